@@ -318,6 +318,110 @@ tn_status tn_sdpa_decode_noalloc(void* stream, int dtype, const void* q, const v
                                  int64_t D, const int32_t* lens, int64_t max_len, double scale,
                                  void* out, float* lse);
 
+/* ---- a key/value cache in pages, held in 4 bits ----
+ * The serving counterpart of tn_kv_append and tn_sdpa_decode: the sequences of
+ * a batch share one pool of pages, and every key and value row is held as
+ * q4_0 blocks (4.5 bits an element). The reference has no paged or quantised
+ * cache (its PreallocatedLayer is one contiguous cache a sequence,
+ * kernels/kv_cache.py:92-114); block values are q4_0's (k_quants.rs:219-277).
+ *
+ * tn_q4_cache names one layer's four planes, caller-owned device memory,
+ * 16-byte aligned. With P = pages, H = n_kv_heads, S = page_size (a power of
+ * two, 16 to 256), D = head_dim (a multiple of 32, at most 256), nb = D / 32:
+ *   k_codes  [P][H][S][4][nb][4] bytes: part g (0..3) of a row holds bytes
+ *            4g .. 4g+3 of each of its blocks (byte j of a block: element j
+ *            low, element j + 16 high, as in every q4_0 block);
+ *   k_scales [P][H][S][nb] f16;
+ *   v_codes  [P][H][S/8][16][nb][8] bytes: byte c of block b of eight
+ *            consecutive tokens, in the order 0 2 1 3 4 6 5 7;
+ *   v_scales [P][H][S/8][nb][8] f16, tokens in order.
+ * So the planes hold P * H * S * D / 2 bytes of codes and P * H * S * nb
+ * scales each. Token o of page p is slot p * S + o (int32; P * S < 2^31).
+ * A page may stand in the tables of several requests (a shared prefix). */
+typedef struct tn_q4_cache {
+    uint8_t* k_codes;
+    uint16_t* k_scales;
+    uint8_t* v_codes;
+    uint16_t* v_scales;
+    int64_t pages, page_size, n_kv_heads, head_dim;
+} tn_q4_cache;
+
+/* One step of the page bookkeeping of n requests (n <= 4096), wholly on the
+ * device, so that a captured decode loop can replay it.
+ *   fresh [n]: tokens that request r adds in this step; negative: it has
+ *     ended, and its pages go back.
+ *   lens [n]: tokens it holds. lens_out [n] (may be lens): after the step; 0
+ *     for an ended one.
+ *   table [n][width]: its pages in order; entries for added tokens are
+ *     written, all others are left as they were.
+ *   free_pages [pages]: a stack of free pages, state[0] of them. Ended
+ *     requests' pages are pushed first, in order of requests and pages; then
+ *     each request in order pops the pages that it needs.
+ *   state_out [2] (may be state): free pages after the step, and the pages
+ *     that refused requests lacked (0: none was refused).
+ * A request is refused when its pages run out (it and every later one that
+ * needs any), when it would outgrow its table row, or when its rows would
+ * pass `tokens`: it keeps its length and its pages.
+ *   row_start [n + 1]: the prefix sums of max(fresh, 0), at most `tokens`:
+ *     the rows of request r among the step's rows.
+ *   base [n]: the position of its first new token, -1 if it was refused.
+ *   slots, pos [tokens]: slot and position of each row; slot -1 (and position
+ *     0) for rows of refused requests and behind the last row.
+ * Lengths are taken as lying in [0, width * page_size], state[0] in
+ * [0, pages]; a popped page outside [0, pages) gives slots of -1. */
+tn_status tn_paged_plan(void* stream, int64_t n, const int32_t* fresh, const int32_t* lens, int32_t* lens_out,
+                        int32_t* table, int64_t width, int64_t page_size, int32_t* free_pages, int64_t pages,
+                        const int32_t* state, int32_t* state_out, int64_t tokens, int32_t* row_start, int32_t* base,
+                        int32_t* slots, int32_t* pos);
+
+/* Rows k, v [m][H][D] in `dtype` (TN_F32, TN_BF16, TN_F16), `stride` elements
+ * from one token's row to the next (H * D when dense; more for parts of stacked
+ * projections), into the cache at `slots` [m]. A slot outside the cache is
+ * skipped; slots of one call are distinct (one given twice holds a mix of its
+ * rows). Blocks are those of tn_q4_0_quantize, except that the scale max / -8
+ * is held to +-8188, so that a cached value is finite and at most 65504 in
+ * size, f16's largest: infinities and larger values saturate there. */
+tn_status tn_kv_append_q4_0(void* stream, const tn_q4_cache* cache, int dtype, const void* k, const void* v,
+                            int64_t m, int64_t stride, const int32_t* slots);
+/* The cached rows at `slots` [m], (code - 8) * scale rounded to `dtype`, to k
+ * and v [m][H][D], dense. A slot outside the cache gives rows of NaN. */
+tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t* slots, int64_t m, int dtype,
+                          void* k, void* v);
+
+/* Attention of the last rows of n requests over their cached tokens.
+ *   q [tokens][Hq][D] in `dtype` (TN_F32, TN_BF16, TN_F16), q_stride elements
+ *   from one token's row to the next; out [tokens][Hq][D] in `dtype`, lse
+ *   nullable f32 [tokens][Hq], dense. Query head h reads key/value head
+ *   h / (Hq / H).
+ *   Request r has rows row_start[r] .. row_start[r+1] - 1, its last tokens, and
+ *   lens[r] cached ones, those rows' own among them (tn_paged_plan's
+ *   row_start and lens_out, after tn_kv_append_q4_0): row j of c attends keys
+ *   0 .. lens[r] - c + j. Token t of it lies at table[r][t / S], t % S.
+ *   max_rows, max_len: host upper bounds of a request's rows and length (they
+ *   size the grid); max_len <= width * S. Rows past max_rows are not computed,
+ *   lengths past max_len are cut to it.
+ *   scale: NaN selects 1/sqrt(D); any sign.
+ * A row with no key to attend gives NaN and lse -inf; one whose keys' page is
+ * outside the cache, NaN and lse NaN. Rows that no request has (behind
+ * row_start[n]) are left as they were. What pages hold past a request's
+ * length, of whatever kind, has no effect. Values that were not written by
+ * tn_kv_append_q4_0 and are past 65504 in size may count as infinite, and an
+ * infinite or NaN value may reach rows of its request ahead of it.
+ * Sums, maxima and the softmax are f32; codes enter the matrix products
+ * exactly for keys of few rows, else as f16 (for f32 and f16 rows in two
+ * parts), probabilities and values as f16 (in two parts where `dtype` needs
+ * them); the output is rounded once.
+ * `work`: scratch of at least tn_sdpa_paged_q4_0_work_floats() floats, 16-byte
+ * aligned, the caller's, so that nothing is allocated and graphs with a
+ * buffer each can run at once; its contents need no preparation and calls on
+ * one stream may share it. */
+int64_t tn_sdpa_paged_q4_0_work_floats(const tn_q4_cache* cache, int64_t n, int64_t tokens, int64_t Hq,
+                                       int64_t max_rows, int64_t max_len);
+tn_status tn_sdpa_paged_q4_0(void* stream, const tn_q4_cache* cache, int dtype, const void* q, int64_t q_stride,
+                             int64_t tokens, int64_t Hq, int64_t n, const int32_t* row_start, const int32_t* lens,
+                             const int32_t* table, int64_t width, int64_t max_rows, int64_t max_len, double scale,
+                             float* work, int64_t work_floats, void* out, float* lse);
+
 /* ---- decode-step ops ----
  * The per-token aten ops around the linear and the attention in a Llama-style
  * decoder step, f32, as the reference runs them for an f32 model

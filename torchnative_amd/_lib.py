@@ -44,6 +44,14 @@ class LlamaLayer(ctypes.Structure):
     ]
 
 
+class Q4Cache(ctypes.Structure):
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v_codes", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p), ("pages", ctypes.c_int64), ("page_size", ctypes.c_int64),
+        ("n_kv_heads", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+    ]
+
+
 class Llama(ctypes.Structure):
     _fields_ = [
         ("n_layers", ctypes.c_int64), ("hidden", ctypes.c_int64), ("n_heads", ctypes.c_int64),
@@ -106,6 +114,12 @@ SIGNATURES = {
     "tn_sdpa_fwd": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I, _P, _I, _D, _P, _P]),
     "tn_sdpa_decode": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _D, _P, _P]),
     "tn_sdpa_decode_noalloc": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _D, _P, _P]),
+    "tn_paged_plan": (_I, [_P, _I64, _P, _P, _P, _P, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _P, _P, _P]),
+    "tn_kv_append_q4_0": (_I, [_P, ctypes.POINTER(Q4Cache), _I, _P, _P, _I64, _I64, _P]),
+    "tn_kv_read_q4_0": (_I, [_P, ctypes.POINTER(Q4Cache), _P, _I64, _I, _P, _P]),
+    "tn_sdpa_paged_q4_0_work_floats": (_I64, [ctypes.POINTER(Q4Cache), _I64, _I64, _I64, _I64, _I64]),
+    "tn_sdpa_paged_q4_0": (_I, [_P, ctypes.POINTER(Q4Cache), _I, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64,
+                                _I64, _D, _P, _I64, _P, _P]),
     "tn_embedding": (_I, [_P, _P, _I64, _P, _I64, _I64, _P]),
     "tn_rmsnorm": (_I, [_P, _P, _I64, _I64, _P, _D, _P]),
     "tn_rope": (_I, [_P, _P, _I64, _I64, _I64, _P, _P]),
