@@ -23,4 +23,34 @@ tn_status paged_check_planes(const char* op, const Pages& c);
 // half hold two consecutive tokens (bytes 0 and 2, bytes 1 and 3).
 __host__ __device__ inline int v_place(int i) { return (i & 4) | ((i & 1) << 1) | ((i >> 1) & 1); }
 
+// Four consecutive elements as floats, at any element.
+template <int DT>
+__device__ inline void load4(const void* p, int64_t i, float (&v)[4]) {
+    if constexpr (DT == TN_F32) {
+        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+        const f4 x = *reinterpret_cast<const f4*>(static_cast<const float*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = x[j];
+    } else {
+        typedef uint16_t h4 __attribute__((ext_vector_type(4), aligned(2)));
+        const h4 x = *reinterpret_cast<const h4*>(static_cast<const uint16_t*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = DT == TN_BF16 ? bf16_to_f32(x[j]) : f16_bits_hw(x[j]);
+    }
+}
+
+template <int DT>
+__device__ inline void store4(void* p, int64_t i, const float (&v)[4]) {
+    if constexpr (DT == TN_F32) {
+        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+        *reinterpret_cast<f4*>(static_cast<float*>(p) + i) = (f4){v[0], v[1], v[2], v[3]};
+    } else {
+        typedef uint16_t h4 __attribute__((ext_vector_type(4), aligned(2)));
+        h4 x;
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = DT == TN_BF16 ? bf16_out(v[j]) : f16_out(v[j]);
+        *reinterpret_cast<h4*>(static_cast<uint16_t*>(p) + i) = x;
+    }
+}
+
 }  // namespace tn

@@ -200,35 +200,6 @@ __global__ __launch_bounds__(256) void k_plan_rows(const PlanArgs a) {
 
 // ---- rows into the cache and back ------------------------------------------------
 
-template <int DT>
-__device__ inline void load4(const void* p, int64_t i, float (&v)[4]) {
-    if constexpr (DT == TN_F32) {
-        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-        const f4 x = *reinterpret_cast<const f4*>(static_cast<const float*>(p) + i);
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = x[j];
-    } else {
-        typedef uint16_t h4 __attribute__((ext_vector_type(4), aligned(2)));
-        const h4 x = *reinterpret_cast<const h4*>(static_cast<const uint16_t*>(p) + i);
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = DT == TN_BF16 ? bf16_to_f32(x[j]) : f16_bits_hw(x[j]);
-    }
-}
-
-template <int DT>
-__device__ inline void store4(void* p, int64_t i, const float (&v)[4]) {
-    if constexpr (DT == TN_F32) {
-        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-        *reinterpret_cast<f4*>(static_cast<float*>(p) + i) = (f4){v[0], v[1], v[2], v[3]};
-    } else {
-        typedef uint16_t h4 __attribute__((ext_vector_type(4), aligned(2)));
-        h4 x;
-#pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = DT == TN_BF16 ? bf16_out(v[j]) : f16_out(v[j]);
-        *reinterpret_cast<h4*>(static_cast<uint16_t*>(p) + i) = x;
-    }
-}
-
 constexpr float KV_MAX_SCALE = 8188.0f;  // 8 * 8188 = 65504, f16's largest
 
 // Four lanes a block: lane g holds elements 4g .. 4g+3 and 16+4g .. 16+4g+3, so

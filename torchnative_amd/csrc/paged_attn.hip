@@ -1,5 +1,11 @@
 // Attention of ragged rows over the paged 4-bit cache (tnhip.h describes the
 // planes and the rows).
+//
+// Rows of a request are folded over the query heads that share a key/value head:
+// row i of (request, key/value head) is token i / G, head h * G + i % G, so that
+// G heads read each key once. Scores are computed transposed, S^T = K Q^T, and so
+// is the output, O^T = V^T P^T: the lane that holds a column's scores then holds
+// them as P^T's operand, with no exchange between lanes (below).
 #include "paged.h"
 
 #include <algorithm>
@@ -10,6 +16,9 @@
 namespace tn {
 namespace {
 
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
 struct PagedArgs {
     Pages c;
     const void* q;
@@ -17,95 +26,368 @@ struct PagedArgs {
     float* lse;  // nullable
     const int32_t *row_start, *lens, *table;
     int64_t q_stride;
-    int n, Hq, G, width, tokens, max_rows, max_len;  // G = Hq / H
-    float sl2;                                      // scale * log2(e)
+    int n, Hq, G, width, max_rows, max_len;  // G = Hq / H
+    float sl2;                               // scale * log2(e)
+    int nsplit, few;                         // splits of the keys; rows of a (request, key/value head) in the partials
+    float* part_o;                           // [n][H][few][nsplit][D] and
+    float2* part_ml;                         // [n][H][few][nsplit], above one split
 };
 
-// One workgroup a (row, query head).
+// Probabilities are kept at 2^P_BIAS times their size over the running maximum,
+// which may lag by RESCALE_SLACK: at most 2^14, so that f16 holds them, and those
+// far below the maximum stay out of its subnormal range as long as they count.
+constexpr float P_BIAS = 6.0f;
+
+// Parts of each 16-bit operand: a 16-bit query is one f16 (a bf16 row scaled by a
+// power of two), an f32 one two; probabilities are two for an output of 11 or 24
+// bits, one for 8; values (code * scale, 15 bits) two for 24.
 template <int DT>
-__global__ __launch_bounds__(256) void k_paged_plain(const PagedArgs a) {
-    __shared__ float sq[256], sp[256], red[4];
-    const int t = blockIdx.x, hq = blockIdx.y, tid = threadIdx.x;
-    if (t >= a.row_start[a.n]) return;
-    int lo = 0, hi = a.n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.row_start[mid] <= t) lo = mid;
-        else hi = mid;
+struct Parts {
+    static constexpr int Q = DT == TN_F32 ? 2 : 1, P = DT == TN_BF16 ? 1 : 2, V = DT == TN_F32 ? 2 : 1;
+};
+
+// Eight codes of a dword as f16, exactly: nibbles 0 4, 2 6, 1 5, 3 7 of it, each
+// pair under the bits of 1024 (low nibbles) or as 16 times its value (high ones).
+__device__ __attribute__((always_inline)) inline void codes4(uint32_t w, h2& a, h2& b) {  // low nibbles
+    const h2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+    a = __builtin_bit_cast(h2, (w & 0x000F000Fu) | 0x64006400u) + off;
+    b = __builtin_bit_cast(h2, ((w >> 8) & 0x000F000Fu) | 0x64006400u) + off;
+}
+__device__ __attribute__((always_inline)) inline void codes4_high(uint32_t w, h2& a, h2& b) {
+    const h2 r = {(_Float16)0.0625f, (_Float16)0.0625f}, off = {(_Float16)-72.0f, (_Float16)-72.0f};
+    a = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x00F000F0u) | 0x64006400u), r, off);
+    b = __builtin_elementwise_fma(__builtin_bit_cast(h2, ((w >> 8) & 0x00F000F0u) | 0x64006400u), r, off);
+}
+__device__ __attribute__((always_inline)) inline h8 join(h2 a, h2 b, h2 c, h2 d) {
+    return (h8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+__device__ __attribute__((always_inline)) inline h8 codes8(uint32_t w) {
+    h2 a, b, c, d;
+    codes4(w, a, b);
+    codes4_high(w, c, d);
+    return join(a, b, c, d);
+}
+
+__device__ __attribute__((always_inline)) inline f32x4 mfma16(h8 a, h8 b, f32x4 c) {
+#if __HIP_DEVICE_COMPILE__
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+#else
+    (void)a, (void)b;
+    return c;
+#endif
+}
+
+// A row's power of two: 2^-e with the largest element of size 2^e .. 2^(e+1), so
+// that bf16 and f32 queries of any size fit f16, the smallest that count above its
+// subnormals; 1 for rows of zeros, infinities and NaN.
+__device__ inline float row_scale(float top) {
+    const uint32_t e = (__builtin_bit_cast(uint32_t, top) >> 23) & 0xffu;
+    // 2^(14 - (e - 127)), a normal number for e up to 254; a subnormal top counts as the smallest normal
+    if (top == 0.0f || e == 255u) return 1.0f;
+    const int x = 14 + 127 - (int)(e < 1u ? 1u : e) + 127;
+    return __builtin_bit_cast(float, (uint32_t)(x > 254 ? 254 : x < 1 ? 1 : x) << 23);
+}
+
+
+// ---- few rows ---------------------------------------------------------------------
+//
+// A wave takes 32 keys at a time. A 16 x 16 x 32 product contracts over one block of
+// 32 elements, so the f32 result is scaled by the block's own scale: codes enter
+// the product exactly. Tile t (0, 1) of S^T has keys 8 g + 4 t + i in row 4 g + i
+// (lane c + 16 g holds rows 4 g .. 4 g + 3 of column c), so that a lane holds eight
+// consecutive keys, the operand of its part of the 32-key product O^T += V^T P^T,
+// whose values it reads as two dwords a block and column (tnhip.h: v_codes).
+template <int NB>
+struct KeyTile {
+    uint32_t k[2][NB];        // rows of the two score tiles: this lane's part of each block
+    uint32_t kd[4 * NB];      // scales of its eight keys, [8][NB] f16
+    uint32_t v[2 * NB];       // values of its eight keys, a byte column of each block
+    uint32_t vd[4 * NB];      // their scales, [NB][8]
+    int bad;                  // its page is outside the cache
+};
+
+template <int N>
+__device__ __attribute__((always_inline)) inline void load_words(const void* p, uint32_t (&w)[N]) {
+    // the widest pieces that N dwords come in; planes are 16-byte aligned, rows of N dwords N-aligned
+    typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef uint32_t u2 __attribute__((ext_vector_type(2), aligned(4)));
+    const uint32_t* s = static_cast<const uint32_t*>(p);
+    constexpr int Q = N / 4 * 4;
+#pragma unroll
+    for (int i = 0; i < Q; i += 4) {
+        const u4 x = *reinterpret_cast<const u4*>(s + i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[i + j] = x[j];
     }
-    const int r = lo, j = t - a.row_start[r], c = a.row_start[r + 1] - a.row_start[r];
-    if (j >= a.max_rows) return;
-    const int len = max(0, min(a.lens[r], a.max_len)), keys = max(0, len - c + j + 1);
-    const int nb = a.c.nb, D = 32 * nb, h = hq / a.G;
+    if constexpr (N % 4 >= 2) {
+        const u2 x = *reinterpret_cast<const u2*>(s + Q);
+        w[Q] = x[0], w[Q + 1] = x[1];
+    }
+    if constexpr (N % 2) w[N - 1] = s[N - 1];
+}
+
+__device__ __attribute__((always_inline)) inline float half_of(uint32_t w, int i) {
+    return (float)__builtin_bit_cast(h2, w)[i];
+}
+
+template <int DT, int NB>
+__global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
+    constexpr int PQ = Parts<DT>::Q, PP = Parts<DT>::P, PV = Parts<DT>::V, D = 32 * NB;
+    __shared__ __align__(16) float so[4][16][D + 4];
+    __shared__ float2 sml[4][16];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const int r = blockIdx.z, h = (int)blockIdx.y % a.c.H, first = (int)blockIdx.y / a.c.H * 16;
+    const int start = a.row_start[r], all = a.row_start[r + 1] - start;
+    const int c = min(all, a.max_rows), rows = c * a.G;
+    if (first >= rows) return;
+    const int len = max(0, min(a.lens[r], a.max_len));
     const int S = 1 << a.c.shift;
-    auto qv = [&](int d) {
-        const int64_t i = t * a.q_stride + (int64_t)hq * D + d;
-        if constexpr (DT == TN_F32) return static_cast<const float*>(a.q)[i];
-        else if constexpr (DT == TN_BF16) return bf16_to_f32(static_cast<const uint16_t*>(a.q)[i]);
-        else return f16_bits_hw(static_cast<const uint16_t*>(a.q)[i]);
+    // this lane's column: its row, and the keys it attends
+    const int i = first + col, j = min(i, rows - 1) / a.G;
+    const int hq = h * a.G + min(i, rows - 1) % a.G;
+    const int keys = max(0, len - all + j + 1);
+    const int most = max(0, len - all + (min(first + 16, rows) - 1) / a.G + 1);  // of any row
+    const int least = max(0, len - all + first / a.G + 1);                       // of every row
+    const int64_t at = (int64_t)(start + j) * a.Hq + hq;
+
+    // the query, as f16 parts in the order of the codes' elements
+    h8 q[PQ][NB];
+    float rs = a.sl2;
+    {
+        float x[NB][8], top = 0.0f;
+        const int64_t qi = (int64_t)(start + j) * a.q_stride + (int64_t)hq * D;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            float lo[4], hi[4];
+            load4<DT>(a.q, qi + 32 * b + 4 * g, lo);
+            load4<DT>(a.q, qi + 32 * b + 16 + 4 * g, hi);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[b][e] = lo[((e & 1) << 1) | (e >> 1)], x[b][4 + e] = hi[((e & 1) << 1) | (e >> 1)];
+                top = fmaxf(top, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
+            }
+        }
+        float sc = 1.0f;
+        if constexpr (DT != TN_F16) {
+            sc = row_scale(wave_xor_max(top));
+            rs = a.sl2 / sc;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = x[b][e] * sc;
+                const _Float16 hi = (_Float16)v;
+                q[0][b][e] = hi;
+                if constexpr (PQ == 2) q[1][b][e] = (_Float16)(v - (float)hi);
+            }
+    }
+
+    f32x4 o[2 * NB];
+#pragma unroll
+    for (int t = 0; t < 2 * NB; t++) o[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.0f;
+
+    // this wave's tiles
+    const int nt = (most + 31) >> 5, nw = a.nsplit * 4, gw = (int)blockIdx.x * 4 + w;
+    const int lo = (int)((int64_t)gw * nt / nw), hi = (int)((int64_t)(gw + 1) * nt / nw);
+    const int32_t* table = a.table + (int64_t)r * a.width;
+    auto pages = [&](int t) {  // the pages of the tile's halves
+        const int last = a.width - 1;
+        return make_int2(table[min((32 * t) >> a.c.shift, last)], table[min((32 * t + 16) >> a.c.shift, last)]);
     };
-    if (tid < D) sq[tid] = qv(tid);
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int k0 = 0; k0 < keys; k0 += 256) {
-        const int key = k0 + tid;
-        float s = -INFINITY;
-        __syncthreads();
-        if (key < keys) {
-            const int page = a.table[(int64_t)r * a.width + (key >> a.c.shift)];
-            if (page < 0 || page >= a.c.pages) {
-                s = NAN;
-            } else {
-                const int64_t row = (((int64_t)page * a.c.H + h) << a.c.shift) + (key & (S - 1));
-                s = 0.0f;
-                for (int b = 0; b < nb; b++) {
-                    float x = 0.0f;
-                    for (int g = 0; g < 4; g++) {
-                        const uint32_t w = *reinterpret_cast<const uint32_t*>(a.c.kc + row * (16 * nb) + (g * nb + b) * 4);
-                        for (int e = 0; e < 4; e++) {
-                            x += sq[32 * b + 4 * g + e] * (float)((int)((w >> (8 * e)) & 15) - 8);
-                            x += sq[32 * b + 16 + 4 * g + e] * (float)((int)((w >> (8 * e + 4)) & 15) - 8);
-                        }
-                    }
-                    s += x * f16_bits_hw(a.c.kd[row * nb + b]);
+    auto load = [&](KeyTile<NB>& x, int t, int2 pg) __attribute__((always_inline)) {
+        const int p0 = __builtin_amdgcn_readfirstlane(pg.x), p1 = __builtin_amdgcn_readfirstlane(pg.y);
+        const bool b0 = (unsigned)p0 >= (unsigned)a.c.pages, b1 = (unsigned)p1 >= (unsigned)a.c.pages;
+        const int64_t r0 = (((int64_t)(b0 ? 0 : p0) * a.c.H + h) << a.c.shift) + ((32 * t) & (S - 1));
+        const int64_t r1 = (((int64_t)(b1 ? 0 : p1) * a.c.H + h) << a.c.shift) + ((32 * t + 16) & (S - 1));
+        const int64_t rk = (col & 8 ? r1 : r0) + (col & 4) * 2 + (col & 3), rg = (g & 2 ? r1 : r0) + (g & 1) * 8;
+        x.bad = g & 2 ? b1 : b0;
+        const uint8_t* kp = a.c.kc + rk * (16 * NB) + g * (4 * NB);
+        load_words(kp, x.k[0]);
+        load_words(kp + 4 * 16 * NB, x.k[1]);
+        load_words(a.c.kd + rg * NB, x.kd);
+        load_words(a.c.vc + rg * (16 * NB) + col * (8 * NB), x.v);
+        load_words(a.c.vd + rg * NB, x.vd);
+    };
+    auto compute = [&](KeyTile<NB>& x, int t) __attribute__((always_inline)) {
+        f32x4 s[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            s[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const h8 kf = codes8(x.k[u][b]);
+                f32x4 y = {0.f, 0.f, 0.f, 0.f};
+                if constexpr (PQ == 2) y = mfma16(kf, q[1][b], y);
+                y = mfma16(kf, q[0][b], y);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int n = (4 * u + e) * NB + b;  // [8][NB]
+                    s[u][e] = fmaf(y[e], half_of(x.kd[n >> 1], n & 1), s[u][e]);
                 }
-                s *= a.sl2;
             }
         }
-        // a NaN score has to reach the maximum
-        float mx = s;
-        for (int i = 32; i; i >>= 1) {
-            const float u = __shfl_xor(mx, i);
-            mx = mx != mx || u != u ? NAN : fmaxf(mx, u);
-        }
-        if ((tid & 63) == 0) red[tid >> 6] = mx;
-        __syncthreads();
-        float mn = m;
-        for (int i = 0; i < 4; i++) mn = mn != mn || red[i] != red[i] ? NAN : fmaxf(mn, red[i]);
-        const float mu = mn == -INFINITY ? 0.0f : mn, al = exp2f(m - mu);
-        m = mn;
-        sp[tid] = exp2f(s - mu);
-        __syncthreads();
-        l *= al;
-        o *= al;
-        for (int i = 0; i < min(256, keys - k0); i++) {
-            l += sp[i];
-            if (tid < D) {
-                const int kk = k0 + i, page = a.table[(int64_t)r * a.width + (kk >> a.c.shift)];
-                if (page < 0 || page >= a.c.pages) continue;
-                const int off = kk & (S - 1), b = tid / 32, e = tid % 32;
-                const int64_t group = (((int64_t)page * a.c.H + h) << (a.c.shift - 3)) + (off >> 3);
-                const int w = a.c.vc[group * (128 * nb) + ((e & 15) * nb + b) * 8 + v_place(off & 7)];
-                o += sp[i] * ((float)((e < 16 ? w & 15 : w >> 4) - 8) * f16_bits_hw(a.c.vd[(group * nb + b) * 8 + (off & 7)]));
+        const int k0 = 32 * t + 8 * g;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[u][e] = s[u][e] * rs;
+        const bool edge = 32 * t + 32 > least || __any(x.bad);
+        if (edge) {
+#pragma unroll
+            for (int n = 0; n < 8; n++) {
+                const float v = s[n >> 2][n & 3];
+                s[n >> 2][n & 3] = k0 + n >= keys ? -INFINITY : x.bad ? NAN : v;
+            }
+            // values that no row attends count as zeros, whatever their page holds
+#pragma unroll
+            for (int n = 0; n < 8; n += 2) {
+                const uint32_t keep = x.bad ? 0u : (k0 + n < len ? 0xffffu : 0u) | (k0 + n + 1 < len ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int b = 0; b < NB; b++) x.vd[4 * b + (n >> 1)] &= keep;
             }
         }
+        float mx = s[0][0];
+#pragma unroll
+        for (int n = 1; n < 8; n++) mx = fmaxf(mx, s[n >> 2][n & 3]);
+        mx = wave_xor_max(mx);
+        if (__any(mx > m + RESCALE_SLACK)) {
+            const float mn = fmaxf(m, mx), al = exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int b = 0; b < 2 * NB; b++) o[b] = o[b] * al;
+        }
+        const float mu = (m == -INFINITY ? 0.0f : m) - P_BIAS;
+        h8 p[PP];
+#pragma unroll
+        for (int n = 0; n < 8; n++) {
+            const float v = __builtin_amdgcn_exp2f(s[n >> 2][n & 3] - mu);
+            l += v;
+            const _Float16 hv = (_Float16)v;
+            p[0][n] = hv;
+            if constexpr (PP == 2) p[1][n] = (_Float16)(v - (float)hv);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            h2 sc[4];
+#pragma unroll
+            for (int n = 0; n < 4; n++) sc[n] = __builtin_bit_cast(h2, x.vd[4 * b + n]);
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                h2 cd[4], v[4];
+                if (half) codes4_high(x.v[2 * b], cd[0], cd[1]), codes4_high(x.v[2 * b + 1], cd[2], cd[3]);
+                else codes4(x.v[2 * b], cd[0], cd[1]), codes4(x.v[2 * b + 1], cd[2], cd[3]);
+#pragma unroll
+                for (int n = 0; n < 4; n++) v[n] = cd[n] * sc[n];
+                f32x4& acc = o[2 * b + half];
+                const h8 vf = join(v[0], v[1], v[2], v[3]);
+                if constexpr (PV == 2) {
+                    h2 z[4];
+#pragma unroll
+                    for (int n = 0; n < 4; n++) z[n] = __builtin_elementwise_fma(cd[n], sc[n], -v[n]);
+                    acc = mfma16(join(z[0], z[1], z[2], z[3]), p[0], acc);
+                }
+                if constexpr (PP == 2) acc = mfma16(vf, p[1], acc);
+                acc = mfma16(vf, p[0], acc);
+            }
+        }
+    };
+    if (lo < hi) {
+        KeyTile<NB> x, y;
+        int2 pg = pages(lo), next = pages(min(lo + 1, hi - 1));
+        load(x, lo, pg);
+        for (int t = lo; t < hi; t += 2) {
+            pg = pages(min(t + 2, hi - 1));
+            load(y, min(t + 1, hi - 1), next);
+            compute(x, t);
+            if (t + 1 >= hi) break;
+            next = pages(min(t + 3, hi - 1));
+            load(x, min(t + 2, hi - 1), pg);
+            compute(y, t + 1);
+        }
     }
-    const int64_t at = (int64_t)t * a.Hq + hq;
-    if (tid < D) {
-        const float y = o / l;
-        if constexpr (DT == TN_F32) static_cast<float*>(a.out)[at * D + tid] = y;
-        else static_cast<uint16_t*>(a.out)[at * D + tid] = DT == TN_BF16 ? bf16_out(y) : f16_out(y);
+
+    // merge the waves
+    l = wave_xor_sum(l);
+    if (g == 0) sml[w][col] = make_float2(m, l);
+#pragma unroll
+    for (int t = 0; t < 2 * NB; t++) *reinterpret_cast<f32x4*>(&so[w][col][16 * t + 4 * g]) = o[t];
+    __syncthreads();
+    for (int e = tid; e < 16 * (D / 4); e += 256) {
+        const int rc = e / (D / 4), d = e % (D / 4) * 4, ri = first + rc;
+        if (ri >= rows) break;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int s = 0; s < 4; s++) mm = fmaxf(mm, sml[s][rc].x);
+        const float mu = mm == -INFINITY ? 0.0f : mm;
+        float tl = 0.0f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const float f = exp2f(sml[s][rc].x - mu);
+            tl += sml[s][rc].y * f;
+            const f32x4 v = *reinterpret_cast<const f32x4*>(&so[s][rc][d]);
+#pragma unroll
+            for (int n = 0; n < 4; n++) acc[n] += v[n] * f;
+        }
+        if (a.nsplit == 1) {
+            const int64_t row = (int64_t)(start + ri / a.G) * a.Hq + h * a.G + ri % a.G;
+            const float inv = 1.0f / tl, y[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+            store4<DT>(a.out, row * D + d, y);
+            if (a.lse && d == 0) a.lse[row] = tl == 0.0f ? -INFINITY : (mm - P_BIAS) * LN2 + logf(tl);
+        } else {
+            const int64_t row = (((int64_t)r * a.c.H + h) * a.few + ri) * a.nsplit + blockIdx.x;
+            *reinterpret_cast<f32x4*>(a.part_o + row * D + d) = acc;
+            if (d == 0) a.part_ml[row] = make_float2(mm, tl);
+        }
     }
-    if (a.lse && tid == 0) a.lse[at] = m == -INFINITY ? -INFINITY : m * LN2 + logf(l);
+    (void)at;
+}
+
+// The splits of a row, in order: four output columns a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void k_paged_combine(const PagedArgs a) {
+    const int D = 32 * a.c.nb, q4 = D / 4;
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t pr = e / q4;
+    const int d = (int)(e - pr * q4) * 4;
+    const int i = (int)(pr % a.few);
+    const int64_t rh = pr / a.few;
+    const int h = (int)(rh % a.c.H);
+    const int64_t r = rh / a.c.H;
+    if (r >= a.n) return;
+    const int start = a.row_start[r], c = min(a.row_start[r + 1] - start, a.max_rows);
+    if (i >= c * a.G) return;
+    const float2* ml = a.part_ml + pr * a.nsplit;
+    const float* po = a.part_o + pr * a.nsplit * D + d;
+    float mm = -INFINITY, tl = 0.0f;
+    for (int s = 0; s < a.nsplit; s++) mm = fmaxf(mm, ml[s].x);
+    const float mu = mm == -INFINITY ? 0.0f : mm;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < a.nsplit; s++) {
+        const float f = exp2f(ml[s].x - mu);
+        tl += ml[s].y * f;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(po + (int64_t)s * D);
+#pragma unroll
+        for (int n = 0; n < 4; n++) acc[n] += v[n] * f;
+    }
+    const int64_t row = (int64_t)(start + i / a.G) * a.Hq + h * a.G + i % a.G;
+    const float inv = 1.0f / tl, y[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+    store4<DT>(a.out, row * D + d, y);
+    if (a.lse && d == 0) a.lse[row] = tl == 0.0f ? -INFINITY : (mm - P_BIAS) * LN2 + logf(tl);
+}
+
+// Splits of the keys: three workgroups a compute unit, each wave with two tiles or
+// more.
+constexpr int64_t FEW_WGS = 768, FEW_MAX_SPLIT = 64;
+int few_splits(const Pages& c, int64_t n, int64_t G, int64_t max_rows, int64_t max_len) {
+    const int64_t wgs = n * c.H * cdiv(max_rows * G, 16);
+    return (int)std::max<int64_t>(
+        1, std::min<int64_t>({cdiv(FEW_WGS, std::max<int64_t>(wgs, 1)), cdiv(max_len, 256), FEW_MAX_SPLIT}));
 }
 
 tn_status attn_check(const char* op, const tn_q4_cache* cache, int64_t n, int64_t tokens, int64_t Hq, int64_t max_rows,
@@ -121,8 +403,39 @@ tn_status attn_check(const char* op, const tn_q4_cache* cache, int64_t n, int64_
     return TN_OK;
 }
 
-int64_t work_floats(const Pages& c, int64_t n, int64_t tokens, int64_t Hq, int64_t max_rows, int64_t max_len) {
-    return 0;
+// Rows of the partials at most, for this call and every smaller one: above one split
+// there are under FEW_WGS workgroups of 16 rows a split, so under 2 * FEW_WGS in all.
+int64_t part_rows(const Pages& c, int64_t n, int64_t G, int64_t max_rows, int64_t max_len) {
+    const int64_t few = max_rows * G, most = std::min(cdiv(max_len, 256), FEW_MAX_SPLIT);
+    if (most < 2) return 0;
+    return std::min(std::min<int64_t>(few, 16) * 2 * FEW_WGS, n * c.H * few * most);
+}
+
+template <int DT, int NB>
+tn_status launch_few(hipStream_t st, const PagedArgs& a) {
+    const dim3 grid((unsigned)a.nsplit, (unsigned)(a.c.H * cdiv((int64_t)a.max_rows * a.G, 16)), (unsigned)a.n);
+    hipLaunchKernelGGL((k_paged_few<DT, NB>), grid, dim3(256), 0, st, a);
+    TN_LAUNCHED();
+    if (a.nsplit > 1) {
+        const int64_t rows = (int64_t)a.n * a.c.H * a.few;
+        hipLaunchKernelGGL(k_paged_combine<DT>, dim3((unsigned)cdiv(rows * (8 * NB), 256)), dim3(256), 0, st, a);
+        TN_LAUNCHED();
+    }
+    return TN_OK;
+}
+
+template <int DT>
+tn_status launch(hipStream_t st, const PagedArgs& a) {
+    switch (a.c.nb) {
+        case 1: return launch_few<DT, 1>(st, a);
+        case 2: return launch_few<DT, 2>(st, a);
+        case 3: return launch_few<DT, 3>(st, a);
+        case 4: return launch_few<DT, 4>(st, a);
+        case 5: return launch_few<DT, 5>(st, a);
+        case 6: return launch_few<DT, 6>(st, a);
+        case 7: return launch_few<DT, 7>(st, a);
+        default: return launch_few<DT, 8>(st, a);
+    }
 }
 
 }  // namespace
@@ -136,28 +449,30 @@ int64_t tn_sdpa_paged_q4_0_work_floats(const tn_q4_cache* cache, int64_t n, int6
                                        int64_t max_rows, int64_t max_len) {
     Pages c;
     if (attn_check("sdpa_paged_q4_0_work_floats", cache, n, tokens, Hq, max_rows, max_len, &c) != TN_OK) return 0;
-    return work_floats(c, n, tokens, Hq, max_rows, max_len);
+    if (!n || !tokens || !Hq || !max_rows) return 0;
+    return part_rows(c, n, Hq / c.H, std::min(max_rows, tokens), max_len) * (32 * c.nb + 2);
 }
 
 tn_status tn_sdpa_paged_q4_0(void* stream, const tn_q4_cache* cache, int dtype, const void* q, int64_t q_stride,
                              int64_t tokens, int64_t Hq, int64_t n, const int32_t* row_start, const int32_t* lens,
                              const int32_t* table, int64_t width, int64_t max_rows, int64_t max_len, double scale,
-                             float* work, int64_t work_floats_given, void* out, float* lse) {
+                             float* work, int64_t work_floats, void* out, float* lse) {
     const char* op = "sdpa_paged_q4_0";
     PagedArgs a{};
     if (dtype != TN_F32 && dtype != TN_BF16 && dtype != TN_F16)
         return fail(TN_ENOTIMPL, "sdpa_paged_q4_0: rows must be float32, bfloat16 or float16");
     TN_TRY(attn_check(op, cache, n, tokens, Hq, max_rows, max_len, &a.c));
-    const int64_t D = 32 * a.c.nb;
+    const int64_t D = 32 * a.c.nb, G = Hq / a.c.H;
     if (width < 0 || width > INT32_MAX || max_len > (width << a.c.shift))
         return fail(TN_EINVAL, "sdpa_paged_q4_0: max_len " + std::to_string(max_len) + " is past what " +
                                    std::to_string(width) + " pages hold");
     if (tokens > 1 && q_stride < Hq * D) return fail(TN_EINVAL, "sdpa_paged_q4_0: the row stride is shorter than a row");
     if (tokens > 1 && q_stride > INT64_MAX / 8 / tokens)
         return fail(TN_EVALUE, "sdpa_paged_q4_0: shape too large");
-    const int64_t need = work_floats(a.c, n, tokens, Hq, max_rows, max_len);
-    if (work_floats_given < need)
-        return fail(TN_EVALUE, "sdpa_paged_q4_0: work holds " + std::to_string(work_floats_given) +
+    if (max_len && !a.c.pages) return fail(TN_EINVAL, "sdpa_paged_q4_0: the cache has no pages");
+    const int64_t need = tn_sdpa_paged_q4_0_work_floats(cache, n, tokens, Hq, max_rows, max_len);
+    if (work_floats < need)
+        return fail(TN_EVALUE, "sdpa_paged_q4_0: work holds " + std::to_string(work_floats) +
                                    " floats, this call needs " + std::to_string(need));
     if (!n || !tokens || !Hq || !max_rows) return TN_OK;
     if (!q || !out || !row_start || !lens || (max_len && !table) || (need && !work))
@@ -166,16 +481,18 @@ tn_status tn_sdpa_paged_q4_0(void* stream, const tn_q4_cache* cache, int dtype, 
     TN_TRY(paged_check_planes(op, a.c));
     const double sc = std::isnan(scale) ? 1.0 / std::sqrt((double)D) : scale;
     a.q = q, a.out = out, a.lse = lse, a.row_start = row_start, a.lens = lens, a.table = table;
-    a.q_stride = q_stride, a.n = (int)n, a.Hq = (int)Hq, a.G = (int)(Hq / a.c.H), a.width = (int)width;
-    a.tokens = (int)tokens, a.max_rows = (int)std::min<int64_t>(max_rows, INT32_MAX), a.max_len = (int)max_len;
+    a.q_stride = q_stride, a.n = (int)n, a.Hq = (int)Hq, a.G = (int)G, a.width = (int)width;
+    a.max_rows = (int)std::min(max_rows, tokens), a.max_len = (int)max_len;
     a.sl2 = (float)(sc * 1.4426950408889634);
+    a.nsplit = few_splits(a.c, n, G, a.max_rows, max_len);
+    a.few = a.max_rows * a.G;
+    const int64_t rows = part_rows(a.c, n, G, a.max_rows, max_len);
+    a.part_o = work;
+    a.part_ml = reinterpret_cast<float2*>(work + rows * D);
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)tokens, (unsigned)Hq);
-    if (dtype == TN_F32) hipLaunchKernelGGL(k_paged_plain<TN_F32>, grid, dim3(256), 0, st, a);
-    else if (dtype == TN_BF16) hipLaunchKernelGGL(k_paged_plain<TN_BF16>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_paged_plain<TN_F16>, grid, dim3(256), 0, st, a);
-    TN_LAUNCHED();
-    return TN_OK;
+    if (dtype == TN_F32) return launch<TN_F32>(st, a);
+    if (dtype == TN_BF16) return launch<TN_BF16>(st, a);
+    return launch<TN_F16>(st, a);
 }
 
 }  // extern "C"
