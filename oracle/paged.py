@@ -123,20 +123,22 @@ def attend(q, cache, row_start, lens, table, scale=None):
         good = (page >= 0) & (page < cache.P)
         slot = np.where(good, page * S + t % S, 0)
         k, v = cache.rows("k", slot), cache.rows("v", slot)
-        for i in range(a, z):
-            m = max(0, length - (z - a) + (i - a) + 1)
-            for h in range(Hq):
-                kh, vh = k[:m, h // G], v[:m, h // G]
-                s = (kh @ q[i, h]) * scale
-                s[~good[:m]] = np.nan
-                if m == 0:
-                    out[i, h], lse[i, h], pav[i, h], vsum[i, h], qk[i, h] = np.nan, -np.inf, 0, 0, 0
-                    continue
-                e = np.exp(s - s.max())
-                p = e / e.sum()
-                out[i, h], lse[i, h] = p @ vh, s.max() + np.log(e.sum())
-                pav[i, h], vsum[i, h] = p @ np.abs(vh), np.abs(vh).sum(0)
-                qk[i, h] = (np.abs(kh) @ np.abs(q[i, h])).max() * abs(scale)
+        m = np.maximum(0, length - (z - a) + np.arange(z - a) + 1)  # keys of each row
+        none, seen = m == 0, t[None] < m[:, None]
+        for h in range(Hq):
+            kh, vh = k[:, h // G], v[:, h // G]
+            with np.errstate(invalid="ignore", divide="ignore"):
+                s = np.where(good, (q[a:z, h] @ kh.T) * scale, np.nan)
+                s = np.where(seen, s, -np.inf)
+                top = s.max(1, initial=-np.inf)
+                e = np.exp(s - np.where(none, 0, top)[:, None])
+                p = e / e.sum(1, keepdims=True)
+                vz = np.where(good[:, None], vh, 0)
+                out[a:z, h], lse[a:z, h] = p @ vz, top + np.log(e.sum(1))
+                pav[a:z, h] = p @ np.abs(vz)
+            vsum[a:z, h] = seen @ np.abs(vz)
+            qk[a:z, h] = np.where(seen & good, np.abs(q[a:z, h]) @ np.abs(kh).T, 0).max(1, initial=0) * abs(scale)
+            out[a:z, h][none], lse[a:z, h][none], pav[a:z, h][none] = np.nan, -np.inf, 0
     return out, lse, pav, vsum, qk
 
 

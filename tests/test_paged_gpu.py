@@ -312,6 +312,15 @@ def test_chunks_and_whole_prompts(tn, dtype, H, G, D, S, rows, lens):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])
+def test_many_rows_of_many_heads(tn, dtype, D):
+    """131072 folded rows and more: the kernel of 256 rows a workgroup, with a request of few rows among the others."""
+    rows = [250, 1, 600, 0, 700, 513]
+    c = Case(tn, dtype, 8, 8, D, 32, rows, [260, 500, 610, 3, 690, 513], seed=D)
+    c.check(c.run(tn))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_without_keys_and_empty_requests(tn, dtype):
     """More rows than tokens: the first attend nothing. Requests of no rows, of no tokens, and of neither."""
     c = Case(tn, dtype, 2, 2, 64, 16, [5, 1, 0, 0, 40, 20], [2, 0, 33, 0, 17, 0], extra=1)

@@ -2,7 +2,7 @@
 // kernels index them, and the checks that every entry point makes.
 #pragma once
 
-#include "tn_common.h"
+#include "attn_common.h"
 
 namespace tn {
 
@@ -45,11 +45,9 @@ __device__ inline void store4(void* p, int64_t i, const float (&v)[4]) {
         typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
         *reinterpret_cast<f4*>(static_cast<float*>(p) + i) = (f4){v[0], v[1], v[2], v[3]};
     } else {
-        typedef uint16_t h4 __attribute__((ext_vector_type(4), aligned(2)));
-        h4 x;
-#pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = DT == TN_BF16 ? bf16_out(v[j]) : f16_out(v[j]);
-        *reinterpret_cast<h4*>(static_cast<uint16_t*>(p) + i) = x;
+        typedef uint32_t w2 __attribute__((ext_vector_type(2), aligned(2)));
+        using E = El<DT == TN_F16>;
+        *reinterpret_cast<w2*>(static_cast<uint16_t*>(p) + i) = (w2){E::pack_out(v[0], v[1]), E::pack_out(v[2], v[3])};
     }
 }
 

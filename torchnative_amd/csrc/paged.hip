@@ -19,7 +19,7 @@ tn_status paged_check(const char* op, const tn_q4_cache* cache, Pages* out) {
     if (D < 32 || D > 256 || D % 32)
         return fail(TN_ENOTIMPL, name + ": head_dim " + std::to_string(D) +
                                      " is not implemented for a q4_0 cache; it is a multiple of 32 up to 256");
-    if (H < 1 || H > 65535 || P < 0) return fail(TN_EINVAL, name + ": bad cache sizes");
+    if (H < 1 || H > 8192 || P < 0) return fail(TN_EINVAL, name + ": bad cache sizes");
     if (P > INT32_MAX / S) return fail(TN_EVALUE, name + ": a cache holds fewer than 2^31 slots");
     out->kc = cache->k_codes, out->kd = cache->k_scales, out->vc = cache->v_codes, out->vd = cache->v_scales;
     out->pages = (int)P, out->H = (int)H, out->nb = (int)(D / 32);

@@ -28,7 +28,8 @@ struct PagedArgs {
     int64_t q_stride;
     int n, Hq, G, width, max_rows, max_len;  // G = Hq / H
     float sl2;                               // scale * log2(e)
-    int nsplit, few;                         // splits of the keys; rows of a (request, key/value head) in the partials
+    int nsplit;                              // k_paged_few: splits of the keys
+    int few;                                 // requests of more folded rows are k_paged_many's; 0: all are
     float* part_o;                           // [n][H][few][nsplit][D] and
     float2* part_ml;                         // [n][H][few][nsplit], above one split
 };
@@ -46,26 +47,55 @@ struct Parts {
     static constexpr int Q = DT == TN_F32 ? 2 : 1, P = DT == TN_BF16 ? 1 : 2, V = DT == TN_F32 ? 2 : 1;
 };
 
-// Eight codes of a dword as f16, exactly: nibbles 0 4, 2 6, 1 5, 3 7 of it, each
-// pair under the bits of 1024 (low nibbles) or as 16 times its value (high ones).
-__device__ __attribute__((always_inline)) inline void codes4(uint32_t w, h2& a, h2& b) {  // low nibbles
-    const h2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-    a = __builtin_bit_cast(h2, (w & 0x000F000Fu) | 0x64006400u) + off;
-    b = __builtin_bit_cast(h2, ((w >> 8) & 0x000F000Fu) | 0x64006400u) + off;
+#define TN_INLINE __device__ __attribute__((always_inline)) inline
+
+// Pairs of f16 in a dword.
+TN_INLINE h2 as_h2(uint32_t w) { return __builtin_bit_cast(h2, w); }
+TN_INLINE uint32_t pk_mul(uint32_t a, uint32_t b) { return __builtin_bit_cast(uint32_t, as_h2(a) * as_h2(b)); }
+// a * b - c, rounded once: what c, the rounded product, lacks
+TN_INLINE uint32_t pk_rest(uint32_t a, uint32_t b, uint32_t c) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(as_h2(a), as_h2(b), -as_h2(c)));
 }
-__device__ __attribute__((always_inline)) inline void codes4_high(uint32_t w, h2& a, h2& b) {
-    const h2 r = {(_Float16)0.0625f, (_Float16)0.0625f}, off = {(_Float16)-72.0f, (_Float16)-72.0f};
-    a = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & 0x00F000F0u) | 0x64006400u), r, off);
-    b = __builtin_elementwise_fma(__builtin_bit_cast(h2, ((w >> 8) & 0x00F000F0u) | 0x64006400u), r, off);
+TN_INLINE h8 as_h8(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(h8, (u4){a, b, c, d});
 }
-__device__ __attribute__((always_inline)) inline h8 join(h2 a, h2 b, h2 c, h2 d) {
-    return (h8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-__device__ __attribute__((always_inline)) inline h8 codes8(uint32_t w) {
-    h2 a, b, c, d;
-    codes4(w, a, b);
-    codes4_high(w, c, d);
-    return join(a, b, c, d);
+TN_INLINE uint32_t pk_f16(float a, float b) { return El<true>::pack_p(a, b); }
+
+// Eight codes of a dword as f16, exactly: its low nibbles (bytes 0 2, bytes 1 3) under
+// the bits of 1024, its high ones as 16 times their value there. One v_and_or_b32 a
+// pair: an instruction takes one constant, so the bits of 1024 sit in a vector
+// register, where the compiler does not see what they are.
+struct Unpack {
+    uint32_t one;
+    TN_INLINE Unpack() {
+#if __HIP_DEVICE_COMPILE__
+        asm("v_mov_b32 %0, 0x64006400" : "=v"(one));
+#endif
+    }
+    TN_INLINE h2 bits(uint32_t w, uint32_t mask) const { return as_h2((w & mask) | one); }
+    TN_INLINE void low(uint32_t w, uint32_t& a, uint32_t& b) const {
+        const h2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
+        a = __builtin_bit_cast(uint32_t, bits(w, 0x000F000Fu) + off);
+        b = __builtin_bit_cast(uint32_t, bits(w >> 8, 0x000F000Fu) + off);
+    }
+    TN_INLINE void high(uint32_t w, uint32_t& a, uint32_t& b) const {
+        const h2 r = {(_Float16)0.0625f, (_Float16)0.0625f}, off = {(_Float16)-72.0f, (_Float16)-72.0f};
+        a = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(bits(w, 0x00F000F0u), r, off));
+        b = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(bits(w >> 8, 0x00F000F0u), r, off));
+    }
+};
+
+// A pair of probabilities as f16 parts, and their sum, unrounded, onto l.
+template <int PARTS>
+TN_INLINE void split_p(float x, float y, uint32_t& hi, uint32_t& lo, float& l) {
+    hi = pk_f16(x, y);
+    if constexpr (PARTS == 2) {
+        const h2 h = as_h2(hi);
+        lo = pk_f16(x - (float)h[0], y - (float)h[1]);
+    }
+    l += x;
+    l += y;
 }
 
 __device__ __attribute__((always_inline)) inline f32x4 mfma16(h8 a, h8 b, f32x4 c) {
@@ -111,16 +141,22 @@ __device__ __attribute__((always_inline)) inline void load_words(const void* p, 
     // the widest pieces that N dwords come in; planes are 16-byte aligned, rows of N dwords N-aligned
     typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(4)));
     typedef uint32_t u2 __attribute__((ext_vector_type(2), aligned(4)));
-    const uint32_t* s = static_cast<const uint32_t*>(p);
+    // (in the global address space, whatever the compiler can see of where p comes from)
+#if __HIP_DEVICE_COMPILE__
+#define TN_GLOBAL __attribute__((address_space(1)))
+#else
+#define TN_GLOBAL
+#endif
+    const TN_GLOBAL uint32_t* s = (const TN_GLOBAL uint32_t*)reinterpret_cast<uintptr_t>(p);
     constexpr int Q = N / 4 * 4;
 #pragma unroll
     for (int i = 0; i < Q; i += 4) {
-        const u4 x = *reinterpret_cast<const u4*>(s + i);
+        const u4 x = *(const TN_GLOBAL u4*)(s + i);
 #pragma unroll
         for (int j = 0; j < 4; j++) w[i + j] = x[j];
     }
     if constexpr (N % 4 >= 2) {
-        const u2 x = *reinterpret_cast<const u2*>(s + Q);
+        const u2 x = *(const TN_GLOBAL u2*)(s + Q);
         w[Q] = x[0], w[Q + 1] = x[1];
     }
     if constexpr (N % 2) w[N - 1] = s[N - 1];
@@ -140,7 +176,7 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
     const int r = blockIdx.z, h = (int)blockIdx.y % a.c.H, first = (int)blockIdx.y / a.c.H * 16;
     const int start = a.row_start[r], all = a.row_start[r + 1] - start;
     const int c = min(all, a.max_rows), rows = c * a.G;
-    if (first >= rows) return;
+    if (first >= rows || rows > a.few) return;
     const int len = max(0, min(a.lens[r], a.max_len));
     const int S = 1 << a.c.shift;
     // this lane's column: its row, and the keys it attends
@@ -211,6 +247,7 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
         load_words(a.c.vc + rg * (16 * NB) + col * (8 * NB), x.v);
         load_words(a.c.vd + rg * NB, x.vd);
     };
+    const Unpack up;
     auto compute = [&](KeyTile<NB>& x, int t) __attribute__((always_inline)) {
         f32x4 s[2];
 #pragma unroll
@@ -218,7 +255,10 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
             s[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                const h8 kf = codes8(x.k[u][b]);
+                uint32_t kw[4];
+                up.low(x.k[u][b], kw[0], kw[1]);
+                up.high(x.k[u][b], kw[2], kw[3]);
+                const h8 kf = as_h8(kw[0], kw[1], kw[2], kw[3]);
                 f32x4 y = {0.f, 0.f, 0.f, 0.f};
                 if constexpr (PQ == 2) y = mfma16(kf, q[1][b], y);
                 y = mfma16(kf, q[0][b], y);
@@ -261,39 +301,32 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
             for (int b = 0; b < 2 * NB; b++) o[b] = o[b] * al;
         }
         const float mu = (m == -INFINITY ? 0.0f : m) - P_BIAS;
-        h8 p[PP];
+        uint32_t ph[4], pl[4];
 #pragma unroll
-        for (int n = 0; n < 8; n++) {
-            const float v = __builtin_amdgcn_exp2f(s[n >> 2][n & 3] - mu);
-            l += v;
-            const _Float16 hv = (_Float16)v;
-            p[0][n] = hv;
-            if constexpr (PP == 2) p[1][n] = (_Float16)(v - (float)hv);
-        }
+        for (int n = 0; n < 8; n += 2)
+            split_p<PP>(__builtin_amdgcn_exp2f(s[n >> 2][n & 3] - mu), __builtin_amdgcn_exp2f(s[n >> 2][(n & 3) + 1] - mu),
+                        ph[n >> 1], pl[n >> 1], l);
+        const h8 p0 = as_h8(ph[0], ph[1], ph[2], ph[3]);
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            h2 sc[4];
-#pragma unroll
-            for (int n = 0; n < 4; n++) sc[n] = __builtin_bit_cast(h2, x.vd[4 * b + n]);
+        for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-                h2 cd[4], v[4];
-                if (half) codes4_high(x.v[2 * b], cd[0], cd[1]), codes4_high(x.v[2 * b + 1], cd[2], cd[3]);
-                else codes4(x.v[2 * b], cd[0], cd[1]), codes4(x.v[2 * b + 1], cd[2], cd[3]);
+                uint32_t cd[4], v[4];
+                if (half) up.high(x.v[2 * b], cd[0], cd[1]), up.high(x.v[2 * b + 1], cd[2], cd[3]);
+                else up.low(x.v[2 * b], cd[0], cd[1]), up.low(x.v[2 * b + 1], cd[2], cd[3]);
 #pragma unroll
-                for (int n = 0; n < 4; n++) v[n] = cd[n] * sc[n];
+                for (int n = 0; n < 4; n++) v[n] = pk_mul(cd[n], x.vd[4 * b + n]);
                 f32x4& acc = o[2 * b + half];
-                const h8 vf = join(v[0], v[1], v[2], v[3]);
+                const h8 vf = as_h8(v[0], v[1], v[2], v[3]);
                 if constexpr (PV == 2) {
-                    h2 z[4];
+                    uint32_t z[4];
 #pragma unroll
-                    for (int n = 0; n < 4; n++) z[n] = __builtin_elementwise_fma(cd[n], sc[n], -v[n]);
-                    acc = mfma16(join(z[0], z[1], z[2], z[3]), p[0], acc);
+                    for (int n = 0; n < 4; n++) z[n] = pk_rest(cd[n], x.vd[4 * b + n], v[n]);
+                    acc = mfma16(as_h8(z[0], z[1], z[2], z[3]), p0, acc);
                 }
-                if constexpr (PP == 2) acc = mfma16(vf, p[1], acc);
-                acc = mfma16(vf, p[0], acc);
+                if constexpr (PP == 2) acc = mfma16(vf, as_h8(pl[0], pl[1], pl[2], pl[3]), acc);
+                acc = mfma16(vf, p0, acc);
             }
-        }
     };
     if (lo < hi) {
         KeyTile<NB> x, y;
@@ -360,7 +393,7 @@ __global__ __launch_bounds__(256) void k_paged_combine(const PagedArgs a) {
     const int64_t r = rh / a.c.H;
     if (r >= a.n) return;
     const int start = a.row_start[r], c = min(a.row_start[r + 1] - start, a.max_rows);
-    if (i >= c * a.G) return;
+    if (i >= c * a.G || c * a.G > a.few) return;
     const float2* ml = a.part_ml + pr * a.nsplit;
     const float* po = a.part_o + pr * a.nsplit * D + d;
     float mm = -INFINITY, tl = 0.0f;
@@ -381,11 +414,371 @@ __global__ __launch_bounds__(256) void k_paged_combine(const PagedArgs a) {
     if (a.lse && d == 0) a.lse[row] = tl == 0.0f ? -INFINITY : (mm - P_BIAS) * LN2 + logf(tl);
 }
 
+// ---- many rows --------------------------------------------------------------------
+//
+// A workgroup takes 128 folded rows, a wave 32 of them, and keys MANY_KEYS at a time.
+// The codes are unpacked and scaled to f16 once a workgroup, into LDS, a stage ahead
+// of their use: K as rows of D elements in the codes' order (chunk 4 b + g: part g of
+// block b), V transposed, a row an element with its keys in the order in which the
+// score product leaves them in a lane (keys 4 h .. 4 h + 3 of each eight in half h of
+// the wave), so that P^T needs no exchange. For 11- and 24-bit outputs the rounded
+// value and what it lacks are two f16 parts. Rows are padded by 16 bytes, which
+// spreads 16 rows' reads over all banks.
+template <int DT, int NB, int W>
+struct Many {
+    static constexpr int KV = DT == TN_BF16 ? 1 : 2, Q = DT == TN_F32 ? 2 : 1, P = DT == TN_F32 ? 2 : 1;
+    static constexpr int T = 64 * W, ROWS = 32 * W;                    // threads, folded rows
+    static constexpr int D = 32 * NB, KP = 2 * D + 16;                  // K row pitch, bytes
+    static constexpr int stage(int kt) { return KV * (kt * KP + D * (2 * kt + 16)); }
+    static constexpr int LDS = W == 8 ? 160 << 10 : 80 << 10;           // one or two workgroups a unit
+    static constexpr int KT = W == 8 && 2 * stage(128) <= LDS ? 128 : 2 * stage(64) <= LDS ? 64 : 32;  // keys of a stage
+    static constexpr int SUB = NB <= 4 && KT >= 64 ? 64 : 32;           // keys of a product: their scores' registers
+    static constexpr int VP = 2 * KT + 16, KB = KT * KP, VB = D * VP, STAGE = KV * (KB + VB);
+    static constexpr int KI = KT * 4, VI = NB * KT;                    // items: (key, part), (byte column, 16 keys)
+    static constexpr int KN = (KI + T - 1) / T, VN = (VI + T - 1) / T;  // of a thread
+    static constexpr int WAVES = W == 8 || 2 * STAGE > LDS ? W / 4 : 2;  // a SIMD, as launch bounds
+};
+
+// Scales that stand in for those of a page outside the cache: NaN for keys (their
+// scores are NaN), zero for values.
+__device__ const uint32_t paged_stand_in[8] = {0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0, 0, 0, 0};
+
+template <int NB>
+TN_INLINE void load_scales(const uint16_t* p, uint32_t (&d)[(NB + 1) / 2]) {
+    if constexpr (NB % 2 == 0) load_words(p, d);
+    else {
+        const TN_GLOBAL uint16_t* s = (const TN_GLOBAL uint16_t*)reinterpret_cast<uintptr_t>(p);
+#pragma unroll
+        for (int b = 0; b < NB; b += 2) d[b / 2] = s[b] | (b + 1 < NB ? (uint32_t)s[b + 1] << 16 : 0u);
+    }
+}
+
+template <int DT, int NB, int W>
+__global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many(const PagedArgs a, int tiles) {
+    using M = Many<DT, NB, W>;
+    constexpr int KT = M::KT, SUB = M::SUB, D = M::D, KV = M::KV, MANY_ROWS = M::ROWS;
+    __shared__ __align__(16) uint8_t lds[2 * M::STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, hh = lane >> 5;
+    // the longest rows first; a key/value head's workgroups on the same dies when there are eight
+    const int h = (int)blockIdx.x % a.c.H, tile = tiles - 1 - (int)blockIdx.x / a.c.H;
+    int r = 0;
+    {  // request r has tiles row_start[r] G / 128 + r and on: at least as many as its rows need
+        int hi = a.n;
+        while (hi - r > 1) {
+            const int mid = (r + hi) >> 1;
+            if ((int)((int64_t)a.row_start[mid] * a.G / MANY_ROWS) + mid <= tile) r = mid;
+            else hi = mid;
+        }
+    }
+    const int start = a.row_start[r], all = a.row_start[r + 1] - start;
+    const int first = (tile - (int)((int64_t)start * a.G / MANY_ROWS) - r) * MANY_ROWS;
+    const int rows = min(all, a.max_rows) * a.G;
+    if (first < 0 || first >= rows || rows <= a.few) return;  // few rows: k_paged_few's
+    const int len = max(0, min(a.lens[r], a.max_len)), before = len - all;
+    const int S = 1 << a.c.shift;
+    const int i = first + 32 * w + col, j = min(i, rows - 1) / a.G, hq = h * a.G + min(i, rows - 1) % a.G;
+    const int keys = max(0, before + j + 1);
+    const int wfirst = first + 32 * w;  // the wave's rows
+    const int wmost = wfirst < rows ? max(0, before + (min(wfirst + 32, rows) - 1) / a.G + 1) : 0;
+    const int most = max(0, before + (min(first + MANY_ROWS, rows) - 1) / a.G + 1);
+    const int nt = (most + KT - 1) / KT;
+
+    // the query: a step of the product contracts over chunks 2 s and 2 s + 1
+    h8 q[M::Q][2 * NB];
+    float rs = fabsf(a.sl2);
+    {
+        float x[2 * NB][8], top = 0.0f;
+        const int64_t qi = (int64_t)(start + j) * a.q_stride + (int64_t)hq * D;
+#pragma unroll
+        for (int s = 0; s < 2 * NB; s++) {
+            float lo[4], hi[4];
+            const int64_t e0 = qi + 32 * (s >> 1) + 8 * (s & 1) + 4 * hh;  // chunk 2 s + hh: part 2 (s & 1) + hh
+            load4<DT>(a.q, e0, lo);
+            load4<DT>(a.q, e0 + 16, hi);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[s][e] = lo[((e & 1) << 1) | (e >> 1)], x[s][4 + e] = hi[((e & 1) << 1) | (e >> 1)];
+                top = fmaxf(top, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
+            }
+        }
+        float sc = 1.0f;
+        if constexpr (DT != TN_F16) {
+            sc = row_scale(xor32_max(top));
+            rs = rs / sc;
+        }
+        // a positive factor, so that it can be taken out of the maximum
+        rs = fmaxf(rs, 1.1754944e-38f);
+        if (a.sl2 < 0.0f) sc = -sc;
+#pragma unroll
+        for (int s = 0; s < 2 * NB; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = x[s][e] * sc;
+                const _Float16 hi = (_Float16)v;
+                q[0][s][e] = hi;
+                if constexpr (M::Q == 2) q[1][s][e] = (_Float16)(v - (float)hi);
+            }
+    }
+    f32x16 o[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[b][e] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    // ---- the workgroup's loads of a stage, and their way into LDS
+    const int32_t* table = a.table + (int64_t)r * a.width;
+    uint32_t kc[M::KN][NB], vc[M::VN][4];
+    uint32_t ksc[M::KN][(NB + 1) / 2];
+    uint32_t vsc[M::VN][8];
+    int kpage[M::KN], vpage[M::VN];
+    // thread's items: K (key, part) with a wave's lanes on one part (their LDS rows differ), V (16 keys, byte column)
+    auto kitem = [&](int n, int& key, int& g) {
+        const int it = tid + M::T * n;
+        key = it % KT, g = it / KT;
+        return it < M::KI;
+    };
+    auto vitem = [&](int n, int& kg, int& b, int& c) {
+        const int it = (M::KI < M::T ? (tid + M::T - M::KI) % M::T : tid) + M::T * n;
+        kg = it / (16 * NB), b = it % (16 * NB) / 16, c = it % 16;
+        return it < M::VI;
+    };
+    auto pages = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < M::KN; n++) {
+            int key, g;
+            kitem(n, key, g);
+            kpage[n] = table[min((KT * t + key) >> a.c.shift, a.width - 1)];
+        }
+#pragma unroll
+        for (int n = 0; n < M::VN; n++) {
+            int kg, b, c;
+            vitem(n, kg, b, c);
+            vpage[n] = table[min((KT * t + 16 * min(kg, KT / 16 - 1)) >> a.c.shift, a.width - 1)];
+        }
+    };
+    auto load = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < M::KN; n++) {
+            int key, g;
+            kitem(n, key, g);
+            const bool bad = (unsigned)kpage[n] >= (unsigned)a.c.pages;
+            const int64_t row = (((int64_t)(bad ? 0 : kpage[n]) * a.c.H + h) << a.c.shift) + ((KT * t + key) & (S - 1));
+            load_words(a.c.kc + row * (16 * NB) + (g & 3) * (4 * NB), kc[n]);
+            load_scales<NB>(bad ? reinterpret_cast<const uint16_t*>(paged_stand_in) : a.c.kd + row * NB, ksc[n]);
+        }
+#pragma unroll
+        for (int n = 0; n < M::VN; n++) {
+            int kg, b, c;
+            vitem(n, kg, b, c);
+            kg = min(kg, KT / 16 - 1);
+            const bool bad = (unsigned)vpage[n] >= (unsigned)a.c.pages;
+            const int64_t group =
+                (((int64_t)(bad ? 0 : vpage[n]) * a.c.H + h) << (a.c.shift - 3)) + (((KT * t + 16 * kg) & (S - 1)) >> 3);
+            const uint8_t* p = a.c.vc + group * (128 * NB) + (c * NB + b) * 8;
+            uint32_t x[2], y[2];
+            load_words(p, x);
+            load_words(p + 128 * NB, y);
+            vc[n][0] = x[0], vc[n][1] = x[1], vc[n][2] = y[0], vc[n][3] = y[1];
+            uint32_t s0[4], s1[4];
+            const uint16_t* zero = reinterpret_cast<const uint16_t*>(paged_stand_in + 4);
+            load_words(bad ? zero : a.c.vd + (group * NB + b) * 8, s0);
+            load_words(bad ? zero : a.c.vd + ((group + 1) * NB + b) * 8, s1);
+#pragma unroll
+            for (int e = 0; e < 4; e++) vsc[n][e] = s0[e], vsc[n][4 + e] = s1[e];
+        }
+    };
+    const Unpack up;
+    auto unpack_k = [&](uint8_t* st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < M::KN; n++) {
+            int key, g;
+            const bool on = kitem(n, key, g);
+            if (M::KI % M::T && !on) continue;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const uint32_t sc = (b & 1 ? ksc[n][b / 2] >> 16 : ksc[n][b / 2] & 0xffffu) * 0x10001u;
+                uint32_t c[4], v[4];
+                up.low(kc[n][b], c[0], c[1]), up.high(kc[n][b], c[2], c[3]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = pk_mul(c[e], sc);
+                uint8_t* p = st + key * M::KP + (4 * b + g) * 16;
+                *reinterpret_cast<h8*>(p) = as_h8(v[0], v[1], v[2], v[3]);
+                if constexpr (KV == 2) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = pk_rest(c[e], sc, v[e]);
+                    *reinterpret_cast<h8*>(p + M::KB) = as_h8(v[0], v[1], v[2], v[3]);
+                }
+            }
+        }
+    };
+    // edge: the stage reaches past the request's length
+    auto unpack_v = [&](auto edge, int t, uint8_t* st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < M::VN; n++) {
+            int kg, b, c;
+            const bool on = vitem(n, kg, b, c);
+            if (M::VI % M::T && !on) continue;
+            if constexpr (decltype(edge)::value) {  // values that no row attends count as zeros
+                const int left = len - KT * t - 16 * kg;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    vsc[n][e] &= (2 * e < left ? 0xffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u);
+            }
+            // dwords 0, 1: tokens 0 .. 7; 2, 3: 8 .. 15. Half 0 holds tokens 0 .. 3 and 8 .. 11
+#pragma unroll
+            for (int high = 0; high < 2; high++)
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    uint32_t x[4], v[4], sc[4];
+                    if (high) up.high(vc[n][half], x[0], x[1]), up.high(vc[n][2 + half], x[2], x[3]);
+                    else up.low(vc[n][half], x[0], x[1]), up.low(vc[n][2 + half], x[2], x[3]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[e] = vsc[n][(e >> 1) * 4 + 2 * half + (e & 1)];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = pk_mul(x[e], sc[e]);
+                    uint8_t* p = st + KV * M::KB + (32 * b + 16 * high + c) * M::VP + (2 * kg + half) * 16;
+                    *reinterpret_cast<h8*>(p) = as_h8(v[0], v[1], v[2], v[3]);
+                    if constexpr (KV == 2) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) v[e] = pk_rest(x[e], sc[e], v[e]);
+                        *reinterpret_cast<h8*>(p + M::VB) = as_h8(v[0], v[1], v[2], v[3]);
+                    }
+                }
+        }
+    };
+
+    f32x16 s[SUB / 32];
+    auto scores = [&](const uint8_t* st, int sub) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < SUB / 32; u++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) s[u][e] = 0.0f;
+            const uint8_t* p = st + (SUB * sub + 32 * u + col) * M::KP + hh * 16;
+#pragma unroll
+            for (int x = 0; x < 2 * NB; x++) {
+                const h8 k = *reinterpret_cast<const h8*>(p + 32 * x);
+                s[u] = El<true>::mfma(k, q[0][x], s[u]);
+                if constexpr (M::Q == 2) s[u] = El<true>::mfma(k, q[1][x], s[u]);
+                if constexpr (KV == 2) s[u] = El<true>::mfma(*reinterpret_cast<const h8*>(p + M::KB + 32 * x), q[0][x], s[u]);
+            }
+        }
+    };
+    auto values = [&](auto edge, const uint8_t* st, int k0, int sub) __attribute__((always_inline)) {
+        if constexpr (decltype(edge)::value) {
+#pragma unroll
+            for (int u = 0; u < SUB / 32; u++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int key = k0 + 32 * u + 8 * (e >> 2) + 4 * hh + (e & 3);
+                    const float v = s[u][e];
+                    s[u][e] = key >= keys ? -INFINITY : v;
+                }
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < SUB / 32; u++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) mx = max3f(mx, s[u][e], s[u][e + 1]);
+        mx = xor32_max(mx) * rs;
+        if (__any(mx > m + RESCALE_SLACK)) {
+            const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[b][e] *= al;
+        }
+        const float mu = P_BIAS - (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+        for (int u = 0; u < SUB / 32; u++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                uint32_t ph[4], pl[4];
+#pragma unroll
+                for (int e = 0; e < 8; e += 2)
+                    split_p<M::P>(__builtin_amdgcn_exp2f(fmaf(s[u][8 * x + e], rs, mu)),
+                                  __builtin_amdgcn_exp2f(fmaf(s[u][8 * x + e + 1], rs, mu)), ph[e >> 1], pl[e >> 1], l);
+                const h8 p0 = as_h8(ph[0], ph[1], ph[2], ph[3]);
+                const uint8_t* vp = st + KV * M::KB + col * M::VP + (SUB / 8 * sub + 4 * u + 2 * x + hh) * 16;
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const h8 v = *reinterpret_cast<const h8*>(vp + 32 * b * M::VP);
+                    if constexpr (KV == 2) o[b] = El<true>::mfma(*reinterpret_cast<const h8*>(vp + M::VB + 32 * b * M::VP), p0, o[b]);
+                    if constexpr (M::P == 2) o[b] = El<true>::mfma(v, as_h8(pl[0], pl[1], pl[2], pl[3]), o[b]);
+                    o[b] = El<true>::mfma(v, p0, o[b]);
+                }
+            }
+    };
+
+    constexpr std::integral_constant<bool, false> INSIDE;
+    constexpr std::integral_constant<bool, true> EDGE;
+    if (nt > 0) {
+        // stages that every row attends in full, and whose successors lie inside the length: no branches
+        const int least = max(0, before + first / a.G + 1), full = min(min(least / KT, len / KT - 1), nt - 1);
+        pages(0);
+        load(0);
+        pages(min(1, nt - 1));
+        unpack_k(lds);
+        unpack_v(EDGE, 0, lds);
+        load(min(1, nt - 1));
+        pages(min(2, nt - 1));
+        __syncthreads();
+        int t = 0;
+        for (; t < full; t++) {
+            uint8_t *st = lds + (t & 1) * M::STAGE, *next = lds + ((t + 1) & 1) * M::STAGE;
+#pragma unroll
+            for (int sub = 0; sub < KT / SUB; sub++) {
+                scores(st, sub);
+                if (sub == 0) unpack_k(next);
+                if (sub == KT / SUB - 1) {
+                    unpack_v(INSIDE, t + 1, next);
+                    load(min(t + 2, nt - 1));
+                    pages(min(t + 3, nt - 1));
+                }
+                values(INSIDE, st, KT * t + SUB * sub, sub);
+            }
+            __syncthreads();
+        }
+        for (; t < nt; t++) {
+            uint8_t *st = lds + (t & 1) * M::STAGE, *next = lds + ((t + 1) & 1) * M::STAGE;
+#pragma unroll 1
+            for (int sub = 0; sub < KT / SUB; sub++)
+                if (KT * t + SUB * sub < wmost) {
+                    scores(st, sub);
+                    values(EDGE, st, KT * t + SUB * sub, sub);
+                }
+            if (t + 1 < nt) {
+                unpack_k(next);
+                unpack_v(EDGE, t + 1, next);
+                load(min(t + 2, nt - 1));
+                pages(min(t + 3, nt - 1));
+            }
+            __syncthreads();
+        }
+    }
+
+    l = xor32_sum(l);
+    if (i >= rows) return;
+    const int64_t row = (int64_t)(start + j) * a.Hq + hq;
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const float y[4] = {o[b][e] * inv, o[b][e + 1] * inv, o[b][e + 2] * inv, o[b][e + 3] * inv};
+            store4<DT>(a.out, row * D + 32 * b + 2 * e + 4 * hh, y);
+        }
+    if (a.lse && hh == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m - P_BIAS) * LN2 + logf(l);
+}
+
 // Splits of the keys: three workgroups a compute unit, each wave with two tiles or
 // more.
 constexpr int64_t FEW_WGS = 768, FEW_MAX_SPLIT = 64;
-int few_splits(const Pages& c, int64_t n, int64_t G, int64_t max_rows, int64_t max_len) {
-    const int64_t wgs = n * c.H * cdiv(max_rows * G, 16);
+int few_splits(const Pages& c, int64_t n, int64_t few, int64_t max_len) {
+    const int64_t wgs = n * c.H * cdiv(few, 16);
     return (int)std::max<int64_t>(
         1, std::min<int64_t>({cdiv(FEW_WGS, std::max<int64_t>(wgs, 1)), cdiv(max_len, 256), FEW_MAX_SPLIT}));
 }
@@ -398,25 +791,48 @@ tn_status attn_check(const char* op, const tn_q4_cache* cache, int64_t n, int64_
     if (Hq % c->H)
         return fail(TN_ENOTIMPL, std::string(op) + ": " + std::to_string(Hq) + " query heads do not divide into " +
                                      std::to_string(c->H) + " key/value heads");
-    if (n > 65535 || Hq > 65535 || tokens > INT32_MAX || tokens * Hq > INT32_MAX || max_len > INT32_MAX)
+    // grids stay under 2^32 threads
+    if (n > 65535 || Hq > 65535 || tokens > INT32_MAX || tokens * Hq > (1 << 30) || n * c->H > (1 << 22) ||
+        max_len > INT32_MAX)
         return fail(TN_EVALUE, std::string(op) + ": shape too large");
     return TN_OK;
 }
 
 // Rows of the partials at most, for this call and every smaller one: above one split
 // there are under FEW_WGS workgroups of 16 rows a split, so under 2 * FEW_WGS in all.
-int64_t part_rows(const Pages& c, int64_t n, int64_t G, int64_t max_rows, int64_t max_len) {
-    const int64_t few = max_rows * G, most = std::min(cdiv(max_len, 256), FEW_MAX_SPLIT);
+int64_t part_rows(const Pages& c, int64_t n, int64_t few, int64_t max_len) {
+    const int64_t most = std::min(cdiv(max_len, 256), FEW_MAX_SPLIT);
     if (most < 2) return 0;
     return std::min(std::min<int64_t>(few, 16) * 2 * FEW_WGS, n * c.H * few * most);
 }
 
+// Folded rows of a request up to which k_paged_few takes it.
+constexpr int FEW_ROWS = 64;
+
+// Folded rows of a request that k_paged_few takes at most in this call; 0: it is not launched. A call of one request
+// is one kernel's.
+int64_t few_limit(int64_t n, int64_t G, int64_t max_rows) {
+    const int64_t rows = max_rows * G;
+    return rows <= FEW_ROWS ? rows : n > 1 ? FEW_ROWS : 0;
+}
+
 template <int DT, int NB>
-tn_status launch_few(hipStream_t st, const PagedArgs& a) {
-    const dim3 grid((unsigned)a.nsplit, (unsigned)(a.c.H * cdiv((int64_t)a.max_rows * a.G, 16)), (unsigned)a.n);
-    hipLaunchKernelGGL((k_paged_few<DT, NB>), grid, dim3(256), 0, st, a);
-    TN_LAUNCHED();
-    if (a.nsplit > 1) {
+tn_status launch_at(hipStream_t st, const PagedArgs& a, int64_t tokens) {
+    if (a.few) {
+        const dim3 grid((unsigned)a.nsplit, (unsigned)(a.c.H * cdiv(a.few, 16)), (unsigned)a.n);
+        hipLaunchKernelGGL((k_paged_few<DT, NB>), grid, dim3(256), 0, st, a);
+        TN_LAUNCHED();
+    }
+    if ((int64_t)a.max_rows * a.G > a.few) {
+        // enough rows for two workgroups of 256 a unit, else of 128 (a unit holds two)
+        const bool wide = tokens * a.G / 256 * a.c.H >= 512;
+        const int64_t tiles = tokens * a.G / (wide ? 256 : 128) + a.n;
+        const dim3 grid((unsigned)(tiles * a.c.H));
+        if (wide) hipLaunchKernelGGL((k_paged_many<DT, NB, 8>), grid, dim3(512), 0, st, a, (int)tiles);
+        else hipLaunchKernelGGL((k_paged_many<DT, NB, 4>), grid, dim3(256), 0, st, a, (int)tiles);
+        TN_LAUNCHED();
+    }
+    if (a.few && a.nsplit > 1) {
         const int64_t rows = (int64_t)a.n * a.c.H * a.few;
         hipLaunchKernelGGL(k_paged_combine<DT>, dim3((unsigned)cdiv(rows * (8 * NB), 256)), dim3(256), 0, st, a);
         TN_LAUNCHED();
@@ -425,16 +841,16 @@ tn_status launch_few(hipStream_t st, const PagedArgs& a) {
 }
 
 template <int DT>
-tn_status launch(hipStream_t st, const PagedArgs& a) {
+tn_status launch(hipStream_t st, const PagedArgs& a, int64_t tokens) {
     switch (a.c.nb) {
-        case 1: return launch_few<DT, 1>(st, a);
-        case 2: return launch_few<DT, 2>(st, a);
-        case 3: return launch_few<DT, 3>(st, a);
-        case 4: return launch_few<DT, 4>(st, a);
-        case 5: return launch_few<DT, 5>(st, a);
-        case 6: return launch_few<DT, 6>(st, a);
-        case 7: return launch_few<DT, 7>(st, a);
-        default: return launch_few<DT, 8>(st, a);
+        case 1: return launch_at<DT, 1>(st, a, tokens);
+        case 2: return launch_at<DT, 2>(st, a, tokens);
+        case 3: return launch_at<DT, 3>(st, a, tokens);
+        case 4: return launch_at<DT, 4>(st, a, tokens);
+        case 5: return launch_at<DT, 5>(st, a, tokens);
+        case 6: return launch_at<DT, 6>(st, a, tokens);
+        case 7: return launch_at<DT, 7>(st, a, tokens);
+        default: return launch_at<DT, 8>(st, a, tokens);
     }
 }
 
@@ -450,7 +866,7 @@ int64_t tn_sdpa_paged_q4_0_work_floats(const tn_q4_cache* cache, int64_t n, int6
     Pages c;
     if (attn_check("sdpa_paged_q4_0_work_floats", cache, n, tokens, Hq, max_rows, max_len, &c) != TN_OK) return 0;
     if (!n || !tokens || !Hq || !max_rows) return 0;
-    return part_rows(c, n, Hq / c.H, std::min(max_rows, tokens), max_len) * (32 * c.nb + 2);
+    return part_rows(c, n, few_limit(n, Hq / c.H, std::min(max_rows, tokens)), max_len) * (32 * c.nb + 2);
 }
 
 tn_status tn_sdpa_paged_q4_0(void* stream, const tn_q4_cache* cache, int dtype, const void* q, int64_t q_stride,
@@ -484,15 +900,15 @@ tn_status tn_sdpa_paged_q4_0(void* stream, const tn_q4_cache* cache, int dtype, 
     a.q_stride = q_stride, a.n = (int)n, a.Hq = (int)Hq, a.G = (int)G, a.width = (int)width;
     a.max_rows = (int)std::min(max_rows, tokens), a.max_len = (int)max_len;
     a.sl2 = (float)(sc * 1.4426950408889634);
-    a.nsplit = few_splits(a.c, n, G, a.max_rows, max_len);
-    a.few = a.max_rows * a.G;
-    const int64_t rows = part_rows(a.c, n, G, a.max_rows, max_len);
+    a.few = (int)few_limit(n, G, a.max_rows);
+    a.nsplit = few_splits(a.c, n, a.few, max_len);
+    const int64_t rows = part_rows(a.c, n, a.few, max_len);
     a.part_o = work;
     a.part_ml = reinterpret_cast<float2*>(work + rows * D);
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == TN_F32) return launch<TN_F32>(st, a);
-    if (dtype == TN_BF16) return launch<TN_BF16>(st, a);
-    return launch<TN_F16>(st, a);
+    if (dtype == TN_F32) return launch<TN_F32>(st, a, tokens);
+    if (dtype == TN_BF16) return launch<TN_BF16>(st, a, tokens);
+    return launch<TN_F16>(st, a, tokens);
 }
 
 }  // extern "C"
