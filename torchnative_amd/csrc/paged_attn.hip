@@ -416,32 +416,60 @@ __global__ __launch_bounds__(256) void k_paged_combine(const PagedArgs a) {
 
 // ---- many rows --------------------------------------------------------------------
 //
-// A workgroup takes 128 folded rows, a wave 32 of them, and keys MANY_KEYS at a time.
-// The codes are unpacked and scaled to f16 once a workgroup, into LDS, a stage ahead
-// of their use: K as rows of D elements in the codes' order (chunk 4 b + g: part g of
-// block b), V transposed, a row an element with its keys in the order in which the
-// score product leaves them in a lane (keys 4 h .. 4 h + 3 of each eight in half h of
-// the wave), so that P^T needs no exchange. For 11- and 24-bit outputs the rounded
-// value and what it lacks are two f16 parts. Rows are padded by 16 bytes, which
-// spreads 16 rows' reads over all banks.
+// A wave takes 32 folded rows, a workgroup 32 W of them, and keys KT at a time. The
+// codes are unpacked and scaled to f16 once a workgroup, into LDS, ahead of their use:
+// K as rows of D elements in the codes' order (chunk 4 b + x + 2 y of 16 bytes: part
+// 2 x + y of block b, so that half x of a wave holds parts 2 x and 2 x + 1), V
+// transposed, a row an element with its keys in the order in which the score product
+// leaves them in a lane (keys 4 h .. 4 h + 3 of each eight in half h of the wave), so
+// that P^T needs no exchange. For 11- and 24-bit outputs the rounded value and what it
+// lacks are two f16 parts. Rows are padded by 16 bytes, which spreads 16 rows' reads
+// over all banks.
+//
+// A wave alternates between a phase of products, O^T += V^T P^T of tile t and S^T of
+// tile t + 1, with its share of the unpacking (V of tile t + 1, K of t + 2) in their
+// shadow, and the softmax of tile t + 1. Eight waves are two groups of one wave a SIMD,
+// half a turn apart: while one group's products run, the other's softmax does. The
+// first group unpacks V and the second K, so that two tiles of each in LDS suffice:
+// with barriers numbered as the first group passes them, it reads V(t) and K(t + 1)
+// and writes V(t + 1) behind barrier 2 t + 2, the second group reads the same and
+// writes K(t + 2) behind 2 t + 3; so V(t + 1) takes the place of V(t - 1), last read
+// behind 2 t + 1, and K(t + 2) that of K(t), last read there too.
 template <int DT, int NB, int W>
 struct Many {
     static constexpr int KV = DT == TN_BF16 ? 1 : 2, Q = DT == TN_F32 ? 2 : 1, P = DT == TN_F32 ? 2 : 1;
-    static constexpr int T = 64 * W, ROWS = 32 * W;                    // threads, folded rows
+    static constexpr int ROWS = 32 * W, GROUPS = W / 4;                // folded rows; groups of four waves
     static constexpr int D = 32 * NB, KP = 2 * D + 16;                  // K row pitch, bytes
     static constexpr int stage(int kt) { return KV * (kt * KP + D * (2 * kt + 16)); }
-    static constexpr int LDS = W == 8 ? 160 << 10 : 80 << 10;           // one or two workgroups a unit
-    static constexpr int KT = W == 8 && 2 * stage(128) <= LDS ? 128 : 2 * stage(64) <= LDS ? 64 : 32;  // keys of a stage
-    static constexpr int SUB = NB <= 4 && KT >= 64 ? 64 : 32;           // keys of a product: their scores' registers
+    static constexpr int LDS = GROUPS == 2 ? 160 << 10 : 80 << 10;      // one or two workgroups a unit
+    static constexpr int KT = NB <= 4 && 2 * stage(64) <= LDS ? 64 : 32;  // keys of a tile
     static constexpr int VP = 2 * KT + 16, KB = KT * KP, VB = D * VP, STAGE = KV * (KB + VB);
     static constexpr int KI = KT * 4, VI = NB * KT;                    // items: (key, part), (byte column, 16 keys)
-    static constexpr int KN = (KI + T - 1) / T, VN = (VI + T - 1) / T;  // of a thread
-    static constexpr int WAVES = W == 8 || 2 * STAGE > LDS ? W / 4 : 2;  // a SIMD, as launch bounds
+    static constexpr int OS = DT == TN_F32 ? 4 : 2, OP = (NB < 4 ? D : 128) * OS + 16;  // output element, row pitch on the way out
+    static constexpr int LDS_BYTES = 2 * STAGE > ROWS * OP ? 2 * STAGE : ROWS * OP;
+    static constexpr int WAVES = GROUPS == 2 || LDS_BYTES <= LDS ? 2 : 1;  // a SIMD, as launch bounds
+    static_assert(KI <= 256 && VI <= 256, "an item a thread");
 };
 
 // Scales that stand in for those of a page outside the cache: NaN for keys (their
 // scores are NaN), zero for values.
 __device__ const uint32_t paged_stand_in[8] = {0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0, 0, 0, 0};
+
+// Eight consecutive elements of a row of type DT, at any element.
+template <int DT>
+struct Eight {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+    u4 w[DT == TN_F32 ? 2 : 1];
+    TN_INLINE void load(const void* p, int64_t i) {
+        const u4* s = reinterpret_cast<const u4*>(static_cast<const char*>(p) + i * (DT == TN_F32 ? 4 : 2));
+        w[0] = s[0];
+        if constexpr (DT == TN_F32) w[1] = s[1];
+    }
+    TN_INLINE float get(int e) const {
+        if constexpr (DT == TN_F32) return __uint_as_float(w[e >> 2][e & 3]);
+        else return e & 1 ? El<DT == TN_F16>::hi(w[0][e >> 1]) : El<DT == TN_F16>::lo(w[0][e >> 1]);
+    }
+};
 
 template <int NB>
 TN_INLINE void load_scales(const uint16_t* p, uint32_t (&d)[(NB + 1) / 2]) {
@@ -456,52 +484,51 @@ TN_INLINE void load_scales(const uint16_t* p, uint32_t (&d)[(NB + 1) / 2]) {
 template <int DT, int NB, int W>
 __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many(const PagedArgs a, int tiles) {
     using M = Many<DT, NB, W>;
-    constexpr int KT = M::KT, SUB = M::SUB, D = M::D, KV = M::KV, MANY_ROWS = M::ROWS;
-    __shared__ __align__(16) uint8_t lds[2 * M::STAGE];
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int KT = M::KT, D = M::D, KV = M::KV, ROWS = M::ROWS;
+    __shared__ __align__(16) uint8_t lds[M::LDS_BYTES];
+    const int tid = threadIdx.x & 255, lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), group = w >> 2;
     const int col = lane & 31, hh = lane >> 5;
-    // the longest rows first; a key/value head's workgroups on the same dies when there are eight
+    // the longest rows first; a key/value head's workgroups on the same die when there are eight
     const int h = (int)blockIdx.x % a.c.H, tile = tiles - 1 - (int)blockIdx.x / a.c.H;
     int r = 0;
-    {  // request r has tiles row_start[r] G / 128 + r and on: at least as many as its rows need
+    {  // request r has tiles row_start[r] G / ROWS + r and on: at least as many as its rows need
         int hi = a.n;
         while (hi - r > 1) {
             const int mid = (r + hi) >> 1;
-            if ((int)((int64_t)a.row_start[mid] * a.G / MANY_ROWS) + mid <= tile) r = mid;
+            if ((int)((int64_t)a.row_start[mid] * a.G / ROWS) + mid <= tile) r = mid;
             else hi = mid;
         }
     }
     const int start = a.row_start[r], all = a.row_start[r + 1] - start;
-    const int first = (tile - (int)((int64_t)start * a.G / MANY_ROWS) - r) * MANY_ROWS;
+    const int first = (tile - (int)((int64_t)start * a.G / ROWS) - r) * ROWS;
     const int rows = min(all, a.max_rows) * a.G;
     if (first < 0 || first >= rows || rows <= a.few) return;  // few rows: k_paged_few's
     const int len = max(0, min(a.lens[r], a.max_len)), before = len - all;
     const int S = 1 << a.c.shift;
     const int i = first + 32 * w + col, j = min(i, rows - 1) / a.G, hq = h * a.G + min(i, rows - 1) % a.G;
     const int keys = max(0, before + j + 1);
-    const int wfirst = first + 32 * w;  // the wave's rows
-    const int wmost = wfirst < rows ? max(0, before + (min(wfirst + 32, rows) - 1) / a.G + 1) : 0;
-    const int most = max(0, before + (min(first + MANY_ROWS, rows) - 1) / a.G + 1);
+    const int least = max(0, before + min(first + 32 * w, rows - 1) / a.G + 1);  // that all of the wave's rows attend
+    const int most = max(0, before + (min(first + ROWS, rows) - 1) / a.G + 1);   // that any of the workgroup's does
     const int nt = (most + KT - 1) / KT;
 
-    // the query: a step of the product contracts over chunks 2 s and 2 s + 1
+    // The query: step 2 b + y of the product contracts over parts y (half 0) and 2 + y
+    // (half 1) of block b, so that a lane's elements of a block are eight low ones in a
+    // row and eight high ones.
     h8 q[M::Q][2 * NB];
     float rs = fabsf(a.sl2);
-    {
-        float x[2 * NB][8], top = 0.0f;
-        const int64_t qi = (int64_t)(start + j) * a.q_stride + (int64_t)hq * D;
+    Eight<DT> qx[NB][2];
+    auto load_q = [&]() __attribute__((always_inline)) {
+        const int64_t qi = (int64_t)(start + j) * a.q_stride + (int64_t)hq * D + 8 * hh;
 #pragma unroll
-        for (int s = 0; s < 2 * NB; s++) {
-            float lo[4], hi[4];
-            const int64_t e0 = qi + 32 * (s >> 1) + 8 * (s & 1) + 4 * hh;  // chunk 2 s + hh: part 2 (s & 1) + hh
-            load4<DT>(a.q, e0, lo);
-            load4<DT>(a.q, e0 + 16, hi);
+        for (int b = 0; b < NB; b++) qx[b][0].load(a.q, qi + 32 * b), qx[b][1].load(a.q, qi + 32 * b + 16);
+    };
+    auto make_q = [&]() __attribute__((always_inline)) {
+        float top = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[s][e] = lo[((e & 1) << 1) | (e >> 1)], x[s][4 + e] = hi[((e & 1) << 1) | (e >> 1)];
-                top = fmaxf(top, fmaxf(fabsf(lo[e]), fabsf(hi[e])));
-            }
-        }
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(qx[b][e >> 3].get(e & 7)));
         float sc = 1.0f;
         if constexpr (DT != TN_F16) {
             sc = row_scale(xor32_max(top));
@@ -511,177 +538,210 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
         rs = fmaxf(rs, 1.1754944e-38f);
         if (a.sl2 < 0.0f) sc = -sc;
 #pragma unroll
-        for (int s = 0; s < 2 * NB; s++)
+        for (int c = 0; c < 2 * NB; c++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = x[s][e] * sc;
+            for (int e = 0; e < 8; e++) {  // elements 0 2 1 3 of the part, low then high
+                const float v = qx[c >> 1][e >> 2].get(4 * (c & 1) + (((e & 1) << 1) | (e >> 1 & 1))) * sc;
                 const _Float16 hi = (_Float16)v;
-                q[0][s][e] = hi;
-                if constexpr (M::Q == 2) q[1][s][e] = (_Float16)(v - (float)hi);
+                q[0][c][e] = hi;
+                if constexpr (M::Q == 2) q[1][c][e] = (_Float16)(v - (float)hi);
             }
-    }
-    f32x16 o[NB];
+    };
+    f32x16 o[NB], s[KT / 32];
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
         for (int e = 0; e < 16; e++) o[b][e] = 0.0f;
     float m = -INFINITY, l = 0.0f;
+    uint32_t ph[KT / 4], pl[KT / 4];
 
-    // ---- the workgroup's loads of a stage, and their way into LDS
+    // ---- this thread's part of a tile: its loads, and their way into LDS
     const int32_t* table = a.table + (int64_t)r * a.width;
-    uint32_t kc[M::KN][NB], vc[M::VN][4];
-    uint32_t ksc[M::KN][(NB + 1) / 2];
-    uint32_t vsc[M::VN][8];
-    int kpage[M::KN], vpage[M::VN];
-    // thread's items: K (key, part) with a wave's lanes on one part (their LDS rows differ), V (16 keys, byte column)
-    auto kitem = [&](int n, int& key, int& g) {
-        const int it = tid + M::T * n;
-        key = it % KT, g = it / KT;
-        return it < M::KI;
-    };
-    auto vitem = [&](int n, int& kg, int& b, int& c) {
-        const int it = (M::KI < M::T ? (tid + M::T - M::KI) % M::T : tid) + M::T * n;
-        kg = it / (16 * NB), b = it % (16 * NB) / 16, c = it % 16;
-        return it < M::VI;
-    };
-    auto pages = [&](int t) __attribute__((always_inline)) {
-#pragma unroll
-        for (int n = 0; n < M::KN; n++) {
-            int key, g;
-            kitem(n, key, g);
-            kpage[n] = table[min((KT * t + key) >> a.c.shift, a.width - 1)];
-        }
-#pragma unroll
-        for (int n = 0; n < M::VN; n++) {
-            int kg, b, c;
-            vitem(n, kg, b, c);
-            vpage[n] = table[min((KT * t + 16 * min(kg, KT / 16 - 1)) >> a.c.shift, a.width - 1)];
-        }
-    };
-    auto load = [&](int t) __attribute__((always_inline)) {
-#pragma unroll
-        for (int n = 0; n < M::KN; n++) {
-            int key, g;
-            kitem(n, key, g);
-            const bool bad = (unsigned)kpage[n] >= (unsigned)a.c.pages;
-            const int64_t row = (((int64_t)(bad ? 0 : kpage[n]) * a.c.H + h) << a.c.shift) + ((KT * t + key) & (S - 1));
-            load_words(a.c.kc + row * (16 * NB) + (g & 3) * (4 * NB), kc[n]);
-            load_scales<NB>(bad ? reinterpret_cast<const uint16_t*>(paged_stand_in) : a.c.kd + row * NB, ksc[n]);
-        }
-#pragma unroll
-        for (int n = 0; n < M::VN; n++) {
-            int kg, b, c;
-            vitem(n, kg, b, c);
-            kg = min(kg, KT / 16 - 1);
-            const bool bad = (unsigned)vpage[n] >= (unsigned)a.c.pages;
-            const int64_t group =
-                (((int64_t)(bad ? 0 : vpage[n]) * a.c.H + h) << (a.c.shift - 3)) + (((KT * t + 16 * kg) & (S - 1)) >> 3);
-            const uint8_t* p = a.c.vc + group * (128 * NB) + (c * NB + b) * 8;
-            uint32_t x[2], y[2];
-            load_words(p, x);
-            load_words(p + 128 * NB, y);
-            vc[n][0] = x[0], vc[n][1] = x[1], vc[n][2] = y[0], vc[n][3] = y[1];
-            uint32_t s0[4], s1[4];
-            const uint16_t* zero = reinterpret_cast<const uint16_t*>(paged_stand_in + 4);
-            load_words(bad ? zero : a.c.vd + (group * NB + b) * 8, s0);
-            load_words(bad ? zero : a.c.vd + ((group + 1) * NB + b) * 8, s1);
-#pragma unroll
-            for (int e = 0; e < 4; e++) vsc[n][e] = s0[e], vsc[n][4 + e] = s1[e];
-        }
-    };
+    // K: (key, part), a wave's lanes on one part (their LDS rows differ); V: (16 keys, byte column)
+    const int ki = tid % M::KI, key = ki % KT, part = ki / KT;
+    const int place = 2 * (part & 1) + (part >> 1);
+    const int vt = M::GROUPS == 1 && M::KI < 256 ? (tid + 256 - M::KI) & 255 : tid;
+    const int vi = vt % M::VI, kg = vi / (16 * NB), vb = vi % (16 * NB) / 16, vcol = vi % 16;
+    const bool kon = M::KI == 256 || tid < M::KI, von = M::VI == 256 || vt < M::VI;
+    struct KPart { uint32_t c[NB], s[(NB + 1) / 2]; } kr;
+    struct VPart { uint32_t c[4], s[8]; } vr;
+    int kpage = 0, vpage = 0;
     const Unpack up;
-    auto unpack_k = [&](uint8_t* st) __attribute__((always_inline)) {
+    // (tiles past the last are the last again)
+    auto kpages = [&](int t) __attribute__((always_inline)) {
+        return table[min((KT * min(t, nt - 1) + key) >> a.c.shift, a.width - 1)];
+    };
+    auto vpages = [&](int t) __attribute__((always_inline)) {
+        return table[min((KT * min(t, nt - 1) + 16 * kg) >> a.c.shift, a.width - 1)];
+    };
+    auto load_k = [&](KPart& x, int page, int t) __attribute__((always_inline)) {
+        t = min(t, nt - 1);
+        const bool bad = (unsigned)page >= (unsigned)a.c.pages;
+        const int64_t row = (((int64_t)(bad ? 0 : page) * a.c.H + h) << a.c.shift) + ((KT * t + key) & (S - 1));
+        load_words(a.c.kc + row * (16 * NB) + part * (4 * NB), x.c);
+        load_scales<NB>(bad ? reinterpret_cast<const uint16_t*>(paged_stand_in) : a.c.kd + row * NB, x.s);
+    };
+    auto load_v = [&](VPart& x, int page, int t) __attribute__((always_inline)) {
+        t = min(t, nt - 1);
+        const bool bad = (unsigned)page >= (unsigned)a.c.pages;
+        const int64_t eight =
+            (((int64_t)(bad ? 0 : page) * a.c.H + h) << (a.c.shift - 3)) + (((KT * t + 16 * kg) & (S - 1)) >> 3);
+        const uint8_t* p = a.c.vc + eight * (128 * NB) + (vcol * NB + vb) * 8;
+        uint32_t c0[2], c1[2], s0[4], s1[4];
+        load_words(p, c0);
+        load_words(p + 128 * NB, c1);
+        x.c[0] = c0[0], x.c[1] = c0[1], x.c[2] = c1[0], x.c[3] = c1[1];
+        const uint16_t* zero = reinterpret_cast<const uint16_t*>(paged_stand_in + 4);
+        load_words(bad ? zero : a.c.vd + (eight * NB + vb) * 8, s0);
+        load_words(bad ? zero : a.c.vd + ((eight + 1) * NB + vb) * 8, s1);
 #pragma unroll
-        for (int n = 0; n < M::KN; n++) {
-            int key, g;
-            const bool on = kitem(n, key, g);
-            if (M::KI % M::T && !on) continue;
+        for (int e = 0; e < 4; e++) x.s[e] = s0[e], x.s[4 + e] = s1[e];
+    };
+    auto unpack_k = [&](const KPart& y, int b, int t) __attribute__((always_inline)) {  // block b of this thread's part of a row
+        const uint32_t sc = (b & 1 ? y.s[b / 2] >> 16 : y.s[b / 2] & 0xffffu) * 0x10001u;
+        uint32_t c[4], v[4];
+        up.low(y.c[b], c[0], c[1]), up.high(y.c[b], c[2], c[3]);
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const uint32_t sc = (b & 1 ? ksc[n][b / 2] >> 16 : ksc[n][b / 2] & 0xffffu) * 0x10001u;
-                uint32_t c[4], v[4];
-                up.low(kc[n][b], c[0], c[1]), up.high(kc[n][b], c[2], c[3]);
+        for (int e = 0; e < 4; e++) v[e] = pk_mul(c[e], sc);
+        uint8_t* p = lds + (t & 1) * M::STAGE + key * M::KP + (4 * b + place) * 16;
+        if (kon) *reinterpret_cast<h8*>(p) = as_h8(v[0], v[1], v[2], v[3]);
+        if constexpr (KV == 2) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = pk_mul(c[e], sc);
-                uint8_t* p = st + key * M::KP + (4 * b + g) * 16;
-                *reinterpret_cast<h8*>(p) = as_h8(v[0], v[1], v[2], v[3]);
-                if constexpr (KV == 2) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = pk_rest(c[e], sc, v[e]);
-                    *reinterpret_cast<h8*>(p + M::KB) = as_h8(v[0], v[1], v[2], v[3]);
-                }
-            }
+            for (int e = 0; e < 4; e++) v[e] = pk_rest(c[e], sc, v[e]);
+            if (kon) *reinterpret_cast<h8*>(p + M::KB) = as_h8(v[0], v[1], v[2], v[3]);
         }
     };
-    // edge: the stage reaches past the request's length
-    auto unpack_v = [&](auto edge, int t, uint8_t* st) __attribute__((always_inline)) {
+    auto edge_v = [&](VPart& y, int t) __attribute__((always_inline)) {  // values that no row attends count as zeros
+        if (KT * t + KT > len) {
+            const int left = len - KT * t - 16 * kg;
 #pragma unroll
-        for (int n = 0; n < M::VN; n++) {
-            int kg, b, c;
-            const bool on = vitem(n, kg, b, c);
-            if (M::VI % M::T && !on) continue;
-            if constexpr (decltype(edge)::value) {  // values that no row attends count as zeros
-                const int left = len - KT * t - 16 * kg;
+            for (int e = 0; e < 8; e++) y.s[e] &= (2 * e < left ? 0xffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u);
+        }
+    };
+    // Half of the elements (low or high nibbles) and of the tokens of this thread's bytes.
+    // Dwords 0, 1: tokens 0 .. 7; 2, 3: 8 .. 15. Half 0 holds tokens 0 .. 3 and 8 .. 11
+    auto unpack_v = [&](const VPart& y, int high, int half, int t) __attribute__((always_inline)) {
+        uint32_t x[4], v[4], sc[4];
+        if (high) up.high(y.c[half], x[0], x[1]), up.high(y.c[2 + half], x[2], x[3]);
+        else up.low(y.c[half], x[0], x[1]), up.low(y.c[2 + half], x[2], x[3]);
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    vsc[n][e] &= (2 * e < left ? 0xffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u);
-            }
-            // dwords 0, 1: tokens 0 .. 7; 2, 3: 8 .. 15. Half 0 holds tokens 0 .. 3 and 8 .. 11
+        for (int e = 0; e < 4; e++) sc[e] = y.s[(e >> 1) * 4 + 2 * half + (e & 1)];
 #pragma unroll
-            for (int high = 0; high < 2; high++)
+        for (int e = 0; e < 4; e++) v[e] = pk_mul(x[e], sc[e]);
+        uint8_t* p = lds + (t & 1) * M::STAGE + KV * M::KB + (32 * vb + 16 * high + vcol) * M::VP + (2 * kg + half) * 16;
+        if (von) *reinterpret_cast<h8*>(p) = as_h8(v[0], v[1], v[2], v[3]);
+        if constexpr (KV == 2) {
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    uint32_t x[4], v[4], sc[4];
-                    if (high) up.high(vc[n][half], x[0], x[1]), up.high(vc[n][2 + half], x[2], x[3]);
-                    else up.low(vc[n][half], x[0], x[1]), up.low(vc[n][2 + half], x[2], x[3]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) sc[e] = vsc[n][(e >> 1) * 4 + 2 * half + (e & 1)];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = pk_mul(x[e], sc[e]);
-                    uint8_t* p = st + KV * M::KB + (32 * b + 16 * high + c) * M::VP + (2 * kg + half) * 16;
-                    *reinterpret_cast<h8*>(p) = as_h8(v[0], v[1], v[2], v[3]);
-                    if constexpr (KV == 2) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) v[e] = pk_rest(x[e], sc[e], v[e]);
-                        *reinterpret_cast<h8*>(p + M::VB) = as_h8(v[0], v[1], v[2], v[3]);
-                    }
-                }
+            for (int e = 0; e < 4; e++) v[e] = pk_rest(x[e], sc[e], v[e]);
+            if (von) *reinterpret_cast<h8*>(p + M::VB) = as_h8(v[0], v[1], v[2], v[3]);
         }
     };
 
-    f32x16 s[SUB / 32];
-    auto scores = [&](const uint8_t* st, int sub) __attribute__((always_inline)) {
+    // ---- the phases
+    // The products of a phase in groups of four fragments out of LDS, each group read
+    // while the one before it is multiplied: PG of O^T += V^T P^T (a group is 16 keys and
+    // BG blocks), then SG of S^T (XG steps of all the tile's keys).
+    constexpr int BG = 4 / KV, PB = (NB + BG - 1) / BG, PG = KT / 16 * PB;
+    constexpr int U = KT / 32, XG = 4 / (KV * U), SG = (2 * NB + XG - 1) / XG;
+    h8 f[2][4];
+    auto fetch = [&](int n, int t) __attribute__((always_inline)) {
+        if (n < PG) {
+            const uint8_t* st = lds + (t & 1) * M::STAGE + KV * M::KB + col * M::VP + hh * 16 + n / PB * 32;
 #pragma unroll
-        for (int u = 0; u < SUB / 32; u++) {
+            for (int e = 0; e < BG; e++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) s[u][e] = 0.0f;
-            const uint8_t* p = st + (SUB * sub + 32 * u + col) * M::KP + hh * 16;
+                for (int p = 0; p < KV; p++)
+                    if (n % PB * BG + e < NB)
+                        f[n & 1][e * KV + p] =
+                            *reinterpret_cast<const h8*>(st + 32 * (n % PB * BG + e) * M::VP + p * M::VB);
+        } else if (n < PG + SG) {
+            const uint8_t* st = lds + ((t + 1) & 1) * M::STAGE + col * M::KP + hh * 16;
 #pragma unroll
-            for (int x = 0; x < 2 * NB; x++) {
-                const h8 k = *reinterpret_cast<const h8*>(p + 32 * x);
-                s[u] = El<true>::mfma(k, q[0][x], s[u]);
-                if constexpr (M::Q == 2) s[u] = El<true>::mfma(k, q[1][x], s[u]);
-                if constexpr (KV == 2) s[u] = El<true>::mfma(*reinterpret_cast<const h8*>(p + M::KB + 32 * x), q[0][x], s[u]);
+            for (int x = 0; x < XG; x++)
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int p = 0; p < KV; p++)
+                        if ((n - PG) * XG + x < 2 * NB)
+                            f[n & 1][(x * U + u) * KV + p] = *reinterpret_cast<const h8*>(
+                                st + 32 * u * M::KP + 32 * ((n - PG) * XG + x) + p * M::KB);
+        }
+    };
+    auto multiply = [&](int n) __attribute__((always_inline)) {
+        if (n < PG) {
+            const int k = 4 * (n / PB);
+            const h8 p0 = as_h8(ph[k], ph[k + 1], ph[k + 2], ph[k + 3]);
+            const h8 p1 = M::P == 2 ? as_h8(pl[k], pl[k + 1], pl[k + 2], pl[k + 3]) : p0;
+#pragma unroll
+            for (int p = KV - 1; p >= 0; p--)
+#pragma unroll
+                for (int e = 0; e < BG; e++) {
+                    const int b = n % PB * BG + e;
+                    if (b >= NB) continue;
+                    if (M::P == 2 && p == 0) o[b] = El<true>::mfma(f[n & 1][e * KV], p1, o[b]);
+                    o[b] = El<true>::mfma(f[n & 1][e * KV + p], p0, o[b]);
+                }
+        } else {
+#pragma unroll
+            for (int x = 0; x < XG; x++) {
+                const int c = (n - PG) * XG + x;
+                if (c >= 2 * NB) continue;
+#pragma unroll
+                for (int p = KV - 1; p >= 0; p--)
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        if (M::Q == 2 && p == 0) s[u] = El<true>::mfma(f[n & 1][(x * U + u) * KV], q[M::Q - 1][c], s[u]);
+                        s[u] = El<true>::mfma(f[n & 1][(x * U + u) * KV + p], q[0][c], s[u]);
+                    }
             }
         }
     };
-    auto values = [&](auto edge, const uint8_t* st, int k0, int sub) __attribute__((always_inline)) {
-        if constexpr (decltype(edge)::value) {
+    // Groups from .. to - 1, the first of which is in registers; between their products,
+    // in their shadow, this thread's part of V of tile t + 1 and K of t + 2 (role: 1 V,
+    // 2 K, 3 both), then the loads of the next ones.
+    auto products = [&](auto role, auto from, auto to, int t) __attribute__((always_inline)) {
+        constexpr int STEPS = to.value - from.value, ROLE = role.value;
+        constexpr int KW = ROLE & 2 ? NB : 0, VW = ROLE & 1 ? 4 : 0, WORK = KW + VW + (ROLE ? 1 : 0);
+        if constexpr (to.value > PG) {
 #pragma unroll
-            for (int u = 0; u < SUB / 32; u++)
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[u][e] = 0.0f;
+        }
+#pragma unroll
+        for (int n = from.value; n < to.value; n++) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (n + 1 < to.value) fetch(n + 1, t);
+            multiply(n);
+#pragma unroll
+            for (int x = (n - from.value) * WORK / STEPS; x < (n - from.value + 1) * WORK / STEPS; x++) {
+                if (x < KW) unpack_k(kr, x, t + 2);
+                else if (x < KW + VW) unpack_v(vr, (x - KW) >> 1, (x - KW) & 1, t + 1);
+                else {
+                    if constexpr (ROLE & 2) load_k(kr, kpage, t + 3), kpage = kpages(t + 4);
+                    if constexpr (ROLE & 1) load_v(vr, vpage, t + 2), vpage = vpages(t + 3);
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto softmax = [&](int t) __attribute__((always_inline)) {
+        if (KT * t + KT > least) {
+#pragma unroll
+            for (int u = 0; u < KT / 32; u++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    const int key = k0 + 32 * u + 8 * (e >> 2) + 4 * hh + (e & 3);
+                    const int k = KT * t + 32 * u + 8 * (e >> 2) + 4 * hh + (e & 3);
                     const float v = s[u][e];
-                    s[u][e] = key >= keys ? -INFINITY : v;
+                    s[u][e] = k >= keys ? -INFINITY : v;
                 }
         }
-        float mx = -INFINITY;
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // short chains
 #pragma unroll
-        for (int u = 0; u < SUB / 32; u++)
+        for (int u = 0; u < KT / 32; u++)
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) mx = max3f(mx, s[u][e], s[u][e + 1]);
-        mx = xor32_max(mx) * rs;
+            for (int e = 0; e < 16; e += 2) mx4[e / 2 & 3] = max3f(mx4[e / 2 & 3], s[u][e], s[u][e + 1]);
+        const float mx = xor32_max(max3f(max3f(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3])) * rs;
         if (__any(mx > m + RESCALE_SLACK)) {
             const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
             m = mn;
@@ -693,85 +753,108 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
         }
         const float mu = P_BIAS - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
-        for (int u = 0; u < SUB / 32; u++)
+        for (int u = 0; u < KT / 32; u++)
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                uint32_t ph[4], pl[4];
+            for (int e = 0; e < 16; e += 2)
+                split_p<M::P>(__builtin_amdgcn_exp2f(fmaf(s[u][e], rs, mu)),
+                              __builtin_amdgcn_exp2f(fmaf(s[u][e + 1], rs, mu)), ph[8 * u + e / 2], pl[8 * u + e / 2], l);
+        // computed here, not where the products take them
+#if __HIP_DEVICE_COMPILE__
 #pragma unroll
-                for (int e = 0; e < 8; e += 2)
-                    split_p<M::P>(__builtin_amdgcn_exp2f(fmaf(s[u][8 * x + e], rs, mu)),
-                                  __builtin_amdgcn_exp2f(fmaf(s[u][8 * x + e + 1], rs, mu)), ph[e >> 1], pl[e >> 1], l);
-                const h8 p0 = as_h8(ph[0], ph[1], ph[2], ph[3]);
-                const uint8_t* vp = st + KV * M::KB + col * M::VP + (SUB / 8 * sub + 4 * u + 2 * x + hh) * 16;
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const h8 v = *reinterpret_cast<const h8*>(vp + 32 * b * M::VP);
-                    if constexpr (KV == 2) o[b] = El<true>::mfma(*reinterpret_cast<const h8*>(vp + M::VB + 32 * b * M::VP), p0, o[b]);
-                    if constexpr (M::P == 2) o[b] = El<true>::mfma(v, as_h8(pl[0], pl[1], pl[2], pl[3]), o[b]);
-                    o[b] = El<true>::mfma(v, p0, o[b]);
-                }
-            }
+        for (int e = 0; e < KT / 4; e++) {
+            asm volatile("" : "+v"(ph[e]));
+            if constexpr (M::P == 2) asm volatile("" : "+v"(pl[e]));
+        }
+        asm volatile("" : "+v"(l));
+#endif
     };
-
-    constexpr std::integral_constant<bool, false> INSIDE;
-    constexpr std::integral_constant<bool, true> EDGE;
-    if (nt > 0) {
-        // stages that every row attends in full, and whose successors lie inside the length: no branches
-        const int least = max(0, before + first / a.G + 1), full = min(min(least / KT, len / KT - 1), nt - 1);
-        pages(0);
-        load(0);
-        pages(min(1, nt - 1));
-        unpack_k(lds);
-        unpack_v(EDGE, 0, lds);
-        load(min(1, nt - 1));
-        pages(min(2, nt - 1));
-        __syncthreads();
-        int t = 0;
-        for (; t < full; t++) {
-            uint8_t *st = lds + (t & 1) * M::STAGE, *next = lds + ((t + 1) & 1) * M::STAGE;
+    auto walk = [&](auto role) __attribute__((always_inline)) {
+        constexpr std::integral_constant<int, 0> BEGIN, NONE;
+        constexpr std::integral_constant<int, PG> MIDDLE;
+        constexpr std::integral_constant<int, PG + SG> END;
+        // all that the first tiles need is asked for before any of it is waited for
+        KPart k0, k1;
+        VPart v0;
+        int kp0 = 0, kp1 = 0, kp2 = 0, vp0 = 0, vp1 = 0;
+        if constexpr (role.value & 2) kp0 = kpages(0), kp1 = kpages(1), kp2 = kpages(2), kpage = kpages(3);
+        if constexpr (role.value & 1) vp0 = vpages(0), vp1 = vpages(1), vpage = vpages(2);
+        load_q();
+        if constexpr (role.value & 2) load_k(k0, kp0, 0), load_k(k1, kp1, 1), load_k(kr, kp2, 2);
+        if constexpr (role.value & 1) load_v(v0, vp0, 0), load_v(vr, vp1, 1);
+        make_q();
+        if constexpr (role.value & 2) {
 #pragma unroll
-            for (int sub = 0; sub < KT / SUB; sub++) {
-                scores(st, sub);
-                if (sub == 0) unpack_k(next);
-                if (sub == KT / SUB - 1) {
-                    unpack_v(INSIDE, t + 1, next);
-                    load(min(t + 2, nt - 1));
-                    pages(min(t + 3, nt - 1));
-                }
-                values(INSIDE, st, KT * t + SUB * sub, sub);
-            }
-            __syncthreads();
+            for (int b = 0; b < NB; b++) unpack_k(k0, b, 0), unpack_k(k1, b, 1);
         }
-        for (; t < nt; t++) {
-            uint8_t *st = lds + (t & 1) * M::STAGE, *next = lds + ((t + 1) & 1) * M::STAGE;
-#pragma unroll 1
-            for (int sub = 0; sub < KT / SUB; sub++)
-                if (KT * t + SUB * sub < wmost) {
-                    scores(st, sub);
-                    values(EDGE, st, KT * t + SUB * sub, sub);
-                }
-            if (t + 1 < nt) {
-                unpack_k(next);
-                unpack_v(EDGE, t + 1, next);
-                load(min(t + 2, nt - 1));
-                pages(min(t + 3, nt - 1));
-            }
-            __syncthreads();
+        if constexpr (role.value & 1) {
+            edge_v(v0, 0);
+#pragma unroll
+            for (int x = 0; x < 4; x++) unpack_v(v0, x >> 1, x & 1, 0);
         }
+        __syncthreads();
+        if (role.value == 2) __syncthreads();  // half a turn behind
+        fetch(PG, -1);
+        products(NONE, MIDDLE, END, -1);
+        for (int t = 0; t + 1 < nt; t++) {
+            __syncthreads();
+            if constexpr (role.value & 1) edge_v(vr, t + 1);
+            softmax(t);
+            fetch(0, t);
+            __syncthreads();
+            __builtin_amdgcn_s_setprio(1);  // the products' few instructions ahead of the other group's many
+            products(role, BEGIN, END, t);
+            __builtin_amdgcn_s_setprio(0);
+        }
+        __syncthreads();
+        softmax(nt - 1);
+        fetch(0, nt - 1);
+        __syncthreads();
+        products(NONE, BEGIN, MIDDLE, nt - 1);
+        if (role.value == 1) __syncthreads();
+    };
+    if (nt > 0) {
+        if constexpr (M::GROUPS == 1) walk(std::integral_constant<int, 3>{});
+        else if (group == 0) walk(std::integral_constant<int, 1>{});
+        else walk(std::integral_constant<int, 2>{});
     }
 
+    // out through LDS, so that a row's bytes leave together
     l = xor32_sum(l);
-    if (i >= rows) return;
-    const int64_t row = (int64_t)(start + j) * a.Hq + hq;
     const float inv = 1.0f / l;
+    uint8_t* mine = lds + w * 32 * M::OP;
+    __syncthreads();
+    if (a.lse && hh == 0 && i < rows)
+        a.lse[(int64_t)(start + j) * a.Hq + hq] = l == 0.0f ? -INFINITY : (m - P_BIAS) * LN2 + logf(l);
 #pragma unroll
-    for (int b = 0; b < NB; b++)
+    for (int b0 = 0; b0 < NB; b0 += 4) {  // four blocks at a time
+        constexpr int SIZE = M::OS;
+        const int nb = NB - b0 < 4 ? NB - b0 : 4, pieces = nb * 2 * SIZE;  // of 16 bytes, a row
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const float y[4] = {o[b][e] * inv, o[b][e + 1] * inv, o[b][e + 2] * inv, o[b][e + 3] * inv};
-            store4<DT>(a.out, row * D + 32 * b + 2 * e + 4 * hh, y);
+        for (int b = b0; b < b0 + nb; b++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const float y[4] = {o[b][e] * inv, o[b][e + 1] * inv, o[b][e + 2] * inv, o[b][e + 3] * inv};
+                uint8_t* p = mine + col * M::OP + (32 * (b - b0) + 2 * e + 4 * hh) * SIZE;
+                if constexpr (DT == TN_F32) {
+                    *reinterpret_cast<f32x4*>(p) = (f32x4){y[0], y[1], y[2], y[3]};
+                } else {
+                    using E = El<DT == TN_F16>;
+                    *reinterpret_cast<uint2*>(p) = make_uint2(E::pack_out(y[0], y[1]), E::pack_out(y[2], y[3]));
+                }
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's own rows
+#pragma unroll
+        for (int k = 0; k < pieces / 2; k++) {
+            const int x = lane + 64 * k, rr = x / pieces, ii = first + 32 * w + rr;
+            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+            typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
+            const u4 v = *reinterpret_cast<const u4*>(mine + rr * M::OP + x % pieces * 16);
+            const int64_t row = (int64_t)(start + ii / a.G) * a.Hq + h * a.G + ii % a.G;
+            if (ii < rows)
+                *reinterpret_cast<v4*>(static_cast<char*>(a.out) + (row * D + 32 * b0) * SIZE + x % pieces * 16) = v;
         }
-    if (a.lse && hh == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m - P_BIAS) * LN2 + logf(l);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
 }
 
 // Splits of the keys: three workgroups a compute unit, each wave with two tiles or
