@@ -312,6 +312,15 @@ def test_chunks_and_whole_prompts(tn, dtype, H, G, D, S, rows, lens):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H, G, D, S", [(2, 3, 64, 16), (1, 4, 128, 32), (1, 2, 96, 16), (1, 1, 256, 64), (1, 2, 32, 16)])
+@pytest.mark.parametrize("rows, lens", [([90], [2100]), ([200, 1, 0, 70, 3], [1500, 900, 40, 70, 1033])])
+def test_chunks_behind_long_contexts(tn, dtype, H, G, D, S, rows, lens):
+    """Keys split over workgroups, with rows whose part of the keys is empty."""
+    c = Case(tn, dtype, H, G, D, S, rows, lens, seed=D + len(rows), extra=2)
+    c.check(c.run(tn))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])
 def test_many_rows_of_many_heads(tn, dtype, D):
     """131072 folded rows and more: the kernel of 256 rows a workgroup, with a request of few rows among the others."""

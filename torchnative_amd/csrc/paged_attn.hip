@@ -32,6 +32,8 @@ struct PagedArgs {
     int few;                                 // requests of more folded rows are k_paged_many's; 0: all are
     float* part_o;                           // [n][H][few][nsplit][D] and
     float2* part_ml;                         // [n][H][few][nsplit], above one split
+    float* many_o;                           // k_paged_many's: [tokens][Hq][splits][D] and
+    float2* many_ml;                         // [tokens][Hq][splits], above one split
 };
 
 // Probabilities are kept at 2^P_BIAS times their size over the running maximum,
@@ -445,7 +447,8 @@ struct Many {
     static constexpr int KT = NB <= 4 && 2 * stage(64) <= LDS ? 64 : 32;  // keys of a tile
     static constexpr int VP = 2 * KT + 16, KB = KT * KP, VB = D * VP, STAGE = KV * (KB + VB);
     static constexpr int KI = KT * 4, VI = NB * KT;                    // items: (key, part), (byte column, 16 keys)
-    static constexpr int OS = DT == TN_F32 ? 4 : 2, OP = (NB < 4 ? D : 128) * OS + 16;  // output element, row pitch on the way out
+    static constexpr int OS = DT == TN_F32 ? 4 : 2;                    // output element
+    static constexpr int OP = (NB < 4 ? D : 128) * (GROUPS == 1 ? 4 : OS) + 16;  // row pitch on the way out
     static constexpr int LDS_BYTES = 2 * STAGE > ROWS * OP ? 2 * STAGE : ROWS * OP;
     static constexpr int WAVES = GROUPS == 2 || LDS_BYTES <= LDS ? 2 : 1;  // a SIMD, as launch bounds
     static_assert(KI <= 256 && VI <= 256, "an item a thread");
@@ -510,7 +513,9 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
     const int keys = max(0, before + j + 1);
     const int least = max(0, before + min(first + 32 * w, rows - 1) / a.G + 1);  // that all of the wave's rows attend
     const int most = max(0, before + (min(first + ROWS, rows) - 1) / a.G + 1);   // that any of the workgroup's does
-    const int nt = (most + KT - 1) / KT;
+    // this workgroup's tiles: one split's share
+    const int all_tiles = (most + KT - 1) / KT, split = blockIdx.y, ns = gridDim.y;
+    const int t0 = (int)((int64_t)split * all_tiles / ns), nt = (int)((int64_t)(split + 1) * all_tiles / ns);
 
     // The query: step 2 b + y of the product contracts over parts y (half 0) and 2 + y
     // (half 1) of block b, so that a lane's elements of a block are eight low ones in a
@@ -776,26 +781,26 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
         KPart k0, k1;
         VPart v0;
         int kp0 = 0, kp1 = 0, kp2 = 0, vp0 = 0, vp1 = 0;
-        if constexpr (role.value & 2) kp0 = kpages(0), kp1 = kpages(1), kp2 = kpages(2), kpage = kpages(3);
-        if constexpr (role.value & 1) vp0 = vpages(0), vp1 = vpages(1), vpage = vpages(2);
+        if constexpr (role.value & 2) kp0 = kpages(t0), kp1 = kpages(t0 + 1), kp2 = kpages(t0 + 2), kpage = kpages(t0 + 3);
+        if constexpr (role.value & 1) vp0 = vpages(t0), vp1 = vpages(t0 + 1), vpage = vpages(t0 + 2);
         load_q();
-        if constexpr (role.value & 2) load_k(k0, kp0, 0), load_k(k1, kp1, 1), load_k(kr, kp2, 2);
-        if constexpr (role.value & 1) load_v(v0, vp0, 0), load_v(vr, vp1, 1);
+        if constexpr (role.value & 2) load_k(k0, kp0, t0), load_k(k1, kp1, t0 + 1), load_k(kr, kp2, t0 + 2);
+        if constexpr (role.value & 1) load_v(v0, vp0, t0), load_v(vr, vp1, t0 + 1);
         make_q();
         if constexpr (role.value & 2) {
 #pragma unroll
-            for (int b = 0; b < NB; b++) unpack_k(k0, b, 0), unpack_k(k1, b, 1);
+            for (int b = 0; b < NB; b++) unpack_k(k0, b, t0), unpack_k(k1, b, t0 + 1);
         }
         if constexpr (role.value & 1) {
-            edge_v(v0, 0);
+            edge_v(v0, t0);
 #pragma unroll
-            for (int x = 0; x < 4; x++) unpack_v(v0, x >> 1, x & 1, 0);
+            for (int x = 0; x < 4; x++) unpack_v(v0, x >> 1, x & 1, t0);
         }
         __syncthreads();
         if (role.value == 2) __syncthreads();  // half a turn behind
-        fetch(PG, -1);
-        products(NONE, MIDDLE, END, -1);
-        for (int t = 0; t + 1 < nt; t++) {
+        fetch(PG, t0 - 1);
+        products(NONE, MIDDLE, END, t0 - 1);
+        for (int t = t0; t + 1 < nt; t++) {
             __syncthreads();
             if constexpr (role.value & 1) edge_v(vr, t + 1);
             softmax(t);
@@ -812,49 +817,91 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
         products(NONE, BEGIN, MIDDLE, nt - 1);
         if (role.value == 1) __syncthreads();
     };
-    if (nt > 0) {
+    if (nt > t0) {
         if constexpr (M::GROUPS == 1) walk(std::integral_constant<int, 3>{});
         else if (group == 0) walk(std::integral_constant<int, 1>{});
         else walk(std::integral_constant<int, 2>{});
     }
 
-    // out through LDS, so that a row's bytes leave together
+    // out through LDS, so that a row's bytes leave together, in `type` to rows of a.out or (many_o) f32
     l = xor32_sum(l);
-    const float inv = 1.0f / l;
     uint8_t* mine = lds + w * 32 * M::OP;
     __syncthreads();
-    if (a.lse && hh == 0 && i < rows)
-        a.lse[(int64_t)(start + j) * a.Hq + hq] = l == 0.0f ? -INFINITY : (m - P_BIAS) * LN2 + logf(l);
+    auto leave = [&](auto type, float f) __attribute__((always_inline)) {
+        constexpr int OT = type.value, SIZE = OT == TN_F32 ? 4 : 2;
 #pragma unroll
-    for (int b0 = 0; b0 < NB; b0 += 4) {  // four blocks at a time
-        constexpr int SIZE = M::OS;
-        const int nb = NB - b0 < 4 ? NB - b0 : 4, pieces = nb * 2 * SIZE;  // of 16 bytes, a row
+        for (int b0 = 0; b0 < NB; b0 += 4) {  // four blocks at a time
+            const int nb = NB - b0 < 4 ? NB - b0 : 4, pieces = nb * 2 * SIZE;  // of 16 bytes, a row
 #pragma unroll
-        for (int b = b0; b < b0 + nb; b++)
+            for (int b = b0; b < b0 + nb; b++)
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const float y[4] = {o[b][e] * inv, o[b][e + 1] * inv, o[b][e + 2] * inv, o[b][e + 3] * inv};
-                uint8_t* p = mine + col * M::OP + (32 * (b - b0) + 2 * e + 4 * hh) * SIZE;
-                if constexpr (DT == TN_F32) {
-                    *reinterpret_cast<f32x4*>(p) = (f32x4){y[0], y[1], y[2], y[3]};
-                } else {
-                    using E = El<DT == TN_F16>;
-                    *reinterpret_cast<uint2*>(p) = make_uint2(E::pack_out(y[0], y[1]), E::pack_out(y[2], y[3]));
+                for (int e = 0; e < 16; e += 4) {
+                    const float y[4] = {o[b][e] * f, o[b][e + 1] * f, o[b][e + 2] * f, o[b][e + 3] * f};
+                    uint8_t* p = mine + col * M::OP + (32 * (b - b0) + 2 * e + 4 * hh) * SIZE;
+                    if constexpr (OT == TN_F32) {
+                        *reinterpret_cast<f32x4*>(p) = (f32x4){y[0], y[1], y[2], y[3]};
+                    } else {
+                        using E = El<OT == TN_F16>;
+                        *reinterpret_cast<uint2*>(p) = make_uint2(E::pack_out(y[0], y[1]), E::pack_out(y[2], y[3]));
+                    }
                 }
-            }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's own rows
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's own rows
 #pragma unroll
-        for (int k = 0; k < pieces / 2; k++) {
-            const int x = lane + 64 * k, rr = x / pieces, ii = first + 32 * w + rr;
-            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-            typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
-            const u4 v = *reinterpret_cast<const u4*>(mine + rr * M::OP + x % pieces * 16);
-            const int64_t row = (int64_t)(start + ii / a.G) * a.Hq + h * a.G + ii % a.G;
-            if (ii < rows)
-                *reinterpret_cast<v4*>(static_cast<char*>(a.out) + (row * D + 32 * b0) * SIZE + x % pieces * 16) = v;
+            for (int k = 0; k < pieces / 2; k++) {
+                const int x = lane + 64 * k, rr = x / pieces, ii = first + 32 * w + rr;
+                typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+                typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
+                const u4 v = *reinterpret_cast<const u4*>(mine + rr * M::OP + x % pieces * 16);
+                int64_t row = (int64_t)(start + ii / a.G) * a.Hq + h * a.G + ii % a.G;
+                if (ns > 1) row = row * ns + split;
+                char* to = ns > 1 ? reinterpret_cast<char*>(a.many_o) : static_cast<char*>(a.out);
+                if (ii < rows) *reinterpret_cast<v4*>(to + (row * D + 32 * b0) * SIZE + x % pieces * 16) = v;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    const int64_t row = (int64_t)(start + j) * a.Hq + hq;
+    if (M::GROUPS == 1 && ns > 1) {  // a split's part: k_paged_join's
+        leave(std::integral_constant<int, TN_F32>{}, 1.0f);
+        if (hh == 0 && i < rows) a.many_ml[row * ns + split] = make_float2(m, l);
+    } else {
+        leave(std::integral_constant<int, DT>{}, 1.0f / l);
+        if (a.lse && hh == 0 && i < rows) a.lse[row] = l == 0.0f ? -INFINITY : (m - P_BIAS) * LN2 + logf(l);
     }
+}
+
+// The splits of k_paged_many's rows, in order: four output columns a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void k_paged_join(const PagedArgs a, int ns) {
+    const int D = 32 * a.c.nb, q4 = D / 4;
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = e / q4;
+    const int d = (int)(e - row * q4) * 4, t = (int)(row / a.Hq);
+    if (t >= a.row_start[a.n]) return;
+    int r = 0, hi = a.n;  // the row's request
+    while (hi - r > 1) {
+        const int mid = (r + hi) >> 1;
+        if (a.row_start[mid] <= t) r = mid;
+        else hi = mid;
+    }
+    const int start = a.row_start[r], c = min(a.row_start[r + 1] - start, a.max_rows);
+    if (t - start >= c || c * a.G <= a.few) return;
+    const float2* ml = a.many_ml + row * ns;
+    const float* po = a.many_o + row * ns * D + d;
+    float mm = -INFINITY, tl = 0.0f;
+    for (int s = 0; s < ns; s++) mm = fmaxf(mm, ml[s].x);
+    const float mu = mm == -INFINITY ? 0.0f : mm;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < ns; s++) {
+        const float f = exp2f(ml[s].x - mu);
+        tl += ml[s].y * f;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(po + (int64_t)s * D);
+#pragma unroll
+        for (int n = 0; n < 4; n++) acc[n] += v[n] * f;
+    }
+    const float inv = 1.0f / tl, y[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+    store4<DT>(a.out, row * D + d, y);
+    if (a.lse && d == 0) a.lse[row] = tl == 0.0f ? -INFINITY : (mm - P_BIAS) * LN2 + logf(tl);
 }
 
 // Splits of the keys: three workgroups a compute unit, each wave with two tiles or
@@ -889,6 +936,21 @@ int64_t part_rows(const Pages& c, int64_t n, int64_t few, int64_t max_len) {
     return std::min(std::min<int64_t>(few, 16) * 2 * FEW_WGS, n * c.H * few * most);
 }
 
+// k_paged_many: 0 for workgroups of 256 rows (rows enough for two a unit), else the
+// splits of the keys for workgroups of 128, two of which a unit holds.
+constexpr int64_t MANY_WGS = 512, MANY_MAX_SPLIT = 8;
+int many_splits(const Pages& c, int64_t n, int64_t tokens, int64_t G, int64_t max_len) {
+    if (tokens * G / 256 * c.H >= MANY_WGS) return 0;
+    const int64_t wgs = (tokens * G / 128 + n) * c.H;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(MANY_WGS, wgs), cdiv(max_len, 512), MANY_MAX_SPLIT}));
+}
+// Rows of its partials at most, for this call and every smaller one: above one split there
+// are under MANY_WGS workgroups of 128 rows a split.
+int64_t many_rows(const Pages& c, int64_t tokens, int64_t G, int64_t max_len) {
+    const int64_t most = std::min(cdiv(max_len, 512), MANY_MAX_SPLIT);
+    return most < 2 ? 0 : std::min(tokens * G * c.H * most, 2 * MANY_WGS * 128);
+}
+
 // Folded rows of a request up to which k_paged_few takes it.
 constexpr int FEW_ROWS = 64;
 
@@ -899,6 +961,12 @@ int64_t few_limit(int64_t n, int64_t G, int64_t max_rows) {
     return rows <= FEW_ROWS ? rows : n > 1 ? FEW_ROWS : 0;
 }
 
+int64_t work_rows(const Pages& c, int64_t n, int64_t tokens, int64_t G, int64_t max_rows, int64_t max_len) {
+    // by the largest number of folded rows that a smaller call could have in k_paged_few
+    const int64_t few = part_rows(c, n, std::min<int64_t>(max_rows * G, FEW_ROWS), max_len);
+    return few + (max_rows * G > FEW_ROWS ? many_rows(c, tokens, G, max_len) : 0);
+}
+
 template <int DT, int NB>
 tn_status launch_at(hipStream_t st, const PagedArgs& a, int64_t tokens) {
     if (a.few) {
@@ -907,13 +975,18 @@ tn_status launch_at(hipStream_t st, const PagedArgs& a, int64_t tokens) {
         TN_LAUNCHED();
     }
     if ((int64_t)a.max_rows * a.G > a.few) {
-        // enough rows for two workgroups of 256 a unit, else of 128 (a unit holds two)
-        const bool wide = tokens * a.G / 256 * a.c.H >= 512;
+        const int ns = many_splits(a.c, a.n, tokens, a.G, a.max_len);
+        const bool wide = ns == 0;
         const int64_t tiles = tokens * a.G / (wide ? 256 : 128) + a.n;
-        const dim3 grid((unsigned)(tiles * a.c.H));
+        const dim3 grid((unsigned)(tiles * a.c.H), wide ? 1u : (unsigned)ns);
         if (wide) hipLaunchKernelGGL((k_paged_many<DT, NB, 8>), grid, dim3(512), 0, st, a, (int)tiles);
         else hipLaunchKernelGGL((k_paged_many<DT, NB, 4>), grid, dim3(256), 0, st, a, (int)tiles);
         TN_LAUNCHED();
+        if (ns > 1) {
+            const int64_t quads = tokens * a.Hq * (8 * NB);
+            hipLaunchKernelGGL(k_paged_join<DT>, dim3((unsigned)cdiv(quads, 256)), dim3(256), 0, st, a, ns);
+            TN_LAUNCHED();
+        }
     }
     if (a.few && a.nsplit > 1) {
         const int64_t rows = (int64_t)a.n * a.c.H * a.few;
@@ -949,7 +1022,7 @@ int64_t tn_sdpa_paged_q4_0_work_floats(const tn_q4_cache* cache, int64_t n, int6
     Pages c;
     if (attn_check("sdpa_paged_q4_0_work_floats", cache, n, tokens, Hq, max_rows, max_len, &c) != TN_OK) return 0;
     if (!n || !tokens || !Hq || !max_rows) return 0;
-    return part_rows(c, n, few_limit(n, Hq / c.H, std::min(max_rows, tokens)), max_len) * (32 * c.nb + 2);
+    return work_rows(c, n, tokens, Hq / c.H, std::min(max_rows, tokens), max_len) * (32 * c.nb + 2);
 }
 
 tn_status tn_sdpa_paged_q4_0(void* stream, const tn_q4_cache* cache, int dtype, const void* q, int64_t q_stride,
@@ -985,9 +1058,11 @@ tn_status tn_sdpa_paged_q4_0(void* stream, const tn_q4_cache* cache, int dtype, 
     a.sl2 = (float)(sc * 1.4426950408889634);
     a.few = (int)few_limit(n, G, a.max_rows);
     a.nsplit = few_splits(a.c, n, a.few, max_len);
-    const int64_t rows = part_rows(a.c, n, a.few, max_len);
-    a.part_o = work;
-    a.part_ml = reinterpret_cast<float2*>(work + rows * D);
+    // f32 rows, then their pairs: the few's and the many's
+    const int64_t few = part_rows(a.c, n, std::min<int64_t>(a.max_rows * G, FEW_ROWS), max_len);
+    const int64_t rows = work_rows(a.c, n, tokens, G, a.max_rows, max_len);
+    a.part_o = work, a.many_o = work + few * D;
+    a.part_ml = reinterpret_cast<float2*>(work + rows * D), a.many_ml = a.part_ml + few;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == TN_F32) return launch<TN_F32>(st, a, tokens);
     if (dtype == TN_BF16) return launch<TN_BF16>(st, a, tokens);
