@@ -69,13 +69,20 @@ TN_INLINE uint32_t pk_f16(float a, float b) { return El<true>::pack_p(a, b); }
 // pair: an instruction takes one constant, so the bits of 1024 sit in a vector
 // register, where the compiler does not see what they are.
 struct Unpack {
-    uint32_t one;
+    uint32_t one, sixty_four;
     TN_INLINE Unpack() {
 #if __HIP_DEVICE_COMPILE__
         asm("v_mov_b32 %0, 0x64006400" : "=v"(one));
+        asm("v_mov_b32 %0, 0x54005400" : "=v"(sixty_four));
 #endif
     }
     TN_INLINE h2 bits(uint32_t w, uint32_t mask) const { return as_h2((w & mask) | one); }
+    // 64 more than the nibbles (72 more than the codes), for a product whose sum starts
+    // from -72 times the other operand's
+    TN_INLINE h8 biased(uint32_t w) const {
+        auto bits64 = [&](uint32_t x) { return (x & 0x00F000F0u) | sixty_four; };
+        return as_h8(bits64(w << 4), bits64(w >> 4), bits64(w), bits64(w >> 8));
+    }
     TN_INLINE void low(uint32_t w, uint32_t& a, uint32_t& b) const {
         const h2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
         a = __builtin_bit_cast(uint32_t, bits(w, 0x000F000Fu) + off);
@@ -131,11 +138,11 @@ __device__ inline float row_scale(float top) {
 // whose values it reads as two dwords a block and column (tnhip.h: v_codes).
 template <int NB>
 struct KeyTile {
-    uint32_t k[2][NB];        // rows of the two score tiles: this lane's part of each block
-    uint32_t kd[4 * NB];      // scales of its eight keys, [8][NB] f16
-    uint32_t v[2 * NB];       // values of its eight keys, a byte column of each block
-    uint32_t vd[4 * NB];      // their scales, [NB][8]
-    int bad;                  // its page is outside the cache
+    uint32_t k[2][NB];    // rows of the two score tiles: this lane's part of each block
+    uint32_t kd[4 * NB];  // scales of its part's eight keys, [8][NB] f16
+    uint32_t v[2 * NB];   // values of its part's eight keys, a byte column of each block
+    uint32_t vd[4 * NB];  // their scales, [NB][8]
+    int bad;              // its part's page is outside the cache
 };
 
 template <int N>
@@ -187,11 +194,14 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
     const int keys = max(0, len - all + j + 1);
     const int most = max(0, len - all + (min(first + 16, rows) - 1) / a.G + 1);  // of any row
     const int least = max(0, len - all + first / a.G + 1);                       // of every row
-    const int64_t at = (int64_t)(start + j) * a.Hq + hq;
 
     // the query, as f16 parts in the order of the codes' elements
+    // (16-bit rows: and what a block's product of codes 72 too large starts from. The f32
+    // sums lose four bits by it, 2^-20 of a score, which an f32 row does not spare)
+    constexpr bool BIASED = DT != TN_F32;
     h8 q[PQ][NB];
-    float rs = a.sl2;
+    f32x4 zero[NB];
+    float rs = fabsf(a.sl2);
     {
         float x[NB][8], top = 0.0f;
         const int64_t qi = (int64_t)(start + j) * a.q_stride + (int64_t)hq * D;
@@ -209,17 +219,29 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
         float sc = 1.0f;
         if constexpr (DT != TN_F16) {
             sc = row_scale(wave_xor_max(top));
-            rs = a.sl2 / sc;
+            rs = rs / sc;
         }
+        // a positive factor, so that it can be taken out of the maximum
+        rs = fmaxf(rs, 1.1754944e-38f);
+        if (a.sl2 < 0.0f) sc = -sc;
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+        for (int b = 0; b < NB; b++) {
+            float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float v = x[b][e] * sc;
                 const _Float16 hi = (_Float16)v;
                 q[0][b][e] = hi;
+                sum += (float)hi;
                 if constexpr (PQ == 2) q[1][b][e] = (_Float16)(v - (float)hi);
             }
+            if constexpr (BIASED) {
+                const float z = -72.0f * wave_xor_sum(sum);
+                zero[b] = (f32x4){z, z, z, z};
+            } else {
+                zero[b] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            }
+        }
     }
 
     f32x4 o[2 * NB];
@@ -235,19 +257,25 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
         const int last = a.width - 1;
         return make_int2(table[min((32 * t) >> a.c.shift, last)], table[min((32 * t + 16) >> a.c.shift, last)]);
     };
+    // this lane's place in the planes, from a half's first row
+    const uint8_t* kbase = a.c.kc + ((col & 4) * 2 + (col & 3)) * (16 * NB) + g * (4 * NB);
+    const uint8_t* vbase = a.c.vc + (g & 1) * (128 * NB) + col * (8 * NB);
+    const uint8_t* kdbase = reinterpret_cast<const uint8_t*>(a.c.kd) + (g & 1) * (16 * NB);
+    const uint8_t* vdbase = reinterpret_cast<const uint8_t*>(a.c.vd) + (g & 1) * (16 * NB);
     auto load = [&](KeyTile<NB>& x, int t, int2 pg) __attribute__((always_inline)) {
         const int p0 = __builtin_amdgcn_readfirstlane(pg.x), p1 = __builtin_amdgcn_readfirstlane(pg.y);
         const bool b0 = (unsigned)p0 >= (unsigned)a.c.pages, b1 = (unsigned)p1 >= (unsigned)a.c.pages;
+        // rows of the halves' first tokens; their bytes in the code planes, 16 NB a row, and in the scales', 2 NB
         const int64_t r0 = (((int64_t)(b0 ? 0 : p0) * a.c.H + h) << a.c.shift) + ((32 * t) & (S - 1));
         const int64_t r1 = (((int64_t)(b1 ? 0 : p1) * a.c.H + h) << a.c.shift) + ((32 * t + 16) & (S - 1));
-        const int64_t rk = (col & 8 ? r1 : r0) + (col & 4) * 2 + (col & 3), rg = (g & 2 ? r1 : r0) + (g & 1) * 8;
+        const int64_t c0 = r0 * (16 * NB), c1 = r1 * (16 * NB), d0 = r0 * (2 * NB), d1 = r1 * (2 * NB);
+        const int64_t ck = col & 8 ? c1 : c0, cv = g & 2 ? c1 : c0, dg = g & 2 ? d1 : d0;
         x.bad = g & 2 ? b1 : b0;
-        const uint8_t* kp = a.c.kc + rk * (16 * NB) + g * (4 * NB);
-        load_words(kp, x.k[0]);
-        load_words(kp + 4 * 16 * NB, x.k[1]);
-        load_words(a.c.kd + rg * NB, x.kd);
-        load_words(a.c.vc + rg * (16 * NB) + col * (8 * NB), x.v);
-        load_words(a.c.vd + rg * NB, x.vd);
+        load_words(kbase + ck, x.k[0]);
+        load_words(kbase + ck + 4 * 16 * NB, x.k[1]);
+        load_words(kdbase + dg, x.kd);
+        load_words(vbase + cv, x.v);
+        load_words(vdbase + dg, x.vd);
     };
     const Unpack up;
     auto compute = [&](KeyTile<NB>& x, int t) __attribute__((always_inline)) {
@@ -257,11 +285,16 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
             s[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                uint32_t kw[4];
-                up.low(x.k[u][b], kw[0], kw[1]);
-                up.high(x.k[u][b], kw[2], kw[3]);
-                const h8 kf = as_h8(kw[0], kw[1], kw[2], kw[3]);
-                f32x4 y = {0.f, 0.f, 0.f, 0.f};
+                h8 kf;
+                if constexpr (BIASED) {
+                    kf = up.biased(x.k[u][b]);
+                } else {
+                    uint32_t kw[4];
+                    up.low(x.k[u][b], kw[0], kw[1]);
+                    up.high(x.k[u][b], kw[2], kw[3]);
+                    kf = as_h8(kw[0], kw[1], kw[2], kw[3]);
+                }
+                f32x4 y = zero[b];
                 if constexpr (PQ == 2) y = mfma16(kf, q[1][b], y);
                 y = mfma16(kf, q[0][b], y);
 #pragma unroll
@@ -272,10 +305,6 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
             }
         }
         const int k0 = 32 * t + 8 * g;
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) s[u][e] = s[u][e] * rs;
         const bool edge = 32 * t + 32 > least || __any(x.bad);
         if (edge) {
 #pragma unroll
@@ -291,10 +320,8 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
                 for (int b = 0; b < NB; b++) x.vd[4 * b + (n >> 1)] &= keep;
             }
         }
-        float mx = s[0][0];
-#pragma unroll
-        for (int n = 1; n < 8; n++) mx = fmaxf(mx, s[n >> 2][n & 3]);
-        mx = wave_xor_max(mx);
+        const float mx = wave_xor_max(max3f(max3f(s[0][0], s[0][1], s[0][2]), max3f(s[0][3], s[1][0], s[1][1]),
+                                            fmaxf(s[1][2], s[1][3]))) * rs;
         if (__any(mx > m + RESCALE_SLACK)) {
             const float mn = fmaxf(m, mx), al = exp2f(m - (mn == -INFINITY ? 0.0f : mn));
             m = mn;
@@ -302,12 +329,12 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
 #pragma unroll
             for (int b = 0; b < 2 * NB; b++) o[b] = o[b] * al;
         }
-        const float mu = (m == -INFINITY ? 0.0f : m) - P_BIAS;
+        const float mu = P_BIAS - (m == -INFINITY ? 0.0f : m);
         uint32_t ph[4], pl[4];
 #pragma unroll
         for (int n = 0; n < 8; n += 2)
-            split_p<PP>(__builtin_amdgcn_exp2f(s[n >> 2][n & 3] - mu), __builtin_amdgcn_exp2f(s[n >> 2][(n & 3) + 1] - mu),
-                        ph[n >> 1], pl[n >> 1], l);
+            split_p<PP>(__builtin_amdgcn_exp2f(fmaf(s[n >> 2][n & 3], rs, mu)),
+                        __builtin_amdgcn_exp2f(fmaf(s[n >> 2][(n & 3) + 1], rs, mu)), ph[n >> 1], pl[n >> 1], l);
         const h8 p0 = as_h8(ph[0], ph[1], ph[2], ph[3]);
 #pragma unroll
         for (int b = 0; b < NB; b++)
@@ -379,7 +406,6 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
             if (d == 0) a.part_ml[row] = make_float2(mm, tl);
         }
     }
-    (void)at;
 }
 
 // The splits of a row, in order: four output columns a thread.
@@ -904,13 +930,14 @@ __global__ __launch_bounds__(256) void k_paged_join(const PagedArgs a, int ns) {
     if (a.lse && d == 0) a.lse[row] = tl == 0.0f ? -INFINITY : (mm - P_BIAS) * LN2 + logf(tl);
 }
 
-// Splits of the keys: three workgroups a compute unit, each wave with two tiles or
-// more.
-constexpr int64_t FEW_WGS = 768, FEW_MAX_SPLIT = 64;
+// Splits of the keys of k_paged_few: one round of the two workgroups that a compute unit
+// holds, each wave with four tiles or more. (Sixteen sequences of 512 to 4096 keys, 128
+// workgroups a split: 17.3 us at 4 splits, 22.4 at 6; twelve of 20000 to 40000, 96 a
+// split: 102 us at 5, 110 at 6; one of 300 keys: 5.3 us unsplit, 7.9 at 2.)
+constexpr int64_t FEW_WGS = 512, FEW_KEYS = 512, FEW_MAX_SPLIT = 64;
 int few_splits(const Pages& c, int64_t n, int64_t few, int64_t max_len) {
-    const int64_t wgs = n * c.H * cdiv(few, 16);
-    return (int)std::max<int64_t>(
-        1, std::min<int64_t>({cdiv(FEW_WGS, std::max<int64_t>(wgs, 1)), cdiv(max_len, 256), FEW_MAX_SPLIT}));
+    const int64_t wgs = std::max<int64_t>(1, n * c.H * cdiv(few, 16));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({FEW_WGS / wgs, cdiv(max_len, FEW_KEYS), FEW_MAX_SPLIT}));
 }
 
 tn_status attn_check(const char* op, const tn_q4_cache* cache, int64_t n, int64_t tokens, int64_t Hq, int64_t max_rows,
@@ -928,12 +955,11 @@ tn_status attn_check(const char* op, const tn_q4_cache* cache, int64_t n, int64_
     return TN_OK;
 }
 
-// Rows of the partials at most, for this call and every smaller one: above one split
-// there are under FEW_WGS workgroups of 16 rows a split, so under 2 * FEW_WGS in all.
+// Rows of its partials at most, for this call and every smaller one: no more than
+// FEW_WGS workgroups of 16 rows, splits counted.
 int64_t part_rows(const Pages& c, int64_t n, int64_t few, int64_t max_len) {
-    const int64_t most = std::min(cdiv(max_len, 256), FEW_MAX_SPLIT);
-    if (most < 2) return 0;
-    return std::min(std::min<int64_t>(few, 16) * 2 * FEW_WGS, n * c.H * few * most);
+    const int64_t most = std::min(cdiv(max_len, FEW_KEYS), FEW_MAX_SPLIT);
+    return most < 2 ? 0 : std::min(std::min<int64_t>(few, 16) * FEW_WGS, n * c.H * few * most);
 }
 
 // k_paged_many: 0 for workgroups of 256 rows (rows enough for two a unit), else the
