@@ -47,10 +47,10 @@ struct PlanArgs {
 };
 
 constexpr int PLAN_MAX_N = 4096;
-constexpr int PLAN_THREADS = 1024;
 
-// Inclusive sums over the workgroup's threads; `red` holds a value per wave and is
+// Inclusive sums over the workgroup's T threads; `red` holds a value per wave and is
 // used again only behind the caller's next barrier.
+template <int T>
 __device__ inline int64_t block_scan(int64_t v, int64_t* red) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
@@ -60,21 +60,27 @@ __device__ inline int64_t block_scan(int64_t v, int64_t* red) {
     }
     if (lane == 63) red[w] = v;
     __syncthreads();
-    int64_t before = 0;
-    for (int i = 0; i < w; i++) before += red[i];
-    return v + before;
+#pragma unroll
+    for (int i = 0; i < T / 64 - 1; i++) v += i < w ? red[i] : 0;
+    return v;
+}
+
+// The last index whose value is at most x, of ascending v[0] <= x .. v[n - 1].
+__device__ inline int last_at_most(const int32_t* v, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (v[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
 }
 
 // The slot and position of row t: its request by a search of the row starts.
 __device__ inline void plan_row(const PlanArgs& a, const int32_t* starts, const int32_t* base, int t) {
     int slot = -1, p = 0;
     if (t < starts[a.n]) {
-        int lo = 0, hi = a.n;  // the last request whose start is at most t and whose next one is past it
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (starts[mid] <= t) lo = mid;
-            else hi = mid;
-        }
+        const int lo = last_at_most(starts, a.n, t);
         const int b = base[lo];
         if (b >= 0) {
             const int q = b + t - starts[lo];
@@ -89,12 +95,14 @@ __device__ inline void plan_row(const PlanArgs& a, const int32_t* starts, const 
     a.pos[t] = p;
 }
 
-// One workgroup: prefix sums over the requests, pages from and to the stack, and
-// the rows' slots where they are few (k_plan_rows otherwise).
-__global__ __launch_bounds__(PLAN_THREADS) void k_plan(const PlanArgs a, int rows_here) {
-    __shared__ int64_t red[2][PLAN_THREADS / 64];
-    __shared__ int32_t s_start[PLAN_MAX_N + 1], s_base[PLAN_MAX_N];
-    __shared__ int64_t s_carry[2];
+// One workgroup: prefix sums over the requests, pages from and to the stack, and the
+// rows' slots where they are few (k_plan_rows otherwise). All latency: three loads that
+// depend on one another (lengths, pages, a row's page), the barriers of two sums.
+template <int T>
+__global__ __launch_bounds__(T) void k_plan(const PlanArgs a, int rows_here) {
+    __shared__ int64_t red[2][T / 64];
+    __shared__ int32_t s_start[PLAN_MAX_N + 1], s_base[PLAN_MAX_N], s_first[PLAN_MAX_N];
+    __shared__ int64_t s_carry[2], s_used[T / 64];
     const int tid = threadIdx.x, lane = tid & 63;
     const int size = 1 << a.shift;
     const int64_t most = (int64_t)a.width << a.shift;
@@ -103,24 +111,22 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_plan(const PlanArgs a, int row
 
     // pages of ended requests go back onto the stack
     int64_t count = min(max(a.state[0], 0), a.pages);
-    for (int r0 = 0; r0 < a.n; r0 += PLAN_THREADS) {
+    for (int r0 = 0; r0 < a.n; r0 += T) {
         const int r = r0 + tid;
         const bool ended = r < a.n && a.fresh[r] < 0;
+        if (!__syncthreads_or(ended)) continue;
         const int give = ended ? pages_of(held_of(r)) : 0;
-        const int64_t end = block_scan(give, red[0]);
-        if (tid == PLAN_THREADS - 1) s_carry[0] = end;
+        const int64_t end = block_scan<T>(give, red[0]);
+        if (tid == T - 1) s_carry[0] = end;
         const int64_t at = count + end - give;
-        // a few pages by the request's own lane, more by its wave
-        for (int j = 0; j < min(give, 4); j++)
-            if (at + j < a.pages) a.free_pages[at + j] = a.table[(int64_t)r * a.width + j];
-        uint64_t long_ones = __ballot(give > 4);
-        while (long_ones) {
-            const int src = __ffsll((unsigned long long)long_ones) - 1;
-            long_ones &= long_ones - 1;
+        uint64_t givers = __ballot(give > 0);  // a wave a request, its lanes a page each
+        while (givers) {
+            const int src = __ffsll((unsigned long long)givers) - 1;
+            givers &= givers - 1;
             const int g = __shfl(give, src);
             const int64_t to = __shfl(at, src);
             const int64_t row = (int64_t)(r - lane + src) * a.width;
-            for (int j = 4 + lane; j < g; j += 64)
+            for (int j = lane; j < g; j += 64)
                 if (to + j < a.pages) a.free_pages[to + j] = a.table[row + j];
         }
         __syncthreads();
@@ -132,62 +138,56 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_plan(const PlanArgs a, int row
     // each request's rows and pages
     int64_t rows = 0, taken = 0, lacking = 0, used = 0;
     if (tid == 0) s_start[0] = 0, a.row_start[0] = 0;
-    for (int r0 = 0; r0 < a.n; r0 += PLAN_THREADS) {
+    for (int r0 = 0; r0 < a.n; r0 += T) {
         const int r = r0 + tid;
         int64_t len = 0, add = 0;
-        bool ended = false;
         if (r < a.n) {
             const int f = a.fresh[r];
-            ended = f < 0;
             add = max(f, 0);
-            len = ended ? 0 : held_of(r);
+            len = f < 0 ? 0 : held_of(r);
         }
         const int held = pages_of(len);
         const int need = (int)min((int64_t)INT32_MAX, ((len + add + size - 1) >> a.shift) - held);
-        const int64_t row_end = rows + block_scan(add, red[0]);
+        const int64_t row_end = rows + block_scan<T>(add, red[0]);
         const bool bad = len + add > most || row_end > a.tokens;
         const int want = bad ? 0 : need;
-        const int64_t asked = taken + block_scan(want, red[1]);
+        const int64_t asked = taken + block_scan<T>(want, red[1]);
         const bool ok = !bad && (need == 0 || asked <= count);
-        const int64_t first = asked - want;
-        if (tid == PLAN_THREADS - 1) s_carry[0] = row_end, s_carry[1] = asked;
+        if (tid == T - 1) s_carry[0] = row_end, s_carry[1] = asked;
         if (r < a.n) {
             a.lens_out[r] = (int)(ok ? len + add : len);
             a.base[r] = s_base[r] = ok ? (int)len : -1;
             a.row_start[r + 1] = s_start[r + 1] = (int)min(row_end, (int64_t)a.tokens);
-        }
-        const int get = ok && r < a.n ? need : 0;
-        if (r < a.n && !ok) lacking += need;
-        if (get) used = max(used, asked);
-        for (int j = 0; j < min(get, 4); j++)
-            a.table[(int64_t)r * a.width + held + j] = a.free_pages[count - 1 - (first + j)];
-        uint64_t long_ones = __ballot(get > 4);
-        while (long_ones) {
-            const int src = __ffsll((unsigned long long)long_ones) - 1;
-            long_ones &= long_ones - 1;
-            const int g = __shfl(get, src), h = __shfl(held, src);
-            const int64_t from = __shfl(first, src);
-            const int64_t row = (int64_t)(r - lane + src) * a.width + h;
-            for (int j = 4 + lane; j < g; j += 64) a.table[row + j] = a.free_pages[count - 1 - (from + j)];
+            s_first[r] = (int)min(asked - want, (int64_t)INT32_MAX);
+            if (!ok) lacking += need;
+            else if (need) used = asked;
         }
         __syncthreads();
         rows = s_carry[0], taken = s_carry[1];
         __syncthreads();
     }
-    // `asked` of the last request that took pages is what left the stack
-    const int64_t lack = block_scan(lacking, red[0]);
+    // what left the stack: `asked` of the last request that took pages
+    const int64_t lack = block_scan<T>(lacking, red[0]);
 #pragma unroll
     for (int o = 32; o; o >>= 1) used = max(used, (int64_t)__shfl_xor(used, o));
+    if (lane == 0) s_used[tid >> 6] = used;
     __syncthreads();
-    if (lane == 0) red[1][tid >> 6] = used;
-    __syncthreads();
-    if (tid == PLAN_THREADS - 1) {
-        for (int i = 0; i < PLAN_THREADS / 64; i++) used = max(used, red[1][i]);
+#pragma unroll
+    for (int i = 0; i < T / 64; i++) used = max(used, s_used[i]);
+    if (tid == T - 1) {
         a.state_out[0] = (int)(count - used);
         a.state_out[1] = (int)min(lack, (int64_t)INT32_MAX);
     }
-    if (rows_here)
-        for (int t = tid; t < a.tokens; t += PLAN_THREADS) plan_row(a, s_start, s_base, t);
+    // the pages in the order in which they were asked for: each its request by a search (a
+    // request that wants none starts where its successor does, which is found)
+    for (int64_t i = tid; i < used; i += T) {
+        const int r = last_at_most(s_first, a.n, (int)i);
+        a.table[(int64_t)r * a.width + pages_of(s_base[r]) + (i - s_first[r])] = a.free_pages[count - 1 - i];
+    }
+    if (rows_here) {
+        __syncthreads();
+        for (int t = tid; t < a.tokens; t += T) plan_row(a, s_start, s_base, t);
+    }
 }
 
 // The slots of many rows: the row starts in LDS, a row a thread.
@@ -241,79 +241,195 @@ struct RowArgs {
     void *ko, *vo;
     int64_t stride;
     const int32_t* slots;
-    int64_t items;  // quarter blocks of K, and as many of V
+    int64_t m;
+    int past;  // read: the output is written past the caches
 };
 
-// A quarter block a lane; blockIdx.y: K or V.
-template <int DT>
-__global__ __launch_bounds__(256) void k_append(const RowArgs a) {
-    const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (item >= a.items) return;  // items is a multiple of 4: blocks stay whole
-    const int g = (int)(item & 3), nb = a.c.nb;
-    const int64_t blk = item >> 2;
-    const int b = (int)(blk % nb);
-    const int64_t th = blk / nb;
-    const int h = (int)(th % a.c.H);
-    const int64_t t = th / a.c.H;
-    const int slot = a.slots[t];
-    if (slot < 0 || (slot >> a.c.shift) >= a.c.pages) return;
-    const int64_t ph = (int64_t)(slot >> a.c.shift) * a.c.H + h;
-    const int o = slot & ((1 << a.c.shift) - 1);
-    uint16_t d;
-    const uint32_t w = quantise_part<DT>(blockIdx.y ? a.v : a.k, t * a.stride + ((int64_t)h * nb + b) * 32, g, &d);
-    if (blockIdx.y == 0) {
-        const int64_t row = (ph << a.c.shift) + o;
-        *reinterpret_cast<uint32_t*>(a.c.kc + row * (16 * nb) + (g * nb + b) * 4) = w;
-        if (g == 0) a.c.kd[row * nb + b] = d;
-    } else {
-        const int64_t group = (ph << (a.c.shift - 3)) + (o >> 3);
-        uint8_t* p = a.c.vc + group * (128 * nb) + v_place(o & 7);
+// A workgroup takes ROWS rows of one head, of K or of V. K rows are whole in their plane;
+// V rows are bytes of eights of slots. Of a run of eight slots from an aligned one on,
+// which a prompt's rows are but for its ends, the bytes leave and come together, 8 a
+// lane; other rows' one by one. (Bytes alone: 8192 rows of 8 heads of 128, 19 us to
+// write and 14 to read; 65536 rows read in 111.)
+constexpr int ROWS = 32;
+
+struct Runs {
+    int slot[ROWS];   // -1: outside the cache
+    int lead[ROWS];   // rows that eight in a row start at, `leads` of them
+    int single[ROWS]; // rows in none of these, `singles` of them
+    int leads, singles;
+};
+
+// The first wave sorts the rows r0 .. of `slots`; all threads wait.
+__device__ inline void sort_runs(Runs& s, const int32_t* slots, int64_t r0, int64_t m, const Pages& c) {
+    const int t = threadIdx.x;
+    if (t < 64) {
+        int slot = -1;
+        if (t < ROWS && r0 + t < m) {
+            slot = slots[r0 + t];
+            if (slot < 0 || (slot >> c.shift) >= c.pages) slot = -1;
+        }
+        // a run starts here: the next seven lanes hold the next seven slots
+        const bool first = slot >= 0 && (slot & 7) == 0;
+        const int prev = __shfl_up(slot, 1);
+        const uint64_t follows = __ballot(t > 0 && slot >= 0 && slot == prev + 1);  // bit t: continues t - 1
+        const bool lead = first && t + 8 <= ROWS && ((follows >> (t + 1)) & 0x7f) == 0x7f;
+        const uint64_t leads = __ballot(lead);
+        uint64_t in = 0;  // lanes of runs
 #pragma unroll
-        for (int j = 0; j < 4; j++) p[((4 * g + j) * nb + b) * 8] = (uint8_t)(w >> (8 * j));
-        if (g == 0) a.c.vd[(group * nb + b) * 8 + (o & 7)] = d;
+        for (int i = 0; i < 8; i++) in |= leads << i;
+        const bool alone = t < ROWS && slot >= 0 && !(in >> t & 1);
+        const uint64_t singles = __ballot(alone), below = (1ull << t) - 1;
+        if (t < ROWS) s.slot[t] = slot;
+        if (lead) s.lead[__popcll(leads & below)] = t;
+        if (alone) s.single[__popcll(singles & below)] = t;
+        if (t == 0) s.leads = __popcll(leads), s.singles = __popcll(singles);
+    }
+    __syncthreads();
+}
+
+// The plane row of a slot and head; the eight that a slot is of.
+__device__ inline int64_t plane_row(const Pages& c, int slot, int h) {
+    return (((int64_t)(slot >> c.shift) * c.H + h) << c.shift) + (slot & ((1 << c.shift) - 1));
+}
+
+template <int DT, int NB>
+__global__ __launch_bounds__(256) void k_append(const RowArgs a) {
+    __shared__ Runs runs;
+    __shared__ uint32_t part[ROWS][4 * NB];  // bytes 4g .. 4g+3 of block b at [g * NB + b]
+    __shared__ uint16_t scale[ROWS][NB];
+    const int tid = threadIdx.x, h = blockIdx.y;
+    const int64_t r0 = (int64_t)blockIdx.x * ROWS;
+    sort_runs(runs, a.slots, r0, a.m, a.c);
+    const bool v = blockIdx.z;
+#pragma unroll
+    for (int it = tid; it < ROWS * NB * 4; it += 256) {
+        const int g = it & 3, b = (it >> 2) % NB, t = (it >> 2) / NB, slot = runs.slot[t];
+        if (slot < 0) continue;  // four lanes together
+        uint16_t d;
+        const uint32_t w = quantise_part<DT>(v ? a.v : a.k, (r0 + t) * a.stride + (h * NB + b) * 32, g, &d);
+        if (v) {
+            part[t][g * NB + b] = w;
+            if (g == 0) scale[t][b] = d;
+        } else {
+            const int64_t row = plane_row(a.c, slot, h);
+            *reinterpret_cast<uint32_t*>(a.c.kc + row * (16 * NB) + (g * NB + b) * 4) = w;
+            if (g == 0) a.c.kd[row * NB + b] = d;
+        }
+    }
+    if (!v) return;
+    __syncthreads();
+    auto byte = [&](int t, int x) {  // byte column x = c * NB + b
+        return part[t][x / NB / 4 * NB + x % NB] >> (x / NB % 4 * 8) & 0xffu;
+    };
+    for (int it = tid; it < runs.leads * 16 * NB; it += 256) {
+        const int t = runs.lead[it / (16 * NB)], x = it % (16 * NB);
+        const int64_t row = plane_row(a.c, runs.slot[t], h);  // of the first of the eight
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i >> 2] |= byte(t + i, x) << (8 * (v_place(i) & 3));
+        *reinterpret_cast<uint2*>(a.c.vc + row * (16 * NB) + x * 8) = make_uint2(w[0], w[1]);
+    }
+    for (int it = tid; it < runs.leads * NB * 8; it += 256) {
+        const int t = runs.lead[it / (8 * NB)], b = it % (8 * NB) / 8, i = it % 8;
+        a.c.vd[plane_row(a.c, runs.slot[t], h) * NB + b * 8 + i] = scale[t + i][b];
+    }
+    for (int it = tid; it < runs.singles * 16 * NB; it += 256) {
+        const int t = runs.single[it / (16 * NB)], x = it % (16 * NB), slot = runs.slot[t];
+        const int64_t row = plane_row(a.c, slot & ~7, h);
+        a.c.vc[row * (16 * NB) + x * 8 + v_place(slot & 7)] = (uint8_t)byte(t, x);
+        if (x < NB) a.c.vd[row * NB + x * 8 + (slot & 7)] = scale[t][x];
+    }
+}
+
+template <int DT, int NB>
+__global__ __launch_bounds__(256) void k_read(const RowArgs a) {
+    constexpr int D = 32 * NB, SIZE = DT == TN_F32 ? 4 : 2, PITCH = D * SIZE + 16;
+    __shared__ Runs runs;
+    __shared__ __align__(16) uint8_t rows[ROWS * PITCH];  // as they leave
+    const int tid = threadIdx.x, h = blockIdx.y;
+    const int64_t r0 = (int64_t)blockIdx.x * ROWS;
+    sort_runs(runs, a.slots, r0, a.m, a.c);
+    auto put = [&](int t, int d, float x) {
+        if constexpr (DT == TN_F32) *reinterpret_cast<float*>(rows + t * PITCH + d * 4) = x;
+        else *reinterpret_cast<uint16_t*>(rows + t * PITCH + d * 2) = DT == TN_BF16 ? bf16_out(x) : f16_out(x);
+    };
+    auto low = [](uint32_t byte) { return (float)((int)(byte & 15) - 8); };
+    if (blockIdx.z == 0) {
+#pragma unroll
+        for (int it = tid; it < ROWS * NB * 4; it += 256) {
+            const int g = it & 3, b = (it >> 2) % NB, t = (it >> 2) / NB, slot = runs.slot[t];
+            if (slot < 0) continue;
+            const int64_t row = plane_row(a.c, slot, h);
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(a.c.kc + row * (16 * NB) + (g * NB + b) * 4);
+            const float s = f16_bits_hw(a.c.kd[row * NB + b]);
+            float y[2][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[0][j] = low(w >> (8 * j)) * s, y[1][j] = low(w >> (8 * j + 4)) * s;
+            store4<DT>(rows + t * PITCH, 32 * b + 4 * g, y[0]);
+            store4<DT>(rows + t * PITCH, 32 * b + 16 + 4 * g, y[1]);
+        }
+    } else {
+        for (int it = tid; it < runs.leads * 16 * NB; it += 256) {
+            const int t = runs.lead[it / (16 * NB)], x = it % (16 * NB), b = x % NB, c = x / NB;
+            const int64_t row = plane_row(a.c, runs.slot[t], h);
+            const uint2 w = *reinterpret_cast<const uint2*>(a.c.vc + row * (16 * NB) + x * 8);
+            const uint4 d = *reinterpret_cast<const uint4*>(a.c.vd + row * NB + b * 8);
+            const uint32_t ws[2] = {w.x, w.y}, ds[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const uint32_t byte = ws[i >> 2] >> (8 * (v_place(i) & 3));
+                const float s = f16_bits_hw((uint16_t)(ds[i >> 1] >> (16 * (i & 1))));
+                put(t + i, 32 * b + c, low(byte) * s);
+                put(t + i, 32 * b + 16 + c, low(byte >> 4) * s);
+            }
+        }
+        for (int it = tid; it < runs.singles * 16 * NB; it += 256) {
+            const int t = runs.single[it / (16 * NB)], x = it % (16 * NB), b = x % NB, c = x / NB, slot = runs.slot[t];
+            const int64_t row = plane_row(a.c, slot & ~7, h);
+            const uint32_t byte = a.c.vc[row * (16 * NB) + x * 8 + v_place(slot & 7)];
+            const float s = f16_bits_hw(a.c.vd[row * NB + b * 8 + (slot & 7)]);
+            put(t, 32 * b + c, low(byte) * s);
+            put(t, 32 * b + 16 + c, low(byte >> 4) * s);
+        }
+    }
+    __syncthreads();
+    constexpr int PIECES = D * SIZE / 16;
+    char* out = static_cast<char*>(blockIdx.z ? a.vo : a.ko);
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
+    constexpr uint32_t NAN2 = DT == TN_F32 ? 0x7fc00000u : DT == TN_BF16 ? 0x7fc07fc0u : 0x7e007e00u;
+#pragma unroll
+    for (int it = tid; it < ROWS * PIECES; it += 256) {
+        const int t = it / PIECES, x = it % PIECES;
+        if (r0 + t >= a.m) continue;
+        const u4 w = runs.slot[t] < 0 ? (u4){NAN2, NAN2, NAN2, NAN2}
+                                      : *reinterpret_cast<const u4*>(rows + t * PITCH + x * 16);
+        v4* to = reinterpret_cast<v4*>(out + (((r0 + t) * a.c.H + h) * D) * SIZE + x * 16);
+        if (a.past) __builtin_nontemporal_store((v4)w, to);
+        else *to = w;
     }
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void k_read(const RowArgs a) {
-    const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (item >= a.items) return;
-    const int g = (int)(item & 3), nb = a.c.nb;
-    const int64_t blk = item >> 2;
-    const int b = (int)(blk % nb);
-    const int64_t th = blk / nb;
-    const int h = (int)(th % a.c.H);
-    const int slot = a.slots[th / a.c.H];
-    float lo[4], hi[4];
-    if (slot < 0 || (slot >> a.c.shift) >= a.c.pages) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) lo[j] = hi[j] = NAN;
-    } else {
-        const int64_t ph = (int64_t)(slot >> a.c.shift) * a.c.H + h;
-        const int o = slot & ((1 << a.c.shift) - 1);
-        uint32_t w = 0;
-        uint16_t d;
-        if (blockIdx.y == 0) {
-            const int64_t row = (ph << a.c.shift) + o;
-            w = *reinterpret_cast<const uint32_t*>(a.c.kc + row * (16 * nb) + (g * nb + b) * 4);
-            d = a.c.kd[row * nb + b];
-        } else {
-            const int64_t group = (ph << (a.c.shift - 3)) + (o >> 3);
-            const uint8_t* p = a.c.vc + group * (128 * nb) + v_place(o & 7);
-#pragma unroll
-            for (int j = 0; j < 4; j++) w |= (uint32_t)p[((4 * g + j) * nb + b) * 8] << (8 * j);
-            d = a.c.vd[(group * nb + b) * 8 + (o & 7)];
-        }
-        const float s = f16_bits_hw(d);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            lo[j] = (float)((int)((w >> (8 * j)) & 15) - 8) * s;
-            hi[j] = (float)((int)((w >> (8 * j + 4)) & 15) - 8) * s;
-        }
+void rows_launch(hipStream_t st, const RowArgs& a, bool append) {
+    const dim3 grid((unsigned)cdiv(a.m, ROWS), (unsigned)a.c.H, 2);
+#define TN_ROWS(NB)                                                                    \
+    case NB:                                                                           \
+        if (append) hipLaunchKernelGGL((k_append<DT, NB>), grid, dim3(256), 0, st, a); \
+        else hipLaunchKernelGGL((k_read<DT, NB>), grid, dim3(256), 0, st, a);          \
+        break;
+    switch (a.c.nb) {
+        TN_ROWS(1) TN_ROWS(2) TN_ROWS(3) TN_ROWS(4) TN_ROWS(5) TN_ROWS(6) TN_ROWS(7) TN_ROWS(8)
     }
-    void* out = blockIdx.y ? a.vo : a.ko;
-    store4<DT>(out, blk * 32 + 4 * g, lo);
-    store4<DT>(out, blk * 32 + 16 + 4 * g, hi);
+#undef TN_ROWS
+}
+
+tn_status rows_at(hipStream_t st, int dtype, const RowArgs& a, bool append) {
+    if (dtype == TN_F32) rows_launch<TN_F32>(st, a, append);
+    else if (dtype == TN_BF16) rows_launch<TN_BF16>(st, a, append);
+    else rows_launch<TN_F16>(st, a, append);
+    TN_LAUNCHED();
+    return TN_OK;
 }
 
 tn_status row_check(const char* op, const tn_q4_cache* cache, int dtype, int64_t m, RowArgs* a) {
@@ -321,9 +437,8 @@ tn_status row_check(const char* op, const tn_q4_cache* cache, int dtype, int64_t
     if (dtype != TN_F32 && dtype != TN_BF16 && dtype != TN_F16)
         return fail(TN_ENOTIMPL, std::string(op) + ": rows must be float32, bfloat16 or float16");
     if (m < 0) return fail(TN_EINVAL, std::string(op) + ": bad sizes");
-    a->items = m * a->c.H * a->c.nb * 4;
-    if (m > INT32_MAX || cdiv(a->items, 256) > WG_ROW * 2)
-        return fail(TN_EVALUE, std::string(op) + ": shape too large");
+    a->m = m;
+    if (m > INT32_MAX) return fail(TN_EVALUE, std::string(op) + ": shape too large");
     return TN_OK;
 }
 
@@ -356,9 +471,10 @@ tn_status tn_paged_plan(void* stream, int64_t n, const int32_t* fresh, const int
     a.free_pages = free_pages, a.state_out = state_out, a.row_start = row_start, a.base = base;
     a.slots = slots, a.pos = pos;
     a.n = (int)n, a.width = (int)width, a.shift = c.shift, a.pages = (int)pages, a.tokens = (int)tokens;
-    const bool here = tokens <= 4 * PLAN_THREADS;
+    const bool here = tokens <= 4096, small = n <= 256 && tokens <= 1024;
     hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(k_plan, dim3(1), dim3(PLAN_THREADS), 0, st, a, (int)here);
+    if (small) hipLaunchKernelGGL(k_plan<256>, dim3(1), dim3(256), 0, st, a, (int)here);
+    else hipLaunchKernelGGL(k_plan<1024>, dim3(1), dim3(1024), 0, st, a, (int)here);
     TN_LAUNCHED();
     if (!here) {
         hipLaunchKernelGGL(k_plan_rows, dim3((unsigned)std::min<int64_t>(cdiv(tokens, 256), 1024)), dim3(256), 0, st, a);
@@ -379,13 +495,7 @@ tn_status tn_kv_append_q4_0(void* stream, const tn_q4_cache* cache, int dtype, c
     if (!k || !v || !slots) return fail(TN_EVALUE, "kv_append_q4_0: null pointer");
     TN_TRY(paged_check_planes(op, a.c));
     a.k = k, a.v = v, a.stride = stride, a.slots = slots;
-    const dim3 grid((unsigned)cdiv(a.items, 256), 2);
-    hipStream_t st = (hipStream_t)stream;
-    if (dtype == TN_F32) hipLaunchKernelGGL(k_append<TN_F32>, grid, dim3(256), 0, st, a);
-    else if (dtype == TN_BF16) hipLaunchKernelGGL(k_append<TN_BF16>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_append<TN_F16>, grid, dim3(256), 0, st, a);
-    TN_LAUNCHED();
-    return TN_OK;
+    return rows_at((hipStream_t)stream, dtype, a, true);
 }
 
 tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t* slots, int64_t m, int dtype, void* k,
@@ -397,13 +507,10 @@ tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t*
     if (!k || !v || !slots) return fail(TN_EVALUE, "kv_read_q4_0: null pointer");
     TN_TRY(paged_check_planes(op, a.c));
     a.ko = k, a.vo = v, a.slots = slots;
-    const dim3 grid((unsigned)cdiv(a.items, 256), 2);
-    hipStream_t st = (hipStream_t)stream;
-    if (dtype == TN_F32) hipLaunchKernelGGL(k_read<TN_F32>, grid, dim3(256), 0, st, a);
-    else if (dtype == TN_BF16) hipLaunchKernelGGL(k_read<TN_BF16>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_read<TN_F16>, grid, dim3(256), 0, st, a);
-    TN_LAUNCHED();
-    return TN_OK;
+    // more than the L2 caches hold between them (65536 rows of 8 heads of 128, bf16: 91 us
+    // through them, 62 past them, 5.6 TB/s; 8192 rows, 33 MB: 11 and 8)
+    a.past = 2 * m * a.c.H * a.c.nb * 32 * (dtype == TN_F32 ? 4 : 2) > (32 << 20);
+    return rows_at((hipStream_t)stream, dtype, a, false);
 }
 
 }  // extern "C"
