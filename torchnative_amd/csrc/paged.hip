@@ -242,7 +242,7 @@ struct RowArgs {
     int64_t stride;
     const int32_t* slots;
     int64_t m;
-    int past;  // read: the output is written past the caches
+    bool past;  // read: the output goes past the caches
 };
 
 // A workgroup takes ROWS rows of one head, of K or of V. K rows are whole in their plane;
@@ -341,7 +341,8 @@ __global__ __launch_bounds__(256) void k_append(const RowArgs a) {
     }
 }
 
-template <int DT, int NB>
+// PAST: the output goes past the caches.
+template <int DT, int NB, bool PAST>
 __global__ __launch_bounds__(256) void k_read(const RowArgs a) {
     constexpr int D = 32 * NB, SIZE = DT == TN_F32 ? 4 : 2, PITCH = D * SIZE + 16;
     __shared__ Runs runs;
@@ -405,7 +406,7 @@ __global__ __launch_bounds__(256) void k_read(const RowArgs a) {
         const u4 w = runs.slot[t] < 0 ? (u4){NAN2, NAN2, NAN2, NAN2}
                                       : *reinterpret_cast<const u4*>(rows + t * PITCH + x * 16);
         v4* to = reinterpret_cast<v4*>(out + (((r0 + t) * a.c.H + h) * D) * SIZE + x * 16);
-        if (a.past) __builtin_nontemporal_store((v4)w, to);
+        if constexpr (PAST) __builtin_nontemporal_store((v4)w, to);
         else *to = w;
     }
 }
@@ -416,7 +417,8 @@ void rows_launch(hipStream_t st, const RowArgs& a, bool append) {
 #define TN_ROWS(NB)                                                                    \
     case NB:                                                                           \
         if (append) hipLaunchKernelGGL((k_append<DT, NB>), grid, dim3(256), 0, st, a); \
-        else hipLaunchKernelGGL((k_read<DT, NB>), grid, dim3(256), 0, st, a);          \
+        else if (a.past) hipLaunchKernelGGL((k_read<DT, NB, true>), grid, dim3(256), 0, st, a); \
+        else hipLaunchKernelGGL((k_read<DT, NB, false>), grid, dim3(256), 0, st, a);   \
         break;
     switch (a.c.nb) {
         TN_ROWS(1) TN_ROWS(2) TN_ROWS(3) TN_ROWS(4) TN_ROWS(5) TN_ROWS(6) TN_ROWS(7) TN_ROWS(8)
