@@ -162,6 +162,29 @@ def test_append_of_large_infinite_and_nan_values_saturates(tn):
     assert all(np.isfinite(t.numpy()).all() for t in dev.read(_ints(tn, [0, 1, 2])))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_large_read_equals_its_pieces(tn, dtype):
+    """Past 32 MB the output goes past the caches; the same values as a few rows at a time, NaN rows among them."""
+    rng = np.random.default_rng(2)
+    H, D, S, m = 8, 128, 64, 9001
+    dev = tn.Q4Cache(-(-m // S), S, H, D)
+    k = _up(tn, rng.standard_normal((m, H, D)).astype(np.float32), dtype)
+    slots = rng.permutation(dev.pages)[np.arange(m) // S] * S + np.arange(m) % S
+    dev.append(k, k, _ints(tn, slots))
+    slots[77] = -1
+    whole = [t.bits() for t in dev.read(_ints(tn, slots), dtype)]
+    for a in range(0, m, 3001):
+        for x, y in zip(whole, dev.read(_ints(tn, slots[a:a + 3001]), dtype)):
+            assert x[a:a + 3001].tobytes() == y.bits().tobytes()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [31, 32, 33])
+def test_rows_around_the_kernels_limit(tn, dtype, rows):
+    c = Case(tn, dtype, 2, 4, 64, 16, [rows, 32, 33], [600, 40, 90])
+    c.check(c.run(tn))
+
+
 def test_append_equals_the_linears_writer(tn):
     """The same blocks as tn_q4_0_quantize gives a weight of the same rows."""
     rng = np.random.default_rng(0)

@@ -977,8 +977,10 @@ int64_t many_rows(const Pages& c, int64_t tokens, int64_t G, int64_t max_len) {
     return most < 2 ? 0 : std::min(tokens * G * c.H * most, 2 * MANY_WGS * 128);
 }
 
-// Folded rows of a request up to which k_paged_few takes it.
-constexpr int FEW_ROWS = 64;
+// Folded rows of a request up to which k_paged_few takes it: it reads and unpacks the
+// codes again for every 16 rows, k_paged_many fills 128. (32 rows of 4 heads behind 4096
+// keys, 8 key/value heads: 17 us there, 25 here; eight such requests 48 and 49.)
+constexpr int FEW_ROWS = 128;
 
 // Folded rows of a request that k_paged_few takes at most in this call; 0: it is not launched. A call of one request
 // is one kernel's.
