@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
     // the query, as f16 parts in the order of the codes' elements
     // (16-bit rows: and what a block's product of codes 72 too large starts from. The f32
     // sums lose four bits by it, 2^-20 of a score, which an f32 row does not spare)
-    constexpr bool BIASED = DT != TN_F32;
+    constexpr bool BIASED = DT != TN_F32 && NB <= 4;  // (more blocks: no registers for it)
     h8 q[PQ][NB];
     f32x4 zero[NB];
     float rs = fabsf(a.sl2);
@@ -357,18 +357,28 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
                 acc = mfma16(vf, p0, acc);
             }
     };
-    if (lo < hi) {
-        KeyTile<NB> x, y;
-        int2 pg = pages(lo), next = pages(min(lo + 1, hi - 1));
-        load(x, lo, pg);
-        for (int t = lo; t < hi; t += 2) {
-            pg = pages(min(t + 2, hi - 1));
-            load(y, min(t + 1, hi - 1), next);
+    if constexpr (NB <= 4) {  // the next tile on its way while one is computed, its pages before that
+        if (lo < hi) {
+            KeyTile<NB> x, y;
+            int2 pg = pages(lo), next = pages(min(lo + 1, hi - 1));
+            load(x, lo, pg);
+            for (int t = lo; t < hi; t += 2) {
+                pg = pages(min(t + 2, hi - 1));
+                load(y, min(t + 1, hi - 1), next);
+                compute(x, t);
+                if (t + 1 >= hi) break;
+                next = pages(min(t + 3, hi - 1));
+                load(x, min(t + 2, hi - 1), pg);
+                compute(y, t + 1);
+            }
+        }
+    } else {  // (two tiles would not fit the registers; two waves a SIMD do)
+        int2 pg = lo < hi ? pages(lo) : make_int2(0, 0);
+        for (int t = lo; t < hi; t++) {
+            KeyTile<NB> x;
+            load(x, t, pg);
+            pg = pages(min(t + 1, hi - 1));
             compute(x, t);
-            if (t + 1 >= hi) break;
-            next = pages(min(t + 3, hi - 1));
-            load(x, min(t + 2, hi - 1), pg);
-            compute(y, t + 1);
         }
     }
 
@@ -757,6 +767,12 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
         __builtin_amdgcn_sched_barrier(0);
     };
     auto softmax = [&](int t) __attribute__((always_inline)) {
+        // the products' wait states: the compiler does not see that max3f's assembly reads their result
+        __builtin_amdgcn_sched_barrier(0);
+#if __HIP_DEVICE_COMPILE__
+        asm volatile("s_nop 15\n\ts_nop 1");
+#endif
+        __builtin_amdgcn_sched_barrier(0);
         if (KT * t + KT > least) {
 #pragma unroll
             for (int u = 0; u < KT / 32; u++)
