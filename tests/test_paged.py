@@ -104,6 +104,20 @@ def test_attention_refusals(L):
         assert call(**kw, q=None, out=None, starts=None, lens=None, table=None) == _lib.TN_OK, kw
 
 
+def test_sizes_past_a_grid_are_refused(L):
+    """A grid holds fewer than 2^32 threads in its first dimension and 2^16 workgroups in its second."""
+    c = ctypes.byref(_cache())
+    for m in ((1 << 28) + 1, (1 << 29) + 1, 1 << 30):
+        assert L.tn_kv_append_q4_0(None, c, 0, 16, 16, m, 128, 16) == _lib.TN_EVALUE and "too large" in _lib.last_error()
+        assert L.tn_kv_read_q4_0(None, c, 16, m, 0, 16, 16) == _lib.TN_EVALUE and "too large" in _lib.last_error()
+    for heads in (4097, 8192):
+        assert L.tn_kv_read_q4_0(None, ctypes.byref(_cache(heads=heads)), 16, 1, 0, 16, 16) == _lib.TN_EINVAL
+    many = ctypes.byref(_cache(heads=4096, pages=1))
+    for n, rows in ((513, 2), (1024, 200), (65535, 1)):
+        args = (None, many, 0, 16, 1 << 30, n, 4096, n, 16, 16, 16, 4, rows, 16, float("nan"), 16, 1 << 60, 16, None)
+        assert L.tn_sdpa_paged_q4_0(*args) == _lib.TN_EVALUE and "too large" in _lib.last_error()
+
+
 def test_work_never_shrinks_with_the_bounds(L):
     """A buffer made for a loop's largest step serves every smaller one: fewer requests, rows or tokens and shorter
     lengths never need more."""

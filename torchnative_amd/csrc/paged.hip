@@ -19,7 +19,8 @@ tn_status paged_check(const char* op, const tn_q4_cache* cache, Pages* out) {
     if (D < 32 || D > 256 || D % 32)
         return fail(TN_ENOTIMPL, name + ": head_dim " + std::to_string(D) +
                                      " is not implemented for a q4_0 cache; it is a multiple of 32 up to 256");
-    if (H < 1 || H > 8192 || P < 0) return fail(TN_EINVAL, name + ": bad cache sizes");
+    // (the attention's grid has up to 8 H workgroups a request in its second dimension)
+    if (H < 1 || H > 4096 || P < 0) return fail(TN_EINVAL, name + ": bad cache sizes");
     if (P > INT32_MAX / S) return fail(TN_EVALUE, name + ": a cache holds fewer than 2^31 slots");
     out->kc = cache->k_codes, out->kd = cache->k_scales, out->vc = cache->v_codes, out->vd = cache->v_scales;
     out->pages = (int)P, out->H = (int)H, out->nb = (int)(D / 32);
@@ -440,7 +441,8 @@ tn_status row_check(const char* op, const tn_q4_cache* cache, int dtype, int64_t
         return fail(TN_ENOTIMPL, std::string(op) + ": rows must be float32, bfloat16 or float16");
     if (m < 0) return fail(TN_EINVAL, std::string(op) + ": bad sizes");
     a->m = m;
-    if (m > INT32_MAX) return fail(TN_EVALUE, std::string(op) + ": shape too large");
+    // 8 threads a row, a grid of fewer than 2^32
+    if (m > 1 << 28) return fail(TN_EVALUE, std::string(op) + ": shape too large");
     return TN_OK;
 }
 

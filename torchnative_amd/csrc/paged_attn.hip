@@ -964,8 +964,8 @@ tn_status attn_check(const char* op, const tn_q4_cache* cache, int64_t n, int64_
     if (Hq % c->H)
         return fail(TN_ENOTIMPL, std::string(op) + ": " + std::to_string(Hq) + " query heads do not divide into " +
                                      std::to_string(c->H) + " key/value heads");
-    // grids stay under 2^32 threads
-    if (n > 65535 || Hq > 65535 || tokens > INT32_MAX || tokens * Hq > (1 << 30) || n * c->H > (1 << 22) ||
+    // k_paged_many has up to 2 tokens * Hq + 512 n * H threads, fewer than 2^32
+    if (n > 65535 || Hq > 65535 || tokens > INT32_MAX || tokens * Hq > (1 << 30) || n * c->H > (1 << 21) ||
         max_len > INT32_MAX)
         return fail(TN_EVALUE, std::string(op) + ": shape too large");
     return TN_OK;
