@@ -397,6 +397,7 @@ tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t*
  *   lens[r] cached ones, those rows' own among them (tn_paged_plan's
  *   row_start and lens_out, after tn_kv_append_q4_0): row j of c attends keys
  *   0 .. lens[r] - c + j. Token t of it lies at table[r][t / S], t % S.
+ *   Entries of row_start ascend; those outside [0, tokens] are cut to it.
  *   max_rows, max_len: host upper bounds of a request's rows and length (they
  *   size the grid); max_len <= width * S. Rows past max_rows are not computed,
  *   lengths past max_len are cut to it.

@@ -109,13 +109,14 @@ class Cache:
 
 
 def attend(q, cache, row_start, lens, table, scale=None):
-    """out, lse and, for the tolerance, sum p |v|, sum |v| and the largest scale sum |q k| of each row, float64.
+    """out, lse and, for the tolerance, sum p |v|, sum |v| and the largest scale sum |q k| and scale sum |q| |d| (d a
+    key block's scale) of each row, float64.
     Rows that no request has are NaN in all of them."""
     T, Hq, D = q.shape
     G, S = Hq // cache.H, cache.S
     scale = D ** -0.5 if scale is None else scale
     out, pav, vsum = (np.full(q.shape, np.nan) for _ in range(3))
-    lse, qk = np.full((T, Hq), np.nan), np.full((T, Hq), np.nan)
+    lse, qk, qd = (np.full((T, Hq), np.nan) for _ in range(3))
     for r, length in enumerate(lens):
         a, z = row_start[r], row_start[r + 1]
         t = np.arange(length)
@@ -123,6 +124,7 @@ def attend(q, cache, row_start, lens, table, scale=None):
         good = (page >= 0) & (page < cache.P)
         slot = np.where(good, page * S + t % S, 0)
         k, v = cache.rows("k", slot), cache.rows("v", slot)
+        kd = np.repeat(np.abs(cache.d["k"][slot].astype(np.float64)), 32, -1)
         m = np.maximum(0, length - (z - a) + np.arange(z - a) + 1)  # keys of each row
         none, seen = m == 0, t[None] < m[:, None]
         for h in range(Hq):
@@ -138,23 +140,29 @@ def attend(q, cache, row_start, lens, table, scale=None):
                 pav[a:z, h] = p @ np.abs(vz)
             vsum[a:z, h] = seen @ np.abs(vz)
             qk[a:z, h] = np.where(seen & good, np.abs(q[a:z, h]) @ np.abs(kh).T, 0).max(1, initial=0) * abs(scale)
+            qd[a:z, h] = np.where(seen & good, np.abs(q[a:z, h]) @ kd[:, h // G].T, 0).max(1, initial=0) * abs(scale)
             out[a:z, h][none], lse[a:z, h][none], pav[a:z, h][none] = np.nan, -np.inf, 0
-    return out, lse, pav, vsum, qk
+    return out, lse, pav, vsum, qk, qd
 
 
-def tolerance(kind, ref, lse, pav, vsum, qk, keys, D):
+def tolerance(kind, ref, lse, pav, vsum, qk, qd, keys, D):
     """Bounds on |got - ref| of out and lse (arrays like them). A half step is 2^-24 in f32 (u), 2^-11 in f16 (h),
     2^-8 in bf16.
 
     A score is off by e: the f32 sum of D products, at most (D + 16) u of sum |q k| (the split of an f32 query in two
     f16 parts, the scale and the argument of exp2 among the 16); in bf16 calls a key may be rounded to f16, h of that
-    sum. A probability is then off by 2 e of itself, exp2 and the running rescales 8 u more. Of sum p |v| the output
+    sum. 16-bit calls of D <= 128 may multiply by codes 72 too large, c + 72 of 64 .. 79, and start a block's sum from
+    z = -72 sum q. With Q = sum |q| of the block's 32 elements: z is 10 additions and a product of 72 Q at most, 11 * 72 u Q;
+    of the 33 terms, any that are summed make at most 79 Q (with z they are -72 of the rest's q and c of their own),
+    33 * 79 u Q; together under 3400 u Q, times the block's scale d. A probability is then off by 2 e of itself, exp2 and the running rescales 8 u more. Of sum p |v| the output
     is off by that and by (keys / 16 + 64) u from the f32 sums (32 keys a product, products in sequence), by 2 h where
     probabilities and values are rounded to f16 (bf16 calls) and by h where one of them is (f16 calls). Probabilities
     are held at 2^6 or more times their size, so one in f16's subnormal range is off by at most 2^-31 of the row's
     largest: 2^-31 sum |v|. The output is rounded once."""
     u, h = 2.0 ** -24, 2.0 ** -11
     e = (D + 16) * u * qk + (h * qk if kind == "bfloat16" else 0)
+    if kind != "float32" and D <= 128:
+        e = e + 3400 * u * qd
     rel = 2 * e + (keys / 16 + 72) * u
     out = pav * (rel[..., None] + {"float32": 0, "float16": h, "bfloat16": 2 * h}[kind]) + 2.0 ** -31 * vsum
     step = {"float32": u, "float16": h, "bfloat16": 2.0 ** -8}[kind]

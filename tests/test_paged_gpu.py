@@ -362,6 +362,17 @@ def test_rows_without_keys_and_empty_requests(tn, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [[1, 1, 2], [40, 3, 200], [300]])
+def test_rows_past_the_calls_are_cut(tn, dtype, rows):
+    """row_start from below zero to past the last row is as if it ran from zero to it."""
+    c = Case(tn, dtype, 2, 2, 64, 16, rows, [x + 70 for x in rows])
+    c.row_start[0], c.row_start[-1] = -5, c.row_start[-1] + 1000
+    got = c.run(tn)
+    c.row_start[0], c.row_start[-1] = 0, c.q.shape[0]
+    c.check(got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [1, 90])
 def test_a_page_outside_the_cache_makes_its_rows_nan(tn, dtype, rows):
     c = Case(tn, dtype, 1, 2, 64, 16, [rows, rows, rows], [100, 100, 100])

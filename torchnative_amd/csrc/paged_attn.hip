@@ -26,7 +26,7 @@ struct PagedArgs {
     float* lse;  // nullable
     const int32_t *row_start, *lens, *table;
     int64_t q_stride;
-    int n, Hq, G, width, max_rows, max_len;  // G = Hq / H
+    int n, tokens, Hq, G, width, max_rows, max_len;  // G = Hq / H
     float sl2;                               // scale * log2(e)
     int nsplit;                              // k_paged_few: splits of the keys
     int few;                                 // requests of more folded rows are k_paged_many's; 0: all are
@@ -50,6 +50,11 @@ struct Parts {
 };
 
 #define TN_INLINE __device__ __attribute__((always_inline)) inline
+
+// row_start[i], and request r's first row and number of rows: within the call's rows,
+// whatever row_start holds.
+TN_INLINE int start_of(const PagedArgs& a, int i) { return min(max(a.row_start[i], 0), a.tokens); }
+TN_INLINE int rows_of(const PagedArgs& a, int r, int start) { return max(start_of(a, r + 1) - start, 0); }
 
 // Pairs of f16 in a dword.
 TN_INLINE h2 as_h2(uint32_t w) { return __builtin_bit_cast(h2, w); }
@@ -183,7 +188,7 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int r = blockIdx.z, h = (int)blockIdx.y % a.c.H, first = (int)blockIdx.y / a.c.H * 16;
-    const int start = a.row_start[r], all = a.row_start[r + 1] - start;
+    const int start = start_of(a, r), all = rows_of(a, r, start);
     const int c = min(all, a.max_rows), rows = c * a.G;
     if (first >= rows || rows > a.few) return;
     const int len = max(0, min(a.lens[r], a.max_len));
@@ -430,7 +435,7 @@ __global__ __launch_bounds__(256) void k_paged_combine(const PagedArgs a) {
     const int h = (int)(rh % a.c.H);
     const int64_t r = rh / a.c.H;
     if (r >= a.n) return;
-    const int start = a.row_start[r], c = min(a.row_start[r + 1] - start, a.max_rows);
+    const int start = start_of(a, r), c = min(rows_of(a, r, start), a.max_rows);
     if (i >= c * a.G || c * a.G > a.few) return;
     const float2* ml = a.part_ml + pr * a.nsplit;
     const float* po = a.part_o + pr * a.nsplit * D + d;
@@ -535,11 +540,11 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
         int hi = a.n;
         while (hi - r > 1) {
             const int mid = (r + hi) >> 1;
-            if ((int)((int64_t)a.row_start[mid] * a.G / ROWS) + mid <= tile) r = mid;
+            if ((int)((int64_t)start_of(a, mid) * a.G / ROWS) + mid <= tile) r = mid;
             else hi = mid;
         }
     }
-    const int start = a.row_start[r], all = a.row_start[r + 1] - start;
+    const int start = start_of(a, r), all = rows_of(a, r, start);
     const int first = (tile - (int)((int64_t)start * a.G / ROWS) - r) * ROWS;
     const int rows = min(all, a.max_rows) * a.G;
     if (first < 0 || first >= rows || rows <= a.few) return;  // few rows: k_paged_few's
@@ -926,7 +931,7 @@ __global__ __launch_bounds__(256) void k_paged_join(const PagedArgs a, int ns) {
         if (a.row_start[mid] <= t) r = mid;
         else hi = mid;
     }
-    const int start = a.row_start[r], c = min(a.row_start[r + 1] - start, a.max_rows);
+    const int start = start_of(a, r), c = min(rows_of(a, r, start), a.max_rows);
     if (t - start >= c || c * a.G <= a.few) return;
     const float2* ml = a.many_ml + row * ns;
     const float* po = a.many_o + row * ns * D + d;
@@ -1097,7 +1102,7 @@ tn_status tn_sdpa_paged_q4_0(void* stream, const tn_q4_cache* cache, int dtype, 
     TN_TRY(paged_check_planes(op, a.c));
     const double sc = std::isnan(scale) ? 1.0 / std::sqrt((double)D) : scale;
     a.q = q, a.out = out, a.lse = lse, a.row_start = row_start, a.lens = lens, a.table = table;
-    a.q_stride = q_stride, a.n = (int)n, a.Hq = (int)Hq, a.G = (int)G, a.width = (int)width;
+    a.q_stride = q_stride, a.n = (int)n, a.tokens = (int)tokens, a.Hq = (int)Hq, a.G = (int)G, a.width = (int)width;
     a.max_rows = (int)std::min(max_rows, tokens), a.max_len = (int)max_len;
     a.sl2 = (float)(sc * 1.4426950408889634);
     a.few = (int)few_limit(n, G, a.max_rows);
