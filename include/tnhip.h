@@ -367,6 +367,9 @@ typedef struct tn_q4_cache {
  *   base [n]: the position of its first new token, -1 if it was refused.
  *   slots, pos [tokens]: slot and position of each row; slot -1 (and position
  *     0) for rows of refused requests and behind the last row.
+ * Pages are not counted: an ended request gives back every page of its row, so
+ * a caller whose requests share pages ends all but the last of them by
+ * bookkeeping of its own (its length set to 0, its own pages pushed).
  * Lengths are taken as lying in [0, width * page_size], state[0] in
  * [0, pages]; a popped page outside [0, pages) gives slots of -1. */
 tn_status tn_paged_plan(void* stream, int64_t n, const int32_t* fresh, const int32_t* lens, int32_t* lens_out,

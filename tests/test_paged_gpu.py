@@ -180,9 +180,10 @@ def test_a_large_read_equals_its_pieces(tn, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [31, 32, 33])
-def test_rows_around_the_kernels_limit(tn, dtype, rows):
+@pytest.mark.parametrize("many", [False, True])
+def test_rows_around_the_kernels_limit(tn, many, dtype, rows):
     c = Case(tn, dtype, 2, 4, 64, 16, [rows, 32, 33], [600, 40, 90])
-    c.check(c.run(tn))
+    c.check(c.run(tn, many=many))
 
 
 def test_append_equals_the_linears_writer(tn):
@@ -258,14 +259,20 @@ class Case:
         self.max_rows, self.max_len = max(rows + [0]), max(lens + [0])
 
     def run(self, tn, dev=None, stream=None, scale=None, fill=7.5, lse=True, table=None, max_len=None, max_rows=None,
-            bits=False):
+            bits=False, many=False):
+        """many: the bound of a length is so loose that the call is one of many products, k_paged_many's."""
         from torchnative_amd import _lib as L
 
         dev = dev or _fill(tn, self.cache)
         T = self.q.shape[0]
         out = _up(tn, np.full(self.q.shape, fill, np.float32), self.dtype)
         ls = _up(tn, np.full((T, self.Hq), fill, np.float32))
-        t = [_ints(tn, a) for a in (self.row_start, self.lens, self.table if table is None else table)]
+        table = self.table if table is None else table
+        if many:
+            short = max(0, (1 << 34) // (T * self.Hq * self.D * self.S) + 1 - table.shape[1])
+            table = np.pad(table, ((0, 0), (0, short)), constant_values=-1)
+            max_len = table.shape[1] * self.S
+        t = [_ints(tn, a) for a in (self.row_start, self.lens, table)]
         most, rows = max_len or self.max_len, max_rows or self.max_rows
         n = len(self.lens)
         floats = dev.work_floats(n, T, self.Hq, rows, most)
@@ -274,7 +281,7 @@ class Case:
               f"{self.lens} work {floats}", flush=True)
         L.check(L.lib().tn_sdpa_paged_q4_0(
             stream, ctypes.byref(dev._c), {"float32": 0, "bfloat16": 1, "float16": 2}[self.dtype], self.q.data_ptr(),
-            self.Hq * self.D, T, self.Hq, n, t[0].data_ptr(), t[1].data_ptr(), t[2].data_ptr(), self.table.shape[1],
+            self.Hq * self.D, T, self.Hq, n, t[0].data_ptr(), t[1].data_ptr(), t[2].data_ptr(), table.shape[1],
             rows, most, float("nan") if scale is None else scale, work.data_ptr(), floats, out.data_ptr(),
             ls.data_ptr() if lse else None))
         tn.synchronize()
@@ -329,57 +336,73 @@ def test_single_tokens_over_long_contexts(tn, dtype, D, G, lens):
 @pytest.mark.parametrize("rows, lens", [
     ([130], [130]), ([3, 0, 70, 1], [90, 40, 70, 200]), ([2, 5, 4], [300, 5, 65]), ([33, 257], [33, 300]),
 ])
-def test_chunks_and_whole_prompts(tn, dtype, H, G, D, S, rows, lens):
+@pytest.mark.parametrize("many", [False, True])
+def test_chunks_and_whole_prompts(tn, many, dtype, H, G, D, S, rows, lens):
     c = Case(tn, dtype, H, G, D, S, rows, lens, seed=D + len(rows), extra=3)
-    c.check(c.run(tn))
+    c.check(c.run(tn, many=many))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("H, G, D, S", [(2, 3, 64, 16), (1, 4, 128, 32), (1, 2, 96, 16), (1, 1, 256, 64), (1, 2, 32, 16)])
 @pytest.mark.parametrize("rows, lens", [([90], [2100]), ([200, 1, 0, 70, 3], [1500, 900, 40, 70, 1033])])
-def test_chunks_behind_long_contexts(tn, dtype, H, G, D, S, rows, lens):
+@pytest.mark.parametrize("many", [False, True])
+def test_chunks_behind_long_contexts(tn, many, dtype, H, G, D, S, rows, lens):
     """Keys split over workgroups, with rows whose part of the keys is empty."""
     c = Case(tn, dtype, H, G, D, S, rows, lens, seed=D + len(rows), extra=2)
-    c.check(c.run(tn))
+    c.check(c.run(tn, many=many))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])
-def test_many_rows_of_many_heads(tn, dtype, D):
-    """131072 folded rows and more: the kernel of 256 rows a workgroup, with a request of few rows among the others."""
-    rows = [250, 1, 600, 0, 700, 513]
+@pytest.mark.parametrize("last", [480, 513])
+def test_many_rows_of_many_heads(tn, dtype, D, last):
+    """131072 folded rows and more: the kernel of 256 rows a workgroup, with a request of few rows among the others;
+    and a little fewer, in workgroups of 128 that take whole rows' keys."""
+    rows = [250, 1, 600, 0, 700, last]
     c = Case(tn, dtype, 8, 8, D, 32, rows, [260, 500, 610, 3, 690, 513], seed=D)
-    c.check(c.run(tn))
+    c.check(c.run(tn, many=True))
+
+
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])
+@pytest.mark.parametrize("H, G", [(8, 8), (2, 2)])
+def test_rows_of_many_keys(tn, D, H, G):
+    """bfloat16 rows from where one part of a key does: some workgroups of a request on either side."""
+    rows = [700, 600, 800] if H == 8 else [300, 5, 70]
+    c = Case(tn, "bfloat16", H, G, D, 32, rows, [1500, 1623, 800] if H == 8 else [1200, 1500, 3001], seed=D)
+    c.check(c.run(tn, many=True))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_rows_without_keys_and_empty_requests(tn, dtype):
+@pytest.mark.parametrize("many", [False, True])
+def test_rows_without_keys_and_empty_requests(tn, many, dtype):
     """More rows than tokens: the first attend nothing. Requests of no rows, of no tokens, and of neither."""
     c = Case(tn, dtype, 2, 2, 64, 16, [5, 1, 0, 0, 40, 20], [2, 0, 33, 0, 17, 0], extra=1)
-    got = c.run(tn)
+    got = c.run(tn, many=many)
     c.check(got)
     assert np.isnan(got[0][:3]).all() and (got[1][:3] == -np.inf).all()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [[1, 1, 2], [40, 3, 200], [300]])
-def test_rows_past_the_calls_are_cut(tn, dtype, rows):
+@pytest.mark.parametrize("many", [False, True])
+def test_rows_past_the_calls_are_cut(tn, many, dtype, rows):
     """row_start from below zero to past the last row is as if it ran from zero to it."""
     c = Case(tn, dtype, 2, 2, 64, 16, rows, [x + 70 for x in rows])
     c.row_start[0], c.row_start[-1] = -5, c.row_start[-1] + 1000
-    got = c.run(tn)
+    got = c.run(tn, many=many)
     c.row_start[0], c.row_start[-1] = 0, c.q.shape[0]
     c.check(got)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [1, 90])
-def test_a_page_outside_the_cache_makes_its_rows_nan(tn, dtype, rows):
+@pytest.mark.parametrize("many", [False, True])
+def test_a_page_outside_the_cache_makes_its_rows_nan(tn, many, dtype, rows):
     c = Case(tn, dtype, 1, 2, 64, 16, [rows, rows, rows], [100, 100, 100])
     for bad in (-1, c.cache.P, 2**31 - 1, -2**31):
         table = c.table.copy()
         table[1, 5] = bad  # tokens 80 .. 95
-        got = c.run(tn, table=table)
+        got = c.run(tn, table=table, many=many)
         c.check(got, table=table)
         first = np.isnan(got[0]).all((1, 2))
         assert not first[:rows].any() and not first[2 * rows:].any() and first[2 * rows - 1]
@@ -388,22 +411,25 @@ def test_a_page_outside_the_cache_makes_its_rows_nan(tn, dtype, rows):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [1, 75])
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 8.0])
-def test_scales_of_any_sign_and_peaked_rows(tn, dtype, rows, scale):
+@pytest.mark.parametrize("many", [False, True])
+def test_scales_of_any_sign_and_peaked_rows(tn, many, dtype, rows, scale):
     c = Case(tn, dtype, 2, 3, 64, 16, [rows, rows], [150, 75], seed=5)
-    c.check(c.run(tn, scale=scale), scale=scale)
+    c.check(c.run(tn, scale=scale, many=many), scale=scale)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows", [1, 75])
 @pytest.mark.parametrize("spread", [1e-4, 300.0, 10000.0])
-def test_small_and_large_values(tn, dtype, rows, spread):
+@pytest.mark.parametrize("many", [False, True])
+def test_small_and_large_values(tn, many, dtype, rows, spread):
     """Scores of one sign past thousands, values from f16's subnormal scales to near its largest."""
     c = Case(tn, dtype, 1, 4, 128, 32, [rows], [180], seed=6, spread=spread)
     scale = 0.1 / spread if spread > 1 else None
-    c.check(c.run(tn, scale=scale), scale=scale)
+    c.check(c.run(tn, scale=scale, many=many), scale=scale)
 
 
-def test_large_queries_of_each_type(tn):
+@pytest.mark.parametrize("many", [False, True])
+def test_large_queries_of_each_type(tn, many):
     """Queries of 1e30 (f32, bf16) and 6e4 (f16) with a scale that brings the scores back; 1e-30 likewise."""
     for dtype, mul in (("float32", 1e30), ("bfloat16", 1e30), ("float16", 6e4), ("float32", 1e-30),
                        ("bfloat16", 1e-30)):
@@ -411,7 +437,7 @@ def test_large_queries_of_each_type(tn):
             c = Case(tn, dtype, 1, 2, 64, 16, [rows], [90], seed=8)
             x = np.clip(c.q.numpy().astype(np.float32), -1, 1) * np.float32(mul)
             c.q = _up(tn, x, dtype)
-            c.check(c.run(tn, scale=0.125 / mul), scale=0.125 / mul)
+            c.check(c.run(tn, scale=0.125 / mul, many=many), scale=0.125 / mul)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -426,11 +452,12 @@ def test_no_lse_and_a_shared_prefix(tn, dtype):
 
 
 @pytest.mark.parametrize("rows", [[1, 1, 1], [90, 1, 4]])
-def test_the_same_bits_every_time_and_whatever_the_bounds_hold(tn, rows):
+@pytest.mark.parametrize("many", [False, True])
+def test_the_same_bits_every_time_and_whatever_the_bounds_hold(tn, many, rows):
     c = Case(tn, "bfloat16", 2, 4, 128, 16, rows, [900, 1300, 40])
-    first = c.run(tn, bits=True)
+    first = c.run(tn, bits=True, many=many)
     for _ in range(3):
-        again = c.run(tn, bits=True)
+        again = c.run(tn, bits=True, many=many)
         assert all(np.array_equal(a, b) for a, b in zip(first, again))
 
 

@@ -478,15 +478,15 @@ __global__ __launch_bounds__(256) void k_paged_combine(const PagedArgs a) {
 // and writes V(t + 1) behind barrier 2 t + 2, the second group reads the same and
 // writes K(t + 2) behind 2 t + 3; so V(t + 1) takes the place of V(t - 1), last read
 // behind 2 t + 1, and K(t + 2) that of K(t), last read there too.
-template <int DT, int NB, int W>
+template <int DT, int NB, int W, int KK>
 struct Many {
     static constexpr int KV = DT == TN_BF16 ? 1 : 2, Q = DT == TN_F32 ? 2 : 1, P = DT == TN_F32 ? 2 : 1;
     static constexpr int ROWS = 32 * W, GROUPS = W / 4;                // folded rows; groups of four waves
     static constexpr int D = 32 * NB, KP = 2 * D + 16;                  // K row pitch, bytes
-    static constexpr int stage(int kt) { return KV * (kt * KP + D * (2 * kt + 16)); }
+    static constexpr int stage(int kt) { return KK * kt * KP + KV * D * (2 * kt + 16); }
     static constexpr int LDS = GROUPS == 2 ? 160 << 10 : 80 << 10;      // one or two workgroups a unit
     static constexpr int KT = NB <= 4 && 2 * stage(64) <= LDS ? 64 : 32;  // keys of a tile
-    static constexpr int VP = 2 * KT + 16, KB = KT * KP, VB = D * VP, STAGE = KV * (KB + VB);
+    static constexpr int VP = 2 * KT + 16, KB = KT * KP, VB = D * VP, STAGE = KK * KB + KV * VB;
     static constexpr int KI = KT * 4, VI = NB * KT;                    // items: (key, part), (byte column, 16 keys)
     static constexpr int OS = DT == TN_F32 ? 4 : 2;                    // output element
     static constexpr int OP = (NB < 4 ? D : 128) * (GROUPS == 1 ? 4 : OS) + 16;  // row pitch on the way out
@@ -525,30 +525,16 @@ TN_INLINE void load_scales(const uint16_t* p, uint32_t (&d)[(NB + 1) / 2]) {
     }
 }
 
-template <int DT, int NB, int W>
-__global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many(const PagedArgs a, int tiles) {
-    using M = Many<DT, NB, W>;
+// Rows first .. first + ROWS of request r, whose rows start at `start` and attend
+// `before` keys more than there are rows ahead of them.
+template <int DT, int NB, int W, int KK>
+TN_INLINE void many_tile(const PagedArgs& a, uint8_t* lds, int h, int r, int start, int rows, int first, int len,
+                         int before) {
+    using M = Many<DT, NB, W, KK>;
     constexpr int KT = M::KT, D = M::D, KV = M::KV, ROWS = M::ROWS;
-    __shared__ __align__(16) uint8_t lds[M::LDS_BYTES];
     const int tid = threadIdx.x & 255, lane = threadIdx.x & 63;
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), group = w >> 2;
     const int col = lane & 31, hh = lane >> 5;
-    // the longest rows first; a key/value head's workgroups on the same die when there are eight
-    const int h = (int)blockIdx.x % a.c.H, tile = tiles - 1 - (int)blockIdx.x / a.c.H;
-    int r = 0;
-    {  // request r has tiles row_start[r] G / ROWS + r and on: at least as many as its rows need
-        int hi = a.n;
-        while (hi - r > 1) {
-            const int mid = (r + hi) >> 1;
-            if ((int)((int64_t)start_of(a, mid) * a.G / ROWS) + mid <= tile) r = mid;
-            else hi = mid;
-        }
-    }
-    const int start = start_of(a, r), all = rows_of(a, r, start);
-    const int first = (tile - (int)((int64_t)start * a.G / ROWS) - r) * ROWS;
-    const int rows = min(all, a.max_rows) * a.G;
-    if (first < 0 || first >= rows || rows <= a.few) return;  // few rows: k_paged_few's
-    const int len = max(0, min(a.lens[r], a.max_len)), before = len - all;
     const int S = 1 << a.c.shift;
     const int i = first + 32 * w + col, j = min(i, rows - 1) / a.G, hq = h * a.G + min(i, rows - 1) % a.G;
     const int keys = max(0, before + j + 1);
@@ -651,7 +637,7 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
         for (int e = 0; e < 4; e++) v[e] = pk_mul(c[e], sc);
         uint8_t* p = lds + (t & 1) * M::STAGE + key * M::KP + (4 * b + place) * 16;
         if (kon) *reinterpret_cast<h8*>(p) = as_h8(v[0], v[1], v[2], v[3]);
-        if constexpr (KV == 2) {
+        if constexpr (KK == 2) {
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = pk_rest(c[e], sc, v[e]);
             if (kon) *reinterpret_cast<h8*>(p + M::KB) = as_h8(v[0], v[1], v[2], v[3]);
@@ -674,7 +660,7 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
         for (int e = 0; e < 4; e++) sc[e] = y.s[(e >> 1) * 4 + 2 * half + (e & 1)];
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = pk_mul(x[e], sc[e]);
-        uint8_t* p = lds + (t & 1) * M::STAGE + KV * M::KB + (32 * vb + 16 * high + vcol) * M::VP + (2 * kg + half) * 16;
+        uint8_t* p = lds + (t & 1) * M::STAGE + KK * M::KB + (32 * vb + 16 * high + vcol) * M::VP + (2 * kg + half) * 16;
         if (von) *reinterpret_cast<h8*>(p) = as_h8(v[0], v[1], v[2], v[3]);
         if constexpr (KV == 2) {
 #pragma unroll
@@ -688,11 +674,11 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
     // while the one before it is multiplied: PG of O^T += V^T P^T (a group is 16 keys and
     // BG blocks), then SG of S^T (XG steps of all the tile's keys).
     constexpr int BG = 4 / KV, PB = (NB + BG - 1) / BG, PG = KT / 16 * PB;
-    constexpr int U = KT / 32, XG = 4 / (KV * U), SG = (2 * NB + XG - 1) / XG;
+    constexpr int U = KT / 32, XG = 4 / (KK * U), SG = (2 * NB + XG - 1) / XG;
     h8 f[2][4];
     auto fetch = [&](int n, int t) __attribute__((always_inline)) {
         if (n < PG) {
-            const uint8_t* st = lds + (t & 1) * M::STAGE + KV * M::KB + col * M::VP + hh * 16 + n / PB * 32;
+            const uint8_t* st = lds + (t & 1) * M::STAGE + KK * M::KB + col * M::VP + hh * 16 + n / PB * 32;
 #pragma unroll
             for (int e = 0; e < BG; e++)
 #pragma unroll
@@ -707,9 +693,9 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
 #pragma unroll
                 for (int u = 0; u < U; u++)
 #pragma unroll
-                    for (int p = 0; p < KV; p++)
+                    for (int p = 0; p < KK; p++)
                         if ((n - PG) * XG + x < 2 * NB)
-                            f[n & 1][(x * U + u) * KV + p] = *reinterpret_cast<const h8*>(
+                            f[n & 1][(x * U + u) * KK + p] = *reinterpret_cast<const h8*>(
                                 st + 32 * u * M::KP + 32 * ((n - PG) * XG + x) + p * M::KB);
         }
     };
@@ -733,11 +719,11 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
                 const int c = (n - PG) * XG + x;
                 if (c >= 2 * NB) continue;
 #pragma unroll
-                for (int p = KV - 1; p >= 0; p--)
+                for (int p = KK - 1; p >= 0; p--)
 #pragma unroll
                     for (int u = 0; u < U; u++) {
-                        if (M::Q == 2 && p == 0) s[u] = El<true>::mfma(f[n & 1][(x * U + u) * KV], q[M::Q - 1][c], s[u]);
-                        s[u] = El<true>::mfma(f[n & 1][(x * U + u) * KV + p], q[0][c], s[u]);
+                        if (M::Q == 2 && p == 0) s[u] = El<true>::mfma(f[n & 1][(x * U + u) * KK], q[M::Q - 1][c], s[u]);
+                        s[u] = El<true>::mfma(f[n & 1][(x * U + u) * KK + p], q[0][c], s[u]);
                     }
             }
         }
@@ -917,6 +903,49 @@ __global__ __launch_bounds__(64 * W, (Many<DT, NB, W>::WAVES)) void k_paged_many
     }
 }
 
+// K's parts are two, so that a score is as exact as the f32 sum. A bf16 call's rows of many
+// keys make do with one, the value rounded to f16: a score is then off by 2^-12 of each
+// of its products, which the output's 8 bits do not show and the lse, a mean over the
+// keys, by less the more they are (random keys, 1024 and on: 3e-7 of the lse; from the
+// first key on 1.1e-6). 4096 rows of 32 heads of 128: 150 us, 144 with one part
+// everywhere and 183 with two.
+constexpr int EXACT_KEYS = 1024;
+
+template <int DT, int NB, int W>
+struct ManyLaunch {
+    static constexpr int KK = DT == TN_BF16 ? 1 : 2;  // of rows of many keys
+    using A = Many<DT, NB, W, 2>;
+    using B = Many<DT, NB, W, KK>;
+    static constexpr int LDS_BYTES = A::LDS_BYTES > B::LDS_BYTES ? A::LDS_BYTES : B::LDS_BYTES;
+    static constexpr int WAVES = A::WAVES < B::WAVES ? A::WAVES : B::WAVES;
+};
+
+template <int DT, int NB, int W>
+__global__ __launch_bounds__(64 * W, (ManyLaunch<DT, NB, W>::WAVES)) void k_paged_many(const PagedArgs a, int tiles) {
+    using L = ManyLaunch<DT, NB, W>;
+    constexpr int ROWS = 32 * W;
+    __shared__ __align__(16) uint8_t lds[L::LDS_BYTES];
+    // the longest rows first; a key/value head's workgroups on the same die when there are eight
+    const int h = (int)blockIdx.x % a.c.H, tile = tiles - 1 - (int)blockIdx.x / a.c.H;
+    int r = 0;
+    {  // request r has tiles row_start[r] G / ROWS + r and on: at least as many as its rows need
+        int hi = a.n;
+        while (hi - r > 1) {
+            const int mid = (r + hi) >> 1;
+            if ((int)((int64_t)start_of(a, mid) * a.G / ROWS) + mid <= tile) r = mid;
+            else hi = mid;
+        }
+    }
+    const int start = start_of(a, r), all = rows_of(a, r, start);
+    const int first = (tile - (int)((int64_t)start * a.G / ROWS) - r) * ROWS;
+    const int rows = min(all, a.max_rows) * a.G;
+    if (first < 0 || first >= rows || rows <= a.few) return;  // few rows: k_paged_few's
+    const int len = max(0, min(a.lens[r], a.max_len)), before = len - all;
+    if (L::KK == 1 && before + first / a.G >= EXACT_KEYS)
+        many_tile<DT, NB, W, L::KK>(a, lds, h, r, start, rows, first, len, before);
+    else many_tile<DT, NB, W, 2>(a, lds, h, r, start, rows, first, len, before);
+}
+
 // The splits of k_paged_many's rows, in order: four output columns a thread.
 template <int DT>
 __global__ __launch_bounds__(256) void k_paged_join(const PagedArgs a, int ns) {
@@ -998,22 +1027,31 @@ int64_t many_rows(const Pages& c, int64_t tokens, int64_t G, int64_t max_len) {
     return most < 2 ? 0 : std::min(tokens * G * c.H * most, 2 * MANY_WGS * 128);
 }
 
-// Folded rows of a request up to which k_paged_few takes it: it reads and unpacks the
-// codes again for every 16 rows, k_paged_many fills 128. (32 rows of 4 heads behind 4096
-// keys, 8 key/value heads: 17 us there, 25 here; eight such requests 48 and 49.)
+// Which kernel takes a request's rows. k_paged_few reads and unpacks the codes again for
+// every 16 folded rows but starts at once and splits finely; k_paged_many fills 128 or 256
+// rows, and its tiles follow one another. So k_paged_few takes all rows of a call whose
+// products (tokens * Hq * max_len * D) are few, twice as many where k_paged_many has K
+// and V in two parts; and of a larger call the requests of up to FEW_ROWS folded rows, if
+// it is of several. (us, few and many, 8 key/value heads of 128 and 32 query heads: bf16,
+// 512 rows of 1024 keys, 2.1e9, 27 and 38; 256 of 4096, 4.3e9, 47 and 42; 512 of 4096,
+// 8.6e9, 85 and 57; f16: 28 and 41, 51 and 54, 92 and 84; f32: 32 and 49, 60 and 65, 110
+// and 105. 4 key/value heads of 64 and 16, f16: 6 requests of 1 to 700 rows and 1000 to
+// 3000 keys, 6.5e9, 55 and 71.) Its grid is as long for every request as for the longest:
+// up to FEW_GRID workgroups of it.
 constexpr int FEW_ROWS = 128;
+constexpr int64_t FEW_WORK = 1ll << 32, FEW_GRID = 8192;
 
-// Folded rows of a request that k_paged_few takes at most in this call; 0: it is not launched. A call of one request
-// is one kernel's.
-int64_t few_limit(int64_t n, int64_t G, int64_t max_rows) {
-    const int64_t rows = max_rows * G;
-    return rows <= FEW_ROWS ? rows : n > 1 ? FEW_ROWS : 0;
+// Folded rows of a request that k_paged_few takes at most in this call; 0: it is not launched.
+int64_t few_limit(const Pages& c, int dtype, int64_t n, int64_t tokens, int64_t G, int64_t max_rows, int64_t max_len) {
+    const int64_t rows = max_rows * G, parts = dtype == TN_BF16 ? 1 : 2;
+    // (tokens * Hq is at most 2^30, D 2^8)
+    const bool little = tokens * G * c.H * 32 * c.nb <= parts * FEW_WORK / std::max<int64_t>(max_len, 1) &&
+                        n * c.H * cdiv(rows, 16) <= FEW_GRID;
+    return rows <= FEW_ROWS || little ? rows : n > 1 ? FEW_ROWS : 0;
 }
 
 int64_t work_rows(const Pages& c, int64_t n, int64_t tokens, int64_t G, int64_t max_rows, int64_t max_len) {
-    // by the largest number of folded rows that a smaller call could have in k_paged_few
-    const int64_t few = part_rows(c, n, std::min<int64_t>(max_rows * G, FEW_ROWS), max_len);
-    return few + (max_rows * G > FEW_ROWS ? many_rows(c, tokens, G, max_len) : 0);
+    return part_rows(c, n, max_rows * G, max_len) + (max_rows * G > FEW_ROWS ? many_rows(c, tokens, G, max_len) : 0);
 }
 
 template <int DT, int NB>
@@ -1105,10 +1143,10 @@ tn_status tn_sdpa_paged_q4_0(void* stream, const tn_q4_cache* cache, int dtype, 
     a.q_stride = q_stride, a.n = (int)n, a.tokens = (int)tokens, a.Hq = (int)Hq, a.G = (int)G, a.width = (int)width;
     a.max_rows = (int)std::min(max_rows, tokens), a.max_len = (int)max_len;
     a.sl2 = (float)(sc * 1.4426950408889634);
-    a.few = (int)few_limit(n, G, a.max_rows);
+    a.few = (int)few_limit(a.c, dtype, n, tokens, G, a.max_rows, max_len);
     a.nsplit = few_splits(a.c, n, a.few, max_len);
     // f32 rows, then their pairs: the few's and the many's
-    const int64_t few = part_rows(a.c, n, std::min<int64_t>(a.max_rows * G, FEW_ROWS), max_len);
+    const int64_t few = part_rows(a.c, n, a.max_rows * G, max_len);
     const int64_t rows = work_rows(a.c, n, tokens, G, a.max_rows, max_len);
     a.part_o = work, a.many_o = work + few * D;
     a.part_ml = reinterpret_cast<float2*>(work + rows * D), a.many_ml = a.part_ml + few;
