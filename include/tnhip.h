@@ -402,7 +402,7 @@ tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t*
  *   0 .. lens[r] - c + j. Token t of it lies at table[r][t / S], t % S.
  *   Entries of row_start ascend; those outside [0, tokens] are cut to it.
  *   max_rows, max_len: host upper bounds of a request's rows and length (they
- *   size the grid); max_len <= width * S. Rows past max_rows are not computed,
+ *   size the grid); max_len <= width * S and 2^30. Rows past max_rows are not computed,
  *   lengths past max_len are cut to it.
  *   scale: NaN selects 1/sqrt(D); any sign.
  * A row with no key to attend gives NaN and lse -inf; one whose keys' page is
@@ -411,10 +411,10 @@ tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t*
  * length, of whatever kind, has no effect. Values that were not written by
  * tn_kv_append_q4_0 and are past 65504 in size may count as infinite, and an
  * infinite or NaN value may reach rows of its request ahead of it.
- * Sums, maxima and the softmax are f32; codes enter the matrix products
- * exactly for keys of few rows, else as f16 (for f32 and f16 rows in two
- * parts), probabilities and values as f16 (in two parts where `dtype` needs
- * them); the output is rounded once.
+ * Sums, maxima and the softmax are f32. Keys enter the matrix products exactly
+ * or as two f16 parts (bf16 rows of 1024 keys and more: rounded to f16),
+ * probabilities and values as f16, in two parts where `dtype` needs them; the
+ * output is rounded once.
  * `work`: scratch of at least tn_sdpa_paged_q4_0_work_floats() floats, 16-byte
  * aligned, the caller's, so that nothing is allocated and graphs with a
  * buffer each can run at once; its contents need no preparation and calls on

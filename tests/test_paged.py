@@ -113,6 +113,9 @@ def test_sizes_past_a_grid_are_refused(L):
     for heads in (4097, 8192):
         assert L.tn_kv_read_q4_0(None, ctypes.byref(_cache(heads=heads)), 16, 1, 0, 16, 16) == _lib.TN_EINVAL
     many = ctypes.byref(_cache(heads=4096, pages=1))
+    for most in ((1 << 30) + 1, 1 << 31):
+        args = (None, c, 0, 16, 256, 2, 4, 1, 16, 16, 16, 1 << 28, 2, most, float("nan"), 16, 1 << 60, 16, None)
+        assert L.tn_sdpa_paged_q4_0(*args) == _lib.TN_EVALUE and "too large" in _lib.last_error()
     for n, rows in ((513, 2), (1024, 200), (65535, 1)):
         args = (None, many, 0, 16, 1 << 30, n, 4096, n, 16, 16, 16, 4, rows, 16, float("nan"), 16, 1 << 60, 16, None)
         assert L.tn_sdpa_paged_q4_0(*args) == _lib.TN_EVALUE and "too large" in _lib.last_error()

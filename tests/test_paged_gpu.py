@@ -354,11 +354,10 @@ def test_chunks_behind_long_contexts(tn, many, dtype, H, G, D, S, rows, lens):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [32, 64, 96, 128, 160, 192, 224, 256])
-@pytest.mark.parametrize("last", [480, 513])
-def test_many_rows_of_many_heads(tn, dtype, D, last):
-    """131072 folded rows and more: the kernel of 256 rows a workgroup, with a request of few rows among the others;
+@pytest.mark.parametrize("rows", [[250, 1, 600, 0, 700, 513], [150, 1, 300, 0, 350, 199]])
+def test_many_rows_of_many_heads(tn, dtype, D, rows):
+    """More than 65536 folded rows: the kernel of 256 rows a workgroup, with a request of few rows among the others;
     and a little fewer, in workgroups of 128 that take whole rows' keys."""
-    rows = [250, 1, 600, 0, 700, last]
     c = Case(tn, dtype, 8, 8, D, 32, rows, [260, 500, 610, 3, 690, 513], seed=D)
     c.check(c.run(tn, many=True))
 

@@ -249,8 +249,9 @@ struct RowArgs {
 // A workgroup takes ROWS rows of one head, of K or of V. K rows are whole in their plane;
 // V rows are bytes of eights of slots. Of a run of eight slots from an aligned one on,
 // which a prompt's rows are but for its ends, the bytes leave and come together, 8 a
-// lane; other rows' one by one. (Bytes alone: 8192 rows of 8 heads of 128, 19 us to
-// write and 14 to read; 65536 rows read in 111.)
+// lane; other rows' one by one. Bound by memory where rows are many: 8192 bf16 rows of 8
+// heads of 128 written in 13.4 us (19 byte by byte), 3.2 TB/s, and read in 10.6 (14),
+// 4.1; 65536 read in 60 (111), 5.7; 16 rows are a launch, 3.7 us.
 constexpr int ROWS = 32;
 
 struct Runs {
@@ -475,7 +476,13 @@ tn_status tn_paged_plan(void* stream, int64_t n, const int32_t* fresh, const int
     a.free_pages = free_pages, a.state_out = state_out, a.row_start = row_start, a.base = base;
     a.slots = slots, a.pos = pos;
     a.n = (int)n, a.width = (int)width, a.shift = c.shift, a.pages = (int)pages, a.tokens = (int)tokens;
-    const bool here = tokens <= 4096, small = n <= 256 && tokens <= 1024;
+    // rows in the workgroup that plans, or in a launch of their own (us: 256 requests, 4096
+    // rows, 11.5 and 11.8; 100 of 8192, 14.5 and 10.9; 16 of 16, 6.6 and 7.9)
+    const bool here = tokens <= 4096;
+    // 256 threads, or 1024 and their longer barriers (16 requests, 6.6 and 10.5; 256 of 1024
+    // rows, 7.5 and 8.9; of 4096, 17.6 and 11.5; 500 requests, 18.1 and 15.4; 100 with rows of
+    // their own launch, 8.8 and 10.9)
+    const bool small = n <= 256 && (tokens <= 1024 || !here);
     hipStream_t st = (hipStream_t)stream;
     if (small) hipLaunchKernelGGL(k_plan<256>, dim3(1), dim3(256), 0, st, a, (int)here);
     else hipLaunchKernelGGL(k_plan<1024>, dim3(1), dim3(1024), 0, st, a, (int)here);

@@ -27,13 +27,13 @@ struct PagedArgs {
     const int32_t *row_start, *lens, *table;
     int64_t q_stride;
     int n, tokens, Hq, G, width, max_rows, max_len;  // G = Hq / H
-    float sl2;                               // scale * log2(e)
-    int nsplit;                              // k_paged_few: splits of the keys
-    int few;                                 // requests of more folded rows are k_paged_many's; 0: all are
-    float* part_o;                           // [n][H][few][nsplit][D] and
-    float2* part_ml;                         // [n][H][few][nsplit], above one split
-    float* many_o;                           // k_paged_many's: [tokens][Hq][splits][D] and
-    float2* many_ml;                         // [tokens][Hq][splits], above one split
+    float sl2;        // scale * log2(e)
+    int nsplit;       // k_paged_few: splits of the keys
+    int few;          // requests of more folded rows are k_paged_many's; 0: all are
+    float* part_o;    // [n][H][few][nsplit][D] and
+    float2* part_ml;  // [n][H][few][nsplit], above one split
+    float* many_o;    // k_paged_many's: [tokens][Hq][splits][D] and
+    float2* many_ml;  // [tokens][Hq][splits], above one split
 };
 
 // Probabilities are kept at 2^P_BIAS times their size over the running maximum,
@@ -41,9 +41,9 @@ struct PagedArgs {
 // far below the maximum stay out of its subnormal range as long as they count.
 constexpr float P_BIAS = 6.0f;
 
-// Parts of each 16-bit operand: a 16-bit query is one f16 (a bf16 row scaled by a
-// power of two), an f32 one two; probabilities are two for an output of 11 or 24
-// bits, one for 8; values (code * scale, 15 bits) two for 24.
+// k_paged_few's parts of each 16-bit operand: a 16-bit query is one f16 (a bf16 row
+// scaled by a power of two), an f32 one two; probabilities are two for an output of 11
+// or 24 bits, one for 8; values (code * scale, 15 bits) two for 24.
 template <int DT>
 struct Parts {
     static constexpr int Q = DT == TN_F32 ? 2 : 1, P = DT == TN_BF16 ? 1 : 2, V = DT == TN_F32 ? 2 : 1;
@@ -141,6 +141,15 @@ __device__ inline float row_scale(float top) {
 // (lane c + 16 g holds rows 4 g .. 4 g + 3 of column c), so that a lane holds eight
 // consecutive keys, the operand of its part of the 32-key product O^T += V^T P^T,
 // whose values it reads as two dwords a block and column (tnhip.h: v_codes).
+//
+// Single rows are bound by the cache's bytes: nothing of a key goes through LDS, a wave
+// loads its next tile whole while it computes one, and the splits make one round of the
+// resident workgroups. Twelve requests of 20000 to 40000 keys, 8 key/value heads of 128,
+// f16: 97 us with the merge, 4.3 TB/s; 5.2 of requests of one length (else the shorter
+// ones' workgroups wait for the longest's). Sixteen of 512 to 4096, bf16: 14 us and 3 of
+// merge, 2.4 TB/s: eight tiles a wave, so that starting and merging count; one of 300, 9
+// heads of 64, f32: 5.4 us, a launch and one tile's chain of loads, products, softmax.
+// Many rows are bound by the vector unit, which unpacks the codes anew for every 16.
 template <int NB>
 struct KeyTile {
     uint32_t k[2][NB];    // rows of the two score tiles: this lane's part of each block
@@ -423,7 +432,8 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
     }
 }
 
-// The splits of a row, in order: four output columns a thread.
+// The splits of a row, in order (the same bits every time): four output columns a thread.
+// A launch of its own, 3 to 4 us: of 17 us for sixteen single rows.
 template <int DT>
 __global__ __launch_bounds__(256) void k_paged_combine(const PagedArgs a) {
     const int D = 32 * a.c.nb, q4 = D / 4;
@@ -465,8 +475,8 @@ __global__ __launch_bounds__(256) void k_paged_combine(const PagedArgs a) {
 // 2 x + y of block b, so that half x of a wave holds parts 2 x and 2 x + 1), V
 // transposed, a row an element with its keys in the order in which the score product
 // leaves them in a lane (keys 4 h .. 4 h + 3 of each eight in half h of the wave), so
-// that P^T needs no exchange. For 11- and 24-bit outputs the rounded value and what it
-// lacks are two f16 parts. Rows are padded by 16 bytes, which spreads 16 rows' reads
+// that P^T needs no exchange. Values are the rounded product and, but for bf16 outputs,
+// what it lacks, two f16 parts; so are keys (one part: EXACT_KEYS below). Rows are padded by 16 bytes, which spreads 16 rows' reads
 // over all banks.
 //
 // A wave alternates between a phase of products, O^T += V^T P^T of tile t and S^T of
@@ -478,6 +488,14 @@ __global__ __launch_bounds__(256) void k_paged_combine(const PagedArgs a) {
 // and writes V(t + 1) behind barrier 2 t + 2, the second group reads the same and
 // writes K(t + 2) behind 2 t + 3; so V(t + 1) takes the place of V(t - 1), last read
 // behind 2 t + 1, and K(t + 2) that of K(t), last read there too.
+//
+// Bound by the products, at the clock that they leave: 4096 causal rows of 32 heads of
+// 128, bf16, 150 us, 920 TF/s of 1300 that a large product of matrices reaches; the clock
+// falls to 1.9 GHz of 2.4. (Step by step: a workgroup of 128 rows, all in one phase, 185;
+// packed operations and no branch in the loop, 178; 256 rows, 167; the two groups half a
+// turn apart, 154; tiles asked for together at the start, output through LDS, 149.)
+// Fewer rows than fill the chip with 256 a workgroup run as 128 a workgroup, two a unit,
+// with their keys in up to 8 splits: 512 rows behind 20000 keys, 192 us, 277 unsplit.
 template <int DT, int NB, int W, int KK>
 struct Many {
     static constexpr int KV = DT == TN_BF16 ? 1 : 2, Q = DT == TN_F32 ? 2 : 1, P = DT == TN_F32 ? 2 : 1;
@@ -906,8 +924,8 @@ TN_INLINE void many_tile(const PagedArgs& a, uint8_t* lds, int h, int r, int sta
 // K's parts are two, so that a score is as exact as the f32 sum. A bf16 call's rows of many
 // keys make do with one, the value rounded to f16: a score is then off by 2^-12 of each
 // of its products, which the output's 8 bits do not show and the lse, a mean over the
-// keys, by less the more they are (random keys, 1024 and on: 3e-7 of the lse; from the
-// first key on 1.1e-6). 4096 rows of 32 heads of 128: 150 us, 144 with one part
+// keys, by less the more they are (a prompt of 4096 random keys: 7e-7 of its lse; one of
+// 1000, in two parts, 7e-8; with one part everywhere, past 1e-6). 4096 rows of 32 heads of 128: 150 us, 144 with one part
 // everywhere and 183 with two.
 constexpr int EXACT_KEYS = 1024;
 
@@ -998,9 +1016,10 @@ tn_status attn_check(const char* op, const tn_q4_cache* cache, int64_t n, int64_
     if (Hq % c->H)
         return fail(TN_ENOTIMPL, std::string(op) + ": " + std::to_string(Hq) + " query heads do not divide into " +
                                      std::to_string(c->H) + " key/value heads");
-    // k_paged_many has up to 2 tokens * Hq + 512 n * H threads, fewer than 2^32
+    // k_paged_many has up to 2 tokens * Hq + 512 n * H threads, fewer than 2^32; keys past a
+    // length's last tile are still numbers of 32 bits
     if (n > 65535 || Hq > 65535 || tokens > INT32_MAX || tokens * Hq > (1 << 30) || n * c->H > (1 << 21) ||
-        max_len > INT32_MAX)
+        max_len > (1 << 30))
         return fail(TN_EVALUE, std::string(op) + ": shape too large");
     return TN_OK;
 }
@@ -1012,11 +1031,14 @@ int64_t part_rows(const Pages& c, int64_t n, int64_t few, int64_t max_len) {
     return most < 2 ? 0 : std::min(std::min<int64_t>(few, 16) * FEW_WGS, n * c.H * few * most);
 }
 
-// k_paged_many: 0 for workgroups of 256 rows (rows enough for two a unit), else the
-// splits of the keys for workgroups of 128, two of which a unit holds.
-constexpr int64_t MANY_WGS = 512, MANY_MAX_SPLIT = 8;
+// k_paged_many: 0 for workgroups of 256 rows (rows enough for one a unit), else the
+// splits of the keys for workgroups of 128, two of which a unit holds. (us, 256 and 128 a
+// workgroup, 4 heads on each of 8 of 128: bf16, 2500 rows of 2500 keys, 312 workgroups of
+// 256, 75 and 77; 4000 of 4000, 145 and 161; 6000 of 6000, 307 and 334; f16, 2048 of 2048,
+// 90 and 102. Unsplit, 512 rows behind 20000 keys take 277, split 192.)
+constexpr int64_t MANY_WIDE = 256, MANY_WGS = 512, MANY_MAX_SPLIT = 8;
 int many_splits(const Pages& c, int64_t n, int64_t tokens, int64_t G, int64_t max_len) {
-    if (tokens * G / 256 * c.H >= MANY_WGS) return 0;
+    if (tokens * G / 256 * c.H >= MANY_WIDE) return 0;
     const int64_t wgs = (tokens * G / 128 + n) * c.H;
     return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(MANY_WGS, wgs), cdiv(max_len, 512), MANY_MAX_SPLIT}));
 }

@@ -131,7 +131,8 @@ class Q4Cache:
     def attend(self, q: Tensor, pages: PageTable, max_rows: int, max_len: int, scale: float | None = None,
                work: Tensor | None = None, out: Tensor | None = None, lse: Tensor | None = None):
         """The rows q [tokens, heads, head_dim] of `pages`' last step over their requests' cached tokens, the rows'
-        own among them. max_rows, max_len: upper bounds of a request's rows and length. Returns (out, lse).
+        own among them. max_rows, max_len: upper bounds of a request's rows and length. Returns (out, lse), whose rows
+        behind the last request's are left as they were.
 
         `work`, `out` and `lse` are made where they are not given. Code that captures passes its own, so that the
         graph's buffers live as long as it does, a `work` of its own for each graph."""
