@@ -999,13 +999,20 @@ __global__ __launch_bounds__(256) void k_paged_join(const PagedArgs a, int ns) {
 }
 
 // Splits of the keys of k_paged_few: one round of the two workgroups that a compute unit
-// holds, each wave with four tiles or more. (Sixteen sequences of 512 to 4096 keys, 128
-// workgroups a split: 17.3 us at 4 splits, 22.4 at 6; twelve of 20000 to 40000, 96 a
-// split: 102 us at 5, 110 at 6; one of 300 keys: 5.3 us unsplit, 7.9 at 2.)
+// holds (sixteen sequences of 512 to 4096 keys, 128 workgroups a split: 17.3 us at 4
+// splits, 22.4 at 6; twelve of 20000 to 40000, 96 a split: 102 us at 5, 110 at 6), of 512
+// keys or more, up to eight of them of 256 (one of 1000 keys, 8 heads of 128: 8.9 us at 4,
+// 10.4 at 2; eight of 100 to 3000, 4 rows each: 12.8 at 8, 13.7 at 6; but four of 1000 to
+// 4000: 13.7 at 15, 11.9 at 8; one of 8000: 13.5 at 32, 12.9 at 16). Up to 512 keys are
+// not worth a merge (300 keys: 5.6 us, 7.9 at 2).
 constexpr int64_t FEW_WGS = 512, FEW_KEYS = 512, FEW_MAX_SPLIT = 64;
+int64_t few_most(int64_t max_len) {
+    if (max_len <= FEW_KEYS) return 1;
+    return std::max(std::min<int64_t>(cdiv(max_len, 256), 8), std::min(cdiv(max_len, FEW_KEYS), FEW_MAX_SPLIT));
+}
 int few_splits(const Pages& c, int64_t n, int64_t few, int64_t max_len) {
     const int64_t wgs = std::max<int64_t>(1, n * c.H * cdiv(few, 16));
-    return (int)std::max<int64_t>(1, std::min<int64_t>({FEW_WGS / wgs, cdiv(max_len, FEW_KEYS), FEW_MAX_SPLIT}));
+    return (int)std::max<int64_t>(1, std::min(FEW_WGS / wgs, few_most(max_len)));
 }
 
 tn_status attn_check(const char* op, const tn_q4_cache* cache, int64_t n, int64_t tokens, int64_t Hq, int64_t max_rows,
@@ -1027,7 +1034,7 @@ tn_status attn_check(const char* op, const tn_q4_cache* cache, int64_t n, int64_
 // Rows of its partials at most, for this call and every smaller one: no more than
 // FEW_WGS workgroups of 16 rows, splits counted.
 int64_t part_rows(const Pages& c, int64_t n, int64_t few, int64_t max_len) {
-    const int64_t most = std::min(cdiv(max_len, FEW_KEYS), FEW_MAX_SPLIT);
+    const int64_t most = few_most(max_len);
     return most < 2 ? 0 : std::min(std::min<int64_t>(few, 16) * FEW_WGS, n * c.H * few * most);
 }
 
