@@ -58,20 +58,25 @@ class PageTable:
         self.slots, self.pos = ints(tokens, fill=-1), ints(tokens)
 
     def step(self, fresh=None) -> None:
-        """Adds fresh[r] tokens to request r, or ends it (negative). `fresh` is a device int32 tensor, or host numbers
-        (uploaded), or None for `self.fresh` as it stands (a captured loop writes it on the device)."""
-        if fresh is None:
-            fresh = self.fresh
-        elif not isinstance(fresh, Tensor):
-            fresh = tensor(np.asarray(fresh, np.int32), device="hip")
+        """Adds fresh[r] tokens to request r, or ends it (negative). `fresh` is a device int32 tensor or host numbers,
+        copied into `self.fresh`, or None for `self.fresh` as it stands (a captured loop writes it on the device).
+        `self.fresh` is one buffer for the table's life: captured steps hold its address."""
         op = "paged_plan"
-        _require_hip(op, fresh)
-        _int32(op, fresh=fresh)
-        if fresh.shape != (self.requests,):
-            raise RuntimeError(f"{op}: fresh {list(fresh.shape)} does not give {self.requests} requests a count each")
-        self.fresh = fresh  # the stream may read it after this call returns
+        own = self.fresh
+        if fresh is not None:
+            given = fresh if isinstance(fresh, Tensor) else np.ascontiguousarray(fresh, np.int32)
+            if isinstance(given, Tensor):
+                _require_hip(op, given)
+                _int32(op, fresh=given)
+            if np.shape(fresh) != own.shape:
+                raise RuntimeError(
+                    f"{op}: fresh {list(np.shape(fresh))} does not give {self.requests} requests a count each")
+            if not isinstance(given, Tensor):
+                check(lib().tn_memcpy_h2d(own.data_ptr(), given.ctypes.data, own.nbytes, current_stream()))
+            elif given.data_ptr() != own.data_ptr():
+                check(lib().tn_memcpy_d2d(own.data_ptr(), given.data_ptr(), own.nbytes, current_stream()))
         check(lib().tn_paged_plan(
-            current_stream(), self.requests, fresh.data_ptr(), self.lens.data_ptr(), self.lens.data_ptr(),
+            current_stream(), self.requests, own.data_ptr(), self.lens.data_ptr(), self.lens.data_ptr(),
             self.table.data_ptr(), self.width, self.page_size, self.free_pages.data_ptr(), self.pages,
             self.state.data_ptr(), self.state.data_ptr(), self.tokens, self.row_start.data_ptr(),
             self.base.data_ptr(), self.slots.data_ptr(), self.pos.data_ptr()))
