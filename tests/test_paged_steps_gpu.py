@@ -105,3 +105,37 @@ def test_eager_admissions_between_replays_of_a_captured_step(tn):
             w.check(fresh, *got, f"step {i}, {how}")
             assert t.fresh.data_ptr() == held
         L.check(lib.tn_graph_destroy(graph))
+
+
+@pytest.mark.parametrize("tokens", [2**31 - 1, 2**31 - (1 << 18) + 7])
+def test_a_plan_of_nearly_2_to_the_31_rows(tn, tokens):
+    """The rows' loop ends where another stride would pass 2^31: slots and positions to the last, and nothing ahead of
+    them."""
+    from torchnative_amd import _lib as L
+
+    lib, guard = L.lib(), 1 << 18
+    rows = tn.empty((2, guard + tokens), "int32", "hip")  # both outputs, each behind ints that no row is at
+    at = [rows.data_ptr() + 4 * (i * (guard + tokens) + guard) for i in range(2)]
+    L.check(lib.tn_memset(rows.data_ptr(), 0x55, rows.nbytes, None))
+    up = lambda a: tn.tensor(np.asarray(a, np.int32), device="hip")  # noqa: E731
+    width, pages, size = 20, 20, 256
+    fresh, lens, table = up([3000, 5, 100]), up([10, 0, 20]), up(np.array([[7] + [-1] * (width - 1)] * 3))
+    free, state, start, base = up(np.arange(pages)), up([pages, 0]), up([0] * 4), up([0] * 3)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    print("tokens", tokens, flush=True)
+    L.check(lib.tn_paged_plan(None, 3, p(fresh), p(lens), p(lens), p(table), width, size, p(free), pages, p(state),
+                              p(state), tokens, p(start), p(base), at[0], at[1]))
+    tn.synchronize()
+
+    def ints(ptr, n):
+        a = np.empty(n, np.int32)
+        L.check(lib.tn_memcpy_d2h(a.ctypes.data, ptr, a.nbytes, None))
+        return a
+
+    want = P.plan(np.array([3000, 5, 100]), np.array([10, 0, 20]), np.array([[7] + [-1] * (width - 1)] * 3), size,
+                  np.arange(pages), np.array([pages, 0]), 4000)
+    for ptr, name, none in zip(at, ("slots", "pos"), (-1, 0)):
+        assert np.array_equal(ints(ptr, 4000), want[name])
+        for i in (4000, tokens // 2, tokens - (1 << 19)):
+            assert (ints(ptr + 4 * i, 1 << 19) == none).all(), (name, i)
+        assert (ints(ptr - 4 * guard, guard) == 0x55555555).all(), name

@@ -84,7 +84,7 @@ __device__ inline void plan_row(const PlanArgs& a, const int32_t* starts, const 
         const int lo = last_at_most(starts, a.n, t);
         const int b = base[lo];
         if (b >= 0) {
-            const int q = b + t - starts[lo];
+            const int q = b + (t - starts[lo]);
             const int page = a.table[(int64_t)lo * a.width + (q >> a.shift)];
             if (page >= 0 && page < a.pages) {
                 slot = (page << a.shift) + (q & ((1 << a.shift) - 1));
@@ -196,7 +196,9 @@ __global__ __launch_bounds__(256) void k_plan_rows(const PlanArgs a) {
     __shared__ int32_t s_start[PLAN_MAX_N + 1];
     for (int i = threadIdx.x; i <= a.n; i += 256) s_start[i] = a.row_start[i];
     __syncthreads();
-    for (int t = blockIdx.x * 256 + threadIdx.x; t < a.tokens; t += gridDim.x * 256) plan_row(a, s_start, a.base, t);
+    // (a step past the last of nearly 2^31 rows is no number of 32 bits)
+    for (int64_t t = blockIdx.x * 256 + threadIdx.x; t < a.tokens; t += gridDim.x * 256)
+        plan_row(a, s_start, a.base, (int)t);
 }
 
 // ---- rows into the cache and back ------------------------------------------------
