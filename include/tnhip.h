@@ -406,9 +406,9 @@ tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t*
  *   lengths past max_len are cut to it.
  *   scale: NaN selects 1/sqrt(D); any sign.
  * A row with no key to attend gives NaN and lse -inf; one whose keys' page is
- * outside the cache, NaN and lse NaN. Rows that no request has (behind
- * row_start[n]) are left as they were. What pages hold past a request's
- * length, of whatever kind, has no effect. Values that were not written by
+ * outside the cache, NaN and lse NaN. Rows that no request has (ahead of
+ * row_start[0], behind row_start[n]) are left as they were. What pages hold
+ * past a request's length, of whatever kind, has no effect. Values that were not written by
  * tn_kv_append_q4_0 and are past 65504 in size may count as infinite, and an
  * infinite or NaN value may reach rows of its request ahead of it.
  * Sums, maxima and the softmax are f32. Keys enter the matrix products exactly

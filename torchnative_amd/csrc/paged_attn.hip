@@ -979,7 +979,7 @@ __global__ __launch_bounds__(256) void k_paged_join(const PagedArgs a, int ns) {
         else hi = mid;
     }
     const int start = start_of(a, r), c = min(rows_of(a, r, start), a.max_rows);
-    if (t - start >= c || c * a.G <= a.few) return;
+    if (t < start || t - start >= c || c * a.G <= a.few) return;  // (rows ahead of the first request's are no one's)
     const float2* ml = a.many_ml + row * ns;
     const float* po = a.many_o + row * ns * D + d;
     float mm = -INFINITY, tl = 0.0f;
