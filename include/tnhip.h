@@ -358,10 +358,11 @@ typedef struct tn_q4_cache {
  *     requests' pages are pushed first, in order of requests and pages; then
  *     each request in order pops the pages that it needs.
  *   state_out [2] (may be state): free pages after the step, and the pages
- *     that refused requests lacked (0: none was refused).
+ *     that refused requests asked for, at least one each (0: none was refused).
  * A request is refused when its pages run out (it and every later one that
  * needs any), when it would outgrow its table row, or when its rows would
- * pass `tokens`: it keeps its length and its pages.
+ * pass `tokens`: it keeps its length and its pages. (One that adds nothing
+ * behind such rows has a base of -1 too, and counts nothing.)
  *   row_start [n + 1]: the prefix sums of max(fresh, 0), at most `tokens`:
  *     the rows of request r among the step's rows.
  *   base [n]: the position of its first new token, -1 if it was refused.

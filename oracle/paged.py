@@ -41,7 +41,7 @@ def plan(fresh, lens, table, page_size, free_pages, state, tokens):
                 taken += 1
             lens[r] += add
         else:
-            lacking += need
+            lacking += max(need, min(add, 1))
         start.append(min(total, tokens))
     slots, pos = np.full(tokens, -1, np.int32), np.zeros(tokens, np.int32)
     for r in range(n):

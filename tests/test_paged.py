@@ -172,3 +172,24 @@ def test_the_oracles_bookkeeping_keeps_every_page_once(seed):
         assert sorted(every) == list(range(pages))
         live = o["slots"][o["slots"] >= 0]
         assert len(set(live)) == len(live)
+
+
+# lengths, fresh, tokens -> base, lens, state behind the step, of requests of up to three pages of 16 and six free ones
+REFUSALS = [
+    ([5, 5], [3, 4], 5, [5, -1], [8, 5], [6, 1]),           # rows past `tokens` that its last page would hold
+    ([5, 5, 0], [3, 4, 0], 5, [5, -1, -1], [8, 5, 0], [6, 1]),  # and one behind it that adds nothing
+    ([5, 40], [3, 20], 99, [5, -1], [8, 40], [6, 1]),       # a table row that is full
+    ([0, 48], [1, 1], 99, [0, -1], [1, 48], [5, 1]),        # one that was full already
+    ([16, 0, 0], [33, 48, 48], 99, [-1, 0, -1], [16, 48, 0], [3, 6]),
+    ([0, 0, 0, 3], [48, 40, 2, 2], 99, [0, 0, -1, 3], [48, 40, 0, 5], [0, 1]),  # pages
+    ([5, 5], [3, 0], 3, [5, 5], [8, 5], [6, 0]),
+    ([5, 5], [-1, 3], 3, [0, 5], [0, 8], [7, 0]),
+]
+
+
+@pytest.mark.parametrize("lens, fresh, tokens, base, after, state", REFUSALS)
+def test_every_refusal_shows_in_the_state(lens, fresh, tokens, base, after, state):
+    n = len(lens)
+    o = P.plan(np.array(fresh, np.int32), np.array(lens, np.int32), np.full((n, 3), 8, np.int32), 16,
+               np.array([3, 1, 4, 0, 5, 2, -1, -1, -1], np.int32), np.array([6, 0], np.int32), tokens)
+    assert (o["base"].tolist(), o["lens"].tolist(), o["state"].tolist()) == (base, after, state)

@@ -7,6 +7,8 @@ import numpy as np
 import pytest
 
 from oracle import paged as P
+from test_paged import REFUSALS
+from test_paged_gpu import _run_plan, _same_plan
 from torchnative_amd.tensor import current_stream
 
 pytestmark = pytest.mark.gpu
@@ -139,3 +141,16 @@ def test_a_plan_of_nearly_2_to_the_31_rows(tn, tokens):
         for i in (4000, tokens // 2, tokens - (1 << 19)):
             assert (ints(ptr + 4 * i, 1 << 19) == none).all(), (name, i)
         assert (ints(ptr - 4 * guard, guard) == 0x55555555).all(), name
+
+
+@pytest.mark.parametrize("lens, fresh, tokens, base, after, state", REFUSALS)
+@pytest.mark.parametrize("behind", [0, 300, 2000])
+def test_every_refusal_shows_in_the_state(tn, behind, lens, fresh, tokens, base, after, state):
+    """behind: requests more, which add nothing (each workgroup size, and sums over several turns of it)."""
+    n = len(lens) + behind
+    lens, fresh = (np.array(x + [0] * behind, np.int32) for x in (lens, fresh))
+    args = (fresh, lens, np.full((n, 3), 8, np.int32), 16, np.array([3, 1, 4, 0, 5, 2, -1, -1, -1], np.int32),
+            np.array([6, 0], np.int32), tokens)
+    got = _run_plan(tn, *args)
+    _same_plan(got, P.plan(*args))
+    assert (got["base"].tolist()[: len(base)], got["state"].tolist()) == (base, state)

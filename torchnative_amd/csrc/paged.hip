@@ -160,7 +160,7 @@ __global__ __launch_bounds__(T) void k_plan(const PlanArgs a, int rows_here) {
             a.base[r] = s_base[r] = ok ? (int)len : -1;
             a.row_start[r + 1] = s_start[r + 1] = (int)min(row_end, (int64_t)a.tokens);
             s_first[r] = (int)min(asked - want, (int64_t)INT32_MAX);
-            if (!ok) lacking += need;
+            if (!ok) lacking += max(need, (int)min(add, (int64_t)1));  // its rows or its table may be what ran out
             else if (need) used = asked;
         }
         __syncthreads();
