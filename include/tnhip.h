@@ -368,6 +368,9 @@ typedef struct tn_q4_cache {
  *   base [n]: the position of its first new token, -1 if it was refused.
  *   slots, pos [tokens]: slot and position of each row; slot -1 (and position
  *     0) for rows of refused requests and behind the last row.
+ * Rows of refused requests keep their place in row_start, so that the caller's
+ * rows stay where it laid them; they are not in the cache, and what attention
+ * gives for them is nothing of theirs (tn_sdpa_paged_q4_0).
  * Pages are not counted: an ended request gives back every page of its row, so
  * a caller whose requests share pages ends all but the last of them by
  * bookkeeping of its own (its length set to 0, its own pages pushed).
@@ -409,7 +412,11 @@ tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t*
  * A row with no key to attend gives NaN and lse -inf; one whose keys' page is
  * outside the cache, NaN and lse NaN. Rows that no request has (ahead of
  * row_start[0], behind row_start[n]) are left as they were. What pages hold
- * past a request's length, of whatever kind, has no effect. Values that were not written by
+ * past a request's length, of whatever kind, has no effect.
+ * Nothing here tells a request that tn_paged_plan refused: its c rows are taken
+ * for those of its last c cached tokens, so that out and lse hold other tokens'
+ * keys (NaN where it has fewer). A caller drops the rows of a base of -1 (the
+ * slots are -1) and gives them again in a later step. Values that were not written by
  * tn_kv_append_q4_0 and are past 65504 in size may count as infinite, and an
  * infinite or NaN value may reach rows of its request ahead of it.
  * Sums, maxima and the softmax are f32. Keys enter the matrix products exactly

@@ -154,3 +154,48 @@ def test_every_refusal_shows_in_the_state(tn, behind, lens, fresh, tokens, base,
     got = _run_plan(tn, *args)
     _same_plan(got, P.plan(*args))
     assert (got["base"].tolist()[: len(base)], got["state"].tolist()) == (base, state)
+
+
+@pytest.mark.parametrize("how", ["rows", "table", "pages"])
+def test_rows_of_a_refused_request_and_its_tokens_given_again(tn, how):
+    """A refused request's rows get the attention of its earlier tokens (NaN where it has fewer), the others theirs; the
+    same tokens in a later step get their own."""
+    w = Loop(tn, seed=3)
+    first, second = {"rows": ([20, 0, 40, 9], [10, 0, 88, 1]), "table": ([20, 0, 120, 9], [1, 0, 30, 1]),
+                     "pages": ([96, 96, 120, 9], [1, 0, 8, 70])}[how]
+    refused = {"rows": 2, "table": 2, "pages": 3}[how]
+    for fresh in ([f if i == j else 0 for j, f in enumerate(first)] for i in range(4)):
+        for part in (min(80, max(fresh)), max(fresh) - min(80, max(fresh))):  # at most TOKENS rows a step
+            if part:
+                step = [part if f else 0 for f in fresh]
+                w.inputs()
+                w.table.step(step)
+                w.dev.append(w.k, w.v, w.table.slots)
+                w.check(step, *w.dev.attend(w.q, w.table, TOKENS, MOST), f"filling {step}")
+    w.inputs()
+    w.table.step(second)
+    w.dev.append(w.k, w.v, w.table.slots)
+    out, lse = w.dev.attend(w.q, w.table, TOKENS, MOST)
+    ref = w.check(second, out, lse, how)
+    base = w.o["base"]
+    assert base[refused] == -1 and w.o["state"][1] > 0 and (base[:refused] >= 0).all()
+    a, z = w.o["row_start"][refused:refused + 2]
+    assert z > a
+    tol, ltol = P.tolerance("float32", np.nan_to_num(ref[0]), ref[1], *(np.nan_to_num(x) for x in ref[2:]), MOST, D)
+    out, lse = out.numpy(), lse.numpy()
+    none = np.isneginf(ref[1][a:z])  # more rows than it has tokens
+    assert np.array_equal(np.isneginf(lse[a:z]), none) and np.isnan(out[a:z][none]).all()
+    assert none.any() == (z - a > w.o["lens"][refused])
+    some = a + np.flatnonzero(~none.any(1))
+    assert (np.abs(out[some] - ref[0][some]) <= tol[some]).all() and (np.abs(lse[some] - ref[1][some]) <= ltol[some]).all()
+    if how == "rows":  # fits once it is not behind the others' rows
+        again = [0, 0, 40, 0]
+    elif how == "table":
+        again = [0, 0, 8, 0]
+    else:
+        again = [-1, 0, 0, 70]
+    w.inputs()
+    w.table.step(again)
+    w.dev.append(w.k, w.v, w.table.slots)
+    w.check(again, *w.dev.attend(w.q, w.table, TOKENS, MOST), "again")
+    assert (w.o["base"][[i for i, f in enumerate(again) if f > 0]] >= 0).all()

@@ -40,7 +40,8 @@ def _int32(op, **named):
 class PageTable:
     """The pages of `requests` slots, at most `width` each, out of a pool of `pages`; a step has at most `tokens`
     rows. `lens`, `row_start`, `base`, `slots`, `pos`, `table` and `state` are device int32 tensors that `step`
-    updates in place (include/tnhip.h, tn_paged_plan)."""
+    updates in place (include/tnhip.h, tn_paged_plan). A request whose tokens do not fit is refused: `base` -1, its rows'
+    `slots` -1, its length as it was; `state[1]` is 0 where none was."""
 
     def __init__(self, requests: int, width: int, page_size: int, pages: int, tokens: int):
         self.requests, self.width, self.page_size = int(requests), int(width), int(page_size)
@@ -138,6 +139,8 @@ class Q4Cache:
         """The rows q [tokens, heads, head_dim] of `pages`' last step over their requests' cached tokens, the rows'
         own among them. max_rows, max_len: upper bounds of a request's rows and length. Returns (out, lse), whose rows
         behind the last request's are left as they were.
+        Rows of a request that the step refused (`pages.base` -1, `pages.slots` -1) are not in the cache; what they get
+        here is the attention of the request's earlier tokens, to be dropped.
 
         `work`, `out` and `lse` are made where they are not given. Code that captures passes its own, so that the
         graph's buffers live as long as it does, a `work` of its own for each graph."""
