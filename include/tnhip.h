@@ -420,9 +420,9 @@ tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t*
  * tn_kv_append_q4_0 and are past 65504 in size may count as infinite, and an
  * infinite or NaN value may reach rows of its request ahead of it.
  * Sums, maxima and the softmax are f32. Keys enter the matrix products exactly
- * or as two f16 parts (bf16 rows of 1024 keys and more: rounded to f16),
- * probabilities and values as f16, in two parts where `dtype` needs them; the
- * output is rounded once.
+ * or as two f16 parts (rounded to f16 in bf16 rows of more than 1024 keys,
+ * where a call has many rows), probabilities and values as f16, in two parts
+ * where `dtype` needs them; the output is rounded once.
  * `work`: scratch of at least tn_sdpa_paged_q4_0_work_floats() floats, 16-byte
  * aligned, the caller's, so that nothing is allocated and graphs with a
  * buffer each can run at once; its contents need no preparation and calls on

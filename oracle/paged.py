@@ -145,23 +145,36 @@ def attend(q, cache, row_start, lens, table, scale=None):
     return out, lse, pav, vsum, qk, qd
 
 
-def tolerance(kind, ref, lse, pav, vsum, qk, qd, keys, D):
+def row_keys(row_start, lens, T):
+    """Keys that each of T rows attends; 0 for rows of no request."""
+    m = np.zeros(T, np.int64)
+    for r, length in enumerate(lens):
+        a, z = row_start[r], row_start[r + 1]
+        m[a:z] = np.maximum(0, length - (z - a) + np.arange(z - a) + 1)
+    return m
+
+
+def tolerance(kind, ref, lse, pav, vsum, qk, qd, keys, D, rounded=True, biased=True):
     """Bounds on |got - ref| of out and lse (arrays like them). A half step is 2^-24 in f32 (u), 2^-11 in f16 (h),
     2^-8 in bf16.
 
     A score is off by e: the f32 sum of D products, at most (D + 16) u of sum |q k| (the split of an f32 query in two
     f16 parts, the scale and the argument of exp2 among the 16); in bf16 calls a key may be rounded to f16, h of that
-    sum. 16-bit calls of D <= 128 may multiply by codes 72 too large, c + 72 of 64 .. 79, and start a block's sum from
-    z = -72 sum q. With Q = sum |q| of the block's 32 elements: z is 10 additions and a product of 72 Q at most, 11 * 72 u Q;
-    of the 33 terms, any that are summed make at most 79 Q (with z they are -72 of the rest's q and c of their own),
-    33 * 79 u Q; together under 3400 u Q, times the block's scale d. A probability is then off by 2 e of itself, exp2 and the running rescales 8 u more. Of sum p |v| the output
+    sum, where `rounded` (a truth value, or one a row: rows of more than 1024 keys on the kernel of many rows). 16-bit
+    calls of D <= 128 may, where `biased` (the kernel of few rows), multiply by codes 72 too large, c + 72 of 64 .. 79,
+    and start a block's sum from z = -72 sum q. With Q = sum |q| of the block's 32 elements: z is 10 additions and a
+    product of 72 Q at most, 11 * 72 u Q; of the 33 terms, any that are summed make at most 79 Q (with z they are -72 of
+    the rest's q and c of their own), 33 * 79 u Q; together under 3400 u Q, times the block's scale d. A probability is
+    then off by 2 e of itself, exp2 and the running rescales 8 u more. Of sum p |v| the output
     is off by that and by (keys / 16 + 64) u from the f32 sums (32 keys a product, products in sequence), by 2 h where
     probabilities and values are rounded to f16 (bf16 calls) and by h where one of them is (f16 calls). Probabilities
     are held at 2^6 or more times their size, so one in f16's subnormal range is off by at most 2^-31 of the row's
     largest: 2^-31 sum |v|. The output is rounded once."""
     u, h = 2.0 ** -24, 2.0 ** -11
-    e = (D + 16) * u * qk + (h * qk if kind == "bfloat16" else 0)
-    if kind != "float32" and D <= 128:
+    e = (D + 16) * u * qk
+    if kind == "bfloat16":
+        e = e + np.where(np.reshape(rounded, (-1, 1)), h * qk, 0)
+    if biased and kind != "float32" and D <= 128:
         e = e + 3400 * u * qd
     rel = 2 * e + (keys / 16 + 72) * u
     out = pav * (rel[..., None] + {"float32": 0, "float16": h, "bfloat16": 2 * h}[kind]) + 2.0 ** -31 * vsum

@@ -193,3 +193,34 @@ def test_every_refusal_shows_in_the_state(lens, fresh, tokens, base, after, stat
     o = P.plan(np.array(fresh, np.int32), np.array(lens, np.int32), np.full((n, 3), 8, np.int32), 16,
                np.array([3, 1, 4, 0, 5, 2, -1, -1, -1], np.int32), np.array([6, 0], np.int32), tokens)
     assert (o["base"].tolist(), o["lens"].tolist(), o["state"].tolist()) == (base, after, state)
+
+
+def _short_rows(rows, length, D, seed=0):
+    """bf16 queries of the last rows of a request, its cache, and the oracle's arguments."""
+    rng = np.random.default_rng(seed)
+    c = P.Cache(-(-length // 16), 16, 1, D)
+    c.append(*(rng.standard_normal((length, 1, D)).astype(np.float32) for _ in "kv"), np.arange(length))
+    q = (rng.standard_normal((rows, 4, D)).astype(np.float32).view(np.uint32) & 0xffff0000).view(np.float32)
+    return q.astype(np.float64), c, [0, rows], [length], np.arange(c.P)[None]
+
+
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+def test_the_bound_of_rows_with_exact_keys_rejects_keys_rounded_to_f16(D):
+    """The mistake is planted in the oracle: every key rounded. Rows of few keys show it, whose lse is nearly a score."""
+    rows = length = 60
+    args = _short_rows(rows, length, D)
+    c = args[1]
+    want = P.attend(*args)
+    exact, stored = c.rows, {w: c.rows(w, np.arange(length)) for w in "kv"}
+    c.rows = lambda w, slots: stored[w][slots].astype(np.float16).astype(np.float64) if w == "k" else exact(w, slots)
+    got = P.attend(*args)
+    keys = P.row_keys(*args[2:4], rows)
+    assert keys.max() == length and (keys <= 1024).all()
+    off = np.abs(got[1] - want[1])
+    loose = P.tolerance("bfloat16", want[0], want[1], *want[2:], length, D)[1]
+    tight = P.tolerance("bfloat16", want[0], want[1], *want[2:], length, D, rounded=keys > 1024, biased=False)[1]
+    assert (off <= loose).all() and (off > tight).any()
+
+
+def test_each_rows_keys():
+    assert P.row_keys([0, 2, 2, 6], [5, 9, 2], 7).tolist() == [4, 5, 0, 0, 1, 2, 0]
