@@ -387,7 +387,9 @@ tn_status tn_paged_plan(void* stream, int64_t n, const int32_t* fresh, const int
  * skipped; slots of one call are distinct (one given twice holds a mix of its
  * rows). Blocks are those of tn_q4_0_quantize, except that the scale max / -8
  * is held to +-8188, so that a cached value is finite and at most 65504 in
- * size, f16's largest: infinities and larger values saturate there. */
+ * size, f16's largest: infinities and larger values saturate there. A NaN takes
+ * no part in its block's scale and leaves code 0, -8 scales, with nothing to
+ * tell it by: a caller that may have NaN looks for them ahead of the call. */
 tn_status tn_kv_append_q4_0(void* stream, const tn_q4_cache* cache, int dtype, const void* k, const void* v,
                             int64_t m, int64_t stride, const int32_t* slots);
 /* The cached rows at `slots` [m], (code - 8) * scale rounded to `dtype`, to k
@@ -419,6 +421,7 @@ tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t*
  * slots are -1) and gives them again in a later step. Values that were not written by
  * tn_kv_append_q4_0 and are past 65504 in size may count as infinite, and an
  * infinite or NaN value may reach rows of its request ahead of it.
+ * A query row with an infinite or NaN element gives NaN; no other row does.
  * Sums, maxima and the softmax are f32. Keys enter the matrix products exactly
  * or as two f16 parts (rounded to f16 in bf16 rows of more than 1024 keys,
  * where a call has many rows), probabilities and values as f16, in two parts

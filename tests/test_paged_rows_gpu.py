@@ -53,3 +53,74 @@ def test_bf16_rows_of_up_to_1024_keys_have_them_exact(tn, D, H, G, rows, lens):
     print(f"  lse: up to 1024 keys {worst[keys <= 1024].max():.3f} of the bound, others "
           f"{worst[keys > 1024].max(initial=0):.3f}", flush=True)
     assert worst.max() <= 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D, S", [(64, 16), (128, 32), (192, 16)])
+@pytest.mark.parametrize("rows, lens", [([1, 1, 3], [40, 700, 5]), ([90, 4, 130], [300, 1100, 130])])
+@pytest.mark.parametrize("many", [False, True])
+def test_queries_that_are_not_finite_reach_no_row_but_theirs(tn, many, dtype, D, S, rows, lens):
+    """One element of a head's row NaN or infinite, and a row of nothing else: NaN out of it, every other row as exact
+    as without it. Such rows lie in a wave with others and in a row's first, middle and last block."""
+    c = Case(tn, dtype, 2, 3, D, S, rows, lens, seed=D)
+    x = c.q.numpy().astype(np.float32)
+    clean = x.copy()
+    T = len(x)
+    bad = {}
+    for i, (what, e) in enumerate([(np.nan, 0), (np.inf, D - 1), (-np.inf, 33), (np.nan, D // 2), (None, 0)]):
+        t, h = (i * 7) % T, (i * 5) % 6
+        if (t, h) in bad:
+            continue
+        bad[t, h] = True
+        if what is None:
+            x[t, h] = np.where(np.arange(D) % 2, np.inf, np.nan)
+        else:
+            x[t, h, e] = what
+    c.q = _up(tn, x, dtype)
+    out, lse = c.run(tn, many=many)
+    for t, h in bad:
+        assert np.isnan(out[t, h]).all(), (t, h)
+        assert not np.isposinf(lse[t, h]), (t, h)
+    c.q = _up(tn, clean, dtype)
+    want = c.run(tn, many=many)
+    for t, h in bad:
+        out[t, h], lse[t, h] = want[0][t, h], want[1][t, h]
+    assert np.array_equal(out, want[0]) and np.array_equal(lse, want[1])
+    c.check((out, lse))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, lens", [([3, 1, 5], [40, 700, 5]), ([90, 4, 130, 33], [300, 1100, 130, 2000])])
+@pytest.mark.parametrize("most", [1, 2, 40])
+@pytest.mark.parametrize("many", [False, True])
+def test_rows_past_the_bound_are_not_computed(tn, many, most, dtype, rows, lens):
+    """max_rows below a request's rows: its first ones as ever (their keys counted with all rows), the others left."""
+    c = Case(tn, dtype, 2, 4, 64, 16, rows, lens, extra=2)
+    out, lse = c.run(tn, many=many, max_rows=most)
+    whole = c.run(tn, many=many)
+    for r, n in enumerate(rows):
+        a = c.row_start[r] + min(n, most)
+        z = c.row_start[r + 1]
+        assert (out[a:z] == 7.5).all() and (lse[a:z] == 7.5).all(), r
+        out[a:z], lse[a:z] = whole[0][a:z], whole[1][a:z]
+    c.check((out, lse))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, lens", [([3, 1, 5], [40, 700, 5]), ([90, 4, 130, 33], [300, 1100, 130, 2000])])
+@pytest.mark.parametrize("most", [1, 33, 128, 1030])
+def test_lengths_past_the_bound_are_cut_to_it(tn, most, dtype, rows, lens):
+    """As a call of the shorter lengths, whose first rows may have no keys."""
+    c = Case(tn, dtype, 2, 4, 64, 16, rows, lens, extra=2)
+    got = c.run(tn, max_len=min(most, c.table.shape[1] * 16))  # (never past what the table holds)
+    c.lens = [min(x, most) for x in lens]
+    c.check(got)
+
+
+@pytest.mark.parametrize("rows, lens", [([1, 2], [300, 40]), ([150], [150])])
+@pytest.mark.parametrize("many", [False, True])
+def test_f16_queries_below_the_normal_range(tn, many, rows, lens):
+    """Multiples of 2^-24, f16's smallest number, with a scale that brings the scores back."""
+    c = Case(tn, "float16", 2, 3, 64, 16, rows, lens, seed=4)
+    c.q = _up(tn, c.q.numpy().astype(np.float32) * np.float32(2.0 ** -18), "float16")
+    c.check(c.run(tn, scale=2.0 ** 15, many=many), scale=2.0 ** 15)
