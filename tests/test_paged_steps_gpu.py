@@ -199,3 +199,60 @@ def test_rows_of_a_refused_request_and_its_tokens_given_again(tn, how):
     w.dev.append(w.k, w.v, w.table.slots)
     w.check(again, *w.dev.attend(w.q, w.table, TOKENS, MOST), "again")
     assert (w.o["base"][[i for i, f in enumerate(again) if f > 0]] >= 0).all()
+
+
+def test_a_captured_step_with_counts_of_the_callers(tn):
+    """The graph copies the caller's counts at every replay; eager steps between have their own."""
+    from torchnative_amd import _lib as L
+
+    lib, s = L.lib(), tn.Stream()
+    with s:
+        w = Loop(tn, seed=5)
+        t = w.table
+        mine = tn.tensor(np.zeros(N, np.int32), device="hip")
+        out, lse = tn.zeros((TOKENS, H * G, D)), tn.zeros((TOKENS, H * G))
+        work = tn.empty((w.dev.work_floats(N, TOKENS, H * G, TOKENS, MOST) + 1,), "float32", "hip")
+        L.check(lib.tn_stream_begin_capture(s.handle))
+        t.step(mine)
+        w.dev.append(w.k, w.v, t.slots)
+        w.dev.attend(w.q, t, TOKENS, MOST, work=work, out=out, lse=lse)
+        graph = ctypes.c_void_p()
+        L.check(lib.tn_stream_end_capture(s.handle, ctypes.byref(graph)))
+        for i, fresh in enumerate([[40, 3, 0, 0], [1, 1, 17, 0], [1, -1, 1, 50], [1, 30, 1, 1], [-1, 1, 1, 1], [7, 1, 1, 1]]):
+            w.inputs()
+            if i % 3 == 2:
+                t.step(fresh)
+                w.dev.append(w.k, w.v, t.slots)
+                got = w.dev.attend(w.q, t, TOKENS, MOST)
+            else:
+                w.write(mine, np.asarray(fresh, np.int32))
+                L.check(lib.tn_graph_launch(s.handle, graph))
+                got = out, lse
+            s.synchronize()
+            w.check(fresh, *got, f"step {i}")
+        L.check(lib.tn_graph_destroy(graph))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_two_streams_attend_one_cache_at_once(tn, dtype):
+    """Eager calls without buffers of their own, interleaved on two streams: scratch is a stream's."""
+    rng = np.random.default_rng(1)
+    heads, dim, lens = 4, 128, [1500, 700]
+    t, dev = tn.PageTable(2, 100, 16, 200, 2200), tn.Q4Cache(200, 16, heads, dim)
+    t.step(lens)
+    k, v = (tn.tensor(rng.standard_normal((2200, heads, dim)).astype(np.float32), dtype=dtype, device="hip") for _ in "kv")
+    dev.append(k, v, t.slots)
+    t.step([1, 1])
+    dev.append(k, v, t.slots)
+    qs = [tn.tensor(rng.standard_normal((2, 4 * heads, dim)).astype(np.float32), dtype=dtype, device="hip")
+          for _ in range(6)]
+    want = [[x.bits() for x in dev.attend(q, t, 1, 1600)] for q in qs]
+    tn.synchronize()
+    streams, got = (tn.Stream(), tn.Stream()), []
+    for rnd in range(3):
+        for i, q in enumerate(qs):
+            with streams[i % 2]:
+                got.append((i, dev.attend(q, t, 1, 1600)))
+    tn.synchronize()
+    for i, pair in got:
+        assert all(np.array_equal(x.bits(), y) for x, y in zip(pair, want[i])), i
