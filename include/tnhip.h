@@ -424,8 +424,13 @@ tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t*
  * A query row with an infinite or NaN element gives NaN; no other row does.
  * Sums, maxima and the softmax are f32. Keys enter the matrix products exactly
  * or as two f16 parts (rounded to f16 in bf16 rows of more than 1024 keys,
- * where a call has many rows), probabilities and values as f16, in two parts
- * where `dtype` needs them; the output is rounded once.
+ * where a call has many rows), probabilities and values as f16: both in two
+ * parts for f32 rows, one of them for f16 rows (which, goes by the call's
+ * size), both rounded to f16 for bf16 rows; the output is rounded once. 16-bit
+ * rows of head dims up to 128 may have their codes multiplied 72 too large and
+ * the excess taken off the f32 sum, which costs it up to four bits.
+ * Probabilities are held to 2^-30 of the row's largest, so that `out` is off by
+ * up to 2^-31 of the sum of its keys' |v| (lse counts them all).
  * `work`: scratch of at least tn_sdpa_paged_q4_0_work_floats() floats, 16-byte
  * aligned, the caller's, so that nothing is allocated and graphs with a
  * buffer each can run at once; its contents need no preparation and calls on

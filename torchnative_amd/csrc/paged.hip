@@ -97,8 +97,11 @@ __device__ inline void plan_row(const PlanArgs& a, const int32_t* starts, const 
 }
 
 // One workgroup: prefix sums over the requests, pages from and to the stack, and the
-// rows' slots where they are few (k_plan_rows otherwise). All latency: three loads that
-// depend on one another (lengths, pages, a row's page), the barriers of two sums.
+// rows' slots where they are few (k_plan_rows otherwise). All latency: counts and lengths,
+// three sums over the workgroup one after another (rows, pages, what was lacking; four
+// where a request has ended, whose counts and lengths are loaded for it first), popped
+// pages out to the table and each row's page back from it. 6.5 us for 16 requests of 256
+// rows, 13.0 with k_plan_rows for 500 of 60000; a launch is 3.5.
 template <int T>
 __global__ __launch_bounds__(T) void k_plan(const PlanArgs a, int rows_here) {
     __shared__ int64_t red[2][T / 64];
@@ -252,8 +255,8 @@ struct RowArgs {
 // V rows are bytes of eights of slots. Of a run of eight slots from an aligned one on,
 // which a prompt's rows are but for its ends, the bytes leave and come together, 8 a
 // lane; other rows' one by one. Bound by memory where rows are many: 8192 bf16 rows of 8
-// heads of 128 written in 13.4 us (19 byte by byte), 3.2 TB/s, and read in 10.6 (14),
-// 4.1; 65536 read in 60 (111), 5.7; 16 rows are a launch, 3.7 us.
+// heads of 128 written in 13.4 us (19 with all bytes one by one), 3.2 TB/s, and read in
+// 10.8 (14), 4.0; 65536 read in 56 to 59, 5.8 to 6.1; 16 rows are a launch, 3.7 us.
 constexpr int ROWS = 32;
 
 struct Runs {
@@ -520,8 +523,13 @@ tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t*
     if (!k || !v || !slots) return fail(TN_EVALUE, "kv_read_q4_0: null pointer");
     TN_TRY(paged_check_planes(op, a.c));
     a.ko = k, a.vo = v, a.slots = slots;
-    // more than the L2 caches hold between them (65536 rows of 8 heads of 128, bf16: 91 us
-    // through them, 62 past them, 5.6 TB/s; 8192 rows, 33 MB: 11 and 8)
+    // Outputs that the L2 caches hold between them stay in them for the kernel that reads them
+    // next; larger ones go past. (us, through the caches and past them, rows of 8 heads of 128,
+    // bf16, ten outputs in turn. Alone: 4096 rows, 16 MB, 7.2 and 5.9; 8192 rows, exactly at
+    // the limit and so through, 14.4 and 9.6; 9000, 15.8 and 10.3; 65536, 90 and 56. The
+    // caches' share is written back at a later kernel's cost: with one that reads the output
+    // right after, 4096 rows 12.2 and 11.9, 6000 17.1 and 18.5, 8192 22.7 and 23.0, 9000 24.9
+    // and 25.8, 32768 75 and 74.)
     a.past = 2 * m * a.c.H * a.c.nb * 32 * (dtype == TN_F32 ? 4 : 2) > (32 << 20);
     return rows_at((hipStream_t)stream, dtype, a, false);
 }

@@ -43,7 +43,12 @@ constexpr float P_BIAS = 6.0f;
 
 // k_paged_few's parts of each 16-bit operand: a 16-bit query is one f16 (a bf16 row
 // scaled by a power of two), an f32 one two; probabilities are two for an output of 11
-// or 24 bits, one for 8; values (code * scale, 15 bits) two for 24.
+// or 24 bits, one for 8; values (code * scale, 15 bits) two for 24. One part is a rounding
+// of 2^-12 at the mean, which a bf16 output, 2^-9, does not show (off the exact result by
+// 1.7e-3 of its norm, as f32 throughout is) and an f16 one shows by a quarter (2.6e-4,
+// 2.1e-4 with values in two parts as well). Two parts of both cost bf16 rows 8 % (sixteen
+// of 512 to 4096 keys, 18.2 and 19.9 us), of values f16 rows 11 % (twelve of 20000 to
+// 40000, 100 and 111).
 template <int DT>
 struct Parts {
     static constexpr int Q = DT == TN_F32 ? 2 : 1, P = DT == TN_BF16 ? 1 : 2, V = DT == TN_F32 ? 2 : 1;
@@ -145,10 +150,10 @@ __device__ inline float row_scale(float top) {
 // Single rows are bound by the cache's bytes: nothing of a key goes through LDS, a wave
 // loads its next tile whole while it computes one, and the splits make one round of the
 // resident workgroups. Twelve requests of 20000 to 40000 keys, 8 key/value heads of 128,
-// f16: 97 us with the merge, 4.3 TB/s; 5.2 of requests of one length (else the shorter
-// ones' workgroups wait for the longest's). Sixteen of 512 to 4096, bf16: 14 us and 3 of
+// f16: 96 to 100 us with the merge, 4.2 TB/s; 5.2 of requests of one length (else the shorter
+// ones' workgroups wait for the longest's). Sixteen of 512 to 4096, bf16: 18 us, 14 and 4 of
 // merge, 2.4 TB/s: eight tiles a wave, so that starting and merging count; one of 300, 9
-// heads of 64, f32: 5.4 us, a launch and one tile's chain of loads, products, softmax.
+// heads of 64, f32: 5.7 us, a launch and one tile's chain of loads, products, softmax.
 // Many rows are bound by the vector unit, which unpacks the codes anew for every 16.
 template <int NB>
 struct KeyTile {
@@ -386,7 +391,7 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
                 compute(y, t + 1);
             }
         }
-    } else {  // (two tiles would not fit the registers; two waves a SIMD do)
+    } else {  // (two tiles would not fit the registers; with one, two waves a SIMD do but at head dim 256, f32 224)
         int2 pg = lo < hi ? pages(lo) : make_int2(0, 0);
         for (int t = lo; t < hi; t++) {
             KeyTile<NB> x;
@@ -433,7 +438,7 @@ __global__ __launch_bounds__(256) void k_paged_few(const PagedArgs a) {
 }
 
 // The splits of a row, in order (the same bits every time): four output columns a thread.
-// A launch of its own, 3 to 4 us: of 17 us for sixteen single rows.
+// A launch of its own, 3 to 4 us: of 18 us for sixteen single rows.
 template <int DT>
 __global__ __launch_bounds__(256) void k_paged_combine(const PagedArgs a) {
     const int D = 32 * a.c.nb, q4 = D / 4;
@@ -476,8 +481,11 @@ __global__ __launch_bounds__(256) void k_paged_combine(const PagedArgs a) {
 // transposed, a row an element with its keys in the order in which the score product
 // leaves them in a lane (keys 4 h .. 4 h + 3 of each eight in half h of the wave), so
 // that P^T needs no exchange. Values are the rounded product and, but for bf16 outputs,
-// what it lacks, two f16 parts; so are keys (one part: EXACT_KEYS below). Rows are padded by 16 bytes, which spreads 16 rows' reads
-// over all banks.
+// what it lacks, two f16 parts; so are keys (one part: EXACT_KEYS below); probabilities
+// are one but for f32 outputs. (One part shows as in k_paged_few. f16 prompts, 32 heads on 8
+// of 128, take 233 us for 4096 rows and 93 for 2048; 17 % and 14 % more with probabilities
+// in two parts too. bf16 rows with two of everything: 276 us for the prompt below.) Rows
+// are padded by 16 bytes, which spreads 16 rows' reads over all banks.
 //
 // A wave alternates between a phase of products, O^T += V^T P^T of tile t and S^T of
 // tile t + 1, with its share of the unpacking (V of tile t + 1, K of t + 2) in their
@@ -490,10 +498,14 @@ __global__ __launch_bounds__(256) void k_paged_combine(const PagedArgs a) {
 // behind 2 t + 1, and K(t + 2) that of K(t), last read there too.
 //
 // Bound by the products, at the clock that they leave: 4096 causal rows of 32 heads of
-// 128, bf16, 150 us, 920 TF/s of 1300 that a large product of matrices reaches; the clock
-// falls to 1.9 GHz of 2.4. (Step by step: a workgroup of 128 rows, all in one phase, 185;
-// packed operations and no branch in the loop, 178; 256 rows, 167; the two groups half a
-// turn apart, 154; tiles asked for together at the start, output through LDS, 149.)
+// 128, bf16, 152 us, 900 TF/s of 1300 that a large product of matrices reaches; the clock
+// falls to 1.9 GHz of 2.4. Workgroups of 256 rows keep part of their registers in scratch
+// memory, inside the loop, at head dim 256 (bf16 from 224 on, f32 from 192): 2048 rows of
+// 2048 keys, 32 heads on 8, at 192, 224 and 256: bf16, 98, 112 and 178 us; f16, 156, 182
+// and 249; f32, 296, 437 and 624 (126 at 128). (The prompt step by step: a workgroup of 128
+// rows, all in one phase, 185; packed operations and no branch in the loop, 178; 256 rows,
+// 167; the two groups half a turn apart, 154; tiles asked for together at the start, output
+// through LDS, 149; keys of bf16 rows in two parts up to 1024 of them, 152.)
 // Fewer rows than fill the chip with 256 a workgroup run as 128 a workgroup, two a unit,
 // with their keys in up to 8 splits: 512 rows behind 20000 keys, 192 us, 277 unsplit.
 template <int DT, int NB, int W, int KK>
@@ -925,8 +937,8 @@ TN_INLINE void many_tile(const PagedArgs& a, uint8_t* lds, int h, int r, int sta
 // keys make do with one, the value rounded to f16: a score is then off by 2^-12 of each
 // of its products, which the output's 8 bits do not show and the lse, a mean over the
 // keys, by less the more they are (a prompt of 4096 random keys: 7e-7 of its lse; one of
-// 1000, in two parts, 7e-8; with one part everywhere, past 1e-6). 4096 rows of 32 heads of 128: 150 us, 144 with one part
-// everywhere and 183 with two.
+// 1000, in two parts, 7e-8; with one part everywhere, past 1e-6). 4096 rows of 32 heads of
+// 128: 152 us; when it was 150, 144 with one part everywhere and 183 with two.
 constexpr int EXACT_KEYS = 1024;
 
 template <int DT, int NB, int W>
@@ -1004,7 +1016,9 @@ __global__ __launch_bounds__(256) void k_paged_join(const PagedArgs a, int ns) {
 // keys or more, up to eight of them of 256 (one of 1000 keys, 8 heads of 128: 8.9 us at 4,
 // 10.4 at 2; eight of 100 to 3000, 4 rows each: 12.8 at 8, 13.7 at 6; but four of 1000 to
 // 4000: 13.7 at 15, 11.9 at 8; one of 8000: 13.5 at 32, 12.9 at 16). Up to 512 keys are
-// not worth a merge (300 keys: 5.6 us, 7.9 at 2).
+// not worth a merge (300 keys: 5.6 us, 7.9 at 2). All measured at head dims of 64 to 128.
+// At 256 (f32: 224) a unit holds one, so that 512 are two rounds: 16 sequences of 512 to
+// 4096 keys, 32 heads on 8, take 36 us in bf16 (23 at 192, 26 at 224), 37 in f16, 48 in f32.
 constexpr int64_t FEW_WGS = 512, FEW_KEYS = 512, FEW_MAX_SPLIT = 64;
 int64_t few_most(int64_t max_len) {
     if (max_len <= FEW_KEYS) return 1;
@@ -1042,7 +1056,9 @@ int64_t part_rows(const Pages& c, int64_t n, int64_t few, int64_t max_len) {
 // splits of the keys for workgroups of 128, two of which a unit holds. (us, 256 and 128 a
 // workgroup, 4 heads on each of 8 of 128: bf16, 2500 rows of 2500 keys, 312 workgroups of
 // 256, 75 and 77; 4000 of 4000, 145 and 161; 6000 of 6000, 307 and 334; f16, 2048 of 2048,
-// 90 and 102. Unsplit, 512 rows behind 20000 keys take 277, split 192.)
+// 90 and 102. Unsplit, 512 rows behind 20000 keys take 277, split 192. All at head dim
+// 128. Above it a unit holds one workgroup of 128 in f32, of f16 rows at 160 and 192, and of
+// any type at 224 and 256; the rule counts two all the same.)
 constexpr int64_t MANY_WIDE = 256, MANY_WGS = 512, MANY_MAX_SPLIT = 8;
 int many_splits(const Pages& c, int64_t n, int64_t tokens, int64_t G, int64_t max_len) {
     if (tokens * G / 256 * c.H >= MANY_WIDE) return 0;
