@@ -414,13 +414,14 @@ tn_status tn_kv_read_q4_0(void* stream, const tn_q4_cache* cache, const int32_t*
  * A row with no key to attend gives NaN and lse -inf; one whose keys' page is
  * outside the cache, NaN and lse NaN. Rows that no request has (ahead of
  * row_start[0], behind row_start[n]) are left as they were. What pages hold
- * past a request's length, of whatever kind, has no effect.
+ * past a request's length, of whatever kind, has no effect. Values that were
+ * not written by tn_kv_append_q4_0 and are past 65504 in size may count as
+ * infinite, and an infinite or NaN value may reach rows of its request ahead of
+ * it.
  * Nothing here tells a request that tn_paged_plan refused: its c rows are taken
  * for those of its last c cached tokens, so that out and lse hold other tokens'
  * keys (NaN where it has fewer). A caller drops the rows of a base of -1 (the
- * slots are -1) and gives them again in a later step. Values that were not written by
- * tn_kv_append_q4_0 and are past 65504 in size may count as infinite, and an
- * infinite or NaN value may reach rows of its request ahead of it.
+ * slots are -1) and gives them again in a later step.
  * A query row with an infinite or NaN element gives NaN; no other row does.
  * Sums, maxima and the softmax are f32. Keys enter the matrix products exactly
  * or as two f16 parts (rounded to f16 in bf16 rows of more than 1024 keys,

@@ -61,7 +61,8 @@ class PageTable:
     def step(self, fresh=None) -> None:
         """Adds fresh[r] tokens to request r, or ends it (negative). `fresh` is a device int32 tensor or host numbers,
         copied into `self.fresh`, or None for `self.fresh` as it stands (a captured loop writes it on the device).
-        `self.fresh` is one buffer for the table's life: captured steps hold its address."""
+        `self.fresh` is one buffer for the table's life: captured steps hold its address. Host numbers wait for the
+        stream and cannot be captured."""
         op = "paged_plan"
         own = self.fresh
         if fresh is not None:
