@@ -124,3 +124,65 @@ def test_f16_queries_below_the_normal_range(tn, many, rows, lens):
     c = Case(tn, "float16", 2, 3, 64, 16, rows, lens, seed=4)
     c.q = _up(tn, c.q.numpy().astype(np.float32) * np.float32(2.0 ** -18), "float16")
     c.check(c.run(tn, scale=2.0 ** 15, many=many), scale=2.0 ** 15)
+
+
+def _attend(tn, dev, dtype, q, T, Hq, D, row_start, lens, table, rows, most, out, lse):
+    import ctypes
+
+    from torchnative_amd import _lib as L
+
+    t = [tn.tensor(np.ascontiguousarray(a, np.int32), device="hip") for a in (row_start, lens, table)]
+    floats = dev.work_floats(len(lens), T, Hq, rows, most)
+    work = tn.empty((floats + 1,), "float32", "hip")
+    L.check(L.lib().tn_sdpa_paged_q4_0(
+        None, ctypes.byref(dev._c), {"float32": 0, "bfloat16": 1, "float16": 2}[dtype], q.data_ptr(), Hq * D, T, Hq,
+        len(lens), t[0].data_ptr(), t[1].data_ptr(), t[2].data_ptr(), np.shape(table)[1], rows, most, float("nan"),
+        work.data_ptr(), floats, out.data_ptr(), lse.data_ptr()))
+    tn.synchronize()
+
+
+@pytest.mark.parametrize("rows, many", [(5, False), (200, True)])
+def test_rows_and_outputs_past_two_to_the_31_elements(tn, rows, many):
+    """The last rows of a call whose queries and outputs pass 4 GiB and 2^31 elements."""
+    from test_paged_gpu import _fill
+    from torchnative_amd import _lib as L
+
+    c = Case(tn, "bfloat16", 2, 4, 256, 16, [rows], [rows + 300], seed=2)
+    T = (1 << 20) + 37 + rows
+    small = c.q.numpy().shape
+    q, out = (tn.empty((T, 8, 256), "bfloat16", "hip") for _ in range(2))
+    lse = tn.empty((T, 8), "float32", "hip")
+    row = 8 * 256 * 2
+    L.check(L.lib().tn_memcpy_d2d(q.data_ptr() + (T - rows) * row, c.q.data_ptr(), rows * row, None))
+    guard = tn.tensor(np.full((64, 8, 256), 7.5, np.float32), dtype="bfloat16", device="hip")
+    L.check(L.lib().tn_memcpy_d2d(out.data_ptr() + (T - rows - 64) * row, guard.data_ptr(), 64 * row, None))
+    table = np.pad(c.table, ((0, 0), (0, 1 << 10)), constant_values=-1) if many else c.table
+    most = table.shape[1] * 16 if many else c.max_len
+    print("rows", rows, "of", T, flush=True)
+    _attend(tn, _fill(tn, c.cache), "bfloat16", q, T, 8, 256, [T - rows, T], c.lens, table, rows, most, out, lse)
+    got, glse = tn.empty((rows + 64, 8, 256), "bfloat16", "hip"), tn.empty((rows, 8), "float32", "hip")
+    L.check(L.lib().tn_memcpy_d2d(got.data_ptr(), out.data_ptr() + (T - rows - 64) * row, (rows + 64) * row, None))
+    L.check(L.lib().tn_memcpy_d2d(glse.data_ptr(), lse.data_ptr() + (T - rows) * 32, rows * 32, None))
+    x = got.numpy().astype(np.float64)
+    assert small == (rows, 8, 256) and (x[:64] == 7.5).all()
+    c.check((x[64:], glse.numpy().astype(np.float64)))
+
+
+def test_as_many_requests_as_a_call_takes(tn):
+    """65535 requests of one row over one shared page, 1 to 16 tokens each: those of one length and query are equal, and
+    the first of each right."""
+    from test_paged_gpu import _fill
+
+    n, D, Hq = 65535, 32, 2
+    c = Case(tn, "float32", 1, 2, D, 16, [1] * 16, list(range(1, 17)), seed=9)
+    for r in range(1, 16):  # one page for all
+        c.table[r] = c.table[15]
+    c.table[0] = c.table[15]
+    r = np.arange(n) % 16
+    q = _up(tn, c.q.numpy()[r], "float32")
+    out, lse = tn.zeros((n, Hq, D)), tn.zeros((n, Hq))
+    dev = _fill(tn, c.cache)
+    _attend(tn, dev, "float32", q, n, Hq, D, np.arange(n + 1), r + 1, c.table[r], 1, 16, out, lse)
+    x, y = out.numpy(), lse.numpy()
+    assert np.array_equal(x, x[:16][r]) and np.array_equal(y, y[:16][r])
+    c.check((x[:16].astype(np.float64), y[:16].astype(np.float64)))
