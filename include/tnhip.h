@@ -227,6 +227,42 @@ tn_status tn_dense_dequantize(void* stream, const void* w, int dtype, int64_t co
 tn_status tn_dense_linear(void* stream, const float* x, int64_t m, int64_t k, const void* w, int w_dtype,
                           int64_t n, const float* bias, float* y);
 
+/* ---- rows in 8-bit integers: a scale for each token and channel ----
+ * The linear whose activations and weights are both int8, one f32 scale a row
+ * of either (a token; an output channel), so that the whole of K is one exact
+ * integer product. The reference has no such format: its 8-bit linear is q8_0,
+ * a scale for every 32 elements (k_quants.rs:652-757).
+ *   codes  [rows][pitch] int8 in [-127, 127], pitch = tn_i8_pitch(k): k rounded
+ *          up to 64, zeros behind k; 16-byte aligned;
+ *   scales [rows] f32: a value is code * scale.
+ * quantize: row r of x [m, k] in `dtype` (TN_F32, TN_BF16, TN_F16; dense), in
+ *   f32 steps: a = max |x|, scale = max(a * (1 / 127), 2^-126), 0 for a row of
+ *   zeros; code = rint(x * (1 / scale)), halves to even, held to +-127. A row
+ *   with an infinity or a NaN gets the scale NaN and codes 0: what is multiplied
+ *   with it is NaN. For weights (a row a channel) and activations alike.
+ * matmul: y[m, n] = ((float)(sum over k of a's and w's codes) * w_scales[n]) *
+ *   a_scales[m] (+ bias[n]), each step rounded to f32 once, then to y_dtype
+ *   (TN_F32, TN_BF16, TN_F16); bias nullable f32 [n]. The sum is exact, so a
+ *   row's bits do not depend on the rows around it or on the kernel that a
+ *   call's size selects. Codes of -128 are outside the format; with them sums
+ *   of up to k * 2^14 are exact as long as they are below 2^31.
+ * linear: y = matmul(quantize(x)), the same bits, x_dtype as quantize's. `work`:
+ *   tn_i8_linear_work_bytes(m, k) bytes of scratch, 16-byte aligned, the
+ *   caller's (0 bytes and a null pointer for few rows, which are quantised in
+ *   the launch that multiplies them); calls on one stream may share it, graphs
+ *   that replay at once need one each. Nothing is allocated.
+ * k is 1 to 131072 (a sum stays below 2^31); m <= 2^24 - 1, n <= 2^24 - 1. y overlaps no
+ * input. k <= 0 is refused with TN_EINVAL "mat1 and mat2 shapes cannot be
+ * multiplied" as quant.rs:322-332, other dtypes with TN_ENOTIMPL. */
+int64_t tn_i8_pitch(int64_t k);
+tn_status tn_i8_quantize(void* stream, const void* x, int dtype, int64_t m, int64_t k, int8_t* codes, float* scales);
+tn_status tn_i8_matmul(void* stream, const int8_t* a, const float* a_scales, int64_t m, int64_t k, const int8_t* w,
+                       const float* w_scales, int64_t n, const float* bias, void* y, int y_dtype);
+int64_t tn_i8_linear_work_bytes(int64_t m, int64_t k);
+tn_status tn_i8_linear(void* stream, const void* x, int x_dtype, int64_t m, int64_t k, const int8_t* w,
+                       const float* w_scales, int64_t n, const float* bias, void* work, int64_t work_bytes, void* y,
+                       int y_dtype);
+
 /* ---- scaled dot-product attention ----
  * `aten._scaled_dot_product_flash_attention_for_cpu(q, k, v, dropout_p=0.,
  * is_causal=False, *, attn_mask=None, scale=None) -> (out, logsumexp)`
@@ -443,6 +479,75 @@ tn_status tn_sdpa_paged_q4_0(void* stream, const tn_q4_cache* cache, int dtype, 
                              const int32_t* table, int64_t width, int64_t max_rows, int64_t max_len, double scale,
                              float* work, int64_t work_floats, void* out, float* lse);
 
+/* ---- the same cache, held in 8 bits ----
+ * Keys and values at 8 bits an element, an f32 scale for each block of sixteen
+ * tokens of a head (8.03 bits an element at head dim 64), for models that 4
+ * bits cost too much. Its pages come from the same tn_paged_plan.
+ *
+ * tn_q8_cache names one layer's four planes, caller-owned device memory,
+ * 16-byte aligned. With P = pages, H = n_kv_heads, S = page_size (a power of
+ * two, 16 to 256), D = head_dim (a multiple of 32, at most 256), a byte being
+ * its code (-127 .. 127) + 128:
+ *   k_codes  [P][H][S][D]
+ *   v_codes  [P][H][S/16][D][16]: sixteen tokens of an element together
+ *   k_scales, v_scales [P][H][S/16] f32
+ * Token o of page p is slot p * S + o, as for the 4-bit cache. */
+typedef struct tn_q8_cache {
+    uint8_t* k_codes;
+    float* k_scales;
+    uint8_t* v_codes;
+    float* v_scales;
+    int64_t pages, page_size, n_kv_heads, head_dim;
+} tn_q8_cache;
+
+/* Rows k, v [m][H][D] in `dtype` (TN_F32, TN_BF16, TN_F16), `stride` elements
+ * from one token's row to the next, into the cache at `slots` [m]. The rows that
+ * a call adds to a block of sixteen slots lie within sixteen rows of the call, as
+ * tn_paged_plan's do, in any order, skipped ones among them; of a slot given
+ * twice the last row counts. (Rows further apart leave their block with a mix:
+ * some not written, its scale from some of them.) A slot outside the cache is
+ * skipped.
+ * A row at the first slot of a block begins the block anew: what it held is
+ * forgotten. Rows at later slots join it: its scale becomes
+ *   s' = max(s, a * (1 / 127), 2^-126), a the largest size among the new rows of
+ * that head (s' = s where a is 0), and if that is larger, the codes of its other
+ * slots become rint(code * (s / s')); new rows' codes are rint(x * (1 / s')),
+ * held to +-127, all in f32 steps, halves to even. So a value is off by half
+ * its block's step when written, and by up to half the new step more each time
+ * the block's scale grows (at most fifteen times).
+ * Infinities and NaN take no part in a scale: an infinity is stored as the
+ * block's +-127 * s', a NaN as 0, with nothing to tell it by: a caller that may
+ * have them looks for them ahead of the call. A scale s of a joined block that
+ * is not a positive finite number counts as 0. */
+tn_status tn_kv_append_q8(void* stream, const tn_q8_cache* cache, int dtype, const void* k, const void* v, int64_t m,
+                          int64_t stride, const int32_t* slots);
+/* The cached rows at `slots` [m], (byte - 128) * scale rounded to `dtype`, to k
+ * and v [m][H][D], dense. A slot outside the cache gives rows of NaN. */
+tn_status tn_kv_read_q8(void* stream, const tn_q8_cache* cache, const int32_t* slots, int64_t m, int dtype, void* k,
+                        void* v);
+
+/* Attention of the last rows of n requests over their cached tokens: the
+ * arguments, rows, limits and refusals of tn_sdpa_paged_q4_0 on a tn_q8_cache.
+ * A row with no key to attend gives NaN and lse -inf; one whose keys' page is
+ * outside the cache, NaN and lse NaN; a query row with an infinite or NaN
+ * element gives NaN, and no other row does. Rows that no request has are left
+ * as they were. What pages hold past a request's length has no effect (the
+ * last block's scales, which its held tokens share, do).
+ * Sums, maxima and the softmax are f32. Codes enter the matrix products exactly;
+ * a query is one f16 under a power of two of its own (two f16 parts for f32
+ * rows), probabilities, times their values' block scale over the largest such
+ * scale met, one f16 for bf16 rows and two for others; the output is rounded
+ * once. Probabilities times scales are held to 2^-30 of the row's largest
+ * probability times the largest scale of values (lse counts them all).
+ * Scales are taken as finite and not negative.
+ * `work`: as there, tn_sdpa_paged_q8_work_floats() floats. */
+int64_t tn_sdpa_paged_q8_work_floats(const tn_q8_cache* cache, int64_t n, int64_t tokens, int64_t Hq,
+                                     int64_t max_rows, int64_t max_len);
+tn_status tn_sdpa_paged_q8(void* stream, const tn_q8_cache* cache, int dtype, const void* q, int64_t q_stride,
+                           int64_t tokens, int64_t Hq, int64_t n, const int32_t* row_start, const int32_t* lens,
+                           const int32_t* table, int64_t width, int64_t max_rows, int64_t max_len, double scale,
+                           float* work, int64_t work_floats, void* out, float* lse);
+
 /* ---- decode-step ops ----
  * The per-token aten ops around the linear and the attention in a Llama-style
  * decoder step, f32, as the reference runs them for an f32 model
@@ -473,6 +578,28 @@ tn_status tn_rmsnorm(void* stream, const float* x, int64_t m, int64_t n, const f
  * (1 / theta^(2i/d), computed by the caller as the model does). */
 tn_status tn_rope(void* stream, float* x, int64_t m, int64_t heads, int64_t d, const float* inv_freq,
                   const int32_t* pos);
+
+/* Norms of query and key heads with the rotation of their positions, one pass:
+ * for a head x [d] of a token, z = x * (1 / sqrt(mean(x^2) + eps)) * weight
+ * (weight f32 [d], q_weight for the Hq query heads, k_weight for the Hkv key
+ * heads), then for i < rot / 2
+ *   out[i]           = z[i] cos - z[i + rot/2] sin
+ *   out[i + rot / 2] = z[i + rot/2] cos + z[i] sin
+ * of the angle pos[t] * inv_freq[i], and out[i] = z[i] for i >= rot: what a
+ * decoder with head norms runs as LlamaRMSNorm's ops (as tn_rmsnorm) on each
+ * head and apply_rotary_pos_emb (as tn_rope). The angle is taken in 64 bits,
+ * so that far positions lose nothing (tn_rope rounds it to f32, as the
+ * reference does). f32 steps throughout, rounded to `dtype` once.
+ *   q [m][Hq][d], k [m][Hkv][d] in `dtype` (TN_F32, TN_BF16, TN_F16), q_stride
+ *   and k_stride elements from a token to the next (both may be parts of one
+ *   stacked projection); q_out, k_out the same with strides of their own; an
+ *   output may be its input, of the same stride (in place), and overlaps
+ *   nothing else. Hq or Hkv may be 0. d is even, 2 to 256; rot is even, 0 to d;
+ *   inv_freq f32 [rot / 2] (null for rot 0); pos device int32 [m]. */
+tn_status tn_qk_norm_rope(void* stream, int dtype, const void* q, int64_t q_stride, int64_t Hq, const void* k,
+                          int64_t k_stride, int64_t Hkv, int64_t m, int64_t d, const float* q_weight,
+                          const float* k_weight, double eps, const float* inv_freq, int64_t rot, const int32_t* pos,
+                          void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride);
 
 /* silu(gate) * up: candle's silu x / (1 + exp(-x)) (candle-core op.rs:782-784,
  * aten.rs:15360-15384), then aten.mul.Tensor. out may alias gate or up. */

@@ -18,7 +18,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import check, lib
-from .tensor import Tensor, current_stream
+from .tensor import Scratch, Tensor, current_stream, row_stride
 
 QK4_0 = 32
 Q4_0_TYPE_SIZE = 18
@@ -318,6 +318,144 @@ def linear(input: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tensor:
                                 weight.data_ptr(), _lib.TN_F32, out_features,
                                 bias.data_ptr() if bias is not None else None, out.data_ptr()))
     return out
+
+
+class I8Rows:
+    """Rows [m, k] in 8-bit integers: int8 codes [m, pitch] and an f32 scale a
+    row (include/tnhip.h, tn_i8_quantize): a weight with a scale a channel, or
+    activations with a scale a token."""
+
+    def __init__(self, shape, device="hip", codes=None, scales=None):
+        m, k = (int(x) for x in shape)
+        self.shape, self.device = (m, k), device
+        self.codes = Tensor((m, (k + 63) // 64 * 64), "int8", device) if codes is None else codes
+        self.scales = Tensor((m,), "float32", device) if scales is None else scales
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.nbytes + self.scales.nbytes
+
+    def to(self, device) -> "I8Rows":
+        """The same codes and scales on another device."""
+        codes = self.codes.to(device)
+        return I8Rows(self.shape, codes.device, codes, self.scales.to(device))
+
+    def __repr__(self):
+        return f"I8Rows(shape={self.shape}, device={self.device})"
+
+
+def i8_quantize(t: Tensor, out: I8Rows | None = None) -> I8Rows:
+    """Rows of t [..., k] (float32, bfloat16 or float16) in 8-bit integers, a
+    scale a row (tn_i8_quantize)."""
+    op = "i8_quantize"
+    _require_hip(op, t)
+    if t.dim() == 0:
+        raise NotImplementedError(f"{op}: a 0-d tensor cannot be quantised")
+    k = t.shape[-1]
+    m = t.numel // k if k else math.prod(t.shape[:-1])
+    rows = I8Rows((m, k)) if out is None else out
+    _require_hip(op, rows)
+    if rows.shape != (m, k):
+        raise RuntimeError(f"{op}: out {list(rows.shape)} does not hold rows {[m, k]}")
+    check(lib().tn_i8_quantize(current_stream(), t.data_ptr(), _dt(t.dtype), m, k, rows.codes.data_ptr(),
+                               rows.scales.data_ptr()))
+    return rows
+
+
+def _i8_out(op, rows, weight, bias, out, odt):
+    """Checks of a product of rows (shape [..., k]) with a weight; its output."""
+    if not isinstance(weight, I8Rows):
+        raise TypeError(f"{op}: weight must be rows in 8-bit integers (i8_quantize), got {type(weight)}")
+    out_features, in_features = weight.shape
+    _require_hip(op, rows, weight, bias, out)
+    if len(rows.shape) == 0 or rows.shape[-1] != in_features:
+        raise RuntimeError(
+            f"{op}: mat1 and mat2 shapes cannot be multiplied ({list(rows.shape)} and {in_features}x{out_features})")
+    if bias is not None and bias.dtype != "float32":
+        raise NotImplementedError(f"{op}: the bias must be float32, got torch.{bias.dtype}")
+    if bias is not None and bias.shape != (out_features,):
+        raise RuntimeError(f"{op}: bias shape {list(bias.shape)} does not match out_features {out_features}")
+    shape = tuple(rows.shape[:-1]) + (out_features,)
+    if out is None:
+        return Tensor(shape, odt, "hip")
+    if out.shape != shape or out.dtype != odt:
+        raise RuntimeError(f"{op}: out {list(out.shape)} {out.dtype} is not {list(shape)} {odt}")
+    return out
+
+
+def i8_matmul(a: I8Rows, weight: I8Rows, bias: Tensor | None = None, *, out_dtype="float32",
+              out: Tensor | None = None) -> Tensor:
+    """a @ weight.T (+ bias) of rows in 8-bit integers (tn_i8_matmul)."""
+    op = "i8_matmul"
+    if not isinstance(a, I8Rows):
+        raise TypeError(f"{op}: the rows must be in 8-bit integers (i8_quantize), got {type(a)}")
+    out = _i8_out(op, a, weight, bias, out, out_dtype)
+    (m, k), n = a.shape, weight.shape[0]
+    check(lib().tn_i8_matmul(current_stream(), a.codes.data_ptr(), a.scales.data_ptr(), m, k, weight.codes.data_ptr(),
+                             weight.scales.data_ptr(), n, bias.data_ptr() if bias is not None else None,
+                             out.data_ptr(), _dt(out_dtype)))
+    return out
+
+
+_i8_work = Scratch()
+
+
+def i8_linear(input: Tensor, weight: I8Rows, bias: Tensor | None = None, *, out_dtype=None,
+              work: Tensor | None = None, out: Tensor | None = None) -> Tensor:
+    """input @ weight.T (+ bias), the input's rows quantised to 8-bit integers
+    first, a scale a token (tn_i8_linear). out_dtype: the input's by default.
+    `work` (tn_i8_linear_work_bytes(m, k) bytes) and `out` are made where they
+    are not given; code that captures passes its own, a `work` of its own for
+    each graph."""
+    op = "i8_linear"
+    odt = out_dtype or (out.dtype if out is not None else input.dtype)
+    out = _i8_out(op, input, weight, bias, out, odt)
+    n, k = weight.shape
+    m = math.prod(input.shape[:-1])
+    need = int(lib().tn_i8_linear_work_bytes(m, k))
+    work = _i8_work.get(need) if work is None else work
+    _require_hip(op, work)
+    check(lib().tn_i8_linear(current_stream(), input.data_ptr(), _dt(input.dtype), m, k, weight.codes.data_ptr(),
+                             weight.scales.data_ptr(), n, bias.data_ptr() if bias is not None else None,
+                             work.data_ptr(), work.nbytes, out.data_ptr(), _dt(odt)))
+    return out
+
+
+def qk_norm_rope(q, k, q_weight: Tensor, k_weight: Tensor, inv_freq: Tensor, pos: Tensor, eps: float = 1e-6,
+                 q_out=None, k_out=None):
+    """RMSNorm of each head of q [m, heads, d] and k [m, kv_heads, d] (weights
+    float32 [d]), then the rotation of its first 2 * len(inv_freq) elements to
+    the token's position, in one pass (tn_qk_norm_rope). q and k are tensors or
+    Heads of stacked rows; outputs go to q_out and k_out, in place by default.
+    Returns (q_out, k_out)."""
+    op = "qk_norm_rope"
+    q_out, k_out = q if q_out is None else q_out, k if k_out is None else k_out
+    _require_hip(op, q, k, q_weight, k_weight, inv_freq, pos, q_out, k_out)
+    for name, t in (("q", q), ("k", k)):
+        if t.dim() != 3:
+            raise RuntimeError(f"{op}: {name} {list(t.shape)} is not [tokens, heads, head_dim]")
+    m, Hq, d = q.shape
+    Hkv = k.shape[1]
+    if k.shape[0] != m or k.shape[2] != d or k.dtype != q.dtype:
+        raise RuntimeError(f"{op}: q {list(q.shape)} {q.dtype} and k {list(k.shape)} {k.dtype} do not describe one "
+                           "set of tokens")
+    for a, b in ((q, q_out), (k, k_out)):
+        if b.shape != a.shape or b.dtype != a.dtype:
+            raise RuntimeError(f"{op}: out {list(b.shape)} {b.dtype} is not {list(a.shape)} {a.dtype}")
+    for name, t in (("q_weight", q_weight), ("k_weight", k_weight), ("inv_freq", inv_freq)):
+        if t.dtype != "float32":
+            raise NotImplementedError(f"{op}: {name} must be float32, got {t.dtype}")
+        if t.dim() != 1 or (name != "inv_freq" and t.shape != (d,)):
+            raise RuntimeError(f"{op}: {name} {list(t.shape)} does not fit heads of {d}")
+    if pos.dtype != "int32":
+        raise NotImplementedError(f"{op}: pos must be int32, got {pos.dtype}")
+    if pos.dim() != 1 or pos.shape[0] < m:
+        raise RuntimeError(f"{op}: pos {list(pos.shape)} does not give {m} tokens a position each")
+    check(lib().tn_qk_norm_rope(
+        current_stream(), _dt(q.dtype), q.data_ptr(), row_stride(q), Hq, k.data_ptr(), row_stride(k), Hkv, m, d,
+        q_weight.data_ptr(), k_weight.data_ptr(), float(eps), inv_freq.data_ptr(), 2 * inv_freq.shape[0],
+        pos.data_ptr(), q_out.data_ptr(), row_stride(q_out), k_out.data_ptr(), row_stride(k_out)))
+    return q_out, k_out
 
 
 def _dt(name):

@@ -6,6 +6,7 @@ libtnhip.so) and a Python mirror of the reference's `torch._C` entry points.
 
 from . import _C, device, gguf, nn, paged, quant, tensor
 from ._C import (
+    I8Rows,
     QTensor,
     _aten_dispatch,
     _dequantize,
@@ -20,16 +21,21 @@ from ._C import (
     _quantized_linear,
     _quantized_nbytes,
     _quantized_to,
+    i8_linear,
+    i8_matmul,
+    i8_quantize,
+    qk_norm_rope,
     scaled_dot_product_attention,
     sdpa_decode,
 )
-from .paged import PageTable, Q4Cache
-from .quant import QuantizedLinear, QuantizeReport, quantize_
-from .tensor import Event, Stream, Tensor, empty, synchronize, tensor, zeros
+from .paged import PageTable, Q4Cache, Q8Cache
+from .quant import Int8Linear, QuantizedLinear, QuantizeReport, quantize_
+from .tensor import Event, Heads, Stream, Tensor, empty, synchronize, tensor, zeros
 
 __all__ = [
     "QTensor", "QuantizedLinear", "QuantizeReport", "quantize_", "Tensor", "Stream", "Event", "empty", "zeros", "tensor",
     "synchronize", "_quantize", "_dequantize", "_quantized_linear", "_quantized_to", "_quantized_blob",
     "_quantized_from_blob", "_quantized_format", "_quantized_formats", "_quantized_nbytes", "_aten_dispatch",
-    "scaled_dot_product_attention", "sdpa_decode", "PageTable", "Q4Cache", "_hip_probe", "_hip_counters", "_hip_ops",
+    "scaled_dot_product_attention", "sdpa_decode", "PageTable", "Q4Cache", "Q8Cache",
+    "I8Rows", "Int8Linear", "i8_quantize", "i8_matmul", "i8_linear", "qk_norm_rope", "Heads", "_hip_probe", "_hip_counters", "_hip_ops",
 ]

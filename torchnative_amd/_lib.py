@@ -52,6 +52,10 @@ class Q4Cache(ctypes.Structure):
     ]
 
 
+class Q8Cache(ctypes.Structure):
+    _fields_ = Q4Cache._fields_
+
+
 class Llama(ctypes.Structure):
     _fields_ = [
         ("n_layers", ctypes.c_int64), ("hidden", ctypes.c_int64), ("n_heads", ctypes.c_int64),
@@ -110,6 +114,11 @@ SIGNATURES = {
     "tn_dense_quantize": (_I, [_P, _P, _I64, _I, _P]),
     "tn_dense_dequantize": (_I, [_P, _P, _I, _I64, _P]),
     "tn_dense_linear": (_I, [_P, _P, _I64, _I64, _P, _I, _I64, _P, _P]),
+    "tn_i8_pitch": (_I64, [_I64]),
+    "tn_i8_quantize": (_I, [_P, _P, _I, _I64, _I64, _P, _P]),
+    "tn_i8_matmul": (_I, [_P, _P, _P, _I64, _I64, _P, _P, _I64, _P, _P, _I]),
+    "tn_i8_linear_work_bytes": (_I64, [_I64, _I64]),
+    "tn_i8_linear": (_I, [_P, _P, _I, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _P, _I]),
     "tn_q4_0_linear_decode": (_I, [_P, _P, _I64, _I, _P, _D, _P, _P, _I64, _P, _P]),
     "tn_sdpa_fwd": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I, _P, _I, _D, _P, _P]),
     "tn_sdpa_decode": (_I, [_P, _I, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _D, _P, _P]),
@@ -120,9 +129,16 @@ SIGNATURES = {
     "tn_sdpa_paged_q4_0_work_floats": (_I64, [ctypes.POINTER(Q4Cache), _I64, _I64, _I64, _I64, _I64]),
     "tn_sdpa_paged_q4_0": (_I, [_P, ctypes.POINTER(Q4Cache), _I, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64,
                                 _I64, _D, _P, _I64, _P, _P]),
+    "tn_kv_append_q8": (_I, [_P, ctypes.POINTER(Q8Cache), _I, _P, _P, _I64, _I64, _P]),
+    "tn_kv_read_q8": (_I, [_P, ctypes.POINTER(Q8Cache), _P, _I64, _I, _P, _P]),
+    "tn_sdpa_paged_q8_work_floats": (_I64, [ctypes.POINTER(Q8Cache), _I64, _I64, _I64, _I64, _I64]),
+    "tn_sdpa_paged_q8": (_I, [_P, ctypes.POINTER(Q8Cache), _I, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _I64, _I64,
+                              _I64, _D, _P, _I64, _P, _P]),
     "tn_embedding": (_I, [_P, _P, _I64, _P, _I64, _I64, _P]),
     "tn_rmsnorm": (_I, [_P, _P, _I64, _I64, _P, _D, _P]),
     "tn_rope": (_I, [_P, _P, _I64, _I64, _I64, _P, _P]),
+    "tn_qk_norm_rope": (_I, [_P, _I, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P, _P, _D, _P, _I64, _P, _P, _I64,
+                             _P, _I64]),
     "tn_silu_mul": (_I, [_P, _P, _P, _I64, _P]),
     "tn_add": (_I, [_P, _P, _P, _I64, _P]),
     "tn_argmax": (_I, [_P, _P, _I64, _I64, _P]),

@@ -1,5 +1,6 @@
-// The paged 4-bit key/value cache (paged.hip, paged_attn.hip): its planes as the
-// kernels index them, and the checks that every entry point makes.
+// The paged key/value caches of 4 bits (paged.hip, paged_attn.hip) and of 8
+// (paged8.hip, paged8_attn.hip): their planes as the kernels index them, and the
+// checks that every entry point makes.
 #pragma once
 
 #include "attn_common.h"
@@ -14,9 +15,19 @@ struct Pages {
     int pages, shift, H, nb;  // page size 1 << shift, head dim 32 nb
 };
 
+struct Pages8 {
+    uint8_t* kc;  // [pages][H][S][D]
+    float* ks;    // [pages][H][S/16]
+    uint8_t* vc;  // [pages][H][S/16][D][16]
+    float* vs;    // [pages][H][S/16]
+    int pages, shift, H, nb;  // as above
+};
+
 // The cache's own numbers, then (planes) its pointers.
 tn_status paged_check(const char* op, const tn_q4_cache* cache, Pages* out);
+tn_status paged_check(const char* op, const tn_q8_cache* cache, Pages8* out);
 tn_status paged_check_planes(const char* op, const Pages& c);
+tn_status paged_check_planes(const char* op, const Pages8& c);
 
 // The place of token i (0..7) among the eight bytes of v_codes: tokens 0 2 1 3 of
 // each four, so that the halves of a dword masked to one nibble of each 16-bit

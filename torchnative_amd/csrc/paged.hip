@@ -8,8 +8,10 @@
 #include "q8.h"
 
 namespace tn {
+namespace {
 
-tn_status paged_check(const char* op, const tn_q4_cache* cache, Pages* out) {
+template <class Cache, class Planes>
+tn_status check_sizes(const char* op, const char* format, const Cache* cache, Planes* out) {
     const std::string name(op);
     if (!cache) return fail(TN_EVALUE, name + ": null cache");
     const int64_t S = cache->page_size, D = cache->head_dim, H = cache->n_kv_heads, P = cache->pages;
@@ -17,24 +19,46 @@ tn_status paged_check(const char* op, const tn_q4_cache* cache, Pages* out) {
         return fail(TN_ENOTIMPL, name + ": page_size " + std::to_string(S) +
                                      " is not implemented; it is a power of two from 16 to 256");
     if (D < 32 || D > 256 || D % 32)
-        return fail(TN_ENOTIMPL, name + ": head_dim " + std::to_string(D) +
-                                     " is not implemented for a q4_0 cache; it is a multiple of 32 up to 256");
+        return fail(TN_ENOTIMPL, name + ": head_dim " + std::to_string(D) + " is not implemented for a " + format +
+                                     " cache; it is a multiple of 32 up to 256");
     // (the attention's grid has up to 8 H workgroups a request in its second dimension)
     if (H < 1 || H > 4096 || P < 0) return fail(TN_EINVAL, name + ": bad cache sizes");
     if (P > INT32_MAX / S) return fail(TN_EVALUE, name + ": a cache holds fewer than 2^31 slots");
-    out->kc = cache->k_codes, out->kd = cache->k_scales, out->vc = cache->v_codes, out->vd = cache->v_scales;
     out->pages = (int)P, out->H = (int)H, out->nb = (int)(D / 32);
     out->shift = __builtin_ctzll((unsigned long long)S);
     return TN_OK;
 }
 
-tn_status paged_check_planes(const char* op, const Pages& c) {
-    if (!c.pages) return TN_OK;  // nothing is read or written
-    if (!c.kc || !c.kd || !c.vc || !c.vd) return fail(TN_EVALUE, std::string(op) + ": null cache plane");
-    const uintptr_t all = reinterpret_cast<uintptr_t>(c.kc) | reinterpret_cast<uintptr_t>(c.kd) |
-                          reinterpret_cast<uintptr_t>(c.vc) | reinterpret_cast<uintptr_t>(c.vd);
-    if (all & 15) return fail(TN_EVALUE, std::string(op) + ": cache planes must be 16-byte aligned");
+uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+tn_status check_planes(const char* op, int pages, const void* a, const void* b, const void* c, const void* d) {
+    if (!pages) return TN_OK;  // nothing is read or written
+    if (!a || !b || !c || !d) return fail(TN_EVALUE, std::string(op) + ": null cache plane");
+    if ((address(a) | address(b) | address(c) | address(d)) & 15)
+        return fail(TN_EVALUE, std::string(op) + ": cache planes must be 16-byte aligned");
     return TN_OK;
+}
+
+}  // namespace
+
+tn_status paged_check(const char* op, const tn_q4_cache* cache, Pages* out) {
+    TN_TRY(check_sizes(op, "q4_0", cache, out));
+    out->kc = cache->k_codes, out->kd = cache->k_scales, out->vc = cache->v_codes, out->vd = cache->v_scales;
+    return TN_OK;
+}
+
+tn_status paged_check(const char* op, const tn_q8_cache* cache, Pages8* out) {
+    TN_TRY(check_sizes(op, "q8", cache, out));
+    out->kc = cache->k_codes, out->ks = cache->k_scales, out->vc = cache->v_codes, out->vs = cache->v_scales;
+    return TN_OK;
+}
+
+tn_status paged_check_planes(const char* op, const Pages& c) {
+    return check_planes(op, c.pages, c.kc, c.kd, c.vc, c.vd);
+}
+
+tn_status paged_check_planes(const char* op, const Pages8& c) {
+    return check_planes(op, c.pages, c.kc, c.ks, c.vc, c.vs);
 }
 
 namespace {

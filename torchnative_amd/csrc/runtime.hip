@@ -235,7 +235,8 @@ const char* tn_ops(void) {
            "torch._C._quantized_to,torch._C._quantized_blob,"
            "aten._scaled_dot_product_flash_attention_for_cpu.default,sdpa_decode,"
            "aten.embedding.default,rms_norm,rotary_embedding,silu_mul,aten.add.Tensor,aten.argmax.default,"
-           "kv_append,paged_plan,kv_append_q4_0,kv_read_q4_0,sdpa_paged_q4_0,q4_0_linear_decode,llama_decode_step,llama_prefill";
+           "kv_append,paged_plan,kv_append_q4_0,kv_read_q4_0,sdpa_paged_q4_0,q4_0_linear_decode,llama_decode_step,llama_prefill,"
+           "i8_quantize,i8_matmul,i8_linear,qk_norm_rope,kv_append_q8,kv_read_q8,sdpa_paged_q8";
 }
 
 tn_status tn_probe(char* buf, size_t len) {

@@ -1,11 +1,11 @@
-"""A key/value cache in pages, held in 4 bits, and the attention over it.
+"""Key/value caches in pages, held in 4 or 8 bits, and the attention over them.
 
 The serving counterpart of the reference's per-sequence `PreallocatedLayer`
 (torchnative/python/torchnative/kernels/kv_cache.py:92-114): the sequences of a
-batch share one pool of pages (`Q4Cache`, one a layer), a device-resident
-`PageTable` hands pages to requests and gives each new token its slot, and
-`Q4Cache.attend` runs the rows of all requests, single tokens and prompts alike,
-over what they have cached.
+batch share one pool of pages (`Q4Cache` or `Q8Cache`, one a layer), a
+device-resident `PageTable` hands pages to requests and gives each new token its
+slot, and a cache's `attend` runs the rows of all requests, single tokens and
+prompts alike, over what they have cached.
 
     pages = PageTable(requests=16, width=256, page_size=16, pages=4096, tokens=512)
     cache = Q4Cache(4096, 16, n_kv_heads, head_dim)
@@ -26,9 +26,9 @@ import numpy as np
 from . import _lib
 from ._C import _dt, _require_hip
 from ._lib import check, lib
-from .tensor import Tensor, current_stream, tensor
+from .tensor import Scratch, Tensor, current_stream, row_stride, tensor
 
-__all__ = ["PageTable", "Q4Cache"]
+__all__ = ["PageTable", "Q4Cache", "Q8Cache"]
 
 
 def _int32(op, **named):
@@ -84,22 +84,25 @@ class PageTable:
             self.base.data_ptr(), self.slots.data_ptr(), self.pos.data_ptr()))
 
 
-class Q4Cache:
-    """One layer's keys and values in pages of q4_0 blocks (include/tnhip.h, tn_q4_cache): page_size a power of two
-    from 16 to 256, head_dim a multiple of 32 up to 256."""
+class _Cache:
+    """What the caches of pages have in common; `_kind` names their entry points and `_planes` makes their planes."""
+
+    _kind: str
+    _struct: type
 
     def __init__(self, pages: int, page_size: int, n_kv_heads: int, head_dim: int):
         self.pages, self.page_size = int(pages), int(page_size)
         self.n_kv_heads, self.head_dim = int(n_kv_heads), int(head_dim)
-        rows = self.pages * self.n_kv_heads * self.page_size
-        self.k_codes, self.v_codes = (Tensor((rows * self.head_dim // 2,), "uint8", "hip") for _ in range(2))
-        self.k_scales, self.v_scales = (Tensor((rows * (self.head_dim // 32),), "float16", "hip") for _ in range(2))
-        self._c = _lib.Q4Cache(self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(),
+        self.k_codes, self.k_scales, self.v_codes, self.v_scales = self._planes()
+        self._c = self._struct(self.k_codes.data_ptr(), self.k_scales.data_ptr(), self.v_codes.data_ptr(),
                                self.v_scales.data_ptr(), self.pages, self.page_size, self.n_kv_heads, self.head_dim)
-        self._work = {}
+        self._work = Scratch()
 
     def _ref(self):
         return ctypes.byref(self._c)
+
+    def _fn(self, name):
+        return getattr(lib(), f"tn_{name.format(self._kind)}")
 
     @property
     def nbytes(self) -> int:
@@ -109,43 +112,44 @@ class Q4Cache:
         if t.dim() != 3 or t.shape[1:] != (self.n_kv_heads, self.head_dim):
             raise RuntimeError(f"{op}: rows {list(t.shape)} are not [m, {self.n_kv_heads}, {self.head_dim}]")
 
-    def append(self, k: Tensor, v: Tensor, slots: Tensor) -> None:
-        """Writes rows k, v [m, n_kv_heads, head_dim] to `slots` [m]; a negative slot skips its row."""
-        op = "kv_append_q4_0"
+    def append(self, k, v, slots: Tensor) -> None:
+        """Writes rows k, v [m, n_kv_heads, head_dim] (tensors, or Heads of stacked rows) to `slots` [m]; a negative slot
+        skips its row."""
+        op = f"kv_append_{self._kind}"
         _require_hip(op, k, v, slots)
         _int32(op, slots=slots)
         self._rows(op, k)
-        if v.shape != k.shape or v.dtype != k.dtype or slots.shape != k.shape[:1]:
+        if v.shape != k.shape or v.dtype != k.dtype or slots.shape != k.shape[:1] or row_stride(v) != row_stride(k):
             raise RuntimeError(f"{op}: k {list(k.shape)} {k.dtype}, v {list(v.shape)} {v.dtype} and slots "
                                f"{list(slots.shape)} do not describe one set of rows")
-        check(lib().tn_kv_append_q4_0(current_stream(), self._ref(), _dt(k.dtype), k.data_ptr(), v.data_ptr(),
-                                      k.shape[0], self.n_kv_heads * self.head_dim, slots.data_ptr()))
+        check(self._fn("kv_append_{}")(current_stream(), self._ref(), _dt(k.dtype), k.data_ptr(), v.data_ptr(),
+                                       k.shape[0], row_stride(k), slots.data_ptr()))
 
     def read(self, slots: Tensor, dtype: str = "float32"):
         """The cached rows at `slots` [m], as (k, v) [m, n_kv_heads, head_dim]."""
-        op = "kv_read_q4_0"
+        op = f"kv_read_{self._kind}"
         _require_hip(op, slots)
         _int32(op, slots=slots)
         k, v = (Tensor((slots.numel, self.n_kv_heads, self.head_dim), dtype, "hip") for _ in range(2))
-        check(lib().tn_kv_read_q4_0(current_stream(), self._ref(), slots.data_ptr(), slots.numel, _dt(dtype),
-                                    k.data_ptr(), v.data_ptr()))
+        check(self._fn("kv_read_{}")(current_stream(), self._ref(), slots.data_ptr(), slots.numel, _dt(dtype),
+                                     k.data_ptr(), v.data_ptr()))
         return k, v
 
     def work_floats(self, requests: int, tokens: int, heads: int, max_rows: int, max_len: int) -> int:
         """Floats of scratch that `attend` takes for such a call."""
-        return int(lib().tn_sdpa_paged_q4_0_work_floats(self._ref(), requests, tokens, heads, max_rows, max_len))
+        return int(self._fn("sdpa_paged_{}_work_floats")(self._ref(), requests, tokens, heads, max_rows, max_len))
 
-    def attend(self, q: Tensor, pages: PageTable, max_rows: int, max_len: int, scale: float | None = None,
+    def attend(self, q, pages: PageTable, max_rows: int, max_len: int, scale: float | None = None,
                work: Tensor | None = None, out: Tensor | None = None, lse: Tensor | None = None):
-        """The rows q [tokens, heads, head_dim] of `pages`' last step over their requests' cached tokens, the rows'
-        own among them. max_rows, max_len: upper bounds of a request's rows and length. Returns (out, lse), whose rows
-        behind the last request's are left as they were.
+        """The rows q [tokens, heads, head_dim] (a tensor, or Heads of stacked rows) of `pages`' last step over their
+        requests' cached tokens, the rows' own among them. max_rows, max_len: upper bounds of a request's rows and
+        length. Returns (out, lse), whose rows behind the last request's are left as they were.
         Rows of a request that the step refused (`pages.base` -1, `pages.slots` -1) are not in the cache; what they get
         here is the attention of the request's earlier tokens, to be dropped.
 
         `work`, `out` and `lse` are made where they are not given. Code that captures passes its own, so that the
         graph's buffers live as long as it does, a `work` of its own for each graph."""
-        op = "sdpa_paged_q4_0"
+        op = f"sdpa_paged_{self._kind}"
         _require_hip(op, q)
         if q.dim() != 3 or q.shape[2] != self.head_dim:
             raise RuntimeError(f"{op}: query {list(q.shape)} is not [tokens, heads, {self.head_dim}]")
@@ -153,20 +157,43 @@ class Q4Cache:
             raise RuntimeError(f"{op}: the table's pages hold {pages.page_size} tokens, the cache's {self.page_size}")
         T, Hq, D = q.shape
         need = self.work_floats(pages.requests, T, Hq, max_rows, max_len)
-        if work is None:  # one a stream: calls on a stream are ordered
-            held = self._work.setdefault(current_stream(), [])  # outgrown ones stay: a graph may point at them
-            if not held or held[-1].numel < need:
-                held.append(Tensor((max(need, 2 * held[-1].numel if held else 1),), "float32", "hip"))
-            work = held[-1]
+        floats = need if work is None else work.numel
         out = Tensor(q.shape, q.dtype, "hip") if out is None else out
         lse = Tensor((T, Hq), "float32", "hip") if lse is None else lse
-        _require_hip(op, work, out, lse)
-        if (out.shape, out.dtype, lse.shape, lse.dtype, work.dtype) != (q.shape, q.dtype, (T, Hq), "float32", "float32"):
+        if work is not None and work.dtype != "float32" or (out.shape, out.dtype, lse.shape, lse.dtype) != (
+                q.shape, q.dtype, (T, Hq), "float32"):
             raise RuntimeError(f"{op}: out {list(out.shape)} {out.dtype}, lse {list(lse.shape)} {lse.dtype} or work "
-                               f"{work.dtype} does not fit query {list(q.shape)} {q.dtype}")
+                               f"{work.dtype if work is not None else ''} does not fit query {list(q.shape)} {q.dtype}")
+        work = self._work.get(4 * need) if work is None else work
+        _require_hip(op, work, out, lse)
         sc = float("nan") if scale is None else float(scale)
-        check(lib().tn_sdpa_paged_q4_0(
-            current_stream(), self._ref(), _dt(q.dtype), q.data_ptr(), Hq * D, T, Hq, pages.requests,
+        check(self._fn("sdpa_paged_{}")(
+            current_stream(), self._ref(), _dt(q.dtype), q.data_ptr(), row_stride(q), T, Hq, pages.requests,
             pages.row_start.data_ptr(), pages.lens.data_ptr(), pages.table.data_ptr(), pages.width, max_rows, max_len,
-            sc, work.data_ptr(), work.numel, out.data_ptr(), lse.data_ptr()))
+            sc, work.data_ptr(), floats, out.data_ptr(), lse.data_ptr()))
         return out, lse
+
+
+class Q4Cache(_Cache):
+    """One layer's keys and values in pages of q4_0 blocks (include/tnhip.h, tn_q4_cache): page_size a power of two
+    from 16 to 256, head_dim a multiple of 32 up to 256."""
+
+    _kind, _struct = "q4_0", _lib.Q4Cache
+
+    def _planes(self):
+        rows = self.pages * self.n_kv_heads * self.page_size
+        return [Tensor(shape, dtype, "hip") for _ in "kv" for shape, dtype in (
+            ((rows * self.head_dim // 2,), "uint8"), ((rows * (self.head_dim // 32),), "float16"))]
+
+
+class Q8Cache(_Cache):
+    """One layer's keys and values in pages, 8 bits an element under a scale for each sixteen tokens of a head
+    (include/tnhip.h, tn_q8_cache); page_size and head_dim as Q4Cache's. The rows that one `append` adds to a block of
+    sixteen slots lie within sixteen rows of it, as a `PageTable`'s do."""
+
+    _kind, _struct = "q8", _lib.Q8Cache
+
+    def _planes(self):
+        rows = self.pages * self.n_kv_heads * self.page_size
+        return [Tensor(shape, dtype, "hip") for _ in "kv" for shape, dtype in (
+            ((rows * self.head_dim,), "uint8"), ((rows // 16,), "float32"))]

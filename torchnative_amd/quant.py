@@ -75,6 +75,52 @@ class QuantizedLinear:
                 f"format={self.format}, bias={self.bias is not None}, device={self.device})")
 
 
+class Int8Linear:
+    """A linear layer over a weight in 8-bit integers with a scale a channel;
+    forward quantises each token to 8 bits under a scale of its own and
+    multiplies integers (`_C.i8_linear`). float32, bfloat16 and float16
+    activations; the output is the activation's dtype unless said otherwise."""
+
+    format = "i8"
+
+    def __init__(self, weight: "_C.I8Rows", bias: Tensor | None = None):
+        self.weight, self.bias = weight, bias
+        self.out_features, self.in_features = weight.shape
+
+    @classmethod
+    def from_linear(cls, mod) -> "Int8Linear":
+        """Quantise a dense layer's weight on the device (a host weight is
+        uploaded first)."""
+        bias = mod.bias
+        return cls(_C.i8_quantize(mod.weight.to("hip")), bias.to("hip") if bias is not None else None)
+
+    def _apply(self, device):
+        """Move the codes, the scales and the bias."""
+        self.weight = self.weight.to(device)
+        if self.bias is not None:
+            self.bias = self.bias.to(device)
+        return self
+
+    to = _apply
+
+    @property
+    def device(self) -> str:
+        return self.weight.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.weight.nbytes
+
+    def forward(self, x: Tensor, out_dtype=None, work: Tensor | None = None, out: Tensor | None = None) -> Tensor:
+        return _C.i8_linear(x, self.weight, self.bias, out_dtype=out_dtype, work=work, out=out)
+
+    __call__ = forward
+
+    def __repr__(self):
+        return (f"Int8Linear(in_features={self.in_features}, out_features={self.out_features}, "
+                f"bias={self.bias is not None}, device={self.device})")
+
+
 class QuantizeReport:
     """What `quantize_` did: the layers replaced, the layers skipped with the
     reason for each, and the weight bytes before and after for the replaced
@@ -116,8 +162,8 @@ def _why(exc: Exception) -> str:
 
 
 def quantize_(model, format: str = "q8_0", predicate=None) -> QuantizeReport:
-    """Replace every `Linear` under `model` with a `QuantizedLinear`, in place,
-    and return the report. `predicate(name, module) -> bool` narrows the
+    """Replace every `Linear` under `model` with a `QuantizedLinear` (format
+    "i8": an `Int8Linear`), in place, and return the report. `predicate(name, module) -> bool` narrows the
     choice; lm_head is not treated specially (the reference leaves that
     choice to the predicate, quant/__init__.py:300-312). A layer whose
     weight the format cannot hold stays dense and is reported with the
@@ -143,14 +189,14 @@ def quantize_(model, format: str = "q8_0", predicate=None) -> QuantizeReport:
                 todo.append((parent, child_name, full, child))
     for parent, child_name, full, child in todo:
         try:
-            q = QuantizedLinear.from_linear(child, format)
+            q = Int8Linear.from_linear(child) if format == "i8" else QuantizedLinear.from_linear(child, format)
         except NotImplementedError as e:
             report.skipped.append((full, _why(e)))
             continue
         setattr(parent, child_name, q)
         report.replaced.append(full)
         report.dense_bytes += child.weight.numel * 4
-        report.quantized_bytes += _C._quantized_nbytes(q.qweight)
+        report.quantized_bytes += q.nbytes if format == "i8" else _C._quantized_nbytes(q.qweight)
     if not report.replaced and not report.skipped:
         raise ValueError(f"quantize_: {type(model).__name__} holds no Linear layer, so nothing was quantised")
     return report

@@ -27,6 +27,7 @@ DTYPES = {
     "int32": (np.int32, 4, None),
     "int64": (np.int64, 8, None),
     "uint8": (np.uint8, 1, None),
+    "int8": (np.int8, 1, None),
     "bool": (np.bool_, 1, _lib.TN_BOOL),
 }
 float32, bfloat16, float16, float64 = "float32", "bfloat16", "float16", "float64"
@@ -172,7 +173,7 @@ class Tensor:
         if dtype is None:
             dtype = {np.dtype(np.float32): "float32", np.dtype(np.float64): "float64",
                      np.dtype(np.float16): "float16", np.dtype(np.int32): "int32",
-                     np.dtype(np.int64): "int64", np.dtype(np.uint8): "uint8",
+                     np.dtype(np.int64): "int64", np.dtype(np.uint8): "uint8", np.dtype(np.int8): "int8",
                      np.dtype(np.bool_): "bool"}.get(arr.dtype)
             if dtype is None:
                 raise NotImplementedError(f"torchnative_amd: numpy dtype {arr.dtype} has no tensor dtype")
@@ -255,6 +256,49 @@ class Tensor:
         else:
             check(lib().tn_memset(self._buf.ptr, 0, self.nbytes, current_stream()))
         return self
+
+
+class Heads:
+    """Heads `first` .. `first + count - 1` of rows [m, heads, d], read and written where they lie: the q, k or v of
+    stacked projections. Stands for a tensor [m, count, d] where an operator takes rows with a stride."""
+
+    def __init__(self, rows: Tensor, first: int, count: int):
+        if rows.dim() != 3 or first < 0 or count < 0 or first + count > rows.shape[1]:
+            raise RuntimeError(f"heads {first} .. {first + count - 1} are not in rows {list(rows.shape)}")
+        self.rows, self.first = rows, int(first)
+        self.shape = (rows.shape[0], int(count), rows.shape[2])
+        self.dtype, self.device = rows.dtype, rows.device
+        self.row_stride = rows.shape[1] * rows.shape[2]
+
+    def dim(self) -> int:
+        return 3
+
+    def data_ptr(self) -> int:
+        return self.rows.data_ptr() + self.first * self.shape[2] * self.rows.element_size
+
+    def numpy(self) -> np.ndarray:
+        return self.rows.numpy()[:, self.first:self.first + self.shape[1]]
+
+
+def row_stride(t) -> int:
+    """Elements from one token's row [heads, d] to the next."""
+    return t.row_stride if isinstance(t, Heads) else t.shape[1] * t.shape[2]
+
+
+class Scratch:
+    """Scratch bytes of one owner, a buffer a device and stream (calls on a stream are ordered). An outgrown buffer
+    stays: a captured graph may point at it."""
+
+    def __init__(self):
+        self._held = {}
+
+    def get(self, nbytes: int) -> Tensor:
+        device = ctypes.c_int()
+        check(lib().tn_get_device(ctypes.byref(device)))
+        held = self._held.setdefault((device.value, current_stream()), [])
+        if not held or held[-1].nbytes < nbytes:
+            held.append(Tensor((max(nbytes, 2 * held[-1].nbytes if held else 1),), "uint8", "hip"))
+        return held[-1]
 
 
 def tensor(data, dtype: str | None = None, device="cpu") -> Tensor:
