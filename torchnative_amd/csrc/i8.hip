@@ -8,7 +8,8 @@
 #include <algorithm>
 #include <cmath>
 
-#include "paged.h"  // load4
+#include "attn_common.h"  // LdsDma, wait_vmcnt, El
+#include "paged.h"        // load4
 
 namespace tn {
 namespace {
@@ -30,18 +31,54 @@ struct Codes {
 // The scale of a row whose largest finite size is `top`.
 __device__ inline float scale_of(float top) { return top > 0.0f ? fmaxf(top * (1.0f / 127.0f), MIN_SCALE) : 0.0f; }
 
-// Four codes in a dword of four values under 1 / scale; a value that is not finite leaves 0.
-__device__ inline uint32_t codes4(const float (&v)[4], float inv) {
-    uint32_t w = 0;
+// Eight elements from i on of a row of k, zeros behind it.
+template <int DT>
+__device__ __attribute__((always_inline)) inline void load_row8(const void* x, int64_t row, int i, int k, float (&v)[8]) {
+    if (i + 8 <= k) {
+        float a[4], b[4];
+        load4<DT>(x, row + i, a);
+        load4<DT>(x, row + i + 4, b);
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const float c = fminf(fmaxf(rintf(v[j] * inv), -127.0f), 127.0f);
-        w |= ((uint32_t)(int)c & 0xffu) << (8 * j);
+        for (int j = 0; j < 4; j++) v[j] = a[j], v[4 + j] = b[j];
+        return;
     }
-    return w;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        v[j] = 0.0f;
+        if (i + j < k) {
+            if constexpr (DT == TN_F32) v[j] = static_cast<const float*>(x)[row + i + j];
+            else {
+                const uint16_t h = static_cast<const uint16_t*>(x)[row + i + j];
+                v[j] = DT == TN_BF16 ? bf16_to_f32(h) : f16_bits_hw(h);
+            }
+        }
+    }
 }
 
-// A workgroup of T threads a row.
+// Onto the largest finite size, and whether all were finite.
+__device__ inline void measure(const float (&v)[8], float& top, bool& odd) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float a = fabsf(v[j]);
+        odd |= !(a < INFINITY);
+        top = a < INFINITY ? fmaxf(top, a) : top;
+    }
+}
+
+// The eight codes of v under 1 / scale (0 for a row that is not finite).
+__device__ inline uint2 codes8(const float (&v)[8], float inv, bool odd) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float c = fminf(fmaxf(rintf(v[j] * inv), -127.0f), 127.0f);
+        w[j >> 2] |= ((uint32_t)(int)c & 0xffu) << (8 * (j & 3));
+    }
+    return odd ? make_uint2(0, 0) : make_uint2(w[0], w[1]);
+}
+
+// T threads a row, which hold up to eight times HOLD elements each and read what is past
+// these again. Bound by memory where rows are many, by a launch where few.
+constexpr int HOLD = 4;
 template <int DT, int T>
 __global__ __launch_bounds__(256) void k_i8_rows(const void* __restrict__ x, int m, int k, int8_t* __restrict__ codes,
                                                  float* __restrict__ scales) {
@@ -53,34 +90,16 @@ __global__ __launch_bounds__(256) void k_i8_rows(const void* __restrict__ x, int
     const bool on = row < m;
     const int64_t at = (on ? row : 0) * k;
     const int pitch = (int)pitch_of(k);
-    float top = 0.0f;
-    int odd = 0;
-    auto take = [&](float v) {
-        const float a = fabsf(v);
-        if (a < INFINITY) top = fmaxf(top, a);
-        else odd = 1;
-    };
-    auto load = [&](int i, float (&v)[4]) {  // elements i .. i + 3, zeros behind the row
-        if (i + 4 <= k) load4<DT>(x, at + i, v);
-        else {
-            float u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int j = 0; j < 4; j++)
-                if (i + j < k) {
-                    if constexpr (DT == TN_F32) u[j] = static_cast<const float*>(x)[at + i + j];
-                    else {
-                        const uint16_t h = static_cast<const uint16_t*>(x)[at + i + j];
-                        u[j] = DT == TN_BF16 ? bf16_to_f32(h) : f16_bits_hw(h);
-                    }
-                }
+    float v[HOLD][8], top = 0.0f;
+    bool odd = false;
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = u[j];
-        }
-    };
-    for (int i = 4 * tid; i < k; i += 4 * T) {
-        float v[4];
-        load(i, v);
+    for (int h = 0; h < HOLD; h++) load_row8<DT>(x, at, 8 * (h * T + tid), k, v[h]);
 #pragma unroll
-        for (int j = 0; j < 4; j++) take(v[j]);
+    for (int h = 0; h < HOLD; h++) measure(v[h], top, odd);
+    for (int i = 8 * (HOLD * T + tid); i < k; i += 8 * T) {
+        float u[8];
+        load_row8<DT>(x, at, i, k, u);
+        measure(u, top, odd);
     }
     top = xor32_max(xor16_max(row16_max(top)));
     odd = __any(odd);
@@ -91,13 +110,18 @@ __global__ __launch_bounds__(256) void k_i8_rows(const void* __restrict__ x, int
         odd = bad[0] | bad[1] | bad[2] | bad[3];
     }
     if (!on) return;
-    const float s = scale_of(top), inv = odd || s == 0.0f ? 0.0f : 1.0f / s;
+    const float s = scale_of(top), inv = s > 0.0f ? 1.0f / s : 0.0f;
     if (tid == 0) scales[row] = odd ? NAN : s;
-    uint32_t* out = reinterpret_cast<uint32_t*>(codes + row * pitch);
-    for (int i = 4 * tid; i < pitch; i += 4 * T) {
-        float v[4];
-        load(i, v);
-        out[i / 4] = odd ? 0u : codes4(v, inv);
+    int8_t* out = codes + row * pitch;
+#pragma unroll
+    for (int h = 0; h < HOLD; h++) {
+        const int i = 8 * (h * T + tid);
+        if (i < pitch) *reinterpret_cast<uint2*>(out + i) = codes8(v[h], inv, odd);
+    }
+    for (int i = 8 * (HOLD * T + tid); i < pitch; i += 8 * T) {
+        float u[8];
+        load_row8<DT>(x, at, i, k, u);
+        *reinterpret_cast<uint2*>(out + i) = codes8(u, inv, odd);
     }
 }
 
@@ -108,13 +132,7 @@ struct MmArgs {
     int m, n, pitch, y_dtype;
 };
 
-__device__ inline void put(const MmArgs& a, int row, int col, int sum) {
-    float v = ((float)sum * a.w.s[col]) * a.a.s[row];
-    if (a.bias) v = v + a.bias[col];
-    const int64_t i = (int64_t)row * a.n + col;
-    if (a.y_dtype == TN_F32) static_cast<float*>(a.y)[i] = v;
-    else static_cast<uint16_t*>(a.y)[i] = a.y_dtype == TN_BF16 ? bf16_out(v) : f16_out(v);
-}
+typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 __device__ __attribute__((always_inline)) inline i32x4 mfma_i8(i32x4 a, i32x4 b, i32x4 c) {
 #if __HIP_DEVICE_COMPILE__
@@ -124,33 +142,513 @@ __device__ __attribute__((always_inline)) inline i32x4 mfma_i8(i32x4 a, i32x4 b,
     return c;
 #endif
 }
-
-// A wave a 16 x 16 tile, its operands straight from memory.
-__global__ __launch_bounds__(256) void k_i8_tile(const MmArgs a, int mt, int64_t tiles) {
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int64_t tile = (int64_t)wg_number() * 4 + (threadIdx.x >> 6);
-    if (tile >= tiles) return;
-    const int m0 = (int)(tile % mt) * 16, n0 = (int)(tile / mt) * 16;
-    const int8_t* pa = a.a.c + (int64_t)min(m0 + c, a.m - 1) * a.pitch + 16 * g;
-    const int8_t* pw = a.w.c + (int64_t)min(n0 + c, a.n - 1) * a.pitch + 16 * g;
-    i32x4 acc = {0, 0, 0, 0};
-    for (int k = 0; k < a.pitch; k += 64)
-        acc = mfma_i8(*reinterpret_cast<const i32x4*>(pa + k), *reinterpret_cast<const i32x4*>(pw + k), acc);
-#pragma unroll
-    for (int r = 0; r < 4; r++)
-        if (m0 + 4 * g + r < a.m && n0 + c < a.n) put(a, m0 + 4 * g + r, n0 + c, acc[r]);
+__device__ __attribute__((always_inline)) inline i32x16 mfma_i8(i32x4 a, i32x4 b, i32x16 c) {
+#if __HIP_DEVICE_COMPILE__
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+#else
+    (void)a, (void)b;
+    return c;
+#endif
 }
 
-tn_status matmul(hipStream_t st, const MmArgs& a) {
-    const int64_t mt = cdiv(a.m, 16), tiles = mt * cdiv(a.n, 16);
-    hipLaunchKernelGGL(k_i8_tile, wg_grid(cdiv(tiles, 4)), dim3(256), 0, st, a, (int)mt, tiles);
+// The epilogue of one sum.
+__device__ inline float finish(int sum, float sw, float sx, bool biased, float bias) {
+    const float v = ((float)sum * sw) * sx;
+    return biased ? v + bias : v;
+}
+
+// A lane of the lower half gives b and takes the upper half's a, which gives a and takes
+// b: x, y are then the lower lanes' a of both halves (lower half) and the b of both (upper).
+template <class V>
+__device__ __attribute__((always_inline)) inline void trade(V a, V b, V& x, V& y) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false,
+                                                    false);
+    x = __builtin_bit_cast(V, (uint32_t)p[0]);
+    y = __builtin_bit_cast(V, (uint32_t)p[1]);
+}
+
+// Up to eight consecutive elements, at any element.
+__device__ __attribute__((always_inline)) inline void put8(float* to, const float (&y)[8], int count) {
+    typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+    if (count >= 8) {
+        *reinterpret_cast<v4*>(to) = (v4){y[0], y[1], y[2], y[3]};
+        *reinterpret_cast<v4*>(to + 4) = (v4){y[4], y[5], y[6], y[7]};
+        return;
+    }
+#pragma unroll
+    for (int u = 0; u < 7; u++)
+        if (u < count) to[u] = y[u];
+}
+__device__ __attribute__((always_inline)) inline void put8(uint16_t* to, const uint32_t (&y)[4], int count) {
+    typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
+    if (count >= 8) {
+        *reinterpret_cast<v4*>(to) = (v4){y[0], y[1], y[2], y[3]};
+        return;
+    }
+#pragma unroll
+    for (int u = 0; u < 7; u++)
+        if (u < count) to[u] = (uint16_t)(y[u / 2] >> (16 * (u & 1)));
+}
+
+// ---- many rows -----------------------------------------------------------------------
+//
+// A workgroup of WN x WM waves, each RT x CT tiles of 32 channels by 32 tokens (the
+// weights are the product's rows, so that a lane's sums are runs of four channels of a
+// token). K goes KB bytes a stage through a ring of NS stages in LDS, filled by loads
+// that go straight there (KG groups of waves: a stage each has its own KB bytes, and the
+// groups' sums are added up at the end); a row's 16-byte chunks lie permuted by its number, so that
+// sixteen rows' chunks cover every bank. A step of 32 bytes of K is read while the step
+// before it is multiplied; one barrier a stage.
+template <int WN, int WM, int RT, int CT, int KB, int NS, int KG = 1>
+struct Tile {
+    static constexpr int W = WN * WM, BN = 32 * RT * WN, BM = 32 * CT * WM;  // waves of a group
+    static constexpr int LW = BN * KB / 1024 / W, LX = BM * KB / 1024 / W;  // loads of a wave, a stage
+    static_assert(LW * W * 1024 == BN * KB && LX * W * 1024 == BM * KB, "whole loads");
+    static constexpr int PER = LW + LX, OX = BN * KB, PART = (BN + BM) * KB, STAGE = KG * PART, STEPS = KB / 32;
+    static_assert(KG == 1 || NS * STAGE >= (KG - 1) * W * RT * CT * 4096, "room for the groups' sums");
+    static constexpr int SIDE = BN > BM ? BN : BM;
+    static_assert((NS - 2) * PER < 64, "loads in flight");
+};
+
+// The tile of tokens from m0 on and channels from n0 on. ring: NS * STAGE bytes; side: the
+// weights' scales, the bias, the tokens' scales, of SIDE floats each.
+template <int WN, int WM, int RT, int CT, int KB, int NS, int KG = 1>
+__device__ __attribute__((always_inline)) inline void gemm_tile(const MmArgs& a, uint8_t* ring, float* side, int m0,
+                                                                int n0) {
+    using T = Tile<WN, WM, RT, CT, KB, NS, KG>;
+    constexpr int W = T::W, CH = KB / 16, RPL = 1024 / KB;  // chunks of a row, rows of a load
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) % W, group = __builtin_amdgcn_readfirstlane(tid >> 6) / W;
+    float *const side_w = side, *const side_b = side + T::SIDE, *const side_x = side + 2 * T::SIDE;
+    const int pitch = a.pitch;
+    const LdsDma rw(a.w.c + (int64_t)n0 * pitch, (uint32_t)(min(T::BN, a.n - n0) * pitch));
+    const LdsDma rx(a.a.c + (int64_t)m0 * pitch, (uint32_t)(min(T::BM, a.m - m0) * pitch));
+    // chunk c of row r lies at place c ^ swz(r)
+    auto swz = [](int r) { return KB == 128 ? (r >> 1) & 7 : (r >> 2) & 3; };
+    uint32_t vw[T::LW], vx[T::LX];
+    int last[T::LW > T::LX ? T::LW : T::LX];  // this lane's chunk's first byte within a stage
+#pragma unroll
+    for (int j = 0; j < (T::LW > T::LX ? T::LW : T::LX); j++) {
+        const int r = (j * W + wave) * RPL + lane / CH, c = (lane % CH) ^ swz(r);
+        if (j < T::LW) vw[j] = (uint32_t)(r * pitch + c * 16);
+        if (j < T::LX) vx[j] = (uint32_t)(r * pitch + c * 16);
+        last[j] = c * 16;
+    }
+    auto issue = [&](int st, int slot) __attribute__((always_inline)) {
+        uint8_t* const s = ring + slot * T::STAGE + group * T::PART;
+        const int k = (st * KG + group) * KB;
+        const bool cut = k + KB > pitch;  // rows end within the last stage
+#pragma unroll
+        for (int j = 0; j < T::LW; j++)
+            rw.load16(cut && k + last[j] >= pitch ? BUF_OOB : vw[j] + (uint32_t)k, s + (j * W + wave) * 1024);
+#pragma unroll
+        for (int j = 0; j < T::LX; j++)
+            rx.load16(cut && k + last[j] >= pitch ? BUF_OOB : vx[j] + (uint32_t)k, s + T::OX + (j * W + wave) * 1024);
+    };
+    const int r32 = lane & 31, hh = lane >> 5, wn = wave / WM * 32 * RT, wm = wave % WM * 32 * CT;
+    const uint32_t base = (uint32_t)(hh ^ swz(r32)) * 16;
+    uint32_t pw = (uint32_t)((wn + r32) * KB), px = (uint32_t)(T::OX + (wm + r32) * KB);
+    struct Step {
+        i32x4 w[RT], x[CT];
+    } f[2];
+    auto read = [&](const uint8_t* s, int step, Step& y) __attribute__((always_inline)) {
+        const uint32_t o = base ^ (uint32_t)(32 * step);
+#pragma unroll
+        for (int i = 0; i < RT; i++) y.w[i] = *reinterpret_cast<const i32x4*>(s + pw + o + i * 32 * KB);
+#pragma unroll
+        for (int j = 0; j < CT; j++) y.x[j] = *reinterpret_cast<const i32x4*>(s + px + o + j * 32 * KB);
+    };
+    i32x16 acc[RT][CT];
+#pragma unroll
+    for (int i = 0; i < RT; i++)
+#pragma unroll
+        for (int j = 0; j < CT; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
+    auto multiply = [&](const Step& y) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int j = 0; j < CT; j++) acc[i][j] = mfma_i8(y.w[i], y.x[j], acc[i][j]);
+    };
+    const int nst = (pitch + KG * KB - 1) / (KG * KB);
+    // stage st has landed for every wave, and every wave has read the stages before it
+    auto landed = [&](int st) __attribute__((always_inline)) {
+        if (st + NS - 2 < nst) wait_vmcnt<(NS - 2) * T::PER>();
+        else wait_vmcnt<0>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    for (int st = 0; st < min(NS, nst); st++) issue(st, st);
+    for (int i = tid; i < T::BN; i += 64 * W * KG) {
+        side_w[i] = n0 + i < a.n ? a.w.s[n0 + i] : 0.0f;
+        side_b[i] = a.bias && n0 + i < a.n ? a.bias[n0 + i] : 0.0f;
+    }
+    for (int i = tid; i < T::BM; i += 64 * W * KG) side_x[i] = m0 + i < a.m ? a.a.s[m0 + i] : 0.0f;
+    // (the last of these stages is one more than the loop has in flight)
+    if (nst >= NS) wait_vmcnt<(NS - 1) * T::PER>();
+    else wait_vmcnt<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(ring + group * T::PART, 0, f[0]);
+    int slot = 0;
+    static_assert(T::STEPS % 2 == 0, "two sets of operands in turn");
+    auto stage = [&](int st, bool more) __attribute__((always_inline)) {
+        const uint8_t* const s = ring + slot * T::STAGE + group * T::PART;
+        const int next = slot + 1 < NS ? slot + 1 : 0;
+#pragma unroll
+        for (int k = 0; k < T::STEPS; k++) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (k + 1 < T::STEPS) read(s, k + 1, f[(k + 1) & 1]);
+            else if (more) {
+                landed(st + 1);
+                if (st + NS < nst) issue(st + NS, slot);
+                read(ring + next * T::STAGE + group * T::PART, 0, f[(k + 1) & 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(f[k & 1]);
+        }
+        slot = next;
+    };
+    for (int st = 0; st + 1 < nst; st++) stage(st, true);
+    stage(nst - 1, false);
+
+    if constexpr (KG > 1) {  // the groups' sums, added up by the first
+        i32x4* const sums = reinterpret_cast<i32x4*>(ring);
+        __syncthreads();
+        if (group) {
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int j = 0; j < CT; j++)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        sums[((((group - 1) * W + wave) * RT + i) * CT + j) * 256 + e * 16 + lane] =
+                            (i32x4){acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+        }
+        __syncthreads();
+        if (group) return;
+#pragma unroll
+        for (int o = 0; o < KG - 1; o++)
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int j = 0; j < CT; j++)
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const i32x4 v = sums[(((o * W + wave) * RT + i) * CT + j) * 256 + e * 16 + lane];
+#pragma unroll
+                        for (int u = 0; u < 4; u++) acc[i][j][e + u] += v[u];
+                    }
+    }
+
+    // A lane's sums of a tile are channels 8 u + 4 hh .. + 3 (u = 0 .. 3) of its token: its
+    // half trades with the other, so that it has eight in a row, twice.
+    const bool whole = n0 + T::BN <= a.n;  // uniform
+    auto leave = [&](auto type) __attribute__((always_inline)) {
+        constexpr int DT = decltype(type)::value;
+#pragma unroll
+        for (int j = 0; j < CT; j++) {
+            const int m = m0 + wm + 32 * j + r32;
+            const float sx = side_x[wm + 32 * j + r32];
+            const int64_t row = (int64_t)m * a.n;
+#pragma unroll
+            for (int i = 0; i < RT; i++) {
+                float v[16];
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const int n = wn + 32 * i + 2 * e + 4 * hh;
+                    const float4 sw = *reinterpret_cast<const float4*>(side_w + n);
+                    const float4 bias = *reinterpret_cast<const float4*>(side_b + n);
+                    const float s4[4] = {sw.x, sw.y, sw.z, sw.w}, b4[4] = {bias.x, bias.y, bias.z, bias.w};
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+                        v[e + u] = finish(acc[i][j][e + u], s4[u], sx, a.bias != nullptr, b4[u]);
+                }
+#pragma unroll
+                for (int p = 0; p < 2; p++) {  // channels 16 p + 8 hh .. + 7
+                    const int n = n0 + wn + 32 * i + 16 * p + 8 * hh;
+                    if constexpr (DT == TN_F32) {
+                        float y[8];
+#pragma unroll
+                        for (int u = 0; u < 4; u++) trade(v[8 * p + u], v[8 * p + 4 + u], y[u], y[4 + u]);
+                        if (m < a.m) put8(static_cast<float*>(a.y) + row + n, y, whole ? 8 : a.n - n);
+                    } else {
+                        using E = El<DT == TN_F16>;
+                        uint32_t y[4];
+#pragma unroll
+                        for (int u = 0; u < 2; u++)
+                            trade(E::pack_out(v[8 * p + 2 * u], v[8 * p + 2 * u + 1]),
+                                  E::pack_out(v[8 * p + 4 + 2 * u], v[8 * p + 5 + 2 * u]), y[u], y[2 + u]);
+                        if (m < a.m) put8(static_cast<uint16_t*>(a.y) + row + n, y, whole ? 8 : a.n - n);
+                    }
+                }
+            }
+        }
+    };
+    if (a.y_dtype == TN_F32) leave(std::integral_constant<int, TN_F32>{});
+    else if (a.y_dtype == TN_BF16) leave(std::integral_constant<int, TN_BF16>{});
+    else leave(std::integral_constant<int, TN_F16>{});
+}
+
+// Tile t of ntl x mtl: consecutive ones of a die's share; there eight token tiles at a time,
+// then the next channels, so that what a die's tiles read stays in its cache.
+struct Place {
+    int m, n;
+};
+__device__ inline int of_die(int id, int count) {
+    const int q = count / 8, rem = count % 8, die = id % 8;
+    return die * q + min(die, rem) + id / 8;
+}
+__device__ inline Place place_of(int t, int ntl, int mtl) {
+    constexpr int GM = 8;
+    const int gsize = GM * ntl, group = t / gsize, gm = min(GM, mtl - group * GM), in = t - group * gsize;
+    return {group * GM + in % gm, in / gm};
+}
+
+template <int WN, int WM, int RT, int CT, int KB, int NS, int KG = 1>
+__global__ __launch_bounds__(64 * WN * WM * KG, 2) void k_i8_gemm(const MmArgs a, int ntl, int mtl, int nwg) {
+    using T = Tile<WN, WM, RT, CT, KB, NS, KG>;
+    __shared__ __align__(16) uint8_t ring[NS * T::STAGE];
+    __shared__ __align__(16) float side[3 * T::SIDE];
+    const int id = wg_number();
+    if (id >= nwg) return;
+    const Place p = place_of(of_die(id, nwg), ntl, mtl);
+    gemm_tile<WN, WM, RT, CT, KB, NS, KG>(a, ring, side, p.m * T::BM, p.n * T::BN);
+}
+
+// Tiles of 256 x 256, one a compute unit; the last `halved` of them as two of half the
+// tokens, so that a round that would leave half of the units idle takes about half as long.
+__global__ __launch_bounds__(512, 2) void k_i8_large(const MmArgs a, int ntl, int mtl, int halved) {
+    using T = Tile<2, 4, 4, 2, 128, 2>;
+    using H = Tile<2, 4, 4, 1, 128, 2>;
+    __shared__ __align__(16) uint8_t ring[2 * T::STAGE];
+    __shared__ __align__(16) float side[3 * T::SIDE];
+    const int id = wg_number(), whole = ntl * mtl - halved;
+    if (id < whole) {
+        const Place p = place_of(of_die(id, whole), ntl, mtl);
+        gemm_tile<2, 4, 4, 2, 128, 2>(a, ring, side, p.m * T::BM, p.n * T::BN);
+    } else {
+        const int x = id - whole;
+        if (x >= 2 * halved) return;
+        const int t = of_die(x, 2 * halved);
+        const Place p = place_of(whole + t / 2, ntl, mtl);
+        const int m0 = p.m * T::BM + t % 2 * H::BM;
+        if (m0 < a.m) gemm_tile<2, 4, 4, 1, 128, 2>(a, ring, side, m0, p.n * T::BN);
+    }
+}
+
+template <int WN, int WM, int RT, int CT, int KB, int NS, int KG = 1>
+tn_status gemm_launch(hipStream_t st, const MmArgs& a) {
+    using T = Tile<WN, WM, RT, CT, KB, NS, KG>;
+    const int64_t ntl = cdiv(a.n, T::BN), mtl = cdiv(a.m, T::BM);
+    if (ntl * mtl > INT32_MAX) return fail(TN_EVALUE, "i8_matmul: shape too large");
+    hipLaunchKernelGGL((k_i8_gemm<WN, WM, RT, CT, KB, NS, KG>), wg_grid(ntl * mtl), dim3(64 * T::W * KG), 0, st, a, (int)ntl,
+                       (int)mtl, (int)(ntl * mtl));
     TN_LAUNCHED();
     return TN_OK;
 }
 
+tn_status large_launch(hipStream_t st, const MmArgs& a) {
+    const int64_t ntl = cdiv(a.n, 256), mtl = cdiv(a.m, 256), tiles = ntl * mtl;
+    if (tiles + 256 > INT32_MAX) return fail(TN_EVALUE, "i8_matmul: shape too large");
+    const int64_t left = tiles % 256, halved = left <= 128 ? left : 0;
+    hipLaunchKernelGGL(k_i8_large, wg_grid(tiles + halved), dim3(512), 0, st, a, (int)ntl, (int)mtl, (int)halved);
+    TN_LAUNCHED();
+    return TN_OK;
+}
+
+// ---- few rows ------------------------------------------------------------------------
+//
+// A workgroup takes 16 channels of up to 16 tokens; its eight waves an eighth of K each,
+// operands straight from memory, eight steps of 64 at a time, and add their sums up in
+// LDS. Bound by the weights' bytes and, over few channels, by a wave's loads one behind
+// the other.
+constexpr int FEW_W = 8, FEW_U = 8;
+
+struct FewSums {
+    i32x4 part[FEW_W][64];
+};
+
+// The waves' sums (channels 4 g .. 4 g + 3 of token c) to the outputs of tokens m0 on.
+__device__ inline void few_out(const MmArgs& a, FewSums& s, const i32x4& acc, int m0, int n0, const float* sx) {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
+    s.part[wave][lane] = acc;
+    __syncthreads();
+    if (wave) return;
+    i32x4 t = s.part[0][lane];
+#pragma unroll
+    for (int i = 1; i < FEW_W; i++) t += s.part[i][lane];
+    const int m = m0 + c, n = n0 + 4 * g;
+    if (m >= a.m) return;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+        if (n + u >= a.n) break;
+        const float v = finish(t[u], a.w.s[n + u], sx[c], a.bias != nullptr, a.bias ? a.bias[n + u] : 0.0f);
+        const int64_t i = (int64_t)m * a.n + n + u;
+        if (a.y_dtype == TN_F32) static_cast<float*>(a.y)[i] = v;
+        else static_cast<uint16_t*>(a.y)[i] = a.y_dtype == TN_BF16 ? bf16_out(v) : f16_out(v);
+    }
+}
+
+// acc += the products of N steps from step k on.
+template <int N>
+__device__ __attribute__((always_inline)) inline void few_steps(const int8_t* px, const int8_t* pw, int k, i32x4& acc) {
+    i32x4 x[N], w[N];
+#pragma unroll
+    for (int u = 0; u < N; u++) w[u] = *reinterpret_cast<const i32x4*>(pw + 64 * (k + u));
+#pragma unroll
+    for (int u = 0; u < N; u++) x[u] = *reinterpret_cast<const i32x4*>(px + 64 * (k + u));
+#pragma unroll
+    for (int u = 0; u < N; u++) acc = mfma_i8(w[u], x[u], acc);
+}
+
+__global__ __launch_bounds__(64 * FEW_W) void k_i8_few(const MmArgs a, int nwg) {
+    __shared__ FewSums sums;
+    __shared__ float sx[16];
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int id = wg_number();
+    if (id >= nwg) return;
+    const int mtl = (a.m + 15) / 16, m0 = id % mtl * 16, n0 = id / mtl * 16;
+    if (threadIdx.x < 16) sx[threadIdx.x] = a.a.s[min(m0 + (int)threadIdx.x, a.m - 1)];
+    const int8_t* px = a.a.c + (int64_t)min(m0 + c, a.m - 1) * a.pitch + 16 * g;
+    const int8_t* pw = a.w.c + (int64_t)min(n0 + c, a.n - 1) * a.pitch + 16 * g;
+    i32x4 acc = {0, 0, 0, 0};
+    const int steps = a.pitch / 64, hi = (int)((int64_t)steps * (wave + 1) / FEW_W);
+    int k = (int)((int64_t)steps * wave / FEW_W);
+    for (; k + FEW_U <= hi; k += FEW_U) few_steps<FEW_U>(px, pw, k, acc);
+    for (; k < hi; k++) few_steps<1>(px, pw, k, acc);
+    few_out(a, sums, acc, m0, n0, sx);
+}
+
+// The same on rows as they are, up to FUSED_M of them: every workgroup quantises them into
+// LDS, its first weights on their way meanwhile. Saves the prepass's launch.
+constexpr int FUSED_M = 4;
+constexpr int64_t FUSED_BYTES = 32 << 10;  // of codes
+
+template <int DT>
+__global__ __launch_bounds__(64 * FEW_W) void k_i8_fused(const MmArgs a, const void* __restrict__ x, int k_len) {
+    __shared__ __align__(16) int8_t codes[FUSED_BYTES];
+    __shared__ FewSums sums;
+    __shared__ float sx[16], red[FEW_W];
+    __shared__ int bad[FEW_W];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n0 = blockIdx.x * 16;
+    const int8_t* pw = a.w.c + (int64_t)min(n0 + c, a.n - 1) * a.pitch + 16 * g;
+    const int steps = a.pitch / 64, hi = (int)((int64_t)steps * (wave + 1) / FEW_W);
+    int k = (int)((int64_t)steps * wave / FEW_W);
+    i32x4 w[FEW_U];
+#pragma unroll
+    for (int u = 0; u < FEW_U; u++) w[u] = *reinterpret_cast<const i32x4*>(pw + 64 * min(k + u, steps - 1));
+    for (int r = 0; r < a.m; r++) {
+        const int64_t at = (int64_t)r * k_len;
+        float v[8], top = 0.0f;
+        bool odd = false;
+        load_row8<DT>(x, at, 8 * tid, k_len, v);
+        measure(v, top, odd);
+        for (int i = 8 * (64 * FEW_W + tid); i < k_len; i += 8 * 64 * FEW_W) {
+            float y[8];
+            load_row8<DT>(x, at, i, k_len, y);
+            measure(y, top, odd);
+        }
+        top = xor32_max(xor16_max(row16_max(top)));
+        odd = __any(odd);
+        if (lane == 0) red[wave] = top, bad[wave] = odd;
+        __syncthreads();
+        odd = false;
+#pragma unroll
+        for (int i = 0; i < FEW_W; i++) top = fmaxf(top, red[i]), odd |= bad[i] != 0;
+        const float s = scale_of(top), inv = s > 0.0f ? 1.0f / s : 0.0f;
+        if (tid == 0) sx[r] = odd ? NAN : s;
+        int8_t* out = codes + r * a.pitch;
+        if (8 * tid < a.pitch) *reinterpret_cast<uint2*>(out + 8 * tid) = codes8(v, inv, odd);
+        for (int i = 8 * (64 * FEW_W + tid); i < a.pitch; i += 8 * 64 * FEW_W) {
+            float y[8];
+            load_row8<DT>(x, at, i, k_len, y);
+            *reinterpret_cast<uint2*>(out + i) = codes8(y, inv, odd);
+        }
+        __syncthreads();
+    }
+    const int8_t* px = codes + min(c, a.m - 1) * a.pitch + 16 * g;
+    i32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < FEW_U; u++)
+        if (k + u < hi) acc = mfma_i8(w[u], *reinterpret_cast<const i32x4*>(px + 64 * (k + u)), acc);
+    k += FEW_U;
+    for (; k + FEW_U <= hi; k += FEW_U) few_steps<FEW_U>(px, pw, k, acc);
+    for (; k < hi; k++) few_steps<1>(px, pw, k, acc);
+    few_out(a, sums, acc, 0, n0, sx);
+}
+
+bool fused(int64_t m, int64_t k) { return m <= FUSED_M && m * pitch_of(k) <= FUSED_BYTES; }
+
+tn_status few_launch(hipStream_t st, const MmArgs& a) {
+    const int64_t nwg = cdiv(a.m, 16) * cdiv(a.n, 16);
+    if (nwg > INT32_MAX) return fail(TN_EVALUE, "i8_matmul: shape too large");
+    hipLaunchKernelGGL(k_i8_few, wg_grid(nwg), dim3(64 * FEW_W), 0, st, a, (int)nwg);
+    TN_LAUNCHED();
+    return TN_OK;
+}
+
+tn_status fused_launch(hipStream_t st, const MmArgs& a, const void* x, int dtype, int64_t k) {
+    const dim3 grid((unsigned)cdiv(a.n, 16)), block(64 * FEW_W);  // n < 2^24: fewer than 2^30 threads
+    if (dtype == TN_F32) hipLaunchKernelGGL(k_i8_fused<TN_F32>, grid, block, 0, st, a, x, (int)k);
+    else if (dtype == TN_BF16) hipLaunchKernelGGL(k_i8_fused<TN_BF16>, grid, block, 0, st, a, x, (int)k);
+    else hipLaunchKernelGGL(k_i8_fused<TN_F16>, grid, block, 0, st, a, x, (int)k);
+    TN_LAUNCHED();
+    return TN_OK;
+}
+
+// The tile shapes, by what a call takes in rounds of the workgroups that the 256 units
+// hold: us of a round over K = 4096 with one and with two workgroups a unit (it holds one
+// where both are the same), and of a tile's start and end, both fitted to measurements of
+// 1 to 4096 tokens on six weights. (us at the best shape, and at its neighbours; [m, 4096]
+// x [14336, 4096] where not stated: m 32, 64 x 32 13.8, 64 x 64 15.3; m 64, 64 x 64 of two
+// groups 15.2, 64 x 128 18.2; m 128, 64 x 128 of two groups 19.3, 64 x 64 22.9; m 512, 128 x
+// 128 40.8, 64 x 128 53, 256 x 256 45; m 1024, 256 x 256 73, 128 x 128 79. [64, 4096] x
+// [4096, 4096]: 64 x 32 7.9, 64 x 64 9.3, of one group 11.4; [256, 14336] x [4096, 14336]: 64
+// x 64 34.7, 64 x 128 47.8, 128 x 128 97.)
+struct Shape {
+    int bn, bm;
+    float one, two, ends;
+    tn_status (*launch)(hipStream_t, const MmArgs&);
+};
+const Shape SHAPES[] = {
+    {64, 32, 5.3f, 5.3f, 0.6f, gemm_launch<2, 1, 1, 1, 128, 3, 4>},
+    {64, 64, 7.2f, 7.2f, 0.7f, gemm_launch<2, 2, 1, 1, 128, 3, 2>},
+    {64, 64, 9.5f, 14.0f, 0.7f, gemm_launch<2, 2, 1, 1, 128, 4>},
+    {64, 128, 11.8f, 11.8f, 1.2f, gemm_launch<2, 2, 1, 2, 128, 3, 2>},
+    {64, 128, 13.5f, 23.0f, 1.0f, gemm_launch<2, 2, 1, 2, 128, 3>},
+    {128, 128, 24.0f, 38.0f, 2.3f, gemm_launch<2, 2, 2, 2, 128, 2>},
+    {256, 256, 36.5f, 66.0f, 4.5f, large_launch},
+};
+
+tn_status matmul(hipStream_t st, const MmArgs& a) {
+    // (us, here and in tiles of 64 x 32: 16 tokens of [4096, 4096], 7.1 and 7.5, of [4096,
+    // 14336], 17.9 and 24.9, of [5000, 1536], 6.0 and 5.4, of [14336, 4096], 19.8 and 13.5)
+    if (a.m <= 16 && a.n <= 8192) return few_launch(st, a);
+    const Shape* best = SHAPES;
+    double least = INFINITY;
+    for (const Shape& s : SHAPES) {
+        const int64_t tiles = cdiv(a.n, s.bn) * cdiv(a.m, s.bm);
+        const bool large = s.launch == large_launch;  // (its tiles of half the tokens: the short round)
+        const int64_t slots = s.one == s.two || large ? 256 : 512, rest = tiles % slots;
+        const int64_t rounds = cdiv(tiles, slots);
+        double us = (double)(tiles / slots) * s.two;
+        if (rest) us += rest <= (large ? 128 : 256) ? s.one : s.two;
+        us = us * a.pitch / 4096 + (double)rounds * s.ends;
+        if (us < least) least = us, best = &s;
+    }
+    return best->launch(st, a);
+}
+
 template <int DT>
 void rows_launch(hipStream_t st, const void* x, int m, int k, int8_t* codes, float* scales) {
-    if (k <= 1024)
+    if (k <= 64 * 8 * HOLD)
         hipLaunchKernelGGL((k_i8_rows<DT, 64>), dim3((unsigned)cdiv(m, 4)), dim3(256), 0, st, x, m, k, codes, scales);
     else hipLaunchKernelGGL((k_i8_rows<DT, 256>), dim3((unsigned)m), dim3(256), 0, st, x, m, k, codes, scales);
 }
@@ -178,7 +676,7 @@ tn_status size_check(const char* op, int64_t m, int64_t k, int64_t n) {
     return TN_OK;
 }
 
-int64_t work_bytes(int64_t m, int64_t k) { return m * pitch_of(k) + (m * 4 + 15) / 16 * 16; }
+int64_t work_bytes(int64_t m, int64_t k) { return fused(m, k) ? 0 : m * pitch_of(k) + (m * 4 + 15) / 16 * 16; }
 
 }  // namespace
 }  // namespace tn
@@ -229,7 +727,11 @@ tn_status tn_i8_linear(void* stream, const void* x, int x_dtype, int64_t m, int6
         return fail(TN_EVALUE, "i8_linear: work holds " + std::to_string(work_size) + " bytes, this call needs " +
                                    std::to_string(need));
     if (!x || !w || !w_scales || !y || (need && !work)) return fail(TN_EVALUE, "i8_linear: null pointer");
-    if (unaligned(w) || unaligned(work)) return fail(TN_EVALUE, "i8_linear: codes and work must be 16-byte aligned");
+    if (unaligned(w) || (need && unaligned(work))) return fail(TN_EVALUE, "i8_linear: codes and work must be 16-byte aligned");
+    if (fused(m, k)) {
+        const MmArgs p{{nullptr, nullptr}, {w, w_scales}, bias, y, (int)m, (int)n, (int)pitch_of(k), y_dtype};
+        return fused_launch((hipStream_t)stream, p, x, x_dtype, k);
+    }
     int8_t* codes = static_cast<int8_t*>(work);
     float* scales = reinterpret_cast<float*>(codes + m * pitch_of(k));
     TN_TRY(quantize((hipStream_t)stream, x, x_dtype, m, k, codes, scales));
