@@ -536,8 +536,8 @@ tn_status tn_kv_read_q8(void* stream, const tn_q8_cache* cache, const int32_t* s
  * Sums, maxima and the softmax are f32. Codes enter the matrix products exactly;
  * a query is one f16 under a power of two of its own (two f16 parts for f32
  * rows), probabilities, times their values' block scale over the largest such
- * scale met, one f16 for bf16 rows and two for others; the output is rounded
- * once. Probabilities times scales are held to 2^-30 of the row's largest
+ * scale met, one f16 for bf16 rows, two for f32 rows, one of them for f16 rows
+ * (which, goes by the call's size); the output is rounded once. Probabilities times scales are held to 2^-30 of the row's largest
  * probability times the largest scale of values (lse counts them all).
  * Scales are taken as finite and not negative.
  * `work`: as there, tn_sdpa_paged_q8_work_floats() floats. */

@@ -314,6 +314,12 @@ __device__ __attribute__((always_inline)) inline void gemm_tile(const MmArgs& a,
     };
     for (int st = 0; st + 1 < nst; st++) stage(st, true);
     stage(nst - 1, false);
+    // the last products' wait states, whatever their first reader is
+    __builtin_amdgcn_sched_barrier(0);
+#if __HIP_DEVICE_COMPILE__
+    asm volatile("s_nop 15\n\ts_nop 1");
+#endif
+    __builtin_amdgcn_sched_barrier(0);
 
     if constexpr (KG > 1) {  // the groups' sums, added up by the first
         i32x4* const sums = reinterpret_cast<i32x4*>(ring);

@@ -54,6 +54,13 @@ TN_INLINE float vref_for(float scale) {
     const uint32_t e = (__builtin_bit_cast(uint32_t, scale) >> 23) & 0xffu;
     return __builtin_bit_cast(float, min(e + 1u, 253u) << 23);
 }
+// Over the two or four lanes of a quad.
+template <int N>
+TN_INLINE float quad_max(float v) {
+    v = fmaxf(v, dpp_f<0xB1>(v));
+    if constexpr (N == 4) v = fmaxf(v, dpp_f<0x4E>(v));
+    return v;
+}
 constexpr float VREF_MIN = 1.1754943508222875e-38f;  // 2^-126
 
 // ---- few rows ---------------------------------------------------------------------
@@ -327,6 +334,490 @@ __global__ __launch_bounds__(256) void k_paged8_combine(const Paged8Args a) {
              d);
 }
 
+// ---- many rows --------------------------------------------------------------------
+//
+// A wave takes 32 folded rows, a workgroup 32 W of them, and keys KT at a time. The
+// codes are unpacked to f16 once a workgroup, into LDS, ahead of their use: K as rows of
+// D elements, V transposed, a row an element with its keys in the order in which the score
+// product leaves them in a lane (keys 4 h .. 4 h + 3 of each eight in half h of the wave),
+// so that P^T needs no exchange. Codes are exact there in one part; a score tile's rows 0
+// .. 15 and 16 .. 31 are a block each, whose scales the softmax takes in: keys' in the
+// factor that its argument has anyway, values' as one product a probability.
+// Rows are padded by 16 bytes, which spreads 16 rows' reads over all banks.
+//
+// A wave alternates between a phase of products, O^T += V^T P^T of tile t and S^T of
+// tile t + 1, with its share of the unpacking (V of tile t + 1, K of t + 2) in their
+// shadow, and the softmax of tile t + 1. Eight waves are two groups of one wave a SIMD,
+// half a turn apart: while one group's products run, the other's softmax does. The
+// first group unpacks V and the second K, so that two tiles of each in LDS suffice:
+// with barriers numbered as the first group passes them, it reads V(t) and K(t + 1)
+// and writes V(t + 1) behind barrier 2 t + 2, the second group reads the same and
+// writes K(t + 2) behind 2 t + 3; so V(t + 1) takes the place of V(t - 1), last read
+// behind 2 t + 1, and K(t + 2) that of K(t), last read there too. The scales lie with
+// their tiles: those of t are read by the softmax of t, behind 2 t + 1 and 2 t + 2, and
+// overwritten with K(t + 2) behind 2 t + 3 and V(t + 2) behind 2 t + 4.
+// A tile's scales, as the softmax takes them: of its keys; of its values the logarithm of a
+// block's share of the reference, its inverse and itself; the reference's last step and the
+// reference, and the smallest share.
+struct Scales {
+    float ks[4], log[4], inv[4], share[4];
+    float step, vref, low, pad;
+};
+
+template <int DT, int NB, int W>
+struct Many8 {
+    static constexpr int Q = DT == TN_F32 ? 2 : 1, P = DT == TN_F32 ? 2 : 1;
+    static constexpr int ROWS = 32 * W, GROUPS = W / 4;                // folded rows; groups of four waves
+    static constexpr int D = 32 * NB, KT = NB <= 4 ? 64 : 32;           // keys of a tile
+    static constexpr int KP = 2 * D + 16, VP = 2 * KT + 16;             // row pitches, bytes
+    static constexpr int KB = KT * KP, VB = D * VP, STAGE = KB + VB + 80;  // and what Scales holds
+    static constexpr int KI = KT * 4, VI = KT / 16 * D, VN = (VI + 255) / 256;  // items: (key, quarter), (block, element)
+    static constexpr int OS = DT == TN_F32 ? 4 : 2;                    // output element
+    static constexpr int OP = (NB < 4 ? D : 128) * (GROUPS == 1 ? 4 : OS) + 16;  // row pitch on the way out
+    static constexpr int LDS_BYTES = 2 * STAGE > ROWS * OP ? 2 * STAGE : ROWS * OP;
+    // waves a SIMD: one where two do not have the registers (four waves a workgroup then)
+    static constexpr bool BIG = DT == TN_F32 ? NB > 5 : NB > 6;
+    static constexpr int WAVES = GROUPS == 1 && BIG ? 1 : 2;
+    static_assert(KI <= 256, "a key item a thread");
+};
+
+// Rows first .. first + ROWS of request r, whose rows start at `start` and attend
+// `before` keys more than there are rows ahead of them.
+template <int DT, int NB, int W>
+TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, int h, int r, int start, int rows, int first, int len,
+                          int before) {
+    using M = Many8<DT, NB, W>;
+    constexpr int KT = M::KT, D = M::D, ROWS = M::ROWS, VN = M::VN, BL = KT / 16;
+    const int tid = threadIdx.x & 255, lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), group = w >> 2;
+    const int col = lane & 31, hh = lane >> 5;
+    const int S = 1 << a.c.shift;
+    const int i = first + 32 * w + col, j = min(i, rows - 1) / a.G, hq = h * a.G + min(i, rows - 1) % a.G;
+    const int keys = max(0, before + j + 1);
+    const int least = max(0, before + min(first + 32 * w, rows - 1) / a.G + 1);  // that all of the wave's rows attend
+    const int most = max(0, before + (min(first + ROWS, rows) - 1) / a.G + 1);   // that any of the workgroup's does
+    // this workgroup's tiles: one split's share
+    const int all_tiles = (most + KT - 1) / KT, split = blockIdx.y, ns = gridDim.y;
+    const int t0 = (int)((int64_t)split * all_tiles / ns), nt = (int)((int64_t)(split + 1) * all_tiles / ns);
+
+    // The query: step c of the product contracts over elements 16 c + 8 hh .. + 7.
+    h8 q[M::Q][2 * NB];
+    float rs = fabsf(a.sl2);
+    Eight<DT> qx[2 * NB];
+    auto load_q = [&]() __attribute__((always_inline)) {
+        const int64_t qi = (int64_t)(start + j) * a.q_stride + (int64_t)hq * D + 8 * hh;
+#pragma unroll
+        for (int c = 0; c < 2 * NB; c++) qx[c].load(a.q, qi + 16 * c);
+    };
+    auto make_q = [&]() __attribute__((always_inline)) {
+        float top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 2 * NB; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(qx[c].get(e)));
+        float sc = 1.0f;
+        if constexpr (DT != TN_F16) {
+            sc = row_scale(xor32_max(top));
+            rs = rs / sc;
+        }
+        // a positive factor, so that it can be taken out of the maximum
+        rs = fmaxf(rs, 1.1754944e-38f);
+        if (a.sl2 < 0.0f) sc = -sc;
+#pragma unroll
+        for (int c = 0; c < 2 * NB; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = qx[c].get(e) * sc;
+                const _Float16 hi = (_Float16)v;
+                q[0][c][e] = hi;
+                if constexpr (M::Q == 2) q[1][c][e] = (_Float16)(v - (float)hi);
+            }
+    };
+    f32x16 o[NB], s[KT / 32];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[b][e] = 0.0f;
+    float m = -INFINITY, l = 0.0f, vref = VREF_MIN;
+    uint32_t ph[KT / 4], pl[KT / 4];
+
+    // ---- this thread's part of a tile: its loads, and their way into LDS
+    const int32_t* table = a.table + (int64_t)r * a.width;
+    // K: (key, quarter of its row), a wave's lanes on one quarter (their LDS rows differ); V: (block, element)
+    const int ki = tid % M::KI, key = ki % KT, part = ki / KT;
+    const bool kon = M::KI == 256 || tid < M::KI;
+    struct KPart { uint32_t c[2 * NB]; float s; } kr;
+    struct VPart { uint32_t c[VN][4]; float s; } vr;
+    int kpage = 0, vpage[VN + 1] = {};
+    float ref = VREF_MIN;  // (in the lanes that write the scales of values)
+    // (item VN: the block whose scale this thread has)
+    auto vblock = [&](int x) { return x == VN ? tid & (BL - 1) : min(tid + 256 * x, M::VI - 1) / D; };
+    auto velement = [&](int x) { return min(tid + 256 * x, M::VI - 1) % D; };
+    // (tiles past the last are the last again)
+    auto kpages = [&](int t) __attribute__((always_inline)) {
+        return table[min((KT * min(t, nt - 1) + key) >> a.c.shift, a.width - 1)];
+    };
+    auto vpages = [&](int t, int x) __attribute__((always_inline)) {
+        return table[min((KT * min(t, nt - 1) + 16 * vblock(x)) >> a.c.shift, a.width - 1)];
+    };
+    auto load_k = [&](KPart& x, int page, int t) __attribute__((always_inline)) {
+        t = min(t, nt - 1);
+        const bool bad = (unsigned)page >= (unsigned)a.c.pages;
+        const int64_t row = (((int64_t)(bad ? 0 : page) * a.c.H + h) << a.c.shift) + ((KT * t + key) & (S - 1));
+        load_words(a.c.kc + row * D + part * (8 * NB), x.c);
+        const float sc = a.c.ks[row >> 4];
+        x.s = bad ? NAN : sc;  // a row's scores, and so the row, are NaN
+    };
+    auto load_v = [&](VPart& x, const int (&page)[VN + 1], int t) __attribute__((always_inline)) {
+        t = min(t, nt - 1);
+#pragma unroll
+        for (int y = 0; y <= VN; y++) {
+            const bool bad = (unsigned)page[y] >= (unsigned)a.c.pages;
+            const int at = KT * t + 16 * vblock(y);
+            const int64_t row = (((int64_t)(bad ? 0 : page[y]) * a.c.H + h) << a.c.shift) + (at & (S - 1));
+            if (y < VN) {
+                load_words(a.c.vc + row * D + velement(y) * 16, x.c[y < VN ? y : 0]);
+            } else {
+                const float sc = a.c.vs[row >> 4];
+                x.s = bad || at >= len ? 0.0f : sc;  // blocks that no row attends count as zeros
+            }
+        }
+    };
+    auto unpack_k = [&](const KPart& y, int b, int t) __attribute__((always_inline)) {  // eight codes
+        uint8_t* st = lds + (t & 1) * M::STAGE;
+        if (kon) *reinterpret_cast<h8*>(st + key * M::KP + (part * NB + b) * 16) = codes8(y.c[2 * b], y.c[2 * b + 1]);
+        if (b == 0 && kon && part == 0 && (key & 15) == 0)
+            reinterpret_cast<Scales*>(st + M::KB + M::VB)->ks[key >> 4] = y.s;
+    };
+    auto unpack_v = [&](const VPart& y, int x, int half, int t) __attribute__((always_inline)) {
+        uint8_t* st = lds + (t & 1) * M::STAGE;
+        const bool on = M::VI % 256 == 0 || tid + 256 * x < M::VI;
+        // tokens 4 half .. + 3 and 8 + 4 half .. + 3
+        if (on)
+            *reinterpret_cast<h8*>(st + M::KB + velement(x) * M::VP + (2 * vblock(x) + half) * 16) =
+                codes8(y.c[x][half], y.c[x][2 + half]);
+        if (x == 0 && half == 0 && tid < BL) {
+            const float top = quad_max<BL>(y.s), next = top >= ref ? vref_for(top) : ref, share = y.s / next;
+            const float low = -quad_max<BL>(-share);
+            Scales* sc = reinterpret_cast<Scales*>(st + M::KB + M::VB);
+            sc->log[tid] = __builtin_amdgcn_logf(share);
+            sc->inv[tid] = __builtin_amdgcn_rcpf(share);
+            sc->share[tid] = share;
+            if (tid == 0) sc->step = ref / next, sc->vref = next, sc->low = low;
+            ref = next;
+        }
+    };
+
+    // ---- the phases
+    // The products of a phase in groups of four fragments out of LDS, each group read
+    // while the one before it is multiplied: PG of O^T += V^T P^T (a group is 16 keys and
+    // up to four blocks of elements), then SG of S^T (XG steps of all the tile's keys).
+    constexpr int BG = 4, PB = (NB + BG - 1) / BG, PG = KT / 16 * PB;
+    constexpr int U = KT / 32, XG = 4 / U, SG = (2 * NB + XG - 1) / XG;
+    h8 f[2][4];
+    auto fetch = [&](int n, int t) __attribute__((always_inline)) {
+        if (n < PG) {
+            const uint8_t* st = lds + (t & 1) * M::STAGE + M::KB + col * M::VP + hh * 16 + n / PB * 32;
+#pragma unroll
+            for (int e = 0; e < BG; e++)
+                if (n % PB * BG + e < NB) f[n & 1][e] = *reinterpret_cast<const h8*>(st + 32 * (n % PB * BG + e) * M::VP);
+        } else if (n < PG + SG) {
+            const uint8_t* st = lds + ((t + 1) & 1) * M::STAGE + col * M::KP + hh * 16;
+#pragma unroll
+            for (int x = 0; x < XG; x++)
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if ((n - PG) * XG + x < 2 * NB)
+                        f[n & 1][x * U + u] = *reinterpret_cast<const h8*>(st + 32 * u * M::KP + 32 * ((n - PG) * XG + x));
+        }
+    };
+    auto multiply = [&](int n) __attribute__((always_inline)) {
+        if (n < PG) {
+            const int k = 4 * (n / PB);
+            const h8 p0 = as_h8(ph[k], ph[k + 1], ph[k + 2], ph[k + 3]);
+            const h8 p1 = M::P == 2 ? as_h8(pl[k], pl[k + 1], pl[k + 2], pl[k + 3]) : p0;
+#pragma unroll
+            for (int e = 0; e < BG; e++) {
+                const int b = n % PB * BG + e;
+                if (b >= NB) continue;
+                if (M::P == 2) o[b] = El<true>::mfma(f[n & 1][e], p1, o[b]);
+                o[b] = El<true>::mfma(f[n & 1][e], p0, o[b]);
+            }
+        } else {
+#pragma unroll
+            for (int x = 0; x < XG; x++) {
+                const int c = (n - PG) * XG + x;
+                if (c >= 2 * NB) continue;
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (M::Q == 2) s[u] = El<true>::mfma(f[n & 1][x * U + u], q[M::Q - 1][c], s[u]);
+                    s[u] = El<true>::mfma(f[n & 1][x * U + u], q[0][c], s[u]);
+                }
+            }
+        }
+    };
+    // Groups from .. to - 1, the first of which is in registers; between their products,
+    // in their shadow, this thread's part of V of tile t + 1 and K of t + 2 (role: 1 V,
+    // 2 K, 3 both), then the loads of the next ones.
+    auto products = [&](auto role, auto from, auto to, int t) __attribute__((always_inline)) {
+        constexpr int STEPS = to.value - from.value, ROLE = role.value;
+        constexpr int KW = ROLE & 2 ? NB : 0, VW = ROLE & 1 ? 2 * VN : 0, WORK = KW + VW + (ROLE ? 1 : 0);
+        if constexpr (to.value > PG) {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[u][e] = 0.0f;
+        }
+#pragma unroll
+        for (int n = from.value; n < to.value; n++) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (n + 1 < to.value) fetch(n + 1, t);
+            multiply(n);
+#pragma unroll
+            for (int x = (n - from.value) * WORK / STEPS; x < (n - from.value + 1) * WORK / STEPS; x++) {
+                if (x < KW) unpack_k(kr, x, t + 2);
+                else if (x < KW + VW) unpack_v(vr, (x - KW) >> 1, (x - KW) & 1, t + 1);
+                else {
+                    if constexpr (ROLE & 2) load_k(kr, kpage, t + 3), kpage = kpages(t + 4);
+                    if constexpr (ROLE & 1) {
+                        load_v(vr, vpage, t + 2);
+#pragma unroll
+                        for (int y = 0; y <= VN; y++) vpage[y] = vpages(t + 3, y);
+                    }
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto softmax = [&](int t) __attribute__((always_inline)) {
+        const Scales sc = *reinterpret_cast<const Scales*>(lds + (t & 1) * M::STAGE + M::KB + M::VB);
+        float fs[BL];
+#pragma unroll
+        for (int b = 0; b < BL; b++) fs[b] = rs * sc.ks[b];
+        // the products' wait states: the compiler does not see that max3f's assembly reads their result
+        __builtin_amdgcn_sched_barrier(0);
+#if __HIP_DEVICE_COMPILE__
+        asm volatile("s_nop 15\n\ts_nop 1");
+#endif
+        __builtin_amdgcn_sched_barrier(0);
+        if (KT * t + KT > least) {
+#pragma unroll
+            for (int u = 0; u < KT / 32; u++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int k = KT * t + 32 * u + 8 * (e >> 2) + 4 * hh + (e & 3);
+                    const float v = s[u][e] * fs[2 * u + (e >> 3)];
+                    s[u][e] = k >= keys ? -INFINITY : v;
+                }
+#pragma unroll
+            for (int b = 0; b < BL; b++) fs[b] = 1.0f;
+        }
+        float mb[BL];
+#pragma unroll
+        for (int b = 0; b < BL; b++) {
+            const f32x16& x = s[b >> 1];
+            const int e = 8 * (b & 1);
+            mb[b] = max3f(max3f(x[e], x[e + 1], x[e + 2]), max3f(x[e + 3], x[e + 4], x[e + 5]),
+                          max3f(x[e + 6], x[e + 7], x[e + 7])) * fs[b];
+        }
+        const float mx = xor32_max(max3f(mb[0], mb[1], BL == 4 ? fmaxf(mb[BL - 2], mb[BL - 1]) : mb[1]));
+        if (__any(mx > m + RESCALE_SLACK)) {
+            const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[b][e] *= al;
+        }
+        vref = sc.vref;
+        if (__builtin_amdgcn_readfirstlane(sc.step != 1.0f)) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[b][e] *= sc.step;
+        }
+        const float mu = P_BIAS - (m == -INFINITY ? 0.0f : m);
+        // A block's share goes into its probabilities' exponent and out of their sum again: one
+        // operation for eight of them. (Not where it is far below the others' or 0: its
+        // probabilities would be lost to the sum. f32 rows keep the product's digits.)
+        if (DT != TN_F32 && __builtin_amdgcn_readfirstlane(sc.low >= 0x1p-6f)) {
+#pragma unroll
+            for (int b = 0; b < BL; b++) {
+                const float ma = mu + sc.log[b];
+                float lb = 0.0f;
+#pragma unroll
+                for (int e = 8 * (b & 1); e < 8 * (b & 1) + 8; e += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][e], fs[b], ma));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][e + 1], fs[b], ma));
+                    split_p<M::P>(p0, p1, ph[8 * (b >> 1) + e / 2], pl[8 * (b >> 1) + e / 2], lb);
+                }
+                l = fmaf(lb, sc.inv[b], l);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < KT / 32; u++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                    const int b = 2 * u + (e >> 3);
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[u][e], fs[b], mu));
+                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[u][e + 1], fs[b], mu));
+                    l += p0;
+                    l += p1;
+                    float none = 0.0f;
+                    split_p<M::P>(p0 * sc.share[b], p1 * sc.share[b], ph[8 * u + e / 2], pl[8 * u + e / 2], none);
+                }
+        }
+        // computed here, not where the products take them
+#if __HIP_DEVICE_COMPILE__
+#pragma unroll
+        for (int e = 0; e < KT / 4; e++) {
+            asm volatile("" : "+v"(ph[e]));
+            if constexpr (M::P == 2) asm volatile("" : "+v"(pl[e]));
+        }
+        asm volatile("" : "+v"(l));
+#endif
+    };
+    auto walk = [&](auto role) __attribute__((always_inline)) {
+        constexpr std::integral_constant<int, 0> BEGIN, NONE;
+        constexpr std::integral_constant<int, PG> MIDDLE;
+        constexpr std::integral_constant<int, PG + SG> END;
+        // all that the first tiles need is asked for before any of it is waited for
+        KPart k0, k1;
+        VPart v0;
+        int kp0 = 0, kp1 = 0, kp2 = 0, vp0[VN + 1] = {}, vp1[VN + 1] = {};
+        if constexpr (role.value & 2) kp0 = kpages(t0), kp1 = kpages(t0 + 1), kp2 = kpages(t0 + 2), kpage = kpages(t0 + 3);
+        if constexpr (role.value & 1) {
+#pragma unroll
+            for (int y = 0; y <= VN; y++) vp0[y] = vpages(t0, y), vp1[y] = vpages(t0 + 1, y), vpage[y] = vpages(t0 + 2, y);
+        }
+        load_q();
+        if constexpr (role.value & 2) load_k(k0, kp0, t0), load_k(k1, kp1, t0 + 1), load_k(kr, kp2, t0 + 2);
+        if constexpr (role.value & 1) load_v(v0, vp0, t0), load_v(vr, vp1, t0 + 1);
+        make_q();
+        if constexpr (role.value & 2) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) unpack_k(k0, b, t0), unpack_k(k1, b, t0 + 1);
+        }
+        if constexpr (role.value & 1) {
+#pragma unroll
+            for (int x = 0; x < 2 * VN; x++) unpack_v(v0, x >> 1, x & 1, t0);
+        }
+        __syncthreads();
+        if (role.value == 2) __syncthreads();  // half a turn behind
+        fetch(PG, t0 - 1);
+        products(NONE, MIDDLE, END, t0 - 1);
+        for (int t = t0; t + 1 < nt; t++) {
+            __syncthreads();
+            softmax(t);
+            fetch(0, t);
+            __syncthreads();
+            __builtin_amdgcn_s_setprio(1);  // the products' few instructions ahead of the other group's many
+            products(role, BEGIN, END, t);
+            __builtin_amdgcn_s_setprio(0);
+        }
+        __syncthreads();
+        softmax(nt - 1);
+        fetch(0, nt - 1);
+        __syncthreads();
+        products(NONE, BEGIN, MIDDLE, nt - 1);
+        if (role.value == 1) __syncthreads();
+    };
+    if (nt > t0) {
+        if constexpr (M::GROUPS == 1) walk(std::integral_constant<int, 3>{});
+        else if (group == 0) walk(std::integral_constant<int, 1>{});
+        else walk(std::integral_constant<int, 2>{});
+    }
+
+    // out through LDS, so that a row's bytes leave together, in `type` to rows of a.out or (many_o) f32
+    l = xor32_sum(l);
+    uint8_t* mine = lds + w * 32 * M::OP;
+    __syncthreads();
+    auto leave = [&](auto type, float f, float g) __attribute__((always_inline)) {
+        constexpr int OT = type.value, SIZE = OT == TN_F32 ? 4 : 2;
+#pragma unroll
+        for (int b0 = 0; b0 < NB; b0 += 4) {  // four blocks at a time
+            const int nb = NB - b0 < 4 ? NB - b0 : 4, pieces = nb * 2 * SIZE;  // of 16 bytes, a row
+#pragma unroll
+            for (int b = b0; b < b0 + nb; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float y[4] = {o[b][e] * f * g, o[b][e + 1] * f * g, o[b][e + 2] * f * g, o[b][e + 3] * f * g};
+                    uint8_t* p = mine + col * M::OP + (32 * (b - b0) + 2 * e + 4 * hh) * SIZE;
+                    if constexpr (OT == TN_F32) {
+                        *reinterpret_cast<f32x4*>(p) = (f32x4){y[0], y[1], y[2], y[3]};
+                    } else {
+                        using E = El<OT == TN_F16>;
+                        *reinterpret_cast<uint2*>(p) = make_uint2(E::pack_out(y[0], y[1]), E::pack_out(y[2], y[3]));
+                    }
+                }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's own rows
+#pragma unroll
+            for (int k = 0; k < pieces / 2; k++) {
+                const int x = lane + 64 * k, rr = x / pieces, ii = first + 32 * w + rr;
+                typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+                typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
+                const u4 v = *reinterpret_cast<const u4*>(mine + rr * M::OP + x % pieces * 16);
+                int64_t row = (int64_t)(start + ii / a.G) * a.Hq + h * a.G + ii % a.G;
+                if (ns > 1) row = row * ns + split;
+                char* to = ns > 1 ? reinterpret_cast<char*>(a.many_o) : static_cast<char*>(a.out);
+                if (ii < rows) *reinterpret_cast<v4*>(to + (row * D + 32 * b0) * SIZE + x % pieces * 16) = v;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    };
+    const int64_t row = (int64_t)(start + j) * a.Hq + hq;
+    if (M::GROUPS == 1 && ns > 1) {  // a split's part: k_paged8_join's
+        leave(std::integral_constant<int, TN_F32>{}, 1.0f, 1.0f);
+        if (hh == 0 && i < rows) reinterpret_cast<Part*>(a.many_ml)[row * ns + split] = Part{m, l, vref, 0.0f};
+    } else {
+        leave(std::integral_constant<int, DT>{}, 1.0f / l, vref);
+        if (a.lse && hh == 0 && i < rows) a.lse[row] = l == 0.0f ? -INFINITY : (m - P_BIAS) * LN2 + logf(l);
+    }
+}
+
+template <int DT, int NB, int W>
+__global__ __launch_bounds__(64 * W, (Many8<DT, NB, W>::WAVES)) void k_paged8_many(const Paged8Args a, int tiles) {
+    constexpr int ROWS = 32 * W;
+    __shared__ __align__(16) uint8_t lds[Many8<DT, NB, W>::LDS_BYTES];
+    // the longest rows first; a key/value head's workgroups on the same die when there are eight
+    const int h = (int)blockIdx.x % a.c.H, tile = tiles - 1 - (int)blockIdx.x / a.c.H;
+    int r = 0;
+    {  // request r has tiles row_start[r] G / ROWS + r and on: at least as many as its rows need
+        int hi = a.n;
+        while (hi - r > 1) {
+            const int mid = (r + hi) >> 1;
+            if ((int)((int64_t)start_of(a, mid) * a.G / ROWS) + mid <= tile) r = mid;
+            else hi = mid;
+        }
+    }
+    const int start = start_of(a, r), all = rows_of(a, r, start);
+    const int first = (tile - (int)((int64_t)start * a.G / ROWS) - r) * ROWS;
+    const int rows = min(all, a.max_rows) * a.G;
+    if (first < 0 || first >= rows || rows <= a.few) return;  // few rows: k_paged8_few's
+    const int len = max(0, min(a.lens[r], a.max_len)), before = len - all;
+    many8_tile<DT, NB, W>(a, lds, h, r, start, rows, first, len, before);
+}
+
+// The splits of k_paged8_many's rows, in order: four output columns a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void k_paged8_join(const Paged8Args a, int ns) {
+    const int D = 32 * a.c.nb, q4 = D / 4;
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = e / q4;
+    const int d = (int)(e - row * q4) * 4, t = (int)(row / a.Hq);
+    if (t >= start_of(a, a.n)) return;
+    int r = 0, hi = a.n;  // the row's request
+    while (hi - r > 1) {
+        const int mid = (r + hi) >> 1;
+        if (start_of(a, mid) <= t) r = mid;
+        else hi = mid;
+    }
+    const int start = start_of(a, r), c = min(rows_of(a, r, start), a.max_rows);
+    if (t < start || t - start >= c || c * a.G <= a.few) return;  // (rows ahead of the first request's are no one's)
+    join<DT>(a, a.many_o + row * ns * D + d, reinterpret_cast<const Part*>(a.many_ml) + row * ns, ns, row, d);
+}
+
 // Splits of the keys of k_paged8_few: one round of the workgroups that compute units
 // hold, of 512 keys or more, up to eight of them of 256.
 constexpr int64_t FEW_WGS = 512, FEW_KEYS = 512, FEW_MAX_SPLIT = 64;
@@ -360,18 +851,67 @@ int64_t part_rows(const Pages8& c, int64_t n, int64_t few, int64_t max_len) {
     return most < 2 ? 0 : std::min(std::min<int64_t>(few, 16) * FEW_WGS, n * c.H * few * most);
 }
 
+// k_paged8_many: 0 for workgroups of 256 rows (rows enough for one a unit), else the
+// splits of the keys for workgroups of 128, two of which a unit holds.
+constexpr int64_t MANY_WIDE = 256, MANY_WGS = 512, MANY_MAX_SPLIT = 8;
+int many_splits(const Pages8& c, int dtype, int64_t n, int64_t tokens, int64_t G, int64_t max_len) {
+    const bool big = dtype == TN_F32 ? c.nb > 5 : c.nb > 6;  // Many8::BIG: 256 rows do not have the registers
+    if (!big && tokens * G / 256 * c.H >= MANY_WIDE) return 0;
+    const int64_t wgs = (tokens * G / 128 + n) * c.H;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(MANY_WGS, wgs), cdiv(max_len, 512), MANY_MAX_SPLIT}));
+}
+// Rows of its partials at most, for this call and every smaller one: above one split there
+// are under MANY_WGS workgroups of 128 rows a split.
+int64_t many_rows(const Pages8& c, int64_t tokens, int64_t G, int64_t max_len) {
+    const int64_t most = std::min(cdiv(max_len, 512), MANY_MAX_SPLIT);
+    return most < 2 ? 0 : std::min(tokens * G * c.H * most, 2 * MANY_WGS * 128);
+}
+
+// Which kernel takes a request's rows. k_paged8_few reads and unpacks the codes again for
+// every 16 folded rows but starts at once and splits finely; k_paged8_many fills 128 or 256
+// rows, and its tiles follow one another. So k_paged8_few takes all rows of a call whose
+// products (tokens * Hq * max_len * D) are few, and of a larger call the requests of up to
+// FEW_ROWS folded rows, if it is of several. Its grid is as long for every request as for
+// the longest: up to FEW_GRID workgroups of it.
+constexpr int FEW_ROWS = 128;
+constexpr int64_t FEW_WORK = 1ll << 32, FEW_GRID = 8192;
+
+// Folded rows of a request that k_paged8_few takes at most in this call; 0: it is not launched.
+int64_t few_limit(const Pages8& c, int dtype, int64_t n, int64_t tokens, int64_t G, int64_t max_rows, int64_t max_len) {
+    const int64_t rows = max_rows * G;
+    (void)dtype;
+    // (tokens * Hq is at most 2^30, D 2^8)
+    const bool little = tokens * G * c.H * 32 * c.nb <= FEW_WORK / std::max<int64_t>(max_len, 1) &&
+                        n * c.H * cdiv(rows, 16) <= FEW_GRID;
+    return rows <= FEW_ROWS || little ? rows : n > 1 ? FEW_ROWS : 0;
+}
+
 int64_t work_rows(const Pages8& c, int64_t n, int64_t tokens, int64_t G, int64_t max_rows, int64_t max_len) {
-    (void)tokens;
-    return part_rows(c, n, max_rows * G, max_len);
+    return part_rows(c, n, max_rows * G, max_len) + (max_rows * G > FEW_ROWS ? many_rows(c, tokens, G, max_len) : 0);
 }
 
 template <int DT, int NB>
 tn_status launch_at(hipStream_t st, const Paged8Args& a, int64_t tokens) {
-    (void)tokens;
     if (a.few) {
         const dim3 grid((unsigned)a.nsplit, (unsigned)(a.c.H * cdiv(a.few, 16)), (unsigned)a.n);
         hipLaunchKernelGGL((k_paged8_few<DT, NB>), grid, dim3(256), 0, st, a);
         TN_LAUNCHED();
+    }
+    if ((int64_t)a.max_rows * a.G > a.few) {
+        const int ns = many_splits(a.c, DT, a.n, tokens, a.G, a.max_len);
+        const bool wide = ns == 0;
+        const int64_t tiles = tokens * a.G / (wide ? 256 : 128) + a.n;
+        const dim3 grid((unsigned)(tiles * a.c.H), wide ? 1u : (unsigned)ns);
+        if constexpr (!Many8<DT, NB, 8>::BIG) {
+            if (wide) hipLaunchKernelGGL((k_paged8_many<DT, NB, 8>), grid, dim3(512), 0, st, a, (int)tiles);
+        }
+        if (!wide) hipLaunchKernelGGL((k_paged8_many<DT, NB, 4>), grid, dim3(256), 0, st, a, (int)tiles);
+        TN_LAUNCHED();
+        if (ns > 1) {
+            const int64_t quads = tokens * a.Hq * (8 * NB);
+            hipLaunchKernelGGL(k_paged8_join<DT>, dim3((unsigned)cdiv(quads, 256)), dim3(256), 0, st, a, ns);
+            TN_LAUNCHED();
+        }
     }
     if (a.few && a.nsplit > 1) {
         const int64_t rows = (int64_t)a.n * a.c.H * a.few;
@@ -440,11 +980,13 @@ tn_status tn_sdpa_paged_q8(void* stream, const tn_q8_cache* cache, int dtype, co
     a.q_stride = q_stride, a.n = (int)n, a.tokens = (int)tokens, a.Hq = (int)Hq, a.G = (int)G, a.width = (int)width;
     a.max_rows = (int)std::min(max_rows, tokens), a.max_len = (int)max_len;
     a.sl2 = (float)(sc * 1.4426950408889634);
-    a.few = (int)(a.max_rows * G);
+    a.few = (int)few_limit(a.c, dtype, n, tokens, G, a.max_rows, max_len);
     a.nsplit = few_splits(a.c, n, a.few, max_len);
+    // f32 rows, then their parts: the few's and the many's
+    const int64_t few = part_rows(a.c, n, a.max_rows * G, max_len);
     const int64_t rows = work_rows(a.c, n, tokens, G, a.max_rows, max_len);
-    a.part_o = work;
-    a.part_ml = reinterpret_cast<float2*>(work + rows * D);
+    a.part_o = work, a.many_o = work + few * D;
+    a.part_ml = reinterpret_cast<float2*>(work + rows * D), a.many_ml = a.part_ml + 2 * few;  // (Part: two each)
     hipStream_t st = (hipStream_t)stream;
     if (dtype == TN_F32) return launch<TN_F32>(st, a, tokens);
     if (dtype == TN_BF16) return launch<TN_BF16>(st, a, tokens);
