@@ -62,6 +62,10 @@ TN_INLINE float quad_max(float v) {
     return v;
 }
 constexpr float VREF_MIN = 1.1754943508222875e-38f;  // 2^-126
+// Its inverse, exactly.
+TN_INLINE float vref_inverse(float vref) {
+    return __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, vref));
+}
 
 // ---- few rows ---------------------------------------------------------------------
 //
@@ -213,12 +217,12 @@ __global__ __launch_bounds__(256, (NB <= 4 ? 2 : 1)) void k_paged8_few(const Pag
         }
         const float mv = wave_xor_max(x.vs);
         if (__any(mv >= vref)) {
-            const float nv = vref_for(mv), al = vref / nv;
+            const float nv = vref_for(mv), al = vref * vref_inverse(nv);
             vref = nv;
 #pragma unroll
             for (int b = 0; b < 2 * NB; b++) o[b] = o[b] * al;
         }
-        const float mu = P_BIAS - (m == -INFINITY ? 0.0f : m), share = x.vs / vref;
+        const float mu = P_BIAS - (m == -INFINITY ? 0.0f : m), share = x.vs * vref_inverse(vref);
         uint32_t ph[8], pl[8];
 #pragma unroll
         for (int n = 0; n < 16; n += 2) {
@@ -342,54 +346,70 @@ __global__ __launch_bounds__(256) void k_paged8_combine(const Paged8Args a) {
 // product leaves them in a lane (keys 4 h .. 4 h + 3 of each eight in half h of the wave),
 // so that P^T needs no exchange. Codes are exact there in one part; a score tile's rows 0
 // .. 15 and 16 .. 31 are a block each, whose scales the softmax takes in: keys' in the
-// factor that its argument has anyway, values' as one product a probability.
+// factor that its argument has anyway, values' in its exponent, and out of the sum again.
 // Rows are padded by 16 bytes, which spreads 16 rows' reads over all banks.
 //
-// A wave alternates between a phase of products, O^T += V^T P^T of tile t and S^T of
-// tile t + 1, with its share of the unpacking (V of tile t + 1, K of t + 2) in their
-// shadow, and the softmax of tile t + 1. Eight waves are two groups of one wave a SIMD,
-// half a turn apart: while one group's products run, the other's softmax does. The
-// first group unpacks V and the second K, so that two tiles of each in LDS suffice:
-// with barriers numbered as the first group passes them, it reads V(t) and K(t + 1)
-// and writes V(t + 1) behind barrier 2 t + 2, the second group reads the same and
-// writes K(t + 2) behind 2 t + 3; so V(t + 1) takes the place of V(t - 1), last read
-// behind 2 t + 1, and K(t + 2) that of K(t), last read there too. The scales lie with
-// their tiles: those of t are read by the softmax of t, behind 2 t + 1 and 2 t + 2, and
-// overwritten with K(t + 2) behind 2 t + 3 and V(t + 2) behind 2 t + 4.
-// A tile's scales, as the softmax takes them: of its keys; of its values the logarithm of a
-// block's share of the reference, its inverse and itself; the reference's last step and the
-// reference, and the smallest share.
-struct Scales {
-    float ks[4], log[4], inv[4], share[4];
-    float step, vref, low, pad;
-};
-
+// A wave alternates between two phases: the softmax of tile t; and the products, O^T +=
+// V^T P^T of tile t and S^T of tile t + 1, with its share of the unpacking (V of tile
+// t + 1, K of t + 2) in their shadow. Eight waves are
+// two groups of one wave a SIMD, half a turn apart: while one group's products run, the
+// other's softmax does. The first group unpacks V and the second K, so that two tiles
+// of each in LDS suffice: with barriers numbered as the first group passes them, it reads
+// V(t) and K(t + 1) and writes V(t + 1) behind barrier 2 t + 2, the second group reads the
+// same and writes K(t + 2) behind 2 t + 3; so V(t + 1) takes the place of V(t - 1), last
+// read behind 2 t + 1, and K(t + 2) that of K(t), last read there too. What the softmax
+// and the unpacking take of a tile's scales is written two turns ahead of the softmax, by
+// lanes of one wave of the last group, into one of four places. The first group, half a turn
+// ahead, unpacks V(t + 1) by it one turn later, so it reads it only behind the turn's
+// middle barrier.
 template <int DT, int NB, int W>
 struct Many8 {
     static constexpr int Q = DT == TN_F32 ? 2 : 1, P = DT == TN_F32 ? 2 : 1;
-    static constexpr int ROWS = 32 * W, GROUPS = W / 4;                // folded rows; groups of four waves
-    static constexpr int D = 32 * NB, KT = NB <= 4 ? 64 : 32;           // keys of a tile
-    static constexpr int KP = 2 * D + 16, VP = 2 * KT + 16;             // row pitches, bytes
-    static constexpr int KB = KT * KP, VB = D * VP, STAGE = KB + VB + 80;  // and what Scales holds
-    static constexpr int KI = KT * 4, VI = KT / 16 * D, VN = (VI + 255) / 256;  // items: (key, quarter), (block, element)
-    static constexpr int OS = DT == TN_F32 ? 4 : 2;                    // output element
+    static constexpr int ROWS = 32 * W;                                 // folded rows
+    static constexpr int D = 32 * NB, KT = NB <= 4 ? 64 : 32;            // keys of a tile
+    static constexpr int GROUPS = W / 4, BL = KT / 16, WPB = 4 / BL;     // groups of four waves; blocks, waves that unpack one
+    static constexpr int KP = 2 * D + 16, VP = 2 * KT + 16;              // row pitches, bytes
+    static constexpr int KB = KT * KP, VB = D * VP, STAGE = KB + VB;
+    static constexpr int N = (NB + 2 * WPB - 1) / (2 * WPB);             // 16-byte pieces a thread, of K and of V
+    static constexpr int OS = DT == TN_F32 ? 4 : 2;                     // output element
     static constexpr int OP = (NB < 4 ? D : 128) * (GROUPS == 1 ? 4 : OS) + 16;  // row pitch on the way out
     static constexpr int LDS_BYTES = 2 * STAGE > ROWS * OP ? 2 * STAGE : ROWS * OP;
     // waves a SIMD: one where two do not have the registers (four waves a workgroup then)
     static constexpr bool BIG = DT == TN_F32 ? NB > 5 : NB > 6;
-    static constexpr int WAVES = GROUPS == 1 && BIG ? 1 : 2;
-    static_assert(KI <= 256, "a key item a thread");
+    static constexpr int WAVES = W == 4 && BIG ? 1 : 2;
 };
+
+// A tile's scales: of its keys; of its values a block's share of the reference, for 16-bit rows
+// its logarithm and inverse, down to 2^-6 (the probabilities of a smaller one would be lost to
+// the sum: what is left of it, `rest`, goes into its codes); the reference's last step and the
+// reference.
+struct Scales {
+    float ks[4], log[4], inv[4], share[4];
+    uint32_t rest[4];  // two f16
+    float step, vref, pad[2];
+};
+constexpr float LEAST_SHARE = 0x1p-6f;
+constexpr uint32_t ONES = 0x3c003c00u;  // two f16
+
+// What a kernel only reads, through the scalar cache where its address is the wave's.
+template <class T>
+TN_INLINE T scalar(const T* p) {
+#if __HIP_DEVICE_COMPILE__
+    return *(const __attribute__((address_space(4))) T*)reinterpret_cast<uintptr_t>(p);
+#else
+    return *p;
+#endif
+}
 
 // Rows first .. first + ROWS of request r, whose rows start at `start` and attend
 // `before` keys more than there are rows ahead of them.
 template <int DT, int NB, int W>
-TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, int h, int r, int start, int rows, int first, int len,
-                          int before) {
+TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int h, int r, int start, int rows, int first,
+                          int len, int before) {
     using M = Many8<DT, NB, W>;
-    constexpr int KT = M::KT, D = M::D, ROWS = M::ROWS, VN = M::VN, BL = KT / 16;
-    const int tid = threadIdx.x & 255, lane = threadIdx.x & 63;
-    const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), group = w >> 2;
+    constexpr int KT = M::KT, D = M::D, ROWS = M::ROWS, N = M::N, BL = M::BL, WPB = M::WPB;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, hh = lane >> 5;
     const int S = 1 << a.c.shift;
     const int i = first + 32 * w + col, j = min(i, rows - 1) / a.G, hq = h * a.G + min(i, rows - 1) % a.G;
@@ -433,96 +453,113 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, int h, int r, int s
                 if constexpr (M::Q == 2) q[1][c][e] = (_Float16)(v - (float)hi);
             }
     };
-    f32x16 o[NB], s[KT / 32];
+    constexpr int U = KT / 32;
+    struct Scores {
+        f32x16 s[U];
+    };
+    struct Probs {
+        uint32_t h[KT / 4], l[KT / 4];
+    };
+    f32x16 o[NB];
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
         for (int e = 0; e < 16; e++) o[b][e] = 0.0f;
     float m = -INFINITY, l = 0.0f, vref = VREF_MIN;
-    uint32_t ph[KT / 4], pl[KT / 4];
 
-    // ---- this thread's part of a tile: its loads, and their way into LDS
+    // ---- this thread's part of a tile: its loads, and their way into LDS. A wave unpacks of
+    // one block of sixteen keys, WPB waves a block, pieces (key, 16 elements) of K and
+    // (element) of V: of either (two groups) or of both
     const int32_t* table = a.table + (int64_t)r * a.width;
-    // K: (key, quarter of its row), a wave's lanes on one quarter (their LDS rows differ); V: (block, element)
-    const int ki = tid % M::KI, key = ki % KT, part = ki / KT;
-    const bool kon = M::KI == 256 || tid < M::KI;
-    struct KPart { uint32_t c[2 * NB]; float s; } kr;
-    struct VPart { uint32_t c[VN][4]; float s; } vr;
-    int kpage = 0, vpage[VN + 1] = {};
-    float ref = VREF_MIN;  // (in the lanes that write the scales of values)
-    // (item VN: the block whose scale this thread has)
-    auto vblock = [&](int x) { return x == VN ? tid & (BL - 1) : min(tid + 256 * x, M::VI - 1) / D; };
-    auto velement = [&](int x) { return min(tid + 256 * x, M::VI - 1) % D; };
+    const int blk = w % 4 / WPB, id0 = w % WPB * 64 + lane, group = w / 4;
+    auto on = [&](int x) { return 32 * NB % (64 * WPB) == 0 || id0 + 64 * WPB * x < 32 * NB; };
+    struct Pieces {
+        uint32_t c[N][4];
+    } kr, vr;
     // (tiles past the last are the last again)
-    auto kpages = [&](int t) __attribute__((always_inline)) {
-        return table[min((KT * min(t, nt - 1) + key) >> a.c.shift, a.width - 1)];
+    auto page_of = [&](int t) __attribute__((always_inline)) {
+        return scalar(table + min((KT * min(t, nt - 1) + 16 * blk) >> a.c.shift, a.width - 1));
     };
-    auto vpages = [&](int t, int x) __attribute__((always_inline)) {
-        return table[min((KT * min(t, nt - 1) + 16 * vblock(x)) >> a.c.shift, a.width - 1)];
+    // the plane row of the first of the wave's sixteen keys
+    auto row_of = [&](int page, int t) __attribute__((always_inline)) {
+        const bool bad = (unsigned)page >= (unsigned)a.c.pages;  // its scales are written so that it does not count
+        return (((int64_t)(bad ? 0 : page) * a.c.H + h) << a.c.shift) + ((KT * min(t, nt - 1) + 16 * blk) & (S - 1));
     };
-    auto load_k = [&](KPart& x, int page, int t) __attribute__((always_inline)) {
-        t = min(t, nt - 1);
-        const bool bad = (unsigned)page >= (unsigned)a.c.pages;
-        const int64_t row = (((int64_t)(bad ? 0 : page) * a.c.H + h) << a.c.shift) + ((KT * t + key) & (S - 1));
-        load_words(a.c.kc + row * D + part * (8 * NB), x.c);
-        const float sc = a.c.ks[row >> 4];
-        x.s = bad ? NAN : sc;  // a row's scores, and so the row, are NaN
-    };
-    auto load_v = [&](VPart& x, const int (&page)[VN + 1], int t) __attribute__((always_inline)) {
-        t = min(t, nt - 1);
+    auto load_k = [&](Pieces& y, int page, int t) __attribute__((always_inline)) {
+        const uint8_t* p = a.c.kc + row_of(page, t) * D;
 #pragma unroll
-        for (int y = 0; y <= VN; y++) {
-            const bool bad = (unsigned)page[y] >= (unsigned)a.c.pages;
-            const int at = KT * t + 16 * vblock(y);
-            const int64_t row = (((int64_t)(bad ? 0 : page[y]) * a.c.H + h) << a.c.shift) + (at & (S - 1));
-            if (y < VN) {
-                load_words(a.c.vc + row * D + velement(y) * 16, x.c[y < VN ? y : 0]);
-            } else {
-                const float sc = a.c.vs[row >> 4];
-                x.s = bad || at >= len ? 0.0f : sc;  // blocks that no row attends count as zeros
-            }
+        for (int x = 0; x < N; x++) {
+            const int id = on(x) ? id0 + 64 * WPB * x : 0;
+            load_words(p + (uint32_t)((id & 15) * D + (id >> 4) * 16), y.c[x]);
         }
     };
-    auto unpack_k = [&](const KPart& y, int b, int t) __attribute__((always_inline)) {  // eight codes
-        uint8_t* st = lds + (t & 1) * M::STAGE;
-        if (kon) *reinterpret_cast<h8*>(st + key * M::KP + (part * NB + b) * 16) = codes8(y.c[2 * b], y.c[2 * b + 1]);
-        if (b == 0 && kon && part == 0 && (key & 15) == 0)
-            reinterpret_cast<Scales*>(st + M::KB + M::VB)->ks[key >> 4] = y.s;
+    auto load_v = [&](Pieces& y, int page, int t) __attribute__((always_inline)) {
+        const uint8_t* p = a.c.vc + row_of(page, t) * D;
+#pragma unroll
+        for (int x = 0; x < N; x++) load_words(p + (uint32_t)((on(x) ? id0 + 64 * WPB * x : 0) * 16), y.c[x]);
     };
-    auto unpack_v = [&](const VPart& y, int x, int half, int t) __attribute__((always_inline)) {
-        uint8_t* st = lds + (t & 1) * M::STAGE;
-        const bool on = M::VI % 256 == 0 || tid + 256 * x < M::VI;
+    auto unpack_k = [&](int x, int half, int t) __attribute__((always_inline)) {  // eight codes
+        const int id = id0 + 64 * WPB * x;
+        if (on(x))
+            *reinterpret_cast<h8*>(lds + (t & 1) * M::STAGE + (16 * blk + (id & 15)) * M::KP + (id >> 4) * 32 + half * 16) =
+                codes8(kr.c[x][2 * half], kr.c[x][2 * half + 1]);
+    };
+    // rest: what is left of a small block's scale (Scales), for all of the wave's pieces
+    auto rest_of = [&](int t) __attribute__((always_inline)) {
+        return DT == TN_F32 ? ONES : (uint32_t)__builtin_amdgcn_readfirstlane((int)scales[t & 3].rest[blk]);
+    };
+    auto unpack_v = [&](int x, int half, int t, uint32_t rest) __attribute__((always_inline)) {
+        const int id = id0 + 64 * WPB * x;
         // tokens 4 half .. + 3 and 8 + 4 half .. + 3
-        if (on)
-            *reinterpret_cast<h8*>(st + M::KB + velement(x) * M::VP + (2 * vblock(x) + half) * 16) =
-                codes8(y.c[x][half], y.c[x][2 + half]);
-        if (x == 0 && half == 0 && tid < BL) {
-            const float top = quad_max<BL>(y.s), next = top >= ref ? vref_for(top) : ref, share = y.s / next;
-            const float low = -quad_max<BL>(-share);
-            Scales* sc = reinterpret_cast<Scales*>(st + M::KB + M::VB);
-            sc->log[tid] = __builtin_amdgcn_logf(share);
-            sc->inv[tid] = __builtin_amdgcn_rcpf(share);
-            sc->share[tid] = share;
-            if (tid == 0) sc->step = ref / next, sc->vref = next, sc->low = low;
-            ref = next;
+        h8 v = codes8(vr.c[x][half], vr.c[x][2 + half]);
+        if (rest != ONES) v = v * as_h8(rest, rest, rest, rest);
+        if (on(x)) *reinterpret_cast<h8*>(lds + (t & 1) * M::STAGE + M::KB + id * M::VP + (2 * blk + half) * 16) = v;
+    };
+    // The scales, by the first BL lanes of the last wave, a block each.
+    const bool scaler = w == W - 1;
+    float ref = VREF_MIN, sk = 0.0f, sv = 0.0f;
+    int spage = 0;
+    auto scale_page = [&](int t) __attribute__((always_inline)) {
+        spage = table[min((KT * min(t, nt - 1) + 16 * (lane & (BL - 1))) >> a.c.shift, a.width - 1)];
+    };
+    auto load_scales = [&](int t) __attribute__((always_inline)) {
+        const bool bad = (unsigned)spage >= (unsigned)a.c.pages;
+        const int at = KT * min(t, nt - 1) + 16 * (lane & (BL - 1));
+        const int64_t row = ((((int64_t)(bad ? 0 : spage) * a.c.H + h) << a.c.shift) + (at & (S - 1))) >> 4;
+        const float k = a.c.ks[row], v = a.c.vs[row];
+        sk = bad ? NAN : k;                       // its scores, and so the rows that attend it, are NaN
+        sv = bad || at >= len ? 0.0f : v;         // blocks that no row attends count as zeros
+    };
+    auto write_scales = [&](int t) __attribute__((always_inline)) {
+        const float top = quad_max<BL>(sv), next = top >= ref ? vref_for(top) : ref, inv = vref_inverse(next);
+        const float share = sv * inv;
+        const bool small = share < LEAST_SHARE;
+        Scales& sc = scales[t & 3];
+        if (lane < BL) {
+            sc.ks[lane] = sk;
+            sc.log[lane] = small ? -6.0f : __builtin_amdgcn_logf(share);
+            sc.inv[lane] = small ? 64.0f : __builtin_amdgcn_rcpf(share);
+            sc.share[lane] = share;
+            sc.rest[lane] = small ? pk_f16(share * 64.0f, share * 64.0f) : ONES;
+            if (lane == 0) sc.step = ref * inv, sc.vref = next;
         }
+        ref = next;
     };
 
-    // ---- the phases
-    // The products of a phase in groups of four fragments out of LDS, each group read
-    // while the one before it is multiplied: PG of O^T += V^T P^T (a group is 16 keys and
-    // up to four blocks of elements), then SG of S^T (XG steps of all the tile's keys).
+    // ---- products, in groups of four fragments out of LDS, each group read while the one
+    // before it is multiplied: PG of O^T += V^T P^T (a group is 16 keys and up to four blocks
+    // of elements), then SG of S^T (XG steps of all the tile's keys).
     constexpr int BG = 4, PB = (NB + BG - 1) / BG, PG = KT / 16 * PB;
-    constexpr int U = KT / 32, XG = 4 / U, SG = (2 * NB + XG - 1) / XG;
+    constexpr int XG = 4 / U, SG = (2 * NB + XG - 1) / XG, G = PG + SG;
     h8 f[2][4];
-    auto fetch = [&](int n, int t) __attribute__((always_inline)) {
+    auto fetch = [&](int n, int slot) __attribute__((always_inline)) {
         if (n < PG) {
-            const uint8_t* st = lds + (t & 1) * M::STAGE + M::KB + col * M::VP + hh * 16 + n / PB * 32;
+            const uint8_t* st = lds + slot * M::STAGE + M::KB + col * M::VP + hh * 16 + n / PB * 32;
 #pragma unroll
             for (int e = 0; e < BG; e++)
                 if (n % PB * BG + e < NB) f[n & 1][e] = *reinterpret_cast<const h8*>(st + 32 * (n % PB * BG + e) * M::VP);
-        } else if (n < PG + SG) {
-            const uint8_t* st = lds + ((t + 1) & 1) * M::STAGE + col * M::KP + hh * 16;
+        } else if (n < G) {
+            const uint8_t* st = lds + slot * M::STAGE + col * M::KP + hh * 16;
 #pragma unroll
             for (int x = 0; x < XG; x++)
 #pragma unroll
@@ -531,11 +568,11 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, int h, int r, int s
                         f[n & 1][x * U + u] = *reinterpret_cast<const h8*>(st + 32 * u * M::KP + 32 * ((n - PG) * XG + x));
         }
     };
-    auto multiply = [&](int n) __attribute__((always_inline)) {
+    auto multiply = [&](int n, const Probs& p, Scores& s) __attribute__((always_inline)) {
         if (n < PG) {
             const int k = 4 * (n / PB);
-            const h8 p0 = as_h8(ph[k], ph[k + 1], ph[k + 2], ph[k + 3]);
-            const h8 p1 = M::P == 2 ? as_h8(pl[k], pl[k + 1], pl[k + 2], pl[k + 3]) : p0;
+            const h8 p0 = as_h8(p.h[k], p.h[k + 1], p.h[k + 2], p.h[k + 3]);
+            const h8 p1 = M::P == 2 ? as_h8(p.l[k], p.l[k + 1], p.l[k + 2], p.l[k + 3]) : p0;
 #pragma unroll
             for (int e = 0; e < BG; e++) {
                 const int b = n % PB * BG + e;
@@ -544,54 +581,36 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, int h, int r, int s
                 o[b] = El<true>::mfma(f[n & 1][e], p0, o[b]);
             }
         } else {
+            if (n == PG) {
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) s.s[u][e] = 0.0f;
+            }
 #pragma unroll
             for (int x = 0; x < XG; x++) {
                 const int c = (n - PG) * XG + x;
                 if (c >= 2 * NB) continue;
 #pragma unroll
                 for (int u = 0; u < U; u++) {
-                    if (M::Q == 2) s[u] = El<true>::mfma(f[n & 1][x * U + u], q[M::Q - 1][c], s[u]);
-                    s[u] = El<true>::mfma(f[n & 1][x * U + u], q[0][c], s[u]);
+                    if (M::Q == 2) s.s[u] = El<true>::mfma(f[n & 1][x * U + u], q[M::Q - 1][c], s.s[u]);
+                    s.s[u] = El<true>::mfma(f[n & 1][x * U + u], q[0][c], s.s[u]);
                 }
             }
         }
     };
-    // Groups from .. to - 1, the first of which is in registers; between their products,
-    // in their shadow, this thread's part of V of tile t + 1 and K of t + 2 (role: 1 V,
-    // 2 K, 3 both), then the loads of the next ones.
-    auto products = [&](auto role, auto from, auto to, int t) __attribute__((always_inline)) {
-        constexpr int STEPS = to.value - from.value, ROLE = role.value;
-        constexpr int KW = ROLE & 2 ? NB : 0, VW = ROLE & 1 ? 2 * VN : 0, WORK = KW + VW + (ROLE ? 1 : 0);
-        if constexpr (to.value > PG) {
-#pragma unroll
-            for (int u = 0; u < U; u++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[u][e] = 0.0f;
-        }
-#pragma unroll
-        for (int n = from.value; n < to.value; n++) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (n + 1 < to.value) fetch(n + 1, t);
-            multiply(n);
-#pragma unroll
-            for (int x = (n - from.value) * WORK / STEPS; x < (n - from.value + 1) * WORK / STEPS; x++) {
-                if (x < KW) unpack_k(kr, x, t + 2);
-                else if (x < KW + VW) unpack_v(vr, (x - KW) >> 1, (x - KW) & 1, t + 1);
-                else {
-                    if constexpr (ROLE & 2) load_k(kr, kpage, t + 3), kpage = kpages(t + 4);
-                    if constexpr (ROLE & 1) {
-                        load_v(vr, vpage, t + 2);
-#pragma unroll
-                        for (int y = 0; y <= VN; y++) vpage[y] = vpages(t + 3, y);
-                    }
-                }
-            }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    auto softmax = [&](int t) __attribute__((always_inline)) {
-        const Scales sc = *reinterpret_cast<const Scales*>(lds + (t & 1) * M::STAGE + M::KB + M::VB);
-        float fs[BL];
+
+    // 16-bit rows have the blocks' shares in the exponents, f32 rows as a product, which keeps
+    // its digits.
+    constexpr bool FOLD = DT != TN_F32;
+    Scores s;
+    Probs p;
+    // role: what this thread unpacks, 1 V, 2 K, 3 both
+    auto turn = [&](auto roles, auto last_turn, int t) __attribute__((always_inline)) {
+        constexpr bool LAST = decltype(last_turn)::value;
+        constexpr int END = LAST ? PG : G, ROLE = decltype(roles)::value;
+        const Scales& sc = scales[t & 3];
+        float fs[BL], mb[BL];
 #pragma unroll
         for (int b = 0; b < BL; b++) fs[b] = rs * sc.ks[b];
         // the products' wait states: the compiler does not see that max3f's assembly reads their result
@@ -602,126 +621,147 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, int h, int r, int s
         __builtin_amdgcn_sched_barrier(0);
         if (KT * t + KT > least) {
 #pragma unroll
-            for (int u = 0; u < KT / 32; u++)
+            for (int u = 0; u < U; u++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int k = KT * t + 32 * u + 8 * (e >> 2) + 4 * hh + (e & 3);
-                    const float v = s[u][e] * fs[2 * u + (e >> 3)];
-                    s[u][e] = k >= keys ? -INFINITY : v;
+                    const float v = s.s[u][e] * fs[2 * u + (e >> 3)];
+                    s.s[u][e] = k >= keys ? -INFINITY : v;
                 }
 #pragma unroll
             for (int b = 0; b < BL; b++) fs[b] = 1.0f;
         }
-        float mb[BL];
 #pragma unroll
         for (int b = 0; b < BL; b++) {
-            const f32x16& x = s[b >> 1];
+            const f32x16& x = s.s[b >> 1];
             const int e = 8 * (b & 1);
             mb[b] = max3f(max3f(x[e], x[e + 1], x[e + 2]), max3f(x[e + 3], x[e + 4], x[e + 5]),
                           max3f(x[e + 6], x[e + 7], x[e + 7])) * fs[b];
         }
         const float mx = xor32_max(max3f(mb[0], mb[1], BL == 4 ? fmaxf(mb[BL - 2], mb[BL - 1]) : mb[1]));
-        if (__any(mx > m + RESCALE_SLACK)) {
-            const float mn = fmaxf(m, mx), al = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
-            m = mn;
-            l *= al;
+        const float step = sc.step;
+        vref = sc.vref;
+        const bool grew = __any(mx > m + RESCALE_SLACK);
+        if (grew || __builtin_amdgcn_readfirstlane(step != 1.0f)) {
+            float al = step;
+            if (grew) {
+                const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+                m = mn;
+                l *= f;
+                al *= f;
+            }
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[b][e] *= al;
         }
-        vref = sc.vref;
-        if (__builtin_amdgcn_readfirstlane(sc.step != 1.0f)) {
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) o[b][e] *= sc.step;
-        }
         const float mu = P_BIAS - (m == -INFINITY ? 0.0f : m);
-        // A block's share goes into its probabilities' exponent and out of their sum again: one
-        // operation for eight of them. (Not where it is far below the others' or 0: its
-        // probabilities would be lost to the sum. f32 rows keep the product's digits.)
-        if (DT != TN_F32 && __builtin_amdgcn_readfirstlane(sc.low >= 0x1p-6f)) {
+        auto probabilities = [&](int b) __attribute__((always_inline)) {  // of a block
+            const float ma = FOLD ? mu + sc.log[b] : mu, share = FOLD ? 1.0f : sc.share[b];
+            float lb = 0.0f;
 #pragma unroll
-            for (int b = 0; b < BL; b++) {
-                const float ma = mu + sc.log[b];
-                float lb = 0.0f;
-#pragma unroll
-                for (int e = 8 * (b & 1); e < 8 * (b & 1) + 8; e += 2) {
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][e], fs[b], ma));
-                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[b >> 1][e + 1], fs[b], ma));
-                    split_p<M::P>(p0, p1, ph[8 * (b >> 1) + e / 2], pl[8 * (b >> 1) + e / 2], lb);
-                }
-                l = fmaf(lb, sc.inv[b], l);
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < KT / 32; u++)
-#pragma unroll
-                for (int e = 0; e < 16; e += 2) {
-                    const int b = 2 * u + (e >> 3);
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[u][e], fs[b], mu));
-                    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[u][e + 1], fs[b], mu));
+            for (int e = 8 * (b & 1); e < 8 * (b & 1) + 8; e += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s.s[b >> 1][e], fs[b], ma));
+                const float p1 = __builtin_amdgcn_exp2f(fmaf(s.s[b >> 1][e + 1], fs[b], ma));
+                const int x = 8 * (b >> 1) + e / 2;
+                if constexpr (FOLD) {
+                    split_p<M::P>(p0, p1, p.h[x], p.l[x], lb);
+                } else {
+                    float none = 0.0f;
                     l += p0;
                     l += p1;
-                    float none = 0.0f;
-                    split_p<M::P>(p0 * sc.share[b], p1 * sc.share[b], ph[8 * u + e / 2], pl[8 * u + e / 2], none);
+                    split_p<M::P>(p0 * share, p1 * share, p.h[x], p.l[x], none);
                 }
-        }
+            }
+            if constexpr (FOLD) l = fmaf(lb, sc.inv[b], l);
+        };
+#pragma unroll
+        for (int b = 0; b < BL; b++) probabilities(b);
         // computed here, not where the products take them
 #if __HIP_DEVICE_COMPILE__
 #pragma unroll
         for (int e = 0; e < KT / 4; e++) {
-            asm volatile("" : "+v"(ph[e]));
-            if constexpr (M::P == 2) asm volatile("" : "+v"(pl[e]));
+            asm volatile("" : "+v"(p.h[e]));
+            if constexpr (M::P == 2) asm volatile("" : "+v"(p.l[e]));
         }
         asm volatile("" : "+v"(l));
 #endif
+        const int vslot = t & 1;
+        fetch(0, vslot);
+        if constexpr (M::GROUPS == 2) __syncthreads();
+        const uint32_t rest = LAST || !(ROLE & 1) ? ONES : rest_of(t + 1);
+        __builtin_amdgcn_s_setprio(1);  // the products' few instructions ahead of the other wave's many
+        // eight codes of V or of K at a time, then the next loads
+        constexpr int VW = ROLE & 1 ? 2 * N : 0, KW = ROLE & 2 ? 2 * N : 0, WORK = LAST ? 0 : VW + KW + 1;
+        auto work = [&](int x) __attribute__((always_inline)) {
+            if (x < VW) unpack_v(x >> 1, x & 1, t + 1, rest);
+            else if (x < VW + KW) unpack_k((x - VW) >> 1, x & 1, t + 2);
+            else {
+                if constexpr (ROLE & 1) load_v(vr, page_of(t + 2), t + 2);
+                if constexpr (ROLE & 2) load_k(kr, page_of(t + 3), t + 3);
+            }
+        };
+#pragma unroll
+        for (int n = 0; n < END; n++) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (n + 1 < END) fetch(n + 1, n + 1 < PG ? vslot : vslot ^ 1);
+            multiply(n, p, s);
+#pragma unroll
+            for (int x = n * WORK / G; x < (n + 1) * WORK / G; x++) work(x);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!LAST && (ROLE & 2) != 0) {
+            if (scaler) {
+                write_scales(t + 2);
+                load_scales(t + 3);
+                scale_page(t + 4);
+            }
+        }
+        __builtin_amdgcn_s_setprio(0);
+        if constexpr (!LAST) __syncthreads();
     };
-    auto walk = [&](auto role) __attribute__((always_inline)) {
-        constexpr std::integral_constant<int, 0> BEGIN, NONE;
-        constexpr std::integral_constant<int, PG> MIDDLE;
-        constexpr std::integral_constant<int, PG + SG> END;
+    auto walk = [&](auto roles) __attribute__((always_inline)) {
+        constexpr int ROLE = decltype(roles)::value;
         // all that the first tiles need is asked for before any of it is waited for
-        KPart k0, k1;
-        VPart v0;
-        int kp0 = 0, kp1 = 0, kp2 = 0, vp0[VN + 1] = {}, vp1[VN + 1] = {};
-        if constexpr (role.value & 2) kp0 = kpages(t0), kp1 = kpages(t0 + 1), kp2 = kpages(t0 + 2), kpage = kpages(t0 + 3);
-        if constexpr (role.value & 1) {
-#pragma unroll
-            for (int y = 0; y <= VN; y++) vp0[y] = vpages(t0, y), vp1[y] = vpages(t0 + 1, y), vpage[y] = vpages(t0 + 2, y);
-        }
+        Pieces k1;
         load_q();
-        if constexpr (role.value & 2) load_k(k0, kp0, t0), load_k(k1, kp1, t0 + 1), load_k(kr, kp2, t0 + 2);
-        if constexpr (role.value & 1) load_v(v0, vp0, t0), load_v(vr, vp1, t0 + 1);
+        if constexpr (ROLE & 2) load_k(k1, page_of(t0), t0), load_k(kr, page_of(t0 + 1), t0 + 1);
+        if constexpr (ROLE & 1) load_v(vr, page_of(t0), t0);
+        if (scaler) {
+            for (int t = t0; t < t0 + 2; t++) scale_page(t), load_scales(t), write_scales(t);
+            scale_page(t0 + 2);
+            load_scales(t0 + 2);
+            scale_page(t0 + 3);
+        }
         make_q();
-        if constexpr (role.value & 2) {
+        if constexpr (ROLE & 2) {
+            const Pieces k2 = kr;
+            kr = k1;
 #pragma unroll
-            for (int b = 0; b < NB; b++) unpack_k(k0, b, t0), unpack_k(k1, b, t0 + 1);
-        }
-        if constexpr (role.value & 1) {
+            for (int x = 0; x < 2 * N; x++) unpack_k(x >> 1, x & 1, t0);
+            kr = k2;
 #pragma unroll
-            for (int x = 0; x < 2 * VN; x++) unpack_v(v0, x >> 1, x & 1, t0);
+            for (int x = 0; x < 2 * N; x++) unpack_k(x >> 1, x & 1, t0 + 1);
+            load_k(kr, page_of(t0 + 2), t0 + 2);
+        }
+        __syncthreads();  // (the scales are there)
+        if constexpr (ROLE & 1) {
+            const uint32_t rest = rest_of(t0);
+#pragma unroll
+            for (int x = 0; x < 2 * N; x++) unpack_v(x >> 1, x & 1, t0, rest);
+            load_v(vr, page_of(t0 + 1), t0 + 1);
+        }
+        if (ROLE == 2) __syncthreads();  // half a turn behind
+        fetch(PG, t0 & 1);
+#pragma unroll
+        for (int n = PG; n < G; n++) {
+            if (n + 1 < G) fetch(n + 1, t0 & 1);
+            multiply(n, p, s);
         }
         __syncthreads();
-        if (role.value == 2) __syncthreads();  // half a turn behind
-        fetch(PG, t0 - 1);
-        products(NONE, MIDDLE, END, t0 - 1);
-        for (int t = t0; t + 1 < nt; t++) {
-            __syncthreads();
-            softmax(t);
-            fetch(0, t);
-            __syncthreads();
-            __builtin_amdgcn_s_setprio(1);  // the products' few instructions ahead of the other group's many
-            products(role, BEGIN, END, t);
-            __builtin_amdgcn_s_setprio(0);
-        }
-        __syncthreads();
-        softmax(nt - 1);
-        fetch(0, nt - 1);
-        __syncthreads();
-        products(NONE, BEGIN, MIDDLE, nt - 1);
-        if (role.value == 1) __syncthreads();
+        for (int t = t0; t + 1 < nt; t++) turn(roles, std::false_type{}, t);
+        turn(roles, std::true_type{}, nt - 1);
+        if (ROLE == 1) __syncthreads();
     };
     if (nt > t0) {
         if constexpr (M::GROUPS == 1) walk(std::integral_constant<int, 3>{});
@@ -729,6 +769,12 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, int h, int r, int s
         else walk(std::integral_constant<int, 2>{});
     }
 
+    // the last products' wait states, whatever their first reader is
+    __builtin_amdgcn_sched_barrier(0);
+#if __HIP_DEVICE_COMPILE__
+    asm volatile("s_nop 15\n\ts_nop 1");
+#endif
+    __builtin_amdgcn_sched_barrier(0);
     // out through LDS, so that a row's bytes leave together, in `type` to rows of a.out or (many_o) f32
     l = xor32_sum(l);
     uint8_t* mine = lds + w * 32 * M::OP;
@@ -767,7 +813,7 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, int h, int r, int s
         }
     };
     const int64_t row = (int64_t)(start + j) * a.Hq + hq;
-    if (M::GROUPS == 1 && ns > 1) {  // a split's part: k_paged8_join's
+    if (W == 4 && ns > 1) {  // a split's part: k_paged8_join's
         leave(std::integral_constant<int, TN_F32>{}, 1.0f, 1.0f);
         if (hh == 0 && i < rows) reinterpret_cast<Part*>(a.many_ml)[row * ns + split] = Part{m, l, vref, 0.0f};
     } else {
@@ -780,6 +826,7 @@ template <int DT, int NB, int W>
 __global__ __launch_bounds__(64 * W, (Many8<DT, NB, W>::WAVES)) void k_paged8_many(const Paged8Args a, int tiles) {
     constexpr int ROWS = 32 * W;
     __shared__ __align__(16) uint8_t lds[Many8<DT, NB, W>::LDS_BYTES];
+    __shared__ __align__(16) Scales scales[4];
     // the longest rows first; a key/value head's workgroups on the same die when there are eight
     const int h = (int)blockIdx.x % a.c.H, tile = tiles - 1 - (int)blockIdx.x / a.c.H;
     int r = 0;
@@ -796,7 +843,7 @@ __global__ __launch_bounds__(64 * W, (Many8<DT, NB, W>::WAVES)) void k_paged8_ma
     const int rows = min(all, a.max_rows) * a.G;
     if (first < 0 || first >= rows || rows <= a.few) return;  // few rows: k_paged8_few's
     const int len = max(0, min(a.lens[r], a.max_len)), before = len - all;
-    many8_tile<DT, NB, W>(a, lds, h, r, start, rows, first, len, before);
+    many8_tile<DT, NB, W>(a, lds, scales, h, r, start, rows, first, len, before);
 }
 
 // The splits of k_paged8_many's rows, in order: four output columns a thread.
