@@ -538,10 +538,9 @@ tn_status tn_kv_read_q8(void* stream, const tn_q8_cache* cache, const int32_t* s
  * of the largest such scale met: times what that ratio leaves, they are rounded
  * to f16. A query is one f16 under a power of two of its own (two f16 parts for
  * f32 rows); probabilities, times their values' block scale over the largest
- * met, are one f16 for bf16 rows, two for f32 rows, either for f16 rows (which,
- * goes by the call's size). The output is rounded once. Probabilities times
- * scales are held to 2^-30 of the row's largest probability times the largest
- * scale of values (lse counts them all).
+ * met, are one f16 for 16-bit rows, two for f32 rows. The output is rounded
+ * once. Probabilities times scales are held to 2^-30 of the row's largest
+ * probability times the largest scale of values (lse counts them all).
  * Scales are taken as finite and not negative.
  * `work`: as there, tn_sdpa_paged_q8_work_floats() floats. */
 int64_t tn_sdpa_paged_q8_work_floats(const tn_q8_cache* cache, int64_t n, int64_t tokens, int64_t Hq,

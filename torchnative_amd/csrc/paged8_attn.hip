@@ -26,12 +26,13 @@ struct Part {
     float m, l, v, pad;
 };
 
-// k_paged8_few's parts of each 16-bit operand: a 16-bit query is one f16 (a bf16 row
-// scaled by a power of two), an f32 one two; probabilities are two for an output of 11
-// or 24 bits, one for 8.
+// Parts of each 16-bit operand: a 16-bit query is one f16 (a bf16 row scaled by a power
+// of two), an f32 one two. Probabilities are one for an output of 16 bits: each is off by
+// half a step of f16, as the output itself is, and their errors do not add up in step; two
+// for f32 rows.
 template <int DT>
 struct Parts8 {
-    static constexpr int Q = DT == TN_F32 ? 2 : 1, P = DT == TN_BF16 ? 1 : 2;
+    static constexpr int Q = DT == TN_F32 ? 2 : 1, P = Q;
 };
 
 // Eight codes of two dwords as f16, exactly.
@@ -364,7 +365,7 @@ __global__ __launch_bounds__(256) void k_paged8_combine(const Paged8Args a) {
 // middle barrier.
 template <int DT, int NB, int W>
 struct Many8 {
-    static constexpr int Q = DT == TN_F32 ? 2 : 1, P = DT == TN_F32 ? 2 : 1;
+    static constexpr int Q = Parts8<DT>::Q, P = Parts8<DT>::P;
     static constexpr int ROWS = 32 * W;                                 // folded rows
     static constexpr int D = 32 * NB, KT = NB <= 4 ? 64 : 32;            // keys of a tile
     static constexpr int GROUPS = W / 4, BL = KT / 16, WPB = 4 / BL;     // groups of four waves; blocks, waves that unpack one
@@ -918,17 +919,21 @@ int64_t many_rows(const Pages8& c, int64_t tokens, int64_t G, int64_t max_len) {
 // every 16 folded rows but starts at once and splits finely; k_paged8_many fills 128 or 256
 // rows, and its tiles follow one another. So k_paged8_few takes all rows of a call whose
 // products (tokens * Hq * max_len * D) are few, and of a larger call the requests of up to
-// FEW_ROWS folded rows, if it is of several. Its grid is as long for every request as for
-// the longest: up to FEW_GRID workgroups of it.
+// FEW_ROWS folded rows, if it is of several. How many are few: a tile of k_paged8_many has
+// the same softmax and the same barriers for rows of 64 elements as for 128, so those wait
+// longer for it. Few against many, us, bf16: 64 elements, products / 2^30: 2 33 / 40, 4 48 / 50,
+// 9 62 / 66 (six ragged requests 6 45 / 58); 128: 2 31 / 32 and 33 / 36, 4 50 / 43 (ragged: 8
+// 64 / 65, 12 88 / 79); 256: 8 97 / 94, 16 157 / 111. f32, 128: 2 32 / 38, 4 56 / 54, 8 97 / 82. Its grid
+// is as long for every request as for the longest: up to FEW_GRID workgroups of it.
 constexpr int FEW_ROWS = 128;
-constexpr int64_t FEW_WORK = 1ll << 32, FEW_GRID = 8192;
+constexpr int64_t FEW_GRID = 8192;
+int64_t few_products(int nb) { return nb <= 3 ? 10ll << 30 : 3ll << 30; }
 
 // Folded rows of a request that k_paged8_few takes at most in this call; 0: it is not launched.
-int64_t few_limit(const Pages8& c, int dtype, int64_t n, int64_t tokens, int64_t G, int64_t max_rows, int64_t max_len) {
+int64_t few_limit(const Pages8& c, int64_t n, int64_t tokens, int64_t G, int64_t max_rows, int64_t max_len) {
     const int64_t rows = max_rows * G;
-    (void)dtype;
     // (tokens * Hq is at most 2^30, D 2^8)
-    const bool little = tokens * G * c.H * 32 * c.nb <= FEW_WORK / std::max<int64_t>(max_len, 1) &&
+    const bool little = tokens * G * c.H * 32 * c.nb <= few_products(c.nb) / std::max<int64_t>(max_len, 1) &&
                         n * c.H * cdiv(rows, 16) <= FEW_GRID;
     return rows <= FEW_ROWS || little ? rows : n > 1 ? FEW_ROWS : 0;
 }
@@ -1027,7 +1032,7 @@ tn_status tn_sdpa_paged_q8(void* stream, const tn_q8_cache* cache, int dtype, co
     a.q_stride = q_stride, a.n = (int)n, a.tokens = (int)tokens, a.Hq = (int)Hq, a.G = (int)G, a.width = (int)width;
     a.max_rows = (int)std::min(max_rows, tokens), a.max_len = (int)max_len;
     a.sl2 = (float)(sc * 1.4426950408889634);
-    a.few = (int)few_limit(a.c, dtype, n, tokens, G, a.max_rows, max_len);
+    a.few = (int)few_limit(a.c, n, tokens, G, a.max_rows, max_len);
     a.nsplit = few_splits(a.c, n, a.few, max_len);
     // f32 rows, then their parts: the few's and the many's
     const int64_t few = part_rows(a.c, n, a.max_rows * G, max_len);
