@@ -23,7 +23,7 @@ struct Row8Args {
     int64_t stride;
     const int32_t* slots;
     int64_t m;
-    int window;  // append: rows whose blocks a wave takes
+    int window;  // rows of a wave (append: rows whose blocks it takes)
 };
 
 // The plane row (of D bytes) of a slot and head: in v_codes, of its block's first byte
@@ -36,21 +36,77 @@ __device__ inline int checked_slot(const Pages8& c, int slot) {
     return slot >= 0 && (slot >> c.shift) < c.pages ? slot : -1;
 }
 
-// Eight consecutive elements at any element.
+// Eight consecutive elements at any element, as they lie and as numbers.
 template <int DT>
-__device__ inline void load8(const void* p, int64_t i, float (&v)[8]) {
-    float a[4], b[4];
-    load4<DT>(p, i, a);
-    load4<DT>(p, i + 4, b);
+struct Eight8 {
+    static constexpr int W = DT == TN_F32 ? 8 : 4;
+    typedef uint32_t words __attribute__((ext_vector_type(W), aligned(DT == TN_F32 ? 4 : 2)));
+    words w;
+    __device__ inline void load(const void* p, int64_t i) {
+        w = *reinterpret_cast<const words*>(static_cast<const char*>(p) + i * (DT == TN_F32 ? 4 : 2));
+    }
+    __device__ inline void clear() {
 #pragma unroll
-    for (int j = 0; j < 4; j++) v[j] = a[j], v[4 + j] = b[j];
+        for (int j = 0; j < W; j++) w[j] = 0;
+    }
+    __device__ inline float get(int j) const {
+        const uint32_t u = w[DT == TN_F32 ? j : j >> 1];  // (a copy: a cast of a vector's element is one of its first)
+        if constexpr (DT == TN_F32) return __builtin_bit_cast(float, u);
+        const uint16_t x = (uint16_t)(u >> (16 * (j & 1)));
+        return DT == TN_BF16 ? bf16_to_f32(x) : f16_bits_hw(x);
+    }
+};
+
+// The bytes of four values under 1 / scale: a sum with 1.5 * 2^23 rounds to an integer, halves
+// to even, whose low byte is the code's. ODD: values may be NaN, stored as 0 (infinities are
+// held to the largest codes either way).
+template <bool ODD>
+__device__ inline uint32_t bytes_of(const float (&v)[4], float inv) {
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        float c = v[j] * inv;
+        if (ODD) c = c == c ? c : 0.0f;
+        c = fminf(fmaxf(c, -127.0f), 127.0f);
+        u[j] = __builtin_bit_cast(uint32_t, c + 12582912.0f);
+    }
+#if __HIP_DEVICE_COMPILE__
+    const uint32_t lo = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
+    return (lo | hi) ^ 0x80808080u;
+#else
+    return u[0];
+#endif
 }
 
-// The byte of a value under 1 / scale: NaN as 0, infinities as the largest codes.
-__device__ inline uint32_t byte_of(float v, float inv) {
-    float c = v * inv;
-    c = c == c ? fminf(fmaxf(rintf(c), -127.0f), 127.0f) : 0.0f;
-    return (uint32_t)((int)c + 128);
+// Four bytes of each of a quad's lanes, transposed: byte i of lane j is byte j of lane i.
+__device__ inline uint32_t quad_transposed(uint32_t w, int lane) {
+#if __HIP_DEVICE_COMPILE__
+    const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0xB1, 0xf, 0xf, true);  // lane ^ 1
+    const uint32_t v = __builtin_amdgcn_perm(y, w, lane & 1 ? 0x03070105u : 0x06020400u);
+    const uint32_t z = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true);  // lane ^ 2
+    return __builtin_amdgcn_perm(z, v, lane & 2 ? 0x03020706u : 0x05040100u);
+#else
+    return w + (uint32_t)lane;
+#endif
+}
+
+template <int DT>
+__device__ inline void store8(void* p, int64_t i, const float (&lo)[4], const float (&hi)[4]) {
+    if constexpr (DT == TN_F32) {
+        store4<DT>(p, i, lo);
+        store4<DT>(p, i + 4, hi);
+    } else {
+        typedef uint32_t w4 __attribute__((ext_vector_type(4), aligned(2)));
+        using E = El<DT == TN_F16>;
+        *reinterpret_cast<w4*>(static_cast<uint16_t*>(p) + i) =
+            (w4){E::pack_out(lo[0], lo[1]), E::pack_out(lo[2], lo[3]), E::pack_out(hi[0], hi[1]), E::pack_out(hi[2], hi[3])};
+    }
+}
+
+// A dword's bytes as codes.
+__device__ inline void codes_of(uint32_t w, float scale, float (&y)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) y[j] = (float)((int)(w >> (8 * j) & 0xffu) - 128) * scale;
 }
 
 // The bytes of a dword under a scale that grew by 1 / ratio.
@@ -68,7 +124,8 @@ __device__ inline uint32_t lowered(uint32_t w, float ratio) {
 // head, of K or of V: the rows of a block lie within sixteen rows of the call.
 template <int DT, int NB>
 __global__ __launch_bounds__(256) void k_append8(const Row8Args a) {
-    constexpr int D = 32 * NB, C = D / 8;  // pieces of eight elements a row; NB of 64 lanes cover 16 rows
+    // C pieces of eight elements a row: NB of 64 lanes cover 16 rows; U of 64 elements a row
+    constexpr int D = 32 * NB, C = D / 8, U = (D + 63) / 64;
     __shared__ __align__(16) uint8_t tile[4][16 * D];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y;
     const bool v = blockIdx.z;
@@ -79,68 +136,79 @@ __global__ __launch_bounds__(256) void k_append8(const Row8Args a) {
     if (t0 + 15 >= a.m) return;  // (no barrier below)
     const int64_t t = t0 + lane;
     const int slot = t >= 0 && t < a.m ? checked_slot(a.c, a.slots[t]) : -1;
-    const int block = slot < 0 ? -1 - lane : slot >> 4;  // (of no row: its own)
-    bool joins = slot < 0, twice = false;
-#pragma unroll
-    for (int j = 1; j < 16; j++) {
-        joins |= __shfl_up(block, j) == block && lane >= j;
-        twice |= __shfl_down(slot, j) == slot && lane + j < 64;
-    }
-    uint64_t firsts = __ballot(!joins && lane >= 15 && lane < 15 + a.window);
-    const uint64_t again = __ballot(twice && slot >= 0);
-    while (firsts) {
-        const int i = __ffsll((unsigned long long)firsts) - 1;  // the first row's lane
-        firsts &= firsts - 1;
-        const int b = __builtin_amdgcn_readlane(block, i);
-        uint64_t rows = __ballot(block == b) & (0xffffull << i);  // lanes of its rows
-        if (rows & again) {  // of a slot given twice the last counts
-            bool drop = false;
-#pragma unroll
-            for (int j = 1; j < 16; j++)
-                drop |= __shfl_down(slot, j) == slot && lane + j < 64 && (rows >> ((lane + j) & 63) & 1);
-            rows &= ~__ballot(drop);
+    for (uint64_t left = __ballot(slot >= 0 && lane >= 15 && lane < 15 + a.window); left;) {
+        const int i = __ffsll((unsigned long long)left) - 1, first = __builtin_amdgcn_readlane(slot, i), b = first >> 4;
+        const uint64_t same = __ballot(slot >> 4 == b);
+        left &= ~same;
+        if (same & (0x7fffull << (i - 15))) continue;  // an earlier row's
+        uint64_t rows = same & (0xffffull << i);  // lanes of the block's rows
+        uint32_t tokens = (uint32_t)(rows >> i) << (first & 15);
+        if (rows & ~__ballot(slot - first == lane - i)) {  // out of order; of a slot given twice the last counts
+            tokens = 0;
+            for (uint64_t t = rows; t;) {
+                const int last = 63 - __clzll((long long)t);
+                const uint32_t bit = 1u << (__builtin_amdgcn_readlane(slot, last) & 15);
+                t &= ~(1ull << last);
+                if (tokens & bit) rows &= ~(1ull << last);
+                tokens |= bit;
+            }
         }
-        uint32_t tokens = 0;
-        for (uint64_t left = rows; left; left &= left - 1)
-            tokens |= 1u << (__builtin_amdgcn_readlane(slot, __ffsll((unsigned long long)left) - 1) & 15);
-        float x[NB][8];
-        float top = 0.0f;
+        // all that the block's part needs is asked for at once
+        const int64_t prow = plane_row(a.c, b << 4, h);
+        const bool fresh = tokens & 1;  // a row at its first slot begins a block anew
+        float old = fresh ? 0.0f : scales[prow >> 4];
+        uint8_t* to = plane + prow * D;
+        uint4 held[U];
+        if (v && tokens != 0xffff)
+#pragma unroll
+            for (int u = 0; u < U; u++) held[u] = *reinterpret_cast<const uint4*>(to + 16 * min(64 * u + lane, D - 1));
+        Eight8<DT> x[NB];
         int token[NB];  // of this lane's piece of pass p, -1: none
 #pragma unroll
         for (int p = 0; p < NB; p++) {
             const int it = p * 64 + lane, r = it / C, c = it % C;
             const int s = __shfl(slot, i + r);
             token[p] = rows >> (i + r) & 1 ? s & 15 : -1;
-            if (token[p] >= 0) load8<DT>(src, (t0 + i + r) * a.stride + (int64_t)h * D + 8 * c, x[p]);
-            else
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[p][j] = 0.0f;
+            if (token[p] >= 0) x[p].load(src, (t0 + i + r) * a.stride + (int64_t)h * D + 8 * c);
+            else x[p].clear();
         }
+        float top = 0.0f, bad = 0.0f;  // bad: NaN if a value is not finite
 #pragma unroll
         for (int p = 0; p < NB; p++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float s = fabsf(x[p][j]);
-                top = s < INFINITY ? fmaxf(top, s) : top;
+                const float s = x[p].get(j);
+                top = fmaxf(top, fabsf(s));
+                bad = fmaf(s, 0.0f, bad);
             }
+        const bool odd = __any(bad != bad);
+        if (odd) {
+            top = 0.0f;
+#pragma unroll
+            for (int p = 0; p < NB; p++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float s = fabsf(x[p].get(j));
+                    top = s < INFINITY ? fmaxf(top, s) : top;
+                }
+        }
         top = xor32_max(xor16_max(row16_max(top)));
-        const int64_t prow = plane_row(a.c, b << 4, h);
-        const bool fresh = tokens & 1;  // a row at its first slot begins a block anew
-        float old = fresh ? 0.0f : scales[prow >> 4];
         if (!(old > 0.0f && old < INFINITY)) old = 0.0f;
         const float s = fmaxf(old, top > 0.0f ? fmaxf(top * (1.0f / 127.0f), MIN_SCALE) : 0.0f);
         const float inv = s > 0.0f ? 1.0f / s : 0.0f;
         const bool grew = !fresh && s > old;
         const float ratio = grew ? old / s : 1.0f;
         if (lane == 0) scales[prow >> 4] = s;
-        uint8_t* to = plane + prow * D;
         uint8_t* mine = tile[w];
 #pragma unroll
         for (int p = 0; p < NB; p++) {
             if (token[p] < 0) continue;
-            uint32_t o[2] = {0, 0};
+            uint32_t o[2];
 #pragma unroll
-            for (int j = 0; j < 8; j++) o[j >> 2] |= byte_of(x[p][j], inv) << (8 * (j & 3));
+            for (int e = 0; e < 2; e++) {
+                const float y[4] = {x[p].get(4 * e), x[p].get(4 * e + 1), x[p].get(4 * e + 2), x[p].get(4 * e + 3)};
+                o[e] = odd ? bytes_of<true>(y, inv) : bytes_of<false>(y, inv);
+            }
             const int c = (p * 64 + lane) % C;
             *reinterpret_cast<uint2*>((v ? mine : to) + token[p] * D + 8 * c) = make_uint2(o[0], o[1]);
         }
@@ -154,60 +222,105 @@ __global__ __launch_bounds__(256) void k_append8(const Row8Args a) {
             }
         } else {  // through LDS: sixteen tokens of an element leave together
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            for (int d = lane; d < D; d += 64) {
-                uint32_t o[4] = {0, 0, 0, 0};
-                uint4* p = reinterpret_cast<uint4*>(to + d * 16);
+#pragma unroll
+            for (int u = 0; u < U; u++) {  // (D is a multiple of a half wave: a quad's lanes go together)
+                const int d = 64 * u + lane;
+                if (d >= D) break;
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    o[j] = quad_transposed(*reinterpret_cast<const uint32_t*>(mine + (4 * j + (d & 3)) * D + (d & ~3)), lane);
                 if (tokens != 0xffff) {
-                    const uint4 u = *p;
-                    o[0] = u.x, o[1] = u.y, o[2] = u.z, o[3] = u.w;
-                    if (grew)
+                    const uint32_t was[4] = {held[u].x, held[u].y, held[u].z, held[u].w};
 #pragma unroll
-                        for (int j = 0; j < 4; j++) o[j] = lowered(o[j], ratio);
+                    for (int j = 0; j < 4; j++) {
+                        // a byte of ones for each new token
+                        const uint32_t bits = tokens >> (4 * j) & 15u, mask = (bits * 0x00204081u & 0x01010101u) * 0xffu;
+                        const uint32_t w = grew ? lowered(was[j], ratio) : was[j];
+                        o[j] = (o[j] & mask) | (w & ~mask);
+                    }
                 }
-#pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if (tokens >> r & 1)
-                        o[r >> 2] = (o[r >> 2] & ~(0xffu << (8 * (r & 3)))) | (uint32_t)mine[r * D + d] << (8 * (r & 3));
-                *p = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4*>(to + d * 16) = make_uint4(o[0], o[1], o[2], o[3]);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
     }
 }
 
-// A workgroup takes 16 rows of one head, of K or of V: eight elements a thread.
-template <int DT>
+// A wave takes the rows of its window, of one head, of K or of V: K's eight elements a lane;
+// of V all the rows of one block together, whose elements come as sixteen tokens and are
+// turned in quads of lanes.
+template <int DT, int NB>
 __global__ __launch_bounds__(256) void k_read8(const Row8Args a) {
-    const int D = 32 * a.c.nb, C = D / 8, h = blockIdx.y;
-    const bool v = blockIdx.z;
-    const int64_t r0 = (int64_t)blockIdx.x * 16;
-    for (int it = threadIdx.x; it < 16 * C; it += 256) {
-        const int64_t t = r0 + it / C;
-        const int c = it % C;
-        if (t >= a.m) break;
-        const int slot = checked_slot(a.c, a.slots[t]);
-        float y[8];
-        if (slot < 0) {
+    constexpr int D = 32 * NB, C = D / 8, U = (D + 63) / 64;
+    __shared__ int row_at[4][16];  // of a block's token: the wave's row that is to have it
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = blockIdx.y;
+    const int64_t t0 = ((int64_t)blockIdx.x * 4 + w) * a.window;
+    if (t0 >= a.m) return;  // (no barrier below)
+    const bool is_row = lane < a.window && t0 + lane < a.m;
+    const int slot = is_row ? checked_slot(a.c, a.slots[t0 + lane]) : -1;
+    if (blockIdx.z == 0) {
+        uint2 u[NB];
+        float s[NB];
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = NAN;
-        } else if (!v) {
-            const int64_t row = plane_row(a.c, slot, h);
-            const uint2 u = *reinterpret_cast<const uint2*>(a.c.kc + row * D + 8 * c);
-            const float s = a.c.ks[row >> 4];
-#pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = (float)((int)((j < 4 ? u.x : u.y) >> (8 * (j & 3)) & 0xffu) - 128) * s;
-        } else {
-            const int64_t row = plane_row(a.c, slot & ~15, h);
-            const uint8_t* p = a.c.vc + row * D + 8 * c * 16 + (slot & 15);
-            const float s = a.c.vs[row >> 4];
-#pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = (float)((int)p[16 * j] - 128) * s;
+        for (int p = 0; p < NB; p++) {
+            if (p && a.window == 1) break;
+            const int it = p * 64 + lane, at = __shfl(slot, it / C);
+            u[p] = make_uint2(0, 0), s[p] = NAN;
+            if (at < 0) continue;  // (a cache may have no row at all)
+            const int64_t row = plane_row(a.c, at, h);
+            u[p] = *reinterpret_cast<const uint2*>(a.c.kc + row * D + 8 * (it % C));
+            s[p] = a.c.ks[row >> 4];
         }
-        void* out = v ? a.vo : a.ko;
-        const int64_t o = (t * a.c.H + h) * D + 8 * c;
-        const float lo[4] = {y[0], y[1], y[2], y[3]}, hi[4] = {y[4], y[5], y[6], y[7]};
-        store4<DT>(out, o, lo);
-        store4<DT>(out, o + 4, hi);
+#pragma unroll
+        for (int p = 0; p < NB; p++) {
+            if (p && a.window == 1) break;
+            const int it = p * 64 + lane, r = it / C;
+            if (r >= a.window || t0 + r >= a.m) continue;
+            const int64_t o = ((t0 + r) * a.c.H + h) * D + 8 * (it % C);
+            float lo[4], hi[4];
+            codes_of(u[p].x, s[p], lo);
+            codes_of(u[p].y, s[p], hi);
+            store8<DT>(a.ko, o, lo, hi);
+        }
+        return;
+    }
+    auto put = [&](int r, int d, uint32_t word, float scale) __attribute__((always_inline)) {
+        float y[4];
+        codes_of(word, scale, y);
+        store4<DT>(a.vo, ((t0 + r) * a.c.H + h) * D + d, y);
+    };
+    for (uint64_t left = __ballot(is_row && slot < 0); left; left &= left - 1)
+        for (int d = 4 * lane; d < D; d += 256) put(__ffsll((unsigned long long)left) - 1, d, 0, NAN);
+    for (uint64_t left = __ballot(slot >= 0); left;) {
+        const int b = __builtin_amdgcn_readlane(slot, __ffsll((unsigned long long)left) - 1) >> 4;
+        const int64_t row = plane_row(a.c, b << 4, h);
+        uint4 u[U];
+#pragma unroll
+        for (int x = 0; x < U; x++)
+            u[x] = *reinterpret_cast<const uint4*>(a.c.vc + row * D + 16 * min(64 * x + lane, D - 1));
+        const float s = a.c.vs[row >> 4];
+        int* at = row_at[w];
+        const bool mine = (left >> lane & 1) && slot >> 4 == b;
+        if (lane < 16) at[lane] = -1;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (mine) at[slot & 15] = lane;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        left &= ~__ballot(mine && at[slot & 15] == lane);  // (of a slot given twice one row a time)
+        int to[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) to[j] = at[4 * j + (lane & 3)];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int x = 0; x < U; x++) {
+            const int d = 64 * x + (lane & ~3);
+            const uint32_t held[4] = {u[x].x, u[x].y, u[x].z, u[x].w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t word = quad_transposed(held[j], lane);
+                if (to[j] >= 0 && d < D) put(to[j], d, word, s);
+            }
+        }
     }
 }
 
@@ -226,9 +339,19 @@ void append_launch(hipStream_t st, const Row8Args& a) {
 
 template <int DT>
 void read_launch(hipStream_t st, const Row8Args& a) {
-    const dim3 grid((unsigned)cdiv(a.m, 16), (unsigned)a.c.H, 2);
-    hipLaunchKernelGGL(k_read8<DT>, grid, dim3(256), 0, st, a);
+    const dim3 grid((unsigned)cdiv(a.m, 4 * a.window), (unsigned)a.c.H, 2);
+#define TN_READ(NB)                                                                        \
+    case NB:                                                                               \
+        hipLaunchKernelGGL((k_read8<DT, NB>), grid, dim3(256), 0, st, a);                  \
+        break;
+    switch (a.c.nb) {
+        TN_READ(1) TN_READ(2) TN_READ(3) TN_READ(4) TN_READ(5) TN_READ(6) TN_READ(7) TN_READ(8)
+    }
+#undef TN_READ
 }
+
+// Rows of a wave's window: few rows have a wave each, so that no block waits for another.
+int window_of(int64_t m) { return m <= 1024 ? 1 : 16; }
 
 tn_status row_check(const char* op, const tn_q8_cache* cache, int dtype, int64_t m, Row8Args* a) {
     TN_TRY(paged_check(op, cache, &a->c));
@@ -260,7 +383,7 @@ tn_status tn_kv_append_q8(void* stream, const tn_q8_cache* cache, int dtype, con
     if (!k || !v || !slots) return fail(TN_EVALUE, "kv_append_q8: null pointer");
     TN_TRY(paged_check_planes(op, a.c));
     a.k = k, a.v = v, a.stride = stride, a.slots = slots;
-    a.window = m <= 1024 ? 1 : 16;
+    a.window = window_of(m);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == TN_F32) append_launch<TN_F32>(st, a);
     else if (dtype == TN_BF16) append_launch<TN_BF16>(st, a);
@@ -278,6 +401,7 @@ tn_status tn_kv_read_q8(void* stream, const tn_q8_cache* cache, const int32_t* s
     if (!k || !v || !slots) return fail(TN_EVALUE, "kv_read_q8: null pointer");
     TN_TRY(paged_check_planes(op, a.c));
     a.ko = k, a.vo = v, a.slots = slots;
+    a.window = window_of(m);
     hipStream_t st = (hipStream_t)stream;
     if (dtype == TN_F32) read_launch<TN_F32>(st, a);
     else if (dtype == TN_BF16) read_launch<TN_BF16>(st, a);
