@@ -33,81 +33,59 @@ __device__ inline float scale_of(float top) { return top > 0.0f ? fmaxf(top * (1
 
 // Eight elements from i on of a row of k, zeros behind it.
 template <int DT>
-__device__ __attribute__((always_inline)) inline void load_row8(const void* x, int64_t row, int i, int k, float (&v)[8]) {
-    if (i + 8 <= k) {
-        float a[4], b[4];
-        load4<DT>(x, row + i, a);
-        load4<DT>(x, row + i + 4, b);
-#pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = a[j], v[4 + j] = b[j];
-        return;
-    }
+TN_INLINE void load_row8(const void* x, int64_t row, int i, int k, Eight<DT>& v) {
+    if (i + 8 <= k) return v.load(x, row + i);
+    v.clear();
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        v[j] = 0.0f;
-        if (i + j < k) {
-            if constexpr (DT == TN_F32) v[j] = static_cast<const float*>(x)[row + i + j];
-            else {
-                const uint16_t h = static_cast<const uint16_t*>(x)[row + i + j];
-                v[j] = DT == TN_BF16 ? bf16_to_f32(h) : f16_bits_hw(h);
-            }
-        }
+        if (i + j >= k) continue;
+        if constexpr (DT == TN_F32) v.w[j >> 2][j & 3] = static_cast<const uint32_t*>(x)[row + i + j];
+        else v.w[0][j >> 1] |= (uint32_t) static_cast<const uint16_t*>(x)[row + i + j] << (16 * (j & 1));
     }
 }
 
-// Onto the largest finite size, and whether all were finite.
-__device__ inline void measure(const float (&v)[8], float& top, bool& odd) {
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float a = fabsf(v[j]);
-        odd |= !(a < INFINITY);
-        top = a < INFINITY ? fmaxf(top, a) : top;
-    }
-}
-
-// The eight codes of v under 1 / scale (0 for a row that is not finite).
-__device__ inline uint2 codes8(const float (&v)[8], float inv, bool odd) {
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float c = fminf(fmaxf(rintf(v[j] * inv), -127.0f), 127.0f);
-        w[j >> 2] |= ((uint32_t)(int)c & 0xffu) << (8 * (j & 3));
-    }
-    return odd ? make_uint2(0, 0) : make_uint2(w[0], w[1]);
+// The eight codes of v under 1 / scale (0 for a row that is not finite). No value's is past
+// +-127: the scale's two roundings and its inverse's leave 127 (1 + 2^-22) at most.
+template <int DT>
+TN_INLINE uint2 codes8(const Eight<DT>& v, float inv, bool odd) {
+    if (odd) return make_uint2(0, 0);
+    return make_uint2(rounded_bytes(v.get(0) * inv, v.get(1) * inv, v.get(2) * inv, v.get(3) * inv),
+                      rounded_bytes(v.get(4) * inv, v.get(5) * inv, v.get(6) * inv, v.get(7) * inv));
 }
 
 // T threads a row, which hold up to eight times HOLD elements each and read what is past
-// these again. Bound by memory where rows are many, by a launch where few.
-constexpr int HOLD = 4;
-template <int DT, int T>
+// these again: a wave where it holds the row, so that nothing waits at a barrier. Bound by
+// memory where rows are many (bf16, 4096 of 4096 elements 9.5 us, 5.3 TB/s; of 14336 36 us, 4.9),
+// by a launch where few (sixteen of 4096 3.2 us).
+template <int DT, int T, int HOLD>
 __global__ __launch_bounds__(256) void k_i8_rows(const void* __restrict__ x, int m, int k, int8_t* __restrict__ codes,
                                                  float* __restrict__ scales) {
     constexpr int RW = 256 / T;
     __shared__ float red[4];
-    __shared__ int bad[4];
+    __shared__ int bads[4];
     const int tid = threadIdx.x % T, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * RW + threadIdx.x / T;
     const bool on = row < m;
     const int64_t at = (on ? row : 0) * k;
     const int pitch = (int)pitch_of(k);
-    float v[HOLD][8], top = 0.0f;
-    bool odd = false;
+    Eight<DT> v[HOLD];
+    float top = 0.0f, bad = 0.0f;
 #pragma unroll
     for (int h = 0; h < HOLD; h++) load_row8<DT>(x, at, 8 * (h * T + tid), k, v[h]);
 #pragma unroll
-    for (int h = 0; h < HOLD; h++) measure(v[h], top, odd);
+    for (int h = 0; h < HOLD; h++) measure(v[h], top, bad);
     for (int i = 8 * (HOLD * T + tid); i < k; i += 8 * T) {
-        float u[8];
+        Eight<DT> u;
         load_row8<DT>(x, at, i, k, u);
-        measure(u, top, odd);
+        measure(u, top, bad);
     }
     top = xor32_max(xor16_max(row16_max(top)));
-    odd = __any(odd);
+    bool odd = __any(bad != bad);
     if constexpr (T > 64) {
-        if (lane == 0) red[w] = top, bad[w] = odd;
+        if (lane == 0) red[w] = top, bads[w] = odd;
         __syncthreads();
         top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        odd = bad[0] | bad[1] | bad[2] | bad[3];
+        odd = bads[0] | bads[1] | bads[2] | bads[3];
     }
     if (!on) return;
     const float s = scale_of(top), inv = s > 0.0f ? 1.0f / s : 0.0f;
@@ -119,7 +97,7 @@ __global__ __launch_bounds__(256) void k_i8_rows(const void* __restrict__ x, int
         if (i < pitch) *reinterpret_cast<uint2*>(out + i) = codes8(v[h], inv, odd);
     }
     for (int i = 8 * (HOLD * T + tid); i < pitch; i += 8 * T) {
-        float u[8];
+        Eight<DT> u;
         load_row8<DT>(x, at, i, k, u);
         *reinterpret_cast<uint2*>(out + i) = codes8(u, inv, odd);
     }
@@ -552,17 +530,17 @@ __global__ __launch_bounds__(64 * FEW_W) void k_i8_fused(const MmArgs a, const v
     for (int u = 0; u < FEW_U; u++) w[u] = *reinterpret_cast<const i32x4*>(pw + 64 * min(k + u, steps - 1));
     for (int r = 0; r < a.m; r++) {
         const int64_t at = (int64_t)r * k_len;
-        float v[8], top = 0.0f;
-        bool odd = false;
+        Eight<DT> v;
+        float top = 0.0f, nan = 0.0f;
         load_row8<DT>(x, at, 8 * tid, k_len, v);
-        measure(v, top, odd);
+        measure(v, top, nan);
         for (int i = 8 * (64 * FEW_W + tid); i < k_len; i += 8 * 64 * FEW_W) {
-            float y[8];
+            Eight<DT> y;
             load_row8<DT>(x, at, i, k_len, y);
-            measure(y, top, odd);
+            measure(y, top, nan);
         }
         top = xor32_max(xor16_max(row16_max(top)));
-        odd = __any(odd);
+        bool odd = __any(nan != nan);
         if (lane == 0) red[wave] = top, bad[wave] = odd;
         __syncthreads();
         odd = false;
@@ -573,7 +551,7 @@ __global__ __launch_bounds__(64 * FEW_W) void k_i8_fused(const MmArgs a, const v
         int8_t* out = codes + r * a.pitch;
         if (8 * tid < a.pitch) *reinterpret_cast<uint2*>(out + 8 * tid) = codes8(v, inv, odd);
         for (int i = 8 * (64 * FEW_W + tid); i < a.pitch; i += 8 * 64 * FEW_W) {
-            float y[8];
+            Eight<DT> y;
             load_row8<DT>(x, at, i, k_len, y);
             *reinterpret_cast<uint2*>(out + i) = codes8(y, inv, odd);
         }
@@ -654,9 +632,11 @@ tn_status matmul(hipStream_t st, const MmArgs& a) {
 
 template <int DT>
 void rows_launch(hipStream_t st, const void* x, int m, int k, int8_t* codes, float* scales) {
-    if (k <= 64 * 8 * HOLD)
-        hipLaunchKernelGGL((k_i8_rows<DT, 64>), dim3((unsigned)cdiv(m, 4)), dim3(256), 0, st, x, m, k, codes, scales);
-    else hipLaunchKernelGGL((k_i8_rows<DT, 256>), dim3((unsigned)m), dim3(256), 0, st, x, m, k, codes, scales);
+    const dim3 waves((unsigned)cdiv(m, 4)), rows((unsigned)m);
+    if (k <= 2048) hipLaunchKernelGGL((k_i8_rows<DT, 64, 4>), waves, dim3(256), 0, st, x, m, k, codes, scales);
+    else if (k <= 4096)
+        hipLaunchKernelGGL((k_i8_rows<DT, 64, 8>), waves, dim3(256), 0, st, x, m, k, codes, scales);
+    else hipLaunchKernelGGL((k_i8_rows<DT, 256, 4>), rows, dim3(256), 0, st, x, m, k, codes, scales);
 }
 
 tn_status quantize(hipStream_t st, const void* x, int dtype, int64_t m, int64_t k, int8_t* codes, float* scales) {

@@ -5,6 +5,8 @@
 
 #include "attn_common.h"
 
+#define TN_INLINE __device__ __attribute__((always_inline)) inline
+
 namespace tn {
 
 struct Pages {
@@ -60,6 +62,46 @@ __device__ inline void store4(void* p, int64_t i, const float (&v)[4]) {
         using E = El<DT == TN_F16>;
         *reinterpret_cast<w2*>(static_cast<uint16_t*>(p) + i) = (w2){E::pack_out(v[0], v[1]), E::pack_out(v[2], v[3])};
     }
+}
+
+// Eight consecutive elements of a row of type DT, at any element.
+template <int DT>
+struct Eight {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+    u4 w[DT == TN_F32 ? 2 : 1];
+    TN_INLINE void load(const void* p, int64_t i) {
+        const u4* s = reinterpret_cast<const u4*>(static_cast<const char*>(p) + i * (DT == TN_F32 ? 4 : 2));
+        w[0] = s[0];
+        if constexpr (DT == TN_F32) w[1] = s[1];
+    }
+    TN_INLINE void clear() { w[0] = w[DT == TN_F32 ? 1 : 0] = (u4){0, 0, 0, 0}; }
+    TN_INLINE float get(int e) const {
+        if constexpr (DT == TN_F32) return __uint_as_float(w[e >> 2][e & 3]);
+        else return e & 1 ? El<DT == TN_F16>::hi(w[0][e >> 1]) : El<DT == TN_F16>::lo(w[0][e >> 1]);
+    }
+};
+
+// Onto the largest size but NaN's, and onto what is NaN behind an infinity or a NaN.
+template <int DT>
+TN_INLINE void measure(const Eight<DT>& x, float& top, float& bad) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float v = x.get(j);
+        top = fmaxf(top, fabsf(v));
+        bad = fmaf(v, 0.0f, bad);
+    }
+}
+
+// Four numbers of size 2^22 at most rounded to integers, halves to even, of which the low
+// bytes: a sum with 1.5 * 2^23 has a step of one.
+TN_INLINE uint32_t rounded_bytes(float a, float b, float c, float d) {
+#if __HIP_DEVICE_COMPILE__
+    constexpr float M = 12582912.0f;
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(b + M), __float_as_uint(a + M), 0x0c0c0400u);
+    return lo | __builtin_amdgcn_perm(__float_as_uint(d + M), __float_as_uint(c + M), 0x04000c0cu);
+#else
+    return (uint32_t)(a + b + c + d);
+#endif
 }
 
 }  // namespace tn

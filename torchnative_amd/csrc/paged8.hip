@@ -36,46 +36,18 @@ __device__ inline int checked_slot(const Pages8& c, int slot) {
     return slot >= 0 && (slot >> c.shift) < c.pages ? slot : -1;
 }
 
-// Eight consecutive elements at any element, as they lie and as numbers.
-template <int DT>
-struct Eight8 {
-    static constexpr int W = DT == TN_F32 ? 8 : 4;
-    typedef uint32_t words __attribute__((ext_vector_type(W), aligned(DT == TN_F32 ? 4 : 2)));
-    words w;
-    __device__ inline void load(const void* p, int64_t i) {
-        w = *reinterpret_cast<const words*>(static_cast<const char*>(p) + i * (DT == TN_F32 ? 4 : 2));
-    }
-    __device__ inline void clear() {
-#pragma unroll
-        for (int j = 0; j < W; j++) w[j] = 0;
-    }
-    __device__ inline float get(int j) const {
-        const uint32_t u = w[DT == TN_F32 ? j : j >> 1];  // (a copy: a cast of a vector's element is one of its first)
-        if constexpr (DT == TN_F32) return __builtin_bit_cast(float, u);
-        const uint16_t x = (uint16_t)(u >> (16 * (j & 1)));
-        return DT == TN_BF16 ? bf16_to_f32(x) : f16_bits_hw(x);
-    }
-};
-
-// The bytes of four values under 1 / scale: a sum with 1.5 * 2^23 rounds to an integer, halves
-// to even, whose low byte is the code's. ODD: values may be NaN, stored as 0 (infinities are
-// held to the largest codes either way).
+// The bytes of four values under 1 / scale. ODD: values may be NaN, stored as 0 (infinities
+// are held to the largest codes either way).
 template <bool ODD>
-__device__ inline uint32_t bytes_of(const float (&v)[4], float inv) {
-    uint32_t u[4];
+TN_INLINE uint32_t bytes_of(const float (&v)[4], float inv) {
+    float c[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        float c = v[j] * inv;
-        if (ODD) c = c == c ? c : 0.0f;
-        c = fminf(fmaxf(c, -127.0f), 127.0f);
-        u[j] = __builtin_bit_cast(uint32_t, c + 12582912.0f);
+        c[j] = v[j] * inv;
+        if (ODD) c[j] = c[j] == c[j] ? c[j] : 0.0f;
+        c[j] = fminf(fmaxf(c[j], -127.0f), 127.0f);
     }
-#if __HIP_DEVICE_COMPILE__
-    const uint32_t lo = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x04000c0cu);
-    return (lo | hi) ^ 0x80808080u;
-#else
-    return u[0];
-#endif
+    return rounded_bytes(c[0], c[1], c[2], c[3]) ^ 0x80808080u;
 }
 
 // Four bytes of each of a quad's lanes, transposed: byte i of lane j is byte j of lane i.
@@ -165,7 +137,7 @@ __global__ __launch_bounds__(256) void k_append8(const Row8Args a) {
         if (v && tokens != 0xffff)
 #pragma unroll
             for (int u = 0; u < U; u++) held[u] = *reinterpret_cast<const uint4*>(to + 16 * min(64 * u + lane, D - 1));
-        Eight8<DT> x[NB];
+        Eight<DT> x[NB];
         int token[NB];  // of this lane's piece of pass p, -1: none
 #pragma unroll
         for (int p = 0; p < NB; p++) {
@@ -177,13 +149,7 @@ __global__ __launch_bounds__(256) void k_append8(const Row8Args a) {
         }
         float top = 0.0f, bad = 0.0f;  // bad: NaN if a value is not finite
 #pragma unroll
-        for (int p = 0; p < NB; p++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float s = x[p].get(j);
-                top = fmaxf(top, fabsf(s));
-                bad = fmaf(s, 0.0f, bad);
-            }
+        for (int p = 0; p < NB; p++) measure(x[p], top, bad);
         const bool odd = __any(bad != bad);
         if (odd) {
             top = 0.0f;

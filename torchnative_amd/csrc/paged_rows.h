@@ -34,7 +34,6 @@ struct Ragged {
 // far below the maximum stay out of its subnormal range as long as they count.
 constexpr float P_BIAS = 6.0f;
 
-#define TN_INLINE __device__ __attribute__((always_inline)) inline
 
 // row_start[i], and request r's first row and number of rows: within the call's rows,
 // whatever row_start holds.
@@ -117,22 +116,6 @@ __device__ __attribute__((always_inline)) inline void load_words(const void* p, 
 __device__ __attribute__((always_inline)) inline float half_of(uint32_t w, int i) {
     return (float)__builtin_bit_cast(h2, w)[i];
 }
-
-// Eight consecutive elements of a row of type DT, at any element.
-template <int DT>
-struct Eight {
-    typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
-    u4 w[DT == TN_F32 ? 2 : 1];
-    TN_INLINE void load(const void* p, int64_t i) {
-        const u4* s = reinterpret_cast<const u4*>(static_cast<const char*>(p) + i * (DT == TN_F32 ? 4 : 2));
-        w[0] = s[0];
-        if constexpr (DT == TN_F32) w[1] = s[1];
-    }
-    TN_INLINE float get(int e) const {
-        if constexpr (DT == TN_F32) return __uint_as_float(w[e >> 2][e & 3]);
-        else return e & 1 ? El<DT == TN_F16>::hi(w[0][e >> 1]) : El<DT == TN_F16>::lo(w[0][e >> 1]);
-    }
-};
 
 }  // namespace
 }  // namespace tn
