@@ -298,22 +298,43 @@ __global__ __launch_bounds__(256, (NB <= 4 ? 2 : 1)) void k_paged8_few(const Pag
     }
 }
 
-// Splits of a row, in order (the same bits every time), into four output columns.
-template <int DT>
-TN_INLINE void join(const Paged8Args& a, const float* po, const Part* ml, int ns, int64_t row, int d) {
+// Splits of a row, in order (the same bits every time), into four output columns of a row of
+// `out`, -1: none, which row_of() tells. Every load of up to JOINS splits is on its way before
+// anything waits for one; one wave or few a compute unit, so that is what the time goes by.
+constexpr int JOINS = 8;
+template <int DT, class RowOf>
+TN_INLINE void join(const Paged8Args& a, const float* po, const Part* ml, int ns, int d, RowOf row_of) {
     const int D = 32 * a.c.nb;
+    f32x4 v[JOINS];
+    Part p[JOINS];
+    auto load = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < JOINS; s++) {
+            const int at = min(s0 + s, ns - 1);
+            p[s] = ml[at];
+            v[s] = *reinterpret_cast<const f32x4*>(po + (int64_t)at * D);
+        }
+    };
+    load(0);
+    const int64_t row = row_of();
+    if (row < 0) return;
     float mm = -INFINITY, tl = 0.0f, vv = 0.0f;
-    for (int s = 0; s < ns; s++) mm = fmaxf(mm, ml[s].m), vv = fmaxf(vv, ml[s].v);
+#pragma unroll
+    for (int s = 0; s < JOINS; s++) mm = fmaxf(mm, p[s].m), vv = fmaxf(vv, p[s].v);  // (the last more than once)
+    for (int s = JOINS; s < ns; s++) mm = fmaxf(mm, ml[s].m), vv = fmaxf(vv, ml[s].v);
     const float mu = mm == -INFINITY ? 0.0f : mm;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < ns; s++) {
-        const Part p = ml[s];
-        const float f = exp2f(p.m - mu), fv = f * (p.v / vv);
-        tl += p.l * f;
-        const f32x4 v = *reinterpret_cast<const f32x4*>(po + (int64_t)s * D);
+    for (int s0 = 0;;) {
 #pragma unroll
-        for (int n = 0; n < 4; n++) acc[n] += v[n] * fv;
+        for (int s = 0; s < JOINS; s++) {
+            if (s0 + s >= ns) break;
+            const float f = exp2f(p[s].m - mu), fv = f * (p[s].v / vv);
+            tl += p[s].l * f;
+#pragma unroll
+            for (int n = 0; n < 4; n++) acc[n] += v[s][n] * fv;
+        }
+        if ((s0 += JOINS) >= ns) break;
+        load(s0);
     }
     const float inv = 1.0f / tl;
     const float y[4] = {acc[0] * inv * vv, acc[1] * inv * vv, acc[2] * inv * vv, acc[3] * inv * vv};
@@ -322,21 +343,17 @@ TN_INLINE void join(const Paged8Args& a, const float* po, const Part* ml, int ns
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void k_paged8_combine(const Paged8Args a) {
-    const int D = 32 * a.c.nb, q4 = D / 4;
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t pr = e / q4;
-    const int d = (int)(e - pr * q4) * 4;
-    const int i = (int)(pr % a.few);
-    const int64_t rh = pr / a.few;
-    const int h = (int)(rh % a.c.H);
-    const int64_t r = rh / a.c.H;
-    if (r >= a.n) return;
-    const int start = start_of(a, r), c = min(rows_of(a, r, start), a.max_rows);
-    if (i >= c * a.G || c * a.G > a.few) return;
-    const int64_t row = (int64_t)(start + i / a.G) * a.Hq + h * a.G + i % a.G;
-    join<DT>(a, a.part_o + pr * a.nsplit * D + d, reinterpret_cast<const Part*>(a.part_ml) + pr * a.nsplit, a.nsplit, row,
-             d);
+__global__ __launch_bounds__(64) void k_paged8_combine(const Paged8Args a) {
+    const int D = 32 * a.c.nb, q4 = D / 4, h = blockIdx.y, r = blockIdx.z;
+    const uint32_t e = blockIdx.x * 64 + threadIdx.x;
+    const int i = (int)(e / (uint32_t)q4), d = (int)(e - (uint32_t)(i * q4)) * 4;
+    if (i >= a.few) return;
+    const int64_t part = (((int64_t)r * a.c.H + h) * a.few + i) * a.nsplit;
+    join<DT>(a, a.part_o + part * D + d, reinterpret_cast<const Part*>(a.part_ml) + part, a.nsplit, d, [&]() {
+        const int start = start_of(a, r), c = min(rows_of(a, r, start), a.max_rows);
+        if (i >= c * a.G || c * a.G > a.few) return (int64_t)-1;
+        return (int64_t)(start + i / a.G) * a.Hq + h * a.G + i % a.G;
+    });
 }
 
 // ---- many rows --------------------------------------------------------------------
@@ -863,7 +880,7 @@ __global__ __launch_bounds__(256) void k_paged8_join(const Paged8Args a, int ns)
     }
     const int start = start_of(a, r), c = min(rows_of(a, r, start), a.max_rows);
     if (t < start || t - start >= c || c * a.G <= a.few) return;  // (rows ahead of the first request's are no one's)
-    join<DT>(a, a.many_o + row * ns * D + d, reinterpret_cast<const Part*>(a.many_ml) + row * ns, ns, row, d);
+    join<DT>(a, a.many_o + row * ns * D + d, reinterpret_cast<const Part*>(a.many_ml) + row * ns, ns, d, [&]() { return row; });
 }
 
 // Splits of the keys of k_paged8_few: one round of the workgroups that compute units
@@ -966,8 +983,8 @@ tn_status launch_at(hipStream_t st, const Paged8Args& a, int64_t tokens) {
         }
     }
     if (a.few && a.nsplit > 1) {
-        const int64_t rows = (int64_t)a.n * a.c.H * a.few;
-        hipLaunchKernelGGL(k_paged8_combine<DT>, dim3((unsigned)cdiv(rows * (8 * NB), 256)), dim3(256), 0, st, a);
+        const dim3 grid((unsigned)cdiv((int64_t)a.few * (8 * NB), 64), (unsigned)a.c.H, (unsigned)a.n);
+        hipLaunchKernelGGL(k_paged8_combine<DT>, grid, dim3(64), 0, st, a);
         TN_LAUNCHED();
     }
     return TN_OK;
