@@ -75,6 +75,11 @@ TN_INLINE float vref_inverse(float vref) {
 // so that a lane holds the sixteen keys of one block, whose scales are one number each
 // for keys and for values, and the operands of its part of two 32-key products
 // O^T += V^T P^T, whose values it reads as sixteen bytes a column.
+//
+// A wave works alone, on every fourth (times the splits) run of tiles, the next tile's codes in
+// registers while one is computed, which is what a call of single tokens is bound by: twelve f16
+// tokens over 20000 to 40000 keys, 32/8 heads of 128 elements, 737 MB, 138 us, 5.3 TB/s; sixteen
+// bf16 over 512 to 4096 22 us (76 MB, 18 us of it here, the rest its merge's).
 template <int NB>
 struct KeyTile8 {
     uint32_t k[4][2 * NB];  // this lane's part of a row of each score tile
@@ -358,7 +363,7 @@ __global__ __launch_bounds__(64) void k_paged8_combine(const Paged8Args a) {
 
 // ---- many rows --------------------------------------------------------------------
 //
-// A wave takes 32 folded rows, a workgroup 32 W of them, and keys KT at a time. The
+// A wave takes 32 folded rows, a workgroup 128 of them, and keys KT at a time. The
 // codes are unpacked to f16 once a workgroup, into LDS, ahead of their use: K as rows of
 // D elements, V transposed, a row an element with its keys in the order in which the score
 // product leaves them in a lane (keys 4 h .. 4 h + 3 of each eight in half h of the wave),
@@ -369,32 +374,31 @@ __global__ __launch_bounds__(64) void k_paged8_combine(const Paged8Args a) {
 //
 // A wave alternates between two phases: the softmax of tile t; and the products, O^T +=
 // V^T P^T of tile t and S^T of tile t + 1, with its share of the unpacking (V of tile
-// t + 1, K of t + 2) in their shadow. Eight waves are
-// two groups of one wave a SIMD, half a turn apart: while one group's products run, the
-// other's softmax does. The first group unpacks V and the second K, so that two tiles
-// of each in LDS suffice: with barriers numbered as the first group passes them, it reads
-// V(t) and K(t + 1) and writes V(t + 1) behind barrier 2 t + 2, the second group reads the
-// same and writes K(t + 2) behind 2 t + 3; so V(t + 1) takes the place of V(t - 1), last
-// read behind 2 t + 1, and K(t + 2) that of K(t), last read there too. What the softmax
-// and the unpacking take of a tile's scales is written two turns ahead of the softmax, by
-// lanes of one wave of the last group, into one of four places. The first group, half a turn
-// ahead, unpacks V(t + 1) by it one turn later, so it reads it only behind the turn's
-// middle barrier.
-template <int DT, int NB, int W>
+// t + 1, K of t + 2) in their shadow. A compute unit holds two workgroups, whose phases
+// fall beside one another's by themselves: one of 256 rows in two groups held half a turn
+// apart unpacks half as often and took as long (4096 bf16 rows of 32/8 heads of 128
+// elements 171 us either way; 2048 f32 rows 101 against 94). With one barrier a turn two
+// tiles of each in LDS suffice: behind barrier t, V(t) and K(t + 1) are read, V(t + 1) and
+// K(t + 2) written, in the places of V(t - 1) and K(t), last read before it. What the
+// softmax and the unpacking take of a tile's scales is written two turns ahead of the
+// softmax, by lanes of the last wave, into one of four places.
+//
+// 4096 causal bf16 rows as above, 137 GFLOP, 171 us: 803 TFLOP/s; an f16 product of 16384
+// reaches 1263. The softmax's exponentials and the unpacking share the issue slots with the
+// products; neither LDS nor memory bounds it.
+constexpr int MANY_ROWS = 128;  // folded rows of a workgroup
+template <int DT, int NB>
 struct Many8 {
     static constexpr int Q = Parts8<DT>::Q, P = Parts8<DT>::P;
-    static constexpr int ROWS = 32 * W;                                 // folded rows
-    static constexpr int D = 32 * NB, KT = NB <= 4 ? 64 : 32;            // keys of a tile
-    static constexpr int GROUPS = W / 4, BL = KT / 16, WPB = 4 / BL;     // groups of four waves; blocks, waves that unpack one
-    static constexpr int KP = 2 * D + 16, VP = 2 * KT + 16;              // row pitches, bytes
+    static constexpr int D = 32 * NB, KT = NB <= 4 ? 64 : 32;  // keys of a tile
+    static constexpr int BL = KT / 16, WPB = 4 / BL;           // its blocks, waves that unpack one
+    static constexpr int KP = 2 * D + 16, VP = 2 * KT + 16;    // row pitches, bytes
     static constexpr int KB = KT * KP, VB = D * VP, STAGE = KB + VB;
-    static constexpr int N = (NB + 2 * WPB - 1) / (2 * WPB);             // 16-byte pieces a thread, of K and of V
-    static constexpr int OS = DT == TN_F32 ? 4 : 2;                     // output element
-    static constexpr int OP = (NB < 4 ? D : 128) * (GROUPS == 1 ? 4 : OS) + 16;  // row pitch on the way out
-    static constexpr int LDS_BYTES = 2 * STAGE > ROWS * OP ? 2 * STAGE : ROWS * OP;
-    // waves a SIMD: one where two do not have the registers (four waves a workgroup then)
-    static constexpr bool BIG = DT == TN_F32 ? NB > 5 : NB > 6;
-    static constexpr int WAVES = W == 4 && BIG ? 1 : 2;
+    static constexpr int N = (NB + 2 * WPB - 1) / (2 * WPB);   // 16-byte pieces a thread, of K and of V
+    static constexpr int OP = (NB < 4 ? D : 128) * 4 + 16;     // row pitch on the way out
+    static constexpr int LDS_BYTES = 2 * STAGE > MANY_ROWS * OP ? 2 * STAGE : MANY_ROWS * OP;
+    // waves a SIMD: one where two do not have the registers
+    static constexpr int WAVES = NB > (DT == TN_F32 ? 5 : 6) ? 1 : 2;
 };
 
 // A tile's scales: of its keys; of its values a block's share of the reference, for 16-bit rows
@@ -419,13 +423,13 @@ TN_INLINE T scalar(const T* p) {
 #endif
 }
 
-// Rows first .. first + ROWS of request r, whose rows start at `start` and attend
+// Rows first .. first + MANY_ROWS of request r, whose rows start at `start` and attend
 // `before` keys more than there are rows ahead of them.
-template <int DT, int NB, int W>
+template <int DT, int NB>
 TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int h, int r, int start, int rows, int first,
                           int len, int before) {
-    using M = Many8<DT, NB, W>;
-    constexpr int KT = M::KT, D = M::D, ROWS = M::ROWS, N = M::N, BL = M::BL, WPB = M::WPB;
+    using M = Many8<DT, NB>;
+    constexpr int KT = M::KT, D = M::D, ROWS = MANY_ROWS, N = M::N, BL = M::BL, WPB = M::WPB;
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, hh = lane >> 5;
@@ -487,9 +491,9 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
 
     // ---- this thread's part of a tile: its loads, and their way into LDS. A wave unpacks of
     // one block of sixteen keys, WPB waves a block, pieces (key, 16 elements) of K and
-    // (element) of V: of either (two groups) or of both
+    // (element) of V
     const int32_t* table = a.table + (int64_t)r * a.width;
-    const int blk = w % 4 / WPB, id0 = w % WPB * 64 + lane, group = w / 4;
+    const int blk = w / WPB, id0 = w % WPB * 64 + lane;
     auto on = [&](int x) { return 32 * NB % (64 * WPB) == 0 || id0 + 64 * WPB * x < 32 * NB; };
     struct Pieces {
         uint32_t c[N][4];
@@ -534,7 +538,7 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
         if (on(x)) *reinterpret_cast<h8*>(lds + (t & 1) * M::STAGE + M::KB + id * M::VP + (2 * blk + half) * 16) = v;
     };
     // The scales, by the first BL lanes of the last wave, a block each.
-    const bool scaler = w == W - 1;
+    const bool scaler = w == 3;
     float ref = VREF_MIN, sk = 0.0f, sv = 0.0f;
     int spage = 0;
     auto scale_page = [&](int t) __attribute__((always_inline)) {
@@ -623,11 +627,11 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
     constexpr bool FOLD = DT != TN_F32;
     Scores s;
     Probs p;
-    // role: what this thread unpacks, 1 V, 2 K, 3 both
-    auto turn = [&](auto roles, auto last_turn, int t) __attribute__((always_inline)) {
+    auto turn = [&](auto last_turn, int t) __attribute__((always_inline)) {
         constexpr bool LAST = decltype(last_turn)::value;
-        constexpr int END = LAST ? PG : G, ROLE = decltype(roles)::value;
+        constexpr int END = LAST ? PG : G;
         const Scales& sc = scales[t & 3];
+        const uint32_t rest = LAST ? ONES : rest_of(t + 1);
         float fs[BL], mb[BL];
 #pragma unroll
         for (int b = 0; b < BL; b++) fs[b] = rs * sc.ks[b];
@@ -706,17 +710,15 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
 #endif
         const int vslot = t & 1;
         fetch(0, vslot);
-        if constexpr (M::GROUPS == 2) __syncthreads();
-        const uint32_t rest = LAST || !(ROLE & 1) ? ONES : rest_of(t + 1);
         __builtin_amdgcn_s_setprio(1);  // the products' few instructions ahead of the other wave's many
         // eight codes of V or of K at a time, then the next loads
-        constexpr int VW = ROLE & 1 ? 2 * N : 0, KW = ROLE & 2 ? 2 * N : 0, WORK = LAST ? 0 : VW + KW + 1;
+        constexpr int WORK = LAST ? 0 : 4 * N + 1;
         auto work = [&](int x) __attribute__((always_inline)) {
-            if (x < VW) unpack_v(x >> 1, x & 1, t + 1, rest);
-            else if (x < VW + KW) unpack_k((x - VW) >> 1, x & 1, t + 2);
+            if (x < 2 * N) unpack_v(x >> 1, x & 1, t + 1, rest);
+            else if (x < 4 * N) unpack_k(x / 2 - N, x & 1, t + 2);
             else {
-                if constexpr (ROLE & 1) load_v(vr, page_of(t + 2), t + 2);
-                if constexpr (ROLE & 2) load_k(kr, page_of(t + 3), t + 3);
+                load_v(vr, page_of(t + 2), t + 2);
+                load_k(kr, page_of(t + 3), t + 3);
             }
         };
 #pragma unroll
@@ -728,7 +730,7 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
             for (int x = n * WORK / G; x < (n + 1) * WORK / G; x++) work(x);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (!LAST && (ROLE & 2) != 0) {
+        if constexpr (!LAST) {
             if (scaler) {
                 write_scales(t + 2);
                 load_scales(t + 3);
@@ -738,13 +740,12 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
         __builtin_amdgcn_s_setprio(0);
         if constexpr (!LAST) __syncthreads();
     };
-    auto walk = [&](auto roles) __attribute__((always_inline)) {
-        constexpr int ROLE = decltype(roles)::value;
+    if (nt > t0) {
         // all that the first tiles need is asked for before any of it is waited for
         Pieces k1;
         load_q();
-        if constexpr (ROLE & 2) load_k(k1, page_of(t0), t0), load_k(kr, page_of(t0 + 1), t0 + 1);
-        if constexpr (ROLE & 1) load_v(vr, page_of(t0), t0);
+        load_k(k1, page_of(t0), t0), load_k(kr, page_of(t0 + 1), t0 + 1);
+        load_v(vr, page_of(t0), t0);
         if (scaler) {
             for (int t = t0; t < t0 + 2; t++) scale_page(t), load_scales(t), write_scales(t);
             scale_page(t0 + 2);
@@ -752,24 +753,19 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
             scale_page(t0 + 3);
         }
         make_q();
-        if constexpr (ROLE & 2) {
-            const Pieces k2 = kr;
-            kr = k1;
+        const Pieces k2 = kr;
+        kr = k1;
 #pragma unroll
-            for (int x = 0; x < 2 * N; x++) unpack_k(x >> 1, x & 1, t0);
-            kr = k2;
+        for (int x = 0; x < 2 * N; x++) unpack_k(x >> 1, x & 1, t0);
+        kr = k2;
 #pragma unroll
-            for (int x = 0; x < 2 * N; x++) unpack_k(x >> 1, x & 1, t0 + 1);
-            load_k(kr, page_of(t0 + 2), t0 + 2);
-        }
+        for (int x = 0; x < 2 * N; x++) unpack_k(x >> 1, x & 1, t0 + 1);
+        load_k(kr, page_of(t0 + 2), t0 + 2);
         __syncthreads();  // (the scales are there)
-        if constexpr (ROLE & 1) {
-            const uint32_t rest = rest_of(t0);
+        const uint32_t rest = rest_of(t0);
 #pragma unroll
-            for (int x = 0; x < 2 * N; x++) unpack_v(x >> 1, x & 1, t0, rest);
-            load_v(vr, page_of(t0 + 1), t0 + 1);
-        }
-        if (ROLE == 2) __syncthreads();  // half a turn behind
+        for (int x = 0; x < 2 * N; x++) unpack_v(x >> 1, x & 1, t0, rest);
+        load_v(vr, page_of(t0 + 1), t0 + 1);
         fetch(PG, t0 & 1);
 #pragma unroll
         for (int n = PG; n < G; n++) {
@@ -777,14 +773,8 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
             multiply(n, p, s);
         }
         __syncthreads();
-        for (int t = t0; t + 1 < nt; t++) turn(roles, std::false_type{}, t);
-        turn(roles, std::true_type{}, nt - 1);
-        if (ROLE == 1) __syncthreads();
-    };
-    if (nt > t0) {
-        if constexpr (M::GROUPS == 1) walk(std::integral_constant<int, 3>{});
-        else if (group == 0) walk(std::integral_constant<int, 1>{});
-        else walk(std::integral_constant<int, 2>{});
+        for (int t = t0; t + 1 < nt; t++) turn(std::false_type{}, t);
+        turn(std::true_type{}, nt - 1);
     }
 
     // the last products' wait states, whatever their first reader is
@@ -831,7 +821,7 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
         }
     };
     const int64_t row = (int64_t)(start + j) * a.Hq + hq;
-    if (W == 4 && ns > 1) {  // a split's part: k_paged8_join's
+    if (ns > 1) {  // a split's part: k_paged8_join's
         leave(std::integral_constant<int, TN_F32>{}, 1.0f, 1.0f);
         if (hh == 0 && i < rows) reinterpret_cast<Part*>(a.many_ml)[row * ns + split] = Part{m, l, vref, 0.0f};
     } else {
@@ -840,10 +830,10 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
     }
 }
 
-template <int DT, int NB, int W>
-__global__ __launch_bounds__(64 * W, (Many8<DT, NB, W>::WAVES)) void k_paged8_many(const Paged8Args a, int tiles) {
-    constexpr int ROWS = 32 * W;
-    __shared__ __align__(16) uint8_t lds[Many8<DT, NB, W>::LDS_BYTES];
+template <int DT, int NB>
+__global__ __launch_bounds__(256, (Many8<DT, NB>::WAVES)) void k_paged8_many(const Paged8Args a, int tiles) {
+    constexpr int ROWS = MANY_ROWS;
+    __shared__ __align__(16) uint8_t lds[Many8<DT, NB>::LDS_BYTES];
     __shared__ __align__(16) Scales scales[4];
     // the longest rows first; a key/value head's workgroups on the same die when there are eight
     const int h = (int)blockIdx.x % a.c.H, tile = tiles - 1 - (int)blockIdx.x / a.c.H;
@@ -861,7 +851,7 @@ __global__ __launch_bounds__(64 * W, (Many8<DT, NB, W>::WAVES)) void k_paged8_ma
     const int rows = min(all, a.max_rows) * a.G;
     if (first < 0 || first >= rows || rows <= a.few) return;  // few rows: k_paged8_few's
     const int len = max(0, min(a.lens[r], a.max_len)), before = len - all;
-    many8_tile<DT, NB, W>(a, lds, scales, h, r, start, rows, first, len, before);
+    many8_tile<DT, NB>(a, lds, scales, h, r, start, rows, first, len, before);
 }
 
 // The splits of k_paged8_many's rows, in order: four output columns a thread.
@@ -884,7 +874,9 @@ __global__ __launch_bounds__(256) void k_paged8_join(const Paged8Args a, int ns)
 }
 
 // Splits of the keys of k_paged8_few: one round of the workgroups that compute units
-// hold, of 512 keys or more, up to eight of them of 256.
+// hold, of 512 keys or more, up to eight of them of 256. Against a round of 1024 workgroups,
+// us: sixteen bf16 tokens over 512 to 4096 keys, 32/8 heads of 128 elements, 22.3 / 24.5, of 256
+// elements 48.7 / 55.5; sixty-four over 1000 to 3000 56 / 62; one over 8000 13.5 / 13.4.
 constexpr int64_t FEW_WGS = 512, FEW_KEYS = 512, FEW_MAX_SPLIT = 64;
 int64_t few_most(int64_t max_len) {
     if (max_len <= FEW_KEYS) return 1;
@@ -916,35 +908,36 @@ int64_t part_rows(const Pages8& c, int64_t n, int64_t few, int64_t max_len) {
     return most < 2 ? 0 : std::min(std::min<int64_t>(few, 16) * FEW_WGS, n * c.H * few * most);
 }
 
-// k_paged8_many: 0 for workgroups of 256 rows (rows enough for one a unit), else the
-// splits of the keys for workgroups of 128, two of which a unit holds.
-constexpr int64_t MANY_WIDE = 256, MANY_WGS = 512, MANY_MAX_SPLIT = 8;
-int many_splits(const Pages8& c, int dtype, int64_t n, int64_t tokens, int64_t G, int64_t max_len) {
-    const bool big = dtype == TN_F32 ? c.nb > 5 : c.nb > 6;  // Many8::BIG: 256 rows do not have the registers
-    if (!big && tokens * G / 256 * c.H >= MANY_WIDE) return 0;
-    const int64_t wgs = (tokens * G / 128 + n) * c.H;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(MANY_WGS, wgs), cdiv(max_len, 512), MANY_MAX_SPLIT}));
+// Splits of the keys of k_paged8_many: what fills one round of the workgroups that compute units
+// hold, two each, of 512 keys or more of a request's middle row. us at rounds of 256 / 512 / 1024
+// workgroups, bf16, 32/8 heads of 128 elements: 512 rows behind 20000 tokens 297 / 205 / 224,
+// behind 4096 75 / 59 / 72; a prompt of 1024, whose middle row has 512 keys, without splits 37,
+// in two 42.
+constexpr int64_t MANY_WGS = 512, MANY_MAX_SPLIT = 8;
+int many_splits(const Pages8& c, int64_t n, int64_t tokens, int64_t G, int64_t max_rows, int64_t max_len) {
+    const int64_t wgs = (tokens * G / MANY_ROWS + n) * c.H, keys = max_len - std::min(max_rows, max_len) / 2;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({cdiv(MANY_WGS, wgs), cdiv(keys, 512), MANY_MAX_SPLIT}));
 }
 // Rows of its partials at most, for this call and every smaller one: above one split there
-// are under MANY_WGS workgroups of 128 rows a split.
+// are under MANY_WGS workgroups a split.
 int64_t many_rows(const Pages8& c, int64_t tokens, int64_t G, int64_t max_len) {
     const int64_t most = std::min(cdiv(max_len, 512), MANY_MAX_SPLIT);
-    return most < 2 ? 0 : std::min(tokens * G * c.H * most, 2 * MANY_WGS * 128);
+    return most < 2 ? 0 : std::min(tokens * G * c.H * most, 2 * MANY_WGS * MANY_ROWS);
 }
 
 // Which kernel takes a request's rows. k_paged8_few reads and unpacks the codes again for
-// every 16 folded rows but starts at once and splits finely; k_paged8_many fills 128 or 256
+// every 16 folded rows but starts at once and splits finely; k_paged8_many fills 128
 // rows, and its tiles follow one another. So k_paged8_few takes all rows of a call whose
 // products (tokens * Hq * max_len * D) are few, and of a larger call the requests of up to
 // FEW_ROWS folded rows, if it is of several. How many are few: a tile of k_paged8_many has
 // the same softmax and the same barriers for rows of 64 elements as for 128, so those wait
 // longer for it. Few against many, us, bf16: 64 elements, products / 2^30: 2 33 / 40, 4 48 / 50,
-// 9 62 / 66 (six ragged requests 6 45 / 58); 128: 2 31 / 32 and 33 / 36, 4 50 / 43 (ragged: 8
+// 8 62 / 55, 9 62 / 66 (six ragged requests 6 45 / 58); 128: 2 31 / 32 and 33 / 36, 4 50 / 43 (ragged: 8
 // 64 / 65, 12 88 / 79); 256: 8 97 / 94, 16 157 / 111. f32, 128: 2 32 / 38, 4 56 / 54, 8 97 / 82. Its grid
 // is as long for every request as for the longest: up to FEW_GRID workgroups of it.
 constexpr int FEW_ROWS = 128;
 constexpr int64_t FEW_GRID = 8192;
-int64_t few_products(int nb) { return nb <= 3 ? 10ll << 30 : 3ll << 30; }
+int64_t few_products(int nb) { return nb <= 3 ? 7ll << 30 : 3ll << 30; }
 
 // Folded rows of a request that k_paged8_few takes at most in this call; 0: it is not launched.
 int64_t few_limit(const Pages8& c, int64_t n, int64_t tokens, int64_t G, int64_t max_rows, int64_t max_len) {
@@ -967,14 +960,10 @@ tn_status launch_at(hipStream_t st, const Paged8Args& a, int64_t tokens) {
         TN_LAUNCHED();
     }
     if ((int64_t)a.max_rows * a.G > a.few) {
-        const int ns = many_splits(a.c, DT, a.n, tokens, a.G, a.max_len);
-        const bool wide = ns == 0;
-        const int64_t tiles = tokens * a.G / (wide ? 256 : 128) + a.n;
-        const dim3 grid((unsigned)(tiles * a.c.H), wide ? 1u : (unsigned)ns);
-        if constexpr (!Many8<DT, NB, 8>::BIG) {
-            if (wide) hipLaunchKernelGGL((k_paged8_many<DT, NB, 8>), grid, dim3(512), 0, st, a, (int)tiles);
-        }
-        if (!wide) hipLaunchKernelGGL((k_paged8_many<DT, NB, 4>), grid, dim3(256), 0, st, a, (int)tiles);
+        const int ns = many_splits(a.c, a.n, tokens, a.G, a.max_rows, a.max_len);
+        const int64_t tiles = tokens * a.G / MANY_ROWS + a.n;
+        const dim3 grid((unsigned)(tiles * a.c.H), (unsigned)ns);
+        hipLaunchKernelGGL((k_paged8_many<DT, NB>), grid, dim3(256), 0, st, a, (int)tiles);
         TN_LAUNCHED();
         if (ns > 1) {
             const int64_t quads = tokens * a.Hq * (8 * NB);
