@@ -2,12 +2,15 @@
 empty calls touch no pointer, and the oracle holds its own invariants."""
 
 import ctypes
+import os
+import shutil
 
 import numpy as np
 import pytest
 
 from oracle import int8 as I
 from torchnative_amd import _lib
+from torchnative_amd import hazard_scan as H
 
 NAN = float("nan")
 
@@ -230,3 +233,28 @@ def test_oracle_blocks_keep_their_values_as_rows_join():
     whole = I.Cache(1, 16, 2, 32)
     whole.append(x, x, np.arange(16))
     assert np.array_equal(whole.scale["k"], c.scale["k"])
+
+
+@pytest.mark.skipif(shutil.which(H.build.HIPCC) is None and not os.path.exists(H.build.HIPCC),
+                    reason="hipcc is not installed")
+def test_ring_stages_of_the_products_are_read_before_they_are_opened(tmp_path):
+    asm = H.assembly("i8.hip", str(tmp_path))
+    for kernel in ("k_i8_gemm", "k_i8_large"):
+        assert kernel in asm
+        assert H.open_barriers(asm, kernel) == []
+
+
+def test_rows_of_codes_refuse_planes_that_do_not_hold_them():
+    from torchnative_amd import _C
+    from torchnative_amd.tensor import Tensor
+
+    def t(shape, dtype):
+        return Tensor(shape, dtype, "cpu", _host=np.zeros(shape, dtype))
+
+    rows = _C.I8Rows((3, 70), "cpu", t((3, 128), "int8"), t((3,), "float32"))
+    assert rows.shape == (3, 70)
+    for codes, scales in ((t((3, 70), "int8"), t((3,), "float32")), (t((2, 128), "int8"), t((3,), "float32")),
+                          (t((3, 128), "uint8"), t((3,), "float32")), (t((3, 128), "int8"), t((2,), "float32")),
+                          (t((3, 128), "int8"), t((3,), "float64"))):
+        with pytest.raises(RuntimeError, match="do not hold rows"):
+            _C.I8Rows((3, 70), "cpu", codes, scales)

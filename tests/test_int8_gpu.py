@@ -401,6 +401,46 @@ def test_append_of_many_rows(tn, dtype, m):
     _same_planes(dev, c)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H, m", [(1, 900), (2, 1025), (4, 1500), (4, 3001), (8, 3001)])
+@pytest.mark.parametrize("order", ["runs", "any"])
+def test_windows_of_one_to_sixteen_rows(tn, dtype, H, m, order):
+    """A wave's window goes by rows and heads. Rows of a block as they come, or in any order, with holes and repeats;
+    read back with repeats, runs and slots that are none, in every output type."""
+    rng = np.random.default_rng(m + H)
+    D, S = 96, 64
+    P_ = m // S * 4 + 40
+    c = _held(rng, P_, S, H, D)
+    dev = _fill(tn, c)
+    blocks, slots = rng.permutation(P_ * S // 16), []
+    for b in blocks:
+        n = int(rng.choice([1, 2, 9, 16]))
+        if order == "runs":
+            lo = int(rng.integers(0, 17 - n))
+            rows = b * 16 + np.arange(lo, lo + n)
+        else:
+            rows = np.where(rng.random(n) < 0.2, -1, b * 16 + rng.integers(0, 16, n))
+        slots += [int(x) for x in rows]
+    assert len(slots) >= m
+    slots = np.array(slots[:m], np.int32)
+    x = [_up(tn, rng.standard_normal((m, H, D)).astype(np.float32), dtype) for _ in "kv"]
+    print(f"case {dtype} H {H} rows {m} {order}", flush=True)
+    dev.append(*x, _ints(tn, slots))
+    c.append(*(t.numpy().astype(np.float32) for t in x), slots)
+    _same_planes(dev, c)
+    total = P_ * S
+    look = np.concatenate([slots, slots[::-1], np.repeat(slots[:40], 5), np.arange(100, 400), [total, -7, 2**31 - 1]])
+    look = look.astype(np.int32)[: m + 500]
+    live = (look >= 0) & (look < total)
+    for out in DTYPES:
+        for w, t in zip("kv", dev.read(_ints(tn, look), out)):
+            at = np.where(live, look, 0)
+            want = (c.code[w][at].astype(np.float32) * c.scale[w][at // 16][..., None]).astype(np.float32)
+            got = t.bits() if out != "float32" else t.numpy()
+            assert np.array_equal(got[live], _narrow(tn, want, out)[live])
+            assert np.isnan(t.numpy()[~live]).all()
+
+
 def test_append_in_any_order_within_a_block_with_holes_and_repeats(tn):
     rng = np.random.default_rng(7)
     H, D = 2, 96

@@ -330,6 +330,10 @@ class I8Rows:
         self.shape, self.device = (m, k), device
         self.codes = Tensor((m, (k + 63) // 64 * 64), "int8", device) if codes is None else codes
         self.scales = Tensor((m,), "float32", device) if scales is None else scales
+        c, f = self.codes, self.scales
+        if (c.shape, c.dtype, f.shape, f.dtype) != ((m, (k + 63) // 64 * 64), "int8", (m,), "float32"):
+            raise RuntimeError(f"I8Rows: codes {list(c.shape)} {c.dtype} and scales {list(f.shape)} {f.dtype} do not "
+                               f"hold rows {[m, k]}")
 
     @property
     def nbytes(self) -> int:

@@ -46,6 +46,8 @@ __device__ inline void store1(void* p, int64_t i, float v) {
 
 // V pairs at a time (1 or 4), NC of those a lane, LH lanes a head. V = 4 takes heads
 // whose turning and staying halves are multiples of four elements.
+// Bound by memory where tokens are many: 8192 of 32 + 8 bf16 heads of 128 elements, 168 MB in
+// and out, 38 us, 4.4 TB/s; by a launch where few (one token 1.9 us of its own).
 template <int DT, int V, int LH, int NC>
 __global__ __launch_bounds__(256) void k_heads(const HeadArgs a) {
     constexpr int HP = 256 / LH;  // heads of a pass
@@ -123,7 +125,9 @@ __global__ __launch_bounds__(256) void k_heads(const HeadArgs a) {
 template <int DT, int V, int LH, int NC>
 tn_status launch_at(hipStream_t st, HeadArgs& a, int64_t m) {
     const int passes = (int)cdiv(a.heads, 256 / LH);
-    // a token's passes in one workgroup where tokens are many, else a workgroup each
+    // a token's passes in one workgroup where tokens are many, which makes its cosines once, else
+    // a workgroup each (32 + 8 bf16 heads of 128, us, one against each: 16 tokens 3.9 / 3.4, 512
+    // 5.3 / 4.8, 1024 7.4 / 7.4, 2048 10.8 / 11.9, 8192 40 / 47)
     a.passes = m >= 1024 ? passes : 1;
     a.groups = (int)cdiv(passes, a.passes);
     if (m * a.groups > INT32_MAX) return fail(TN_EVALUE, "qk_norm_rope: shape too large");
