@@ -18,7 +18,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import check, lib
-from .tensor import Scratch, Tensor, current_stream, row_stride
+from .tensor import Heads, Scratch, Tensor, current_stream, row_stride
 
 QK4_0 = 32
 Q4_0_TYPE_SIZE = 18
@@ -92,13 +92,19 @@ class QTensor:
         return f"QTensor(shape={self.shape}, format={self.format}, device={self.device})"
 
 
-def _require_hip(op, *tensors):
-    for t in tensors:
+def _require_hip(op, *tensors, rows=()):
+    """Every operand on the device, and dense but for `rows`, whose row stride the call hands on."""
+    for t in (*tensors, *rows):
         if t is not None and getattr(t, "device", None) != "hip":
             raise NotImplementedError(
                 f"{op}: operand on device {getattr(t, 'device', '?')!r}: this backend computes on the hip device "
                 "only and does not fall back to the host; move the operands with .to('hip')"
             )
+    for t in tensors:
+        if isinstance(t, Heads):
+            raise NotImplementedError(
+                f"{op}: heads {t.first} .. {t.first + t.shape[1] - 1} of rows {list(t.rows.shape)}: this operand is taken "
+                "as dense rows, which Heads of stacked rows are not; copy them into a tensor of their own")
 
 
 def _shape2(shape, fmt="q4_0"):
@@ -434,7 +440,7 @@ def qk_norm_rope(q, k, q_weight: Tensor, k_weight: Tensor, inv_freq: Tensor, pos
     Returns (q_out, k_out)."""
     op = "qk_norm_rope"
     q_out, k_out = q if q_out is None else q_out, k if k_out is None else k_out
-    _require_hip(op, q, k, q_weight, k_weight, inv_freq, pos, q_out, k_out)
+    _require_hip(op, q_weight, k_weight, inv_freq, pos, rows=(q, k, q_out, k_out))
     for name, t in (("q", q), ("k", k)):
         if t.dim() != 3:
             raise RuntimeError(f"{op}: {name} {list(t.shape)} is not [tokens, heads, head_dim]")

@@ -116,7 +116,7 @@ class _Cache:
         """Writes rows k, v [m, n_kv_heads, head_dim] (tensors, or Heads of stacked rows) to `slots` [m]; a negative slot
         skips its row."""
         op = f"kv_append_{self._kind}"
-        _require_hip(op, k, v, slots)
+        _require_hip(op, slots, rows=(k, v))
         _int32(op, slots=slots)
         self._rows(op, k)
         if v.shape != k.shape or v.dtype != k.dtype or slots.shape != k.shape[:1] or row_stride(v) != row_stride(k):
@@ -150,7 +150,7 @@ class _Cache:
         `work`, `out` and `lse` are made where they are not given. Code that captures passes its own, so that the
         graph's buffers live as long as it does, a `work` of its own for each graph."""
         op = f"sdpa_paged_{self._kind}"
-        _require_hip(op, q)
+        _require_hip(op, work, out, lse, rows=(q,))
         if q.dim() != 3 or q.shape[2] != self.head_dim:
             raise RuntimeError(f"{op}: query {list(q.shape)} is not [tokens, heads, {self.head_dim}]")
         if pages.page_size != self.page_size:
@@ -165,7 +165,6 @@ class _Cache:
             raise RuntimeError(f"{op}: out {list(out.shape)} {out.dtype}, lse {list(lse.shape)} {lse.dtype} or work "
                                f"{work.dtype if work is not None else ''} does not fit query {list(q.shape)} {q.dtype}")
         work = self._work.get(4 * need) if work is None else work
-        _require_hip(op, work, out, lse)
         sc = float("nan") if scale is None else float(scale)
         check(self._fn("sdpa_paged_{}")(
             current_stream(), self._ref(), _dt(q.dtype), q.data_ptr(), row_stride(q), T, Hq, pages.requests,

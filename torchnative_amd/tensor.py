@@ -260,7 +260,8 @@ class Tensor:
 
 class Heads:
     """Heads `first` .. `first + count - 1` of rows [m, heads, d], read and written where they lie: the q, k or v of
-    stacked projections. Stands for a tensor [m, count, d] where an operator takes rows with a stride."""
+    stacked projections. Stands for a tensor [m, count, d] where an operator takes rows with a stride (qk_norm_rope, a
+    cache's append, the query of its attend); the others refuse it."""
 
     def __init__(self, rows: Tensor, first: int, count: int):
         if rows.dim() != 3 or first < 0 or count < 0 or first + count > rows.shape[1]:
