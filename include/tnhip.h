@@ -533,14 +533,13 @@ tn_status tn_kv_read_q8(void* stream, const tn_q8_cache* cache, const int32_t* s
  * element gives NaN, and no other row does. Rows that no request has are left
  * as they were. What pages hold past a request's length has no effect (the
  * last block's scales, which its held tokens share, do).
- * Sums, maxima and the softmax are f32. Codes enter the matrix products exactly,
- * but for values of 16-bit calls of many rows whose block's scale is under 2^-6
- * of the largest such scale met: times what that ratio leaves, they are rounded
- * to f16. A query is one f16 under a power of two of its own (two f16 parts for
- * f32 rows); probabilities, times their values' block scale over the largest
- * met, are one f16 for 16-bit rows, two for f32 rows. The output is rounded
- * once. Probabilities times scales are held to 2^-30 of the row's largest
- * probability times the largest scale of values (lse counts them all).
+ * Sums, maxima and the softmax are f32. Codes enter the matrix products exactly.
+ * A query is one f16 under a power of two of its own (two f16 parts for f32
+ * rows); probabilities, times their values' block scale over the largest that
+ * the row attends, are one f16 for 16-bit rows, two for f32 rows. The output is
+ * rounded once. Probabilities times scales are held to 2^-30 of the row's
+ * largest probability times the largest scale of values that it attends (lse
+ * counts them all); blocks of later tokens do not count.
  * Scales are taken as finite and not negative.
  * `work`: as there, tn_sdpa_paged_q8_work_floats() floats. */
 int64_t tn_sdpa_paged_q8_work_floats(const tn_q8_cache* cache, int64_t n, int64_t tokens, int64_t Hq,

@@ -139,8 +139,7 @@ def tolerance(kind, ref, lse, pav, qk, keys, D, most):
     off by 2 e of itself; exp2, its block's share of the scale (2^-6 and more in the exponent, whose logarithm is off by
     2^-22 at most, 3 u of the probability) and the running rescales 12 u more. Of sum p |v| the output is off by that, by
     (keys / 16 + 64) u from the f32 sums (32 keys a product, products in sequence) and, 16-bit calls, by h where a
-    probability is one f16 (two f16 parts: 4 u) and by h where a block's share under 2^-6 is rounded into its codes, once
-    itself (another h). A probability times its share is held at 2^6 or
+    probability is one f16 (two f16 parts: 4 u), twice that again allowed. A probability times its share is held at 2^6 or
     more times the row's largest one's size, so one in f16's subnormal range is off by at most 2^-31 of it, times a
     reference for the scales of at most twice their largest: 2^-30 most for each key. The output is rounded once."""
     u, h = 2.0 ** -24, 2.0 ** -11

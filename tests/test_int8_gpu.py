@@ -959,3 +959,51 @@ def test_a_block_served_eager_and_captured(tn, dtype):
     graph = list(_loop(tn, dtype, STEPS, True))
     for i, (a, b) in enumerate(zip(eager, graph)):
         assert all(x.tobytes() == y.tobytes() for x, y in zip(a, b)), f"step {i}"
+
+
+# --- what later tokens hold costs a row nothing -----------------------------------------------
+
+
+def _own_most(c):
+    """For each row the largest size that a value of its own keys can have, [rows, 1, 1]."""
+    most = np.zeros(int(c.row_start[-1]))
+    for r, x in enumerate(c.lens):
+        for i in range(c.rows[r]):
+            t = np.arange(x - c.rows[r] + i + 1)
+            at = np.unique((c.table[r, t // c.S] * c.S + t % c.S) // 16)
+            most[c.row_start[r] + i] = 127.0 * float(np.max(c.cache.scale["v"][at], initial=0))
+    return most[:, None, None]
+
+
+@pytest.mark.parametrize("dtype, climb", [("float32", 12), ("bfloat16", 12), ("float16", 3)])
+@pytest.mark.parametrize("H, G, D, rows, lens", [(2, 1, 64, [200], [200]), (1, 4, 128, [70, 1, 33], [300, 90, 40]),
+                                                 (1, 2, 256, [100], [100]), (2, 3, 32, [150, 5], [150, 64])])
+@MANY
+def test_scales_of_later_tokens_cost_a_row_nothing(tn, many, dtype, climb, H, G, D, rows, lens):
+    """Each block's values are 2^climb times the block's before it, over and over through eight blocks: a row in the
+    middle of a tile is held to the bound of the keys that it attends."""
+    c = Case(tn, dtype, H, G, D, 16, rows, lens, seed=21)
+    for r, x in enumerate(lens):
+        for b in range(-(-x // 16)):
+            c.cache.scale["v"][c.table[r, b]] *= np.float32(2.0 ** (climb * (b % 8) - 4 * climb))
+    out, lse = c.run(tn, many=many)
+    ro, rl, pav, _, qk, _ = P.attend(c.q.numpy().astype(np.float64), c.cache, c.row_start, c.lens, c.table, None)
+    tol, ltol = I.tolerance(dtype, ro, rl, pav, qk, max(lens), D, _own_most(c))
+    worst, lworst = np.max(np.abs(out - ro) / tol), np.max(np.abs(lse - rl) / ltol)
+    print(f"  worst {worst:.3f} of the bound, lse {lworst:.3f}", flush=True)
+    assert worst <= 1 and lworst <= 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@MANY
+def test_a_rows_bits_do_not_depend_on_later_tokens_values(tn, many, dtype):
+    """The same rows with the values of a later block 2^40 and 2^-40 times as large."""
+    c = Case(tn, dtype, 1, 2, 64, 16, [120], [120], seed=22)
+    was, last = c.cache.scale["v"].copy(), c.table[0, 3]  # tokens 48 .. 63, in the same tile as all before
+    got = []
+    for mul in (1.0, 2.0 ** 40, 2.0 ** -40):
+        c.cache.scale["v"][:] = was
+        c.cache.scale["v"][last] *= np.float32(mul)
+        got.append(c.run(tn, bits=True, many=many))
+    for out, lse in got[1:]:
+        assert np.array_equal(out[:48], got[0][0][:48]) and np.array_equal(lse[:48], got[0][1][:48])

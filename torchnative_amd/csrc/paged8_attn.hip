@@ -49,8 +49,9 @@ TN_INLINE h8 codes8(uint32_t a, uint32_t b) {
 #endif
 }
 
-// The scale of values that a wave's sums are held under: a power of two above every block's
-// scale met so far, so that a probability times its block's share of it is at most itself.
+// The scale of values that a row's sums are held under: a power of two above the scale of every
+// block met so far that the row attends, so that a probability times its block's share of it is at
+// most itself, and no later token's values take part.
 TN_INLINE float vref_for(float scale) {
     const uint32_t e = (__builtin_bit_cast(uint32_t, scale) >> 23) & 0xffu;
     return __builtin_bit_cast(float, min(e + 1u, 253u) << 23);
@@ -200,8 +201,9 @@ __global__ __launch_bounds__(256, (NB <= 4 ? 2 : 1)) void k_paged8_few(const Pag
 #pragma unroll
         for (int u = 0; u < 4; u++) s[u] = s[u] * f;
         if (edge) {
-            // values of a block that no row attends count as zeros, whatever its page holds
-            if (k0 >= len || x.bad) x.vs = 0.0f;
+            // values of a block that this lane's row does not attend count as zeros, whatever its page
+            // holds, so that the reference for the scales is of the row's own keys
+            if (k0 >= keys || x.bad) x.vs = 0.0f;
 #pragma unroll
             for (int u = 0; u < 4; u++)
 #pragma unroll
@@ -223,7 +225,7 @@ __global__ __launch_bounds__(256, (NB <= 4 ? 2 : 1)) void k_paged8_few(const Pag
         }
         const float mv = wave_xor_max(x.vs);
         if (__any(mv >= vref)) {
-            const float nv = vref_for(mv), al = vref * vref_inverse(nv);
+            const float nv = mv >= vref ? vref_for(mv) : vref, al = vref * vref_inverse(nv);
             vref = nv;
 #pragma unroll
             for (int b = 0; b < 2 * NB; b++) o[b] = o[b] * al;
@@ -369,7 +371,8 @@ __global__ __launch_bounds__(64) void k_paged8_combine(const Paged8Args a) {
 // product leaves them in a lane (keys 4 h .. 4 h + 3 of each eight in half h of the wave),
 // so that P^T needs no exchange. Codes are exact there in one part; a score tile's rows 0
 // .. 15 and 16 .. 31 are a block each, whose scales the softmax takes in: keys' in the
-// factor that its argument has anyway, values' in its exponent, and out of the sum again.
+// factor that its argument has anyway, values' in its exponent, and out of the sum again
+// (in tiles that end among a wave's rows, of small scales, and of f32 rows: by a product).
 // Rows are padded by 16 bytes, which spreads 16 rows' reads over all banks.
 //
 // A wave alternates between two phases: the softmax of tile t; and the products, O^T +=
@@ -380,8 +383,8 @@ __global__ __launch_bounds__(64) void k_paged8_combine(const Paged8Args a) {
 // elements 171 us either way; 2048 f32 rows 101 against 94). With one barrier a turn two
 // tiles of each in LDS suffice: behind barrier t, V(t) and K(t + 1) are read, V(t + 1) and
 // K(t + 2) written, in the places of V(t - 1) and K(t), last read before it. What the
-// softmax and the unpacking take of a tile's scales is written two turns ahead of the
-// softmax, by lanes of the last wave, into one of four places.
+// softmax takes of a tile's scales is written two turns ahead of it, by lanes of the last
+// wave, into one of four places.
 //
 // 4096 causal bf16 rows as above, 137 GFLOP, 171 us: 803 TFLOP/s; an f16 product of 16384
 // reaches 1263. The softmax's exponentials and the unpacking share the issue slots with the
@@ -401,17 +404,16 @@ struct Many8 {
     static constexpr int WAVES = NB > (DT == TN_F32 ? 5 : 6) ? 1 : 2;
 };
 
-// A tile's scales: of its keys; of its values a block's share of the reference, for 16-bit rows
-// its logarithm and inverse, down to 2^-6 (the probabilities of a smaller one would be lost to
-// the sum: what is left of it, `rest`, goes into its codes); the reference's last step and the
-// reference.
+// A tile's scales: of its keys and of its values; of the latter, for tiles that all of a wave's 16-bit
+// rows attend whole, a block's share of the reference as its logarithm and inverse (small: one is
+// under 2^-6, and probabilities are multiplied by shares instead, where a scale of 0 needs none);
+// the reference's last step and the reference.
 struct Scales {
-    float ks[4], log[4], inv[4], share[4];
-    uint32_t rest[4];  // two f16
-    float step, vref, pad[2];
+    float ks[4], vs[4], log[4], inv[4];
+    float step, vref;
+    int small, pad;
 };
 constexpr float LEAST_SHARE = 0x1p-6f;
-constexpr uint32_t ONES = 0x3c003c00u;  // two f16
 
 // What a kernel only reads, through the scalar cache where its address is the wave's.
 template <class T>
@@ -526,16 +528,11 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
             *reinterpret_cast<h8*>(lds + (t & 1) * M::STAGE + (16 * blk + (id & 15)) * M::KP + (id >> 4) * 32 + half * 16) =
                 codes8(kr.c[x][2 * half], kr.c[x][2 * half + 1]);
     };
-    // rest: what is left of a small block's scale (Scales), for all of the wave's pieces
-    auto rest_of = [&](int t) __attribute__((always_inline)) {
-        return DT == TN_F32 ? ONES : (uint32_t)__builtin_amdgcn_readfirstlane((int)scales[t & 3].rest[blk]);
-    };
-    auto unpack_v = [&](int x, int half, int t, uint32_t rest) __attribute__((always_inline)) {
+    auto unpack_v = [&](int x, int half, int t) __attribute__((always_inline)) {  // tokens 4 half .. + 3 and 8 + 4 half .. + 3
         const int id = id0 + 64 * WPB * x;
-        // tokens 4 half .. + 3 and 8 + 4 half .. + 3
-        h8 v = codes8(vr.c[x][half], vr.c[x][2 + half]);
-        if (rest != ONES) v = v * as_h8(rest, rest, rest, rest);
-        if (on(x)) *reinterpret_cast<h8*>(lds + (t & 1) * M::STAGE + M::KB + id * M::VP + (2 * blk + half) * 16) = v;
+        if (on(x))
+            *reinterpret_cast<h8*>(lds + (t & 1) * M::STAGE + M::KB + id * M::VP + (2 * blk + half) * 16) =
+                codes8(vr.c[x][half], vr.c[x][2 + half]);
     };
     // The scales, by the first BL lanes of the last wave, a block each.
     const bool scaler = w == 3;
@@ -555,15 +552,14 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
     auto write_scales = [&](int t) __attribute__((always_inline)) {
         const float top = quad_max<BL>(sv), next = top >= ref ? vref_for(top) : ref, inv = vref_inverse(next);
         const float share = sv * inv;
-        const bool small = share < LEAST_SHARE;
+        const int small = __any(share < LEAST_SHARE);
         Scales& sc = scales[t & 3];
         if (lane < BL) {
             sc.ks[lane] = sk;
-            sc.log[lane] = small ? -6.0f : __builtin_amdgcn_logf(share);
-            sc.inv[lane] = small ? 64.0f : __builtin_amdgcn_rcpf(share);
-            sc.share[lane] = share;
-            sc.rest[lane] = small ? pk_f16(share * 64.0f, share * 64.0f) : ONES;
-            if (lane == 0) sc.step = ref * inv, sc.vref = next;
+            sc.vs[lane] = sv;
+            sc.log[lane] = __builtin_amdgcn_logf(share);
+            sc.inv[lane] = __builtin_amdgcn_rcpf(share);
+            if (lane == 0) sc.step = ref * inv, sc.vref = next, sc.small = small;
         }
         ref = next;
     };
@@ -622,8 +618,8 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
         }
     };
 
-    // 16-bit rows have the blocks' shares in the exponents, f32 rows as a product, which keeps
-    // its digits.
+    // 16-bit rows have the blocks' shares in the exponents where they can, f32 rows as a product,
+    // which keeps its digits.
     constexpr bool FOLD = DT != TN_F32;
     Scores s;
     Probs p;
@@ -631,7 +627,6 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
         constexpr bool LAST = decltype(last_turn)::value;
         constexpr int END = LAST ? PG : G;
         const Scales& sc = scales[t & 3];
-        const uint32_t rest = LAST ? ONES : rest_of(t + 1);
         float fs[BL], mb[BL];
 #pragma unroll
         for (int b = 0; b < BL; b++) fs[b] = rs * sc.ks[b];
@@ -641,7 +636,17 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
         asm volatile("s_nop 15\n\ts_nop 1");
 #endif
         __builtin_amdgcn_sched_barrier(0);
-        if (KT * t + KT > least) {
+        const bool edge = KT * t + KT > least;  // uniform, and so for all tiles behind
+        float step = sc.step;
+        if (edge) {
+            // keys that a row does not attend, and the reference for scales of its own keys alone: what
+            // later tokens hold costs a row no digits
+            float top = 0.0f;
+#pragma unroll
+            for (int b = 0; b < BL; b++) top = fmaxf(top, KT * t + 16 * b < keys ? sc.vs[b] : 0.0f);
+            const float next = top >= vref ? vref_for(top) : vref;
+            step = vref * vref_inverse(next);
+            vref = next;
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
@@ -652,6 +657,8 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
                 }
 #pragma unroll
             for (int b = 0; b < BL; b++) fs[b] = 1.0f;
+        } else {
+            vref = sc.vref;
         }
 #pragma unroll
         for (int b = 0; b < BL; b++) {
@@ -661,10 +668,8 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
                           max3f(x[e + 6], x[e + 7], x[e + 7])) * fs[b];
         }
         const float mx = xor32_max(max3f(mb[0], mb[1], BL == 4 ? fmaxf(mb[BL - 2], mb[BL - 1]) : mb[1]));
-        const float step = sc.step;
-        vref = sc.vref;
         const bool grew = __any(mx > m + RESCALE_SLACK);
-        if (grew || __builtin_amdgcn_readfirstlane(step != 1.0f)) {
+        if (grew || __any(step != 1.0f)) {
             float al = step;
             if (grew) {
                 const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
@@ -678,27 +683,35 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
                 for (int e = 0; e < 16; e++) o[b][e] *= al;
         }
         const float mu = P_BIAS - (m == -INFINITY ? 0.0f : m);
-        auto probabilities = [&](int b) __attribute__((always_inline)) {  // of a block
-            const float ma = FOLD ? mu + sc.log[b] : mu, share = FOLD ? 1.0f : sc.share[b];
+        auto probabilities = [&](auto fold, int b) __attribute__((always_inline)) {  // of a block
+            constexpr bool IN = decltype(fold)::value;  // its share is in the exponent
+            const float ma = IN ? mu + sc.log[b] : mu;
+            // (of a block that the row does not attend it may be anything: held to 1)
+            const float share = IN ? 1.0f : fminf(sc.vs[b] * vref_inverse(vref), 1.0f);
             float lb = 0.0f;
 #pragma unroll
             for (int e = 8 * (b & 1); e < 8 * (b & 1) + 8; e += 2) {
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(s.s[b >> 1][e], fs[b], ma));
                 const float p1 = __builtin_amdgcn_exp2f(fmaf(s.s[b >> 1][e + 1], fs[b], ma));
                 const int x = 8 * (b >> 1) + e / 2;
-                if constexpr (FOLD) {
+                if constexpr (IN) {
                     split_p<M::P>(p0, p1, p.h[x], p.l[x], lb);
                 } else {
                     float none = 0.0f;
-                    l += p0;
-                    l += p1;
+                    lb += p0;
+                    lb += p1;
                     split_p<M::P>(p0 * share, p1 * share, p.h[x], p.l[x], none);
                 }
             }
-            if constexpr (FOLD) l = fmaf(lb, sc.inv[b], l);
+            l = IN ? fmaf(lb, sc.inv[b], l) : l + lb;
         };
+        if (FOLD && !edge && !__builtin_amdgcn_readfirstlane(sc.small)) {
 #pragma unroll
-        for (int b = 0; b < BL; b++) probabilities(b);
+            for (int b = 0; b < BL; b++) probabilities(std::integral_constant<bool, FOLD>{}, b);
+        } else {
+#pragma unroll
+            for (int b = 0; b < BL; b++) probabilities(std::false_type{}, b);
+        }
         // computed here, not where the products take them
 #if __HIP_DEVICE_COMPILE__
 #pragma unroll
@@ -714,7 +727,7 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
         // eight codes of V or of K at a time, then the next loads
         constexpr int WORK = LAST ? 0 : 4 * N + 1;
         auto work = [&](int x) __attribute__((always_inline)) {
-            if (x < 2 * N) unpack_v(x >> 1, x & 1, t + 1, rest);
+            if (x < 2 * N) unpack_v(x >> 1, x & 1, t + 1);
             else if (x < 4 * N) unpack_k(x / 2 - N, x & 1, t + 2);
             else {
                 load_v(vr, page_of(t + 2), t + 2);
@@ -761,11 +774,10 @@ TN_INLINE void many8_tile(const Paged8Args& a, uint8_t* lds, Scales* scales, int
 #pragma unroll
         for (int x = 0; x < 2 * N; x++) unpack_k(x >> 1, x & 1, t0 + 1);
         load_k(kr, page_of(t0 + 2), t0 + 2);
-        __syncthreads();  // (the scales are there)
-        const uint32_t rest = rest_of(t0);
 #pragma unroll
-        for (int x = 0; x < 2 * N; x++) unpack_v(x >> 1, x & 1, t0, rest);
+        for (int x = 0; x < 2 * N; x++) unpack_v(x >> 1, x & 1, t0);
         load_v(vr, page_of(t0 + 1), t0 + 1);
+        __syncthreads();
         fetch(PG, t0 & 1);
 #pragma unroll
         for (int n = PG; n < G; n++) {
