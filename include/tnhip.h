@@ -18,7 +18,11 @@
  *     device and stream) for the activation quantisation of the prefill GEMM
  *     and the split-KV partials of decode attention.
  *   - `stream` is a hipStream_t (NULL = the default stream). Compute calls are
- *     asynchronous on it and never synchronise the host.
+ *     asynchronous on it and never synchronise the host. Threads may call on one
+ *     stream at once: the launches of a call that uses a workspace, or a `work`
+ *     buffer of the caller's, follow one another, with no other such call's
+ *     between them, so that calls on one stream may share a `work` whichever
+ *     threads make them. Calls on two streams at once need one each.
  *   - Every call returns a tn_status. On failure, tn_last_error() returns a
  *     thread-local message; TN_ENOTIMPL maps to Python's NotImplementedError
  *     (err.rs:11-13, a refusal by name), TN_EINVAL to RuntimeError with the
@@ -249,8 +253,8 @@ tn_status tn_dense_linear(void* stream, const float* x, int64_t m, int64_t k, co
  * linear: y = matmul(quantize(x)), the same bits, x_dtype as quantize's. `work`:
  *   tn_i8_linear_work_bytes(m, k) bytes of scratch, 16-byte aligned, the
  *   caller's (0 bytes and a null pointer for few rows, which are quantised in
- *   the launch that multiplies them); calls on one stream may share it, graphs
- *   that replay at once need one each. Nothing is allocated.
+ *   the launch that multiplies them); calls on one stream may share it, from any
+ *   threads, graphs that replay at once need one each. Nothing is allocated.
  * k is 1 to 131072 (a sum stays below 2^31); m <= 2^24 - 1, n <= 2^24 - 1. y overlaps no
  * input. k <= 0 is refused with TN_EINVAL "mat1 and mat2 shapes cannot be
  * multiplied" as quant.rs:322-332, other dtypes with TN_ENOTIMPL. */

@@ -1007,3 +1007,37 @@ def test_a_rows_bits_do_not_depend_on_later_tokens_values(tn, many, dtype):
         got.append(c.run(tn, bits=True, many=many))
     for out, lse in got[1:]:
         assert np.array_equal(out[:48], got[0][0][:48]) and np.array_equal(lse[:48], got[0][1][:48])
+
+
+# --- threads ------------------------------------------------------------------------------------
+
+
+def test_threads_on_one_stream_share_layers_and_caches(tn):
+    """Each thread's products and attention are its own, bit for bit, where all go through the same scratch."""
+    import threading
+
+    rng = np.random.default_rng(31)
+    layer = tn.Int8Linear(tn.i8_quantize(_up(tn, rng.standard_normal((900, 700)).astype(np.float32))))
+    c = Case(tn, "bfloat16", 2, 4, 128, 16, [1, 1, 1], [900, 1300, 40])
+    dev, table = _fill(tn, c.cache), object.__new__(tn.PageTable)
+    table.requests, table.width, table.page_size = 3, c.table.shape[1], c.S
+    table.row_start, table.lens, table.table = (_ints(tn, a) for a in (c.row_start, c.lens, c.table))
+    xs = [_up(tn, rng.standard_normal((70, 700)).astype(np.float32)) for _ in range(4)]
+    qs = [_up(tn, rng.standard_normal((3, 8, 128)).astype(np.float32), "bfloat16") for _ in range(4)]
+    want = [(layer(x).numpy(), dev.attend(q, table, 1, 1300)[0].bits()) for x, q in zip(xs, qs)]
+    bad, go = [], threading.Barrier(4)
+
+    def work(i):
+        try:
+            go.wait()
+            for n in range(40):
+                y, (a, _) = layer(xs[i]), dev.attend(qs[i], table, 1, 1300)
+                if n % 8 == 7 and not (np.array_equal(y.numpy(), want[i][0]) and np.array_equal(a.bits(), want[i][1])):
+                    bad.append((i, n))
+        except Exception as e:  # noqa: BLE001
+            bad.append((i, repr(e)))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert bad == []

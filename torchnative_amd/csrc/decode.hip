@@ -695,6 +695,7 @@ tn_status tn_llama_step(void* stream, const tn_llama* m) {
     tn_status s = check_model(m);
     if (s != TN_OK) return s;
     hipStream_t st = (hipStream_t)stream;
+    const Turn turn(stream);
     const LlamaWork w = llama_work(m);
     float* h = m->work + w.h;
     float* qkv = m->work + w.qkv;
@@ -842,6 +843,7 @@ tn_status tn_llama_prefill(void* stream, const tn_llama* m, int64_t T, float* wo
     if (m->head_dim % 2 != 0 || m->head_dim > 1024)
         return fail(TN_ENOTIMPL, "tn_llama_prefill: head_dim must be even and at most 1024");
     hipStream_t st = (hipStream_t)stream;
+    const Turn turn(stream);
     const PrefillWork w = prefill_work(m, T);
     const int64_t H = m->hidden, D = m->head_dim, Hq = m->n_heads, Hkv = m->n_kv_heads, I = m->inter;
     const int64_t nqkv = (Hq + 2 * Hkv) * D;
@@ -919,6 +921,7 @@ tn_status tn_llama_capture(void* stream, const tn_llama* m, int64_t steps, void*
     tn_status s = check_model(m);
     if (s != TN_OK) return s;
     hipStream_t st = (hipStream_t)stream;
+    const Turn turn(stream);
     // capture records the stream's work from here on: it must be idle
     TN_HIP(hipStreamSynchronize(st));
     TN_HIP(hipStreamBeginCapture(st, hipStreamCaptureModeThreadLocal));

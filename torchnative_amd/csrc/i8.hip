@@ -720,6 +720,7 @@ tn_status tn_i8_linear(void* stream, const void* x, int x_dtype, int64_t m, int6
     }
     int8_t* codes = static_cast<int8_t*>(work);
     float* scales = reinterpret_cast<float*>(codes + m * pitch_of(k));
+    const Turn turn(stream);
     TN_TRY(quantize((hipStream_t)stream, x, x_dtype, m, k, codes, scales));
     MmArgs p{{codes, scales}, {w, w_scales}, bias, y, (int)m, (int)n, (int)pitch_of(k), y_dtype};
     return matmul((hipStream_t)stream, p);

@@ -1072,6 +1072,7 @@ tn_status tn_sdpa_paged_q4_0(void* stream, const tn_q4_cache* cache, int dtype, 
     a.part_o = work, a.many_o = work + few * D;
     a.part_ml = reinterpret_cast<float2*>(work + rows * D), a.many_ml = a.part_ml + few;
     hipStream_t st = (hipStream_t)stream;
+    const Turn turn(stream);
     if (dtype == TN_F32) return launch<TN_F32>(st, a, tokens);
     if (dtype == TN_BF16) return launch<TN_BF16>(st, a, tokens);
     return launch<TN_F16>(st, a, tokens);

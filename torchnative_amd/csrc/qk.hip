@@ -957,6 +957,7 @@ tn_status tn_q4_k_linear(void* stream, const void* x, int x_dtype, int64_t m, in
         return fail(TN_EINVAL, std::string(OP) + ": x and the q4_k weight must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;
     const int yb = y_dtype == TN_BF16;
+    const Turn turn(stream);
     if (x_dtype == TN_F32) return linear_qk<float>(st, static_cast<const float*>(x), m, k, w, n, bias, y, yb);
     return linear_qk<uint16_t>(st, static_cast<const uint16_t*>(x), m, k, w, n, bias, y, yb);
 }

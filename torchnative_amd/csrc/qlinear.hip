@@ -1084,11 +1084,13 @@ tn_status tn_q4_0_linear_decode(void* stream, const float* x, int64_t k, int pro
 
 tn_status tn_q4_0_linear(void* stream, const void* x, int x_dtype, int64_t m, int64_t k, const uint8_t* qs,
                          const uint16_t* d, int64_t n, const float* bias, void* y, int y_dtype) {
+    const Turn turn(stream);
     return linear_entry<FMT_Q4_0>(stream, x, x_dtype, m, k, qs, d, n, bias, y, y_dtype);
 }
 
 tn_status tn_q8_0_linear(void* stream, const void* x, int x_dtype, int64_t m, int64_t k, const int8_t* qs,
                          const uint16_t* d, int64_t n, const float* bias, void* y, int y_dtype) {
+    const Turn turn(stream);
     return linear_entry<FMT_Q8_0>(stream, x, x_dtype, m, k, reinterpret_cast<const uint8_t*>(qs), d, n, bias, y,
                                   y_dtype);
 }

@@ -38,6 +38,19 @@ Counters& counters() {
 }
 
 namespace {
+// Streams' turns, several streams to a lock where there are more of them: a call holds one
+// at a time, however deep, so no two wait for each other.
+constexpr int TURNS = 64;
+std::recursive_mutex g_turns[TURNS];
+std::recursive_mutex& turn_of(void* stream) {
+    return g_turns[(reinterpret_cast<uintptr_t>(stream) * 0x9E3779B97F4A7C15ull >> 58) % TURNS];
+}
+}  // namespace
+
+Turn::Turn(void* stream) : mu_(turn_of(stream)) { mu_.lock(); }
+Turn::~Turn() { mu_.unlock(); }
+
+namespace {
 // A stream's scratch. A graph captured from a stream keeps the addresses it
 // saw, so once a stream has been captured a buffer outgrown by a later,
 // larger call is retired (kept) rather than freed, and all of them go with

@@ -2470,6 +2470,7 @@ extern "C" {
 tn_status tn_sdpa_fwd(void* stream, int dtype, const void* q, const void* k, const void* v, int64_t B, int64_t Hq,
                       int64_t Hkv, int64_t L, int64_t S, int64_t D, const void* attn_mask, int mask_dtype,
                       const int64_t* mask_strides, int is_causal, double scale, void* out, float* lse) {
+    const Turn turn(stream);
     if (dtype != TN_F32 && dtype != TN_BF16 && dtype != TN_F16 && dtype != TN_F64)
         return fail(TN_EINVAL, "scaled_dot_product_attention_flash_attention: Expected data type in FP32, FP64, BF16, "
                                "FP16");
@@ -2772,6 +2773,7 @@ extern "C" {
 tn_status tn_sdpa_decode(void* stream, int dtype, const void* q, const void* k_cache, const void* v_cache, int64_t B,
                          int64_t Hq, int64_t Hkv, int64_t cap, int64_t D, const int32_t* lens, int64_t max_len,
                          double scale, void* out, float* lse) {
+    const Turn turn(stream);
     return decode_entry(stream, dtype, q, k_cache, v_cache, B, Hq, Hkv, cap, D, lens, max_len, scale, out, lse,
                         workspace);
 }
@@ -2779,6 +2781,7 @@ tn_status tn_sdpa_decode(void* stream, int dtype, const void* q, const void* k_c
 tn_status tn_sdpa_decode_noalloc(void* stream, int dtype, const void* q, const void* k_cache, const void* v_cache,
                                  int64_t B, int64_t Hq, int64_t Hkv, int64_t cap, int64_t D, const int32_t* lens,
                                  int64_t max_len, double scale, void* out, float* lse) {
+    const Turn turn(stream);
     return decode_entry(stream, dtype, q, k_cache, v_cache, B, Hq, Hkv, cap, D, lens, max_len, scale, out, lse,
                         static_scratch);
 }

@@ -8,6 +8,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
+#include <mutex>
 #include <string>
 
 #include "../../include/tnhip.h"
@@ -30,8 +31,23 @@ struct Counters {
 };
 Counters& counters();
 
-// Grow-only device workspace, one per (device, stream). Calls on one stream
-// are ordered, so reuse across them is safe.
+// A call's turn on its stream, from its first launch to its last: launches that
+// share a buffer, the library's or the caller's, have no other thread's between
+// them, and no buffer grows away under a call that holds its address. Entry points
+// of such launches take one; calls within a call share it.
+class Turn {
+  public:
+    explicit Turn(void* stream);
+    ~Turn();
+    Turn(const Turn&) = delete;
+    Turn& operator=(const Turn&) = delete;
+
+  private:
+    std::recursive_mutex& mu_;
+};
+
+// Grow-only device workspace, one per (device, stream), for a call that holds the
+// stream's Turn. Calls on one stream are ordered, so reuse across them is safe.
 tn_status workspace(hipStream_t stream, size_t bytes, void** out);
 // The same for a call that can do without: null, and no refusal, where the
 // stream is under graph capture and its workspace would have to grow.

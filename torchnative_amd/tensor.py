@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 import weakref
 
 import numpy as np
@@ -287,19 +288,21 @@ def row_stride(t) -> int:
 
 
 class Scratch:
-    """Scratch bytes of one owner, a buffer a device and stream (calls on a stream are ordered). An outgrown buffer
-    stays: a captured graph may point at it."""
+    """Scratch bytes of one owner, a buffer a device and stream (calls on a stream are ordered, and the launches of one
+    follow one another whichever thread makes it). An outgrown buffer stays: another thread's call, or a captured graph,
+    may point at it."""
 
     def __init__(self):
-        self._held = {}
+        self._held, self._lock = {}, threading.RLock()
 
     def get(self, nbytes: int) -> Tensor:
         device = ctypes.c_int()
         check(lib().tn_get_device(ctypes.byref(device)))
-        held = self._held.setdefault((device.value, current_stream()), [])
-        if not held or held[-1].nbytes < nbytes:
-            held.append(Tensor((max(nbytes, 2 * held[-1].nbytes if held else 1),), "uint8", "hip"))
-        return held[-1]
+        with self._lock:
+            held = self._held.setdefault((device.value, current_stream()), [])
+            if not held or held[-1].nbytes < nbytes:
+                held.append(Tensor((max(nbytes, 2 * held[-1].nbytes if held else 1),), "uint8", "hip"))
+            return held[-1]
 
 
 def tensor(data, dtype: str | None = None, device="cpu") -> Tensor:
