@@ -1,5 +1,5 @@
 """Several threads on one stream: the launches of a call that share a buffer, the caller's or the library's, follow one
-another with no other call's between them. Run over tests/hip_record.cpp, which records launches and runs none."""
+another with no other call's between them. And scratch that ends with its stream. Run over tests/hip_record.cpp, which records launches and runs none."""
 
 import os
 import shutil
@@ -126,4 +126,66 @@ def test_launches_of_a_call_stay_together(recorder, name):
     r = subprocess.run([sys.executable, "-c", CHILD, recorder, name], capture_output=True, text=True, timeout=120,
                        cwd=os.path.dirname(HERE))
     print(r.stdout)
+    assert r.returncode == 0, r.stdout + r.stderr[-1500:]
+
+
+ENDS = r"""
+import ctypes, gc, sys
+R = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)
+import torchnative_amd as tn
+from torchnative_amd import _C
+T = sys.modules["torchnative_amd.tensor"]
+
+
+def events():
+    n = R.record_events(None, 0)
+    out = (ctypes.c_int64 * (2 * max(n, 1)))()
+    R.record_events(out, n)
+    return [(out[2 * i], out[2 * i + 1]) for i in range(n)]
+
+
+GIVEN, FREED, WAITED, ENDED = 1, 2, 3, 4
+x, w, y = tn.empty((64, 256)), tn.I8Rows((128, 256)), tn.empty((64, 128))
+cache, table = tn.Q8Cache(512, 16, 8, 128), object.__new__(tn.PageTable)
+table.requests, table.width, table.page_size = 1, 512, 16
+table.row_start, table.lens, table.table = (tn.empty((n,), "int32") for n in (2, 1, 512))
+q, out, lse = tn.empty((1, 32, 128)), tn.empty((1, 32, 128)), tn.empty((1, 32))
+
+
+def calls():
+    tn.i8_linear(x, w, out=y)
+    cache.attend(q, table, 1, 8000, out=out, lse=lse)
+
+
+calls()
+always = _C._i8_work._held[0, None] + cache._work._held[0, None]  # the default stream's
+for rnd in range(3):
+    s = tn.Stream()
+    R.record_clear()
+    with s:
+        calls()
+        tn.i8_linear(tn.empty((640, 256)), w, out=tn.empty((640, 128)))  # outgrows the first
+    handle = s.handle
+    held = [t.data_ptr() for o in (_C._i8_work, cache._work) for t in o._held[0, handle]]
+    assert len(held) == 3, held
+    was = events()
+    assert all((GIVEN, p) in was and (FREED, p) not in was for p in held), "another stream's buffer"
+    R.record_clear()
+    del s
+    gc.collect()
+    seen = events()
+    print(seen)
+    end = seen.index((ENDED, handle))
+    for p in held:
+        assert (FREED, p) in seen, "a buffer outlives its stream"
+        assert seen.index((WAITED, handle)) < seen.index((FREED, p)) and seen.index((WAITED, handle)) < end
+    assert list(_C._i8_work._held) == [(0, None)] and list(cache._work._held) == [(0, None)]
+assert _C._i8_work._held[0, None] + cache._work._held[0, None] == always
+"""
+
+
+def test_scratch_ends_with_its_stream(recorder):
+    """Its buffers are free for others only when its work has ended, and none stays behind."""
+    r = subprocess.run([sys.executable, "-c", ENDS, recorder], capture_output=True, text=True, timeout=120,
+                       cwd=os.path.dirname(HERE))
     assert r.returncode == 0, r.stdout + r.stderr[-1500:]

@@ -415,8 +415,8 @@ def i8_linear(input: Tensor, weight: I8Rows, bias: Tensor | None = None, *, out_
     """input @ weight.T (+ bias), the input's rows quantised to 8-bit integers
     first, a scale a token (tn_i8_linear). out_dtype: the input's by default.
     `work` (tn_i8_linear_work_bytes(m, k) bytes) and `out` are made where they
-    are not given; code that captures passes its own, a `work` of its own for
-    each graph."""
+    are not given (a `work` that goes with its stream); code that captures
+    passes its own, a `work` of its own for each graph."""
     op = "i8_linear"
     odt = out_dtype or (out.dtype if out is not None else input.dtype)
     out = _i8_out(op, input, weight, bias, out, odt)

@@ -147,8 +147,9 @@ class _Cache:
         Rows of a request that the step refused (`pages.base` -1, `pages.slots` -1) are not in the cache; what they get
         here is the attention of the request's earlier tokens, to be dropped.
 
-        `work`, `out` and `lse` are made where they are not given. Code that captures passes its own, so that the
-        graph's buffers live as long as it does, a `work` of its own for each graph."""
+        `work`, `out` and `lse` are made where they are not given (a `work` that goes with its stream). Code that
+        captures passes its own, so that the graph's buffers live as long as it does, a `work` of its own for each
+        graph."""
         op = f"sdpa_paged_{self._kind}"
         _require_hip(op, work, out, lse, rows=(q,))
         if q.dim() != 3 or q.shape[2] != self.head_dim:

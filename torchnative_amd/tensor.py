@@ -67,6 +67,10 @@ class Stream:
 
 def _destroy_stream(h):
     try:
+        # taken ahead of the handle's end, which another stream may then have; freed when the stream's work has ended
+        held = Scratch.of_stream(h)
+        if held:
+            check(lib().tn_stream_synchronize(h))
         lib().tn_stream_destroy(h)
     except Exception:  # interpreter shutdown
         pass
@@ -290,10 +294,21 @@ def row_stride(t) -> int:
 class Scratch:
     """Scratch bytes of one owner, a buffer a device and stream (calls on a stream are ordered, and the launches of one
     follow one another whichever thread makes it). An outgrown buffer stays: another thread's call, or a captured graph,
-    may point at it."""
+    may point at it. All go with their stream, as the library's workspaces do."""
+
+    _all = weakref.WeakSet()
+    _lock = threading.RLock()  # (a stream may end, by the garbage collector, inside a call here)
 
     def __init__(self):
-        self._held, self._lock = {}, threading.RLock()
+        self._held = {}
+        with Scratch._lock:
+            Scratch._all.add(self)
+
+    @staticmethod
+    def of_stream(handle) -> list:
+        """The buffers of a stream that ends, taken from their owners."""
+        with Scratch._lock:
+            return [s._held.pop(k) for s in Scratch._all for k in list(s._held) if k[1] == handle]
 
     def get(self, nbytes: int) -> Tensor:
         device = ctypes.c_int()
