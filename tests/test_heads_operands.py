@@ -101,3 +101,16 @@ def test_rows_with_a_stride_hand_it_on(calls):
         (a,) = calls.named(f"tn_sdpa_paged_{kind}")
         assert a[3:5] == (base, 512)
     assert isinstance(cache._c, ctypes.Structure) and _lib.Q8Cache is type(cache._c)
+
+
+def test_rows_of_codes_are_where_their_planes_are(calls):
+    """Whatever the device is called, or not named at all."""
+    for name in ("hip", "cuda", "cuda:0", "hip:0"):
+        w = tn.I8Rows((7, 64), name)
+        assert w.device == "hip"
+        tn.i8_linear(_t(5, 64), w, out=_t(5, 7))
+        assert calls.named("tn_i8_linear")[-1][5] == w.codes.data_ptr()
+    host = [tn.Tensor(s, d, "cpu") for s, d in (((7, 64), "int8"), ((7,), "float32"))]
+    assert tn.I8Rows((7, 64), codes=host[0], scales=host[1]).device == "cpu"
+    with pytest.raises(RuntimeError, match="codes on cpu and scales on hip"):
+        tn.I8Rows((7, 64), codes=host[0], scales=_t(7))

@@ -333,13 +333,16 @@ class I8Rows:
 
     def __init__(self, shape, device="hip", codes=None, scales=None):
         m, k = (int(x) for x in shape)
-        self.shape, self.device = (m, k), device
+        self.shape = (m, k)
         self.codes = Tensor((m, (k + 63) // 64 * 64), "int8", device) if codes is None else codes
         self.scales = Tensor((m,), "float32", device) if scales is None else scales
         c, f = self.codes, self.scales
         if (c.shape, c.dtype, f.shape, f.dtype) != ((m, (k + 63) // 64 * 64), "int8", (m,), "float32"):
             raise RuntimeError(f"I8Rows: codes {list(c.shape)} {c.dtype} and scales {list(f.shape)} {f.dtype} do not "
                                f"hold rows {[m, k]}")
+        if c.device != f.device:
+            raise RuntimeError(f"I8Rows: codes on {c.device} and scales on {f.device}")
+        self.device = c.device
 
     @property
     def nbytes(self) -> int:
