@@ -540,8 +540,8 @@ tn_status tn_kv_read_q8(void* stream, const tn_q8_cache* cache, const int32_t* s
  * Sums, maxima and the softmax are f32. Codes enter the matrix products exactly.
  * A query is one f16 under a power of two of its own (two f16 parts for f32
  * rows); probabilities, times their values' block scale over the largest that
- * the row attends, are one f16 for 16-bit rows, two for f32 rows. The output is
- * rounded once. Probabilities times scales are held to 2^-30 of the row's
+ * the row attends, are one f16 for bf16 rows, two f16 parts for others. The output
+ * is rounded once. Probabilities times scales are held to 2^-30 of the row's
  * largest probability times the largest scale of values that it attends (lse
  * counts them all); blocks of later tokens do not count.
  * Scales are taken as finite and not negative.

@@ -1041,3 +1041,28 @@ def test_threads_on_one_stream_share_layers_and_caches(tn):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert bad == []
+
+
+# --- the digits of a probability ---------------------------------------------------------------
+
+
+@pytest.mark.parametrize("H, G, D, rows, lens", [(2, 4, 64, [1, 1], [700, 300]), (1, 4, 128, [160, 3], [400, 90]),
+                                                 (1, 2, 256, [90], [300])])
+@MANY
+def test_f16_rows_are_off_by_no_more_than_their_rounding(tn, many, H, G, D, rows, lens):
+    """Probabilities are held in two f16 parts: the bound of f32 rows, and a half step of f16 for the output's rounding.
+    In one part each is off by up to another half step, which some of these thousands of elements would show: queries of
+    one element keep the scores' share of the bound small."""
+    h = 2.0 ** -11
+    c = Case(tn, "float16", H, G, D, 16, rows, lens, seed=23)
+    x = 3 * c.q.numpy().astype(np.float32)
+    x[..., 1:] = 0
+    c.q = _up(tn, x, "float16")
+    out, lse = c.run(tn, many=many)
+    ro, rl, pav, _, qk, _ = P.attend(c.q.numpy().astype(np.float64), c.cache, c.row_start, c.lens, c.table, None)
+    tol, ltol = I.tolerance("float32", ro, rl, pav, qk, max(lens), D, c.cache.value_size())
+    tol = tol + h * (np.abs(ro) + tol) + 2.0 ** -25
+    worst, lworst = np.max(np.abs(out - ro) / tol), np.max(np.abs(lse - rl) / ltol)
+    off = float(np.linalg.norm(out - ro) / np.linalg.norm(ro))
+    print(f"  worst {worst:.3f} of the bound, lse {lworst:.3f}, off by {off:.2e} of the norm", flush=True)
+    assert worst <= 1 and lworst <= 1
