@@ -1,4 +1,6 @@
 import os
+import shutil
+import subprocess
 import sys
 
 import pytest
@@ -10,6 +12,17 @@ if ROOT not in sys.path:
 
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an MI355X (gfx950) and the built HIP library")
+
+
+@pytest.fixture(scope="session")
+def recorder(tmp_path_factory):
+    """A HIP runtime that records launches and runs none (hip_record.cpp), for a process to load ahead of the library."""
+    if shutil.which("g++") is None:
+        pytest.skip("g++ is not installed")
+    out = str(tmp_path_factory.mktemp("hip") / "librecord.so")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-pthread", "-o", out,
+                    os.path.join(ROOT, "tests", "hip_record.cpp")], check=True)
+    return out
 
 
 @pytest.fixture(scope="session")

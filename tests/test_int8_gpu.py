@@ -6,6 +6,7 @@ import functools
 
 import numpy as np
 import pytest
+from test_int8_shapes import PRODUCTS
 
 from oracle import int8 as I
 from oracle import paged as P
@@ -1066,3 +1067,29 @@ def test_f16_rows_are_off_by_no_more_than_their_rounding(tn, many, H, G, D, rows
     off = float(np.linalg.norm(out - ro) / np.linalg.norm(ro))
     print(f"  worst {worst:.3f} of the bound, lse {lworst:.3f}, off by {off:.2e} of the norm", flush=True)
     assert worst <= 1 and lworst <= 1
+
+
+# --- every shape of the product -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("m, n, k", PRODUCTS)
+def test_every_product_bit_for_bit(tn, m, n, k):
+    """Quantised on the device and by the oracle; the sums of codes are whole numbers below 2^53, exact in f64."""
+    rng = np.random.default_rng(m + n + k)
+    odt = DTYPES[(m + n) % 3]
+    x = rng.standard_normal((m, k)).astype(np.float32) * (0.5 + rng.random((m, 1))).astype(np.float32)
+    w = rng.standard_normal((n, k)).astype(np.float32)
+    b = rng.standard_normal(n).astype(np.float32)
+    tx, tw = _up(tn, x, DTYPES[m % 3]), tn.i8_quantize(_up(tn, w))
+    cx, sx = I.quantize(tx.numpy().astype(np.float32))
+    cw, sw = I.quantize(w)
+    print(f"case [{m}, {k}] x [{n}, {k}] {tx.dtype} -> {odt}", flush=True)
+    total = (cx.astype(np.float64) @ cw.T.astype(np.float64)).astype(np.float32)
+    want = _narrow(tn, ((total * sw[None]).astype(np.float32) * sx[:, None]).astype(np.float32) + b, odt)
+    got = tn.i8_linear(tx, tw, _up(tn, b), out_dtype=odt)
+    got = got.numpy() if odt == "float32" else got.bits()
+    assert got.tobytes() == want.tobytes(), np.argwhere(got != want)[:5]
+    a = tn.i8_quantize(tx)
+    assert np.array_equal(a.codes.numpy()[:, :k], cx)
+    again = tn.i8_matmul(a, tw, _up(tn, b), out_dtype=odt)
+    assert (again.numpy() if odt == "float32" else again.bits()).tobytes() == want.tobytes()

@@ -2,7 +2,6 @@
 another with no other call's between them. And scratch that ends with its stream. Run over tests/hip_record.cpp, which records launches and runs none."""
 
 import os
-import shutil
 import subprocess
 import sys
 
@@ -109,16 +108,6 @@ for st in (None, stream.value):
 NAMES = ["i8_linear", "sdpa_paged_q8 few", "sdpa_paged_q8 many", "sdpa_paged_q4_0 few", "sdpa_paged_q4_0 many",
          "q4_0_linear", "q8_0_linear", "q4_k_linear", "sdpa_fwd", "sdpa_decode", "sdpa_decode_noalloc", "llama_step",
          "llama_prefill"]
-
-
-@pytest.fixture(scope="session")
-def recorder(tmp_path_factory):
-    if shutil.which("g++") is None:
-        pytest.skip("g++ is not installed")
-    out = str(tmp_path_factory.mktemp("hip") / "librecord.so")
-    subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-pthread", "-o", out,
-                    os.path.join(HERE, "hip_record.cpp")], check=True)
-    return out
 
 
 @pytest.mark.parametrize("name", NAMES)
