@@ -456,8 +456,8 @@ struct FewSums {
     i32x4 part[FEW_W][64];
 };
 
-// The waves' sums (channels 4 g .. 4 g + 3 of token c) to the outputs of tokens m0 on.
-__device__ inline void few_out(const MmArgs& a, FewSums& s, const i32x4& acc, int m0, int n0, const float* sx) {
+// The waves' sums (channels 4 g .. 4 g + 3 of token c) to the outputs.
+__device__ inline void few_out(const MmArgs& a, FewSums& s, const i32x4& acc, int n0, const float* sx) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
     s.part[wave][lane] = acc;
     __syncthreads();
@@ -465,13 +465,13 @@ __device__ inline void few_out(const MmArgs& a, FewSums& s, const i32x4& acc, in
     i32x4 t = s.part[0][lane];
 #pragma unroll
     for (int i = 1; i < FEW_W; i++) t += s.part[i][lane];
-    const int m = m0 + c, n = n0 + 4 * g;
-    if (m >= a.m) return;
+    const int n = n0 + 4 * g;
+    if (c >= a.m) return;
 #pragma unroll
     for (int u = 0; u < 4; u++) {
         if (n + u >= a.n) break;
         const float v = finish(t[u], a.w.s[n + u], sx[c], a.bias != nullptr, a.bias ? a.bias[n + u] : 0.0f);
-        const int64_t i = (int64_t)m * a.n + n + u;
+        const int64_t i = (int64_t)c * a.n + n + u;
         if (a.y_dtype == TN_F32) static_cast<float*>(a.y)[i] = v;
         else static_cast<uint16_t*>(a.y)[i] = a.y_dtype == TN_BF16 ? bf16_out(v) : f16_out(v);
     }
@@ -489,23 +489,21 @@ __device__ __attribute__((always_inline)) inline void few_steps(const int8_t* px
     for (int u = 0; u < N; u++) acc = mfma_i8(w[u], x[u], acc);
 }
 
-__global__ __launch_bounds__(64 * FEW_W) void k_i8_few(const MmArgs a, int nwg) {
+__global__ __launch_bounds__(64 * FEW_W) void k_i8_few(const MmArgs a) {
     __shared__ FewSums sums;
     __shared__ float sx[16];
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int id = wg_number();
-    if (id >= nwg) return;
-    const int mtl = (a.m + 15) / 16, m0 = id % mtl * 16, n0 = id / mtl * 16;
-    if (threadIdx.x < 16) sx[threadIdx.x] = a.a.s[min(m0 + (int)threadIdx.x, a.m - 1)];
-    const int8_t* px = a.a.c + (int64_t)min(m0 + c, a.m - 1) * a.pitch + 16 * g;
+    const int n0 = blockIdx.x * 16;
+    if (threadIdx.x < 16) sx[threadIdx.x] = a.a.s[min((int)threadIdx.x, a.m - 1)];
+    const int8_t* px = a.a.c + (int64_t)min(c, a.m - 1) * a.pitch + 16 * g;
     const int8_t* pw = a.w.c + (int64_t)min(n0 + c, a.n - 1) * a.pitch + 16 * g;
     i32x4 acc = {0, 0, 0, 0};
     const int steps = a.pitch / 64, hi = (int)((int64_t)steps * (wave + 1) / FEW_W);
     int k = (int)((int64_t)steps * wave / FEW_W);
     for (; k + FEW_U <= hi; k += FEW_U) few_steps<FEW_U>(px, pw, k, acc);
     for (; k < hi; k++) few_steps<1>(px, pw, k, acc);
-    few_out(a, sums, acc, m0, n0, sx);
+    few_out(a, sums, acc, n0, sx);
 }
 
 // The same on rows as they are, up to FUSED_M of them: every workgroup quantises them into
@@ -565,15 +563,13 @@ __global__ __launch_bounds__(64 * FEW_W) void k_i8_fused(const MmArgs a, const v
     k += FEW_U;
     for (; k + FEW_U <= hi; k += FEW_U) few_steps<FEW_U>(px, pw, k, acc);
     for (; k < hi; k++) few_steps<1>(px, pw, k, acc);
-    few_out(a, sums, acc, 0, n0, sx);
+    few_out(a, sums, acc, n0, sx);
 }
 
 bool fused(int64_t m, int64_t k) { return m <= FUSED_M && m * pitch_of(k) <= FUSED_BYTES; }
 
 tn_status few_launch(hipStream_t st, const MmArgs& a) {
-    const int64_t nwg = cdiv(a.m, 16) * cdiv(a.n, 16);
-    if (nwg > INT32_MAX) return fail(TN_EVALUE, "i8_matmul: shape too large");
-    hipLaunchKernelGGL(k_i8_few, wg_grid(nwg), dim3(64 * FEW_W), 0, st, a, (int)nwg);
+    hipLaunchKernelGGL(k_i8_few, dim3((unsigned)cdiv(a.n, 16)), dim3(64 * FEW_W), 0, st, a);
     TN_LAUNCHED();
     return TN_OK;
 }
