@@ -383,15 +383,18 @@ __global__ __launch_bounds__(64) void k_paged8_combine(const Paged8Args a) {
 // t + 1, K of t + 2) in their shadow. A compute unit holds two workgroups, whose phases
 // fall beside one another's by themselves: one of 256 rows in two groups held half a turn
 // apart unpacks half as often and took as long (4096 bf16 rows of 32/8 heads of 128
-// elements 171 us either way; 2048 f32 rows 101 against 94). With one barrier a turn two
+// elements took the same; 2048 f32 rows 101 us against 93). With one barrier a turn two
 // tiles of each in LDS suffice: behind barrier t, V(t) and K(t + 1) are read, V(t + 1) and
 // K(t + 2) written, in the places of V(t - 1) and K(t), last read before it. What the
 // softmax takes of a tile's scales is written two turns ahead of it, by lanes of the last
 // wave, into one of four places.
 //
-// 4096 causal bf16 rows as above, 137 GFLOP, 171 us: 803 TFLOP/s; an f16 product of 16384
-// reaches 1263. The softmax's exponentials and the unpacking share the issue slots with the
-// products; neither LDS nor memory bounds it.
+// 4096 causal bf16 rows as above, 137 GFLOP, 155 to 171 us: 803 to 884 TFLOP/s; an f16
+// product of 16384 reaches 1263. By its counters a SIMD issues vector instructions in 58 % of
+// the cycles, the softmax's and the unpacking's for the most part, and its matrix core is busy
+// in 41 %: the two phases all but take turns. LDS is busy in 35 %; as each fragment of 16-bit
+// rows read from it feeds one product, it would be at its limit soon after if the matrix core
+// were busy throughout. Spilled registers: one of f32 rows of 160 elements, outside the loop.
 constexpr int MANY_ROWS = 128;  // folded rows of a workgroup
 template <int DT, int NB>
 struct Many8 {
