@@ -255,8 +255,8 @@ tn_status tn_dense_linear(void* stream, const float* x, int64_t m, int64_t k, co
  *   caller's (0 bytes and a null pointer for few rows, which are quantised in
  *   the launch that multiplies them); calls on one stream may share it, from any
  *   threads, graphs that replay at once need one each. Nothing is allocated.
- * k is 1 to 131072 (a sum stays below 2^31); m <= 2^24 - 1, n <= 2^24 - 1. y overlaps no
- * input. k <= 0 is refused with TN_EINVAL "mat1 and mat2 shapes cannot be
+ * k is 1 to 131072 (a sum stays below 2^31); m <= 2^24 - 1, n <= 2^24 - 1. A y that
+ * overlaps x, codes or work is refused with TN_EINVAL. k <= 0 is refused with TN_EINVAL "mat1 and mat2 shapes cannot be
  * multiplied" as quant.rs:322-332, other dtypes with TN_ENOTIMPL. */
 int64_t tn_i8_pitch(int64_t k);
 tn_status tn_i8_quantize(void* stream, const void* x, int dtype, int64_t m, int64_t k, int8_t* codes, float* scales);

@@ -258,3 +258,23 @@ def test_rows_of_codes_refuse_planes_that_do_not_hold_them():
                           (t((3, 128), "int8"), t((3,), "float64"))):
         with pytest.raises(RuntimeError, match="do not hold rows"):
             _C.I8Rows((3, 70), "cpu", codes, scales)
+
+
+def test_an_output_over_an_input_is_refused(L):
+    """Workgroups would read what others have written: one byte in common is enough, none is not."""
+    m, n, k = 3, 100, 200
+    x, w, far = 1 << 20, 1 << 24, 1 << 28
+
+    def lin(y, work=far, m=m):
+        return L.tn_i8_linear(None, x, _lib.TN_BF16, m, k, w, far, n, None, work, 1 << 40, y, _lib.TN_F32)
+
+    def mm(y):
+        return L.tn_i8_matmul(None, x, far, m, k, w, far, n, None, y, _lib.TN_F32)
+
+    ysize, pitch = m * n * 4, 256
+    for f, size in ((lin, m * k * 2), (mm, m * pitch)):
+        for y in (x, x + size - 4, x - ysize + 4, w, w + n * pitch - 4, w - ysize + 4):
+            assert f(y) == _lib.TN_EINVAL and "y overlaps an input" in _lib.last_error(), (f, y)
+    need = L.tn_i8_linear_work_bytes(300, k)
+    for y in (far, far + need - 4):
+        assert lin(y, m=300) == _lib.TN_EINVAL and "overlaps" in _lib.last_error()

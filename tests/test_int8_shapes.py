@@ -29,7 +29,7 @@ from torchnative_amd import _lib
 L, P, out = _lib.lib(), 1 << 20, []
 for m, n, k in json.loads(sys.argv[2]):
     R.record_clear()
-    _lib.check(L.tn_i8_linear(None, P, 0, m, k, P, P, n, None, P, 1 << 50, P, 0))
+    _lib.check(L.tn_i8_linear(None, P, 0, m, k, P, P, n, None, P, 1 << 50, 1 << 50, 0))
     last = R.record_launches(None, 0) - 1
     out.append((R.record_kernel(last).decode(), R.record_workgroups(last)))
 names, i = [], 0
@@ -59,3 +59,23 @@ def test_every_product_is_reached(recorder):
             assert 0 <= halved <= tiles
             kinds.add((halved > 0, halved < tiles))
     assert kinds == {(False, True), (True, False), (True, True)}, kinds
+
+
+BESIDE = r"""
+import ctypes, sys
+R = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)
+from torchnative_amd import _lib
+L = _lib.lib()
+m, n, k, x, w, far = 3, 100, 200, 1 << 20, 1 << 24, 1 << 28
+for y in (x + m * k * 2, x - m * n * 4, w + n * 256, w - m * n * 4):
+    _lib.check(L.tn_i8_linear(None, x, 1, m, k, w, far, n, None, None, 0, y, 0))
+for y in (x + m * 256, x - m * n * 4, w + n * 256):
+    _lib.check(L.tn_i8_matmul(None, x, far, m, k, w, far, n, None, y, 0))
+assert R.record_launches(None, 0) == 7
+"""
+
+
+def test_an_output_beside_its_inputs_is_taken(recorder):
+    r = subprocess.run([sys.executable, "-c", BESIDE, recorder], capture_output=True, text=True, timeout=120,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stdout + r.stderr[-1500:]

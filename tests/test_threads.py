@@ -50,7 +50,7 @@ def llama():
 
 model = llama()
 CALLS = {
-    "i8_linear": lambda st: L.tn_i8_linear(st, P, 1, 64, 4096, P, P, 4096, None, P, big, P, 1),
+    "i8_linear": lambda st: L.tn_i8_linear(st, P, 1, 64, 4096, P, P, 4096, None, P, big, big, 1),
     "sdpa_paged_q8 few": paged(L.tn_sdpa_paged_q8, q8, 16, 16, 1, 4096),
     "sdpa_paged_q8 many": paged(L.tn_sdpa_paged_q8, q8, 1, 512, 512, 20000),
     "sdpa_paged_q4_0 few": paged(L.tn_sdpa_paged_q4_0, q4, 16, 16, 1, 4096),

@@ -419,7 +419,7 @@ def i8_linear(input: Tensor, weight: I8Rows, bias: Tensor | None = None, *, out_
     first, a scale a token (tn_i8_linear). out_dtype: the input's by default.
     `work` (tn_i8_linear_work_bytes(m, k) bytes) and `out` are made where they
     are not given (a `work` that goes with its stream); code that captures
-    passes its own, a `work` of its own for each graph."""
+    passes its own, a `work` of its own for each graph. `out` is not the input."""
     op = "i8_linear"
     odt = out_dtype or (out.dtype if out is not None else input.dtype)
     out = _i8_out(op, input, weight, bias, out, odt)

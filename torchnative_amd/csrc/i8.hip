@@ -648,6 +648,13 @@ tn_status quantize(hipStream_t st, const void* x, int dtype, int64_t m, int64_t 
 
 bool row_dtype(int dtype) { return dtype == TN_F32 || dtype == TN_BF16 || dtype == TN_F16; }
 bool unaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
+int64_t size_of(int dtype) { return dtype == TN_F32 ? 4 : 2; }
+// Whether y [m, n] and `bytes` bytes at p have any in common: a product writes y while others of
+// its workgroups read.
+bool overlaps(const void* y, int64_t m, int64_t n, int y_dtype, const void* p, int64_t bytes) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(y), b = reinterpret_cast<uintptr_t>(p);
+    return a < b + (uintptr_t)bytes && b < a + (uintptr_t)(m * n * size_of(y_dtype));
+}
 
 tn_status size_check(const char* op, int64_t m, int64_t k, int64_t n) {
     if (k <= 0)
@@ -690,6 +697,8 @@ tn_status tn_i8_matmul(void* stream, const int8_t* a, const float* a_scales, int
     if (m == 0 || n == 0) return TN_OK;
     if (!a || !a_scales || !w || !w_scales || !y) return fail(TN_EVALUE, "i8_matmul: null pointer");
     if (unaligned(a) || unaligned(w)) return fail(TN_EVALUE, "i8_matmul: codes must be 16-byte aligned");
+    if (overlaps(y, m, n, y_dtype, a, m * pitch_of(k)) || overlaps(y, m, n, y_dtype, w, n * pitch_of(k)))
+        return fail(TN_EINVAL, "i8_matmul: y overlaps an input");
     MmArgs p{{a, a_scales}, {w, w_scales}, bias, y, (int)m, (int)n, (int)pitch_of(k), y_dtype};
     return matmul((hipStream_t)stream, p);
 }
@@ -713,6 +722,9 @@ tn_status tn_i8_linear(void* stream, const void* x, int x_dtype, int64_t m, int6
                                    std::to_string(need));
     if (!x || !w || !w_scales || !y || (need && !work)) return fail(TN_EVALUE, "i8_linear: null pointer");
     if (unaligned(w) || (need && unaligned(work))) return fail(TN_EVALUE, "i8_linear: codes and work must be 16-byte aligned");
+    if (overlaps(y, m, n, y_dtype, x, m * k * size_of(x_dtype)) || overlaps(y, m, n, y_dtype, w, n * pitch_of(k)) ||
+        overlaps(y, m, n, y_dtype, work, need))
+        return fail(TN_EINVAL, "i8_linear: y overlaps an input or work");
     if (fused(m, k)) {
         const MmArgs p{{nullptr, nullptr}, {w, w_scales}, bias, y, (int)m, (int)n, (int)pitch_of(k), y_dtype};
         return fused_launch((hipStream_t)stream, p, x, x_dtype, k);
